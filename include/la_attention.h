@@ -226,6 +226,99 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
                           int64_t head_dim, int dtype, int64_t window,
                           void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head.
+ *
+ *   S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T,   out_t = scale * q_t S_t
+ *
+ * with S_{-1} = init_state (zero if null).  The state is fp32 (batch, heads,
+ * d_qk, d_v), contiguous; log_decay is fp32 (heads) in device memory, finite
+ * and <= 0 or -inf (no memory).  d_qk and d_v are at most 128 and need not be
+ * equal.  The reference has no decayed form; the recurrence without decay is
+ * its chunked kernel's (kernels/nki_attention_chunked.py:20-113).
+ *
+ * q, k, v, out and the gradients are (batch, heads, seq_len, d) with a dense
+ * last dimension and any strides {batch, heads, seq_len} (in elements), so a
+ * projection's (batch, seq_len, heads, d) output needs no copy.  Inputs are
+ * never written, and out and the gradients may not overlap them.
+ *
+ * segments: each head's sequence is split into this many segments walked by
+ * different CTAs (0 = let the library choose); more than one needs the
+ * workspace (256-byte aligned) that la_decay_plan reports.  A value that is
+ * not finite reaches every output of its own 128-token tile, and what the
+ * recurrence carries it to.
+ * ------------------------------------------------------------------------- */
+int la_decay_plan(int64_t batch, int64_t heads, int64_t seq_len, int64_t d_qk, int64_t d_v,
+                  int dtype, int backward, int segments_requested, int *segments_out,
+                  size_t *workspace_bytes_out);
+
+/* Whole prompts.  final_state: null, or the state after the last token. */
+int la_decay_chunked_fwd(const void *q, const int64_t *q_strides, const void *k,
+                         const int64_t *k_strides, const void *v, const int64_t *v_strides,
+                         void *out, const int64_t *out_strides, const float *log_decay,
+                         int64_t batch, int64_t heads, int64_t seq_len, int64_t d_qk, int64_t d_v,
+                         int dtype, float scale, const float *init_state, float *final_state,
+                         void *workspace, size_t workspace_bytes, int segments, void *stream);
+
+/* Gradients of la_decay_chunked_fwd for d_out and d_final_state (null: zero).
+ * d_init_state may be null.  log_decay is a constant: it has no gradient. */
+int la_decay_chunked_bwd(const void *q, const int64_t *q_strides, const void *k,
+                         const int64_t *k_strides, const void *v, const int64_t *v_strides,
+                         const void *d_out, const int64_t *d_out_strides, void *dq,
+                         const int64_t *dq_strides, void *dk, const int64_t *dk_strides, void *dv,
+                         const int64_t *dv_strides, const float *log_decay, int64_t batch,
+                         int64_t heads, int64_t seq_len, int64_t d_qk, int64_t d_v, int dtype,
+                         float scale, const float *init_state, const float *d_final_state,
+                         float *d_init_state, void *workspace, size_t workspace_bytes,
+                         int segments, void *stream);
+
+/* One token of every sequence: the state is updated in place and out
+ * (batch, heads, d_v), contiguous, written.  q, k, v: (batch, heads, d) with
+ * strides {batch, heads}; state: dense last two dimensions, strides {batch,
+ * heads}, no two sequences' states overlapping. */
+int la_decay_step(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,
+                  const void *v, const int64_t *v_strides, void *out, float *state,
+                  const int64_t *state_strides, const float *log_decay, int64_t batch,
+                  int64_t heads, int64_t d_qk, int64_t d_v, int dtype, float scale, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Root-mean-square norm of rows of width d <= 16384, with the addition of a
+ * residual:   s = x + residual,  y = s / sqrt(mean(s^2) + eps) * weight.
+ *
+ * Rows are addressed as (shape[0], shape[1], shape[2], d) with a dense last
+ * dimension and strides {0, 1, 2} in elements for each input; y, sum and d_s
+ * are contiguous.  weight (null: ones) is fp32 or bf16 by weight_dtype.
+ * fp32 statistics.  sum (null or s in the inputs' dtype) and rstd (null or
+ * fp32, one per row: 1 / sqrt(mean + eps)) are what the gradient needs.  The
+ * reference has no norm; its module wrapper (benchmarks/
+ * based_attention_benchmark.py:24-69) is the block that these surround.
+ * ------------------------------------------------------------------------- */
+int la_rms_norm_fwd(const void *x, const int64_t *x_strides, const void *residual,
+                    const int64_t *residual_strides, const void *weight, void *y, void *sum,
+                    float *rstd, const int64_t *shape, int64_t d, int dtype, int weight_dtype,
+                    float eps, void *stream);
+
+/* The same with y held in e4m3 and fp32 scales (rows, d / group): a group's
+ * scale is max(amax |y|, 2^-96) / 448 and its values round(y / scale).  group
+ * is d (one scale per row) or 16, 32, 64, 128 or 256 dividing d; groups
+ * narrower than the row need 16-byte aligned rows. */
+int la_rms_norm_fp8(const void *x, const int64_t *x_strides, const void *residual,
+                    const int64_t *residual_strides, const void *weight, void *y, float *scales,
+                    void *sum, const int64_t *shape, int64_t d, int64_t group, int dtype,
+                    int weight_dtype, float eps, void *stream);
+
+/* Bytes of workspace la_rms_norm_bwd needs for d_weight on this device. */
+int la_rms_norm_bwd_workspace_size(int64_t rows, int64_t d, size_t *bytes);
+
+/* Gradient: s (the forward's sum, or x without a residual), rstd, d_y and
+ * d_sum (null: none) give d_s = the gradient of both x and residual, and
+ * d_weight (null: not computed; in weight_dtype; summed in a fixed order). */
+int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight, const void *d_y,
+                    const int64_t *d_y_strides, const void *d_sum, const int64_t *d_sum_strides,
+                    const float *rstd, void *d_s, void *d_weight, const int64_t *shape, int64_t d,
+                    int dtype, int weight_dtype, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,427 @@
+"""Linear attention with a decay for each head: the kernels against the
+definition in 64 bits, the gradients against the formulas and differences, and
+the refusals.
+
+Bounds.  Let A be the definition applied to |q|, |k|, |v| and |S_0|.  A product
+of fp32 sums over at most n terms is off by at most n 2^-24 A; a weight
+lambda^m by a few ulp, and by a few more for each tile that carried it.  With
+bf16 inputs the weights that multiply v and the state that multiplies q are
+rounded once to bf16 (half a step: 2^-8), and so is the output.
+"""
+
+import math
+
+import pytest
+import torch
+
+import trainium_linear_attention_b200 as T
+from trainium_linear_attention_b200 import ops
+
+gpu = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ definition
+def recurrence(q, k, v, g, scale, state):
+    """Token by token in float64 (b, h, t, d); returns (out, state)."""
+    lam = torch.exp(g.double())[:, None, None]
+    outs = []
+    for t in range(q.shape[2]):
+        state = lam * state + k[:, :, t, :, None] * v[:, :, t, None, :]
+        outs.append((q[:, :, t, None, :] @ state).squeeze(-2) * scale)
+    out = torch.stack(outs, 2) if outs else q.new_zeros((*q.shape[:2], 0, v.shape[-1]))
+    return out, state
+
+
+def definition(q, k, v, g, scale, state):
+    """The same, 64 tokens at a time."""
+    outs = []
+    for at in range(0, q.shape[2], 64):
+        qi, ki, vi = (x[:, :, at:at + 64] for x in (q, k, v))
+        out, end = T.ref_decay_attn(qi, ki, vi, g.double(), scale, state)
+        outs.append(out)
+        state = end
+    out = torch.cat(outs, 2) if outs else q.new_zeros((*q.shape[:2], 0, v.shape[-1]))
+    return out, state
+
+
+def bound(dtype, out, absolute, t, d):
+    terms = (2 * d + 128 + 8 * (t // 64 + 1) + 64) * 2.0 ** -24
+    if dtype == torch.float32 or out.dim() == 0:
+        return terms * absolute + 1e-30
+    return 2.0 ** -8 * 1.01 * (out.abs() + absolute) + 1e-30
+
+
+def make(b, h, t, dk, dv, dtype, layout="bhtd", seed=0, device="cuda"):
+    gen = torch.Generator().manual_seed(seed)
+
+    def heads(d):
+        if layout == "bthd":
+            return torch.randn(b, t, h, d, generator=gen).to(dtype).to(device).transpose(1, 2)
+        if layout == "sliced":  # rows inside wider ones, an odd token stride
+            wide = torch.randn(b, h, t, d + 8, generator=gen).to(dtype).to(device)
+            return wide[..., :d]
+        if layout == "odd":  # rows that start at no 16-byte boundary
+            wide = torch.randn(b, h, t, d + 3, generator=gen).to(dtype).to(device)
+            return wide[..., 1:d + 1]
+        return torch.randn(b, h, t, d, generator=gen).to(dtype).to(device)
+
+    q, k, v = heads(dk), heads(dk), heads(dv)
+    g = -torch.exp2(-8.0 * torch.arange(1, h + 1) / h).float().to(device)
+    state = (torch.randn(b, h, dk, dv, generator=gen) * 3).to(device)
+    return q, k, v, g, state
+
+
+def check_forward(q, k, v, g, scale, state, segments=0):
+    t, d = q.shape[2], q.shape[3]
+    s0 = torch.zeros(*q.shape[:2], d, v.shape[-1], device=q.device) if state is None else state
+    out, end = ops.decay_attention(q, k, v, g, scale=scale, initial_state=state,
+                                   return_state=True, segments=segments)
+    wide = [x.double() for x in (q, k, v)]
+    want, want_end = definition(*wide, g, scale, s0.double())
+    a_out, a_end = definition(*(x.abs() for x in wide), g, abs(scale), s0.double().abs())
+    assert out.dtype == q.dtype and out.shape == want.shape
+    assert ((out.double() - want).abs() <= bound(q.dtype, want, a_out, t, d)).all()
+    # bf16 inputs: lambda^m k v enters as two bf16 terms, off by 2^-17 of it
+    slack = 0.0 if q.dtype == torch.float32 else 2.0 ** -17
+    assert ((end.double() - want_end).abs()
+            <= bound(torch.float32, want_end, a_end, t, d) + slack * a_end).all()
+    return out, end
+
+
+# --------------------------------------------------------------------- CPU
+def test_reference_is_the_recurrence():
+    q, k, v, g, state = make(2, 3, 150, 8, 5, torch.float64, device="cpu")
+    want = recurrence(q, k, v, g, 0.3, state.double())
+    for got in (T.ref_decay_attn(q, k, v, g.double(), 0.3, state.double()),
+                definition(q, k, v, g, 0.3, state.double())):
+        for x, y in zip(got, want):
+            assert (x - y).abs().max() <= 1e-12 * y.abs().max()
+    # no memory at all: every token sees itself
+    gone = torch.full((3,), float("-inf"), dtype=torch.float64)
+    out, end = T.ref_decay_attn(q, k, v, gone, 1.0)
+    assert torch.allclose(out, (q * k).sum(-1, keepdim=True) * v, rtol=1e-12, atol=0)
+    assert torch.allclose(end, k[:, :, -1, :, None] * v[:, :, -1, None, :], rtol=1e-12, atol=0)
+
+
+def test_refusals():
+    q, k, v, g, state = make(1, 2, 8, 16, 16, torch.float32, device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        T.decay_linear_attention(q, k, v, g)
+    with pytest.raises(ValueError, match="CUDA"):
+        T.decay_linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g, state)
+    with pytest.raises(ValueError):
+        T.decay_linear_attention_step(q, k, v, g, state)
+    with pytest.raises(TypeError):
+        T.decay_linear_attention(q, k.double(), v, g)
+    for bad in (g[:1], g.double(), g.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="log_decay"):
+            ops._check_log_decay(bad, 2, q.device)
+    with pytest.raises(TypeError):
+        ops._check_log_decay(-0.5, 2, q.device)
+    with pytest.raises(ValueError, match="state"):
+        ops._check_state(state.double(), (1, 2, 16, 16), q.device, "state")
+
+
+def test_c_entry_points_refuse():
+    import ctypes
+
+    from trainium_linear_attention_b200 import _native as N
+
+    lib, p, s = N.lib(), ctypes.c_void_p(256), (ctypes.c_int64 * 3)(1, 1, 1)
+    n, ws = ctypes.c_int(0), ctypes.c_size_t(0)
+    plan = [ctypes.byref(n), ctypes.byref(ws)]
+    assert lib.la_decay_plan(2, 4, 4096, 64, 64, 1, 0, 4, *plan) == N.LA_OK
+    assert n.value == 4 and ws.value == 2 * 4 * 4 * 64 * 64 * 4
+    assert lib.la_decay_plan(2, 4, 4096, 64, 64, 1, 1, 4, *plan) == N.LA_OK
+    assert ws.value == 2 * 2 * 4 * 4 * 64 * 64 * 4
+    assert lib.la_decay_plan(2, 4, 100, 64, 64, 1, 0, 4, *plan) == N.LA_OK
+    assert n.value == 1 and ws.value == 0
+    assert lib.la_decay_plan(2, 4, 4096, 129, 64, 1, 0, 1, *plan) == N.LA_ERR_UNSUPPORTED
+    assert lib.la_decay_plan(2, 4, -1, 64, 64, 1, 0, 1, *plan) == N.LA_ERR_INVALID_ARGUMENT
+    assert lib.la_decay_plan(1 << 15, 4, 8, 64, 64, 1, 0, 1, *plan) == N.LA_ERR_UNSUPPORTED
+
+    def fwd(q=p, qs=s, dtype=1, b=1, t=8, dk=64, g=p, segments=0):
+        return lib.la_decay_chunked_fwd(q, qs, p, s, p, s, p, s, g, b, 2, t, dk, 64, dtype, 1.0,
+                                        None, None, None, 0, segments, None)
+
+    assert fwd(q=None) == fwd(qs=None) == fwd(dtype=5) == fwd(g=None) == N.LA_ERR_INVALID_ARGUMENT
+    assert fwd(segments=-1) == fwd(dk=0) == N.LA_ERR_INVALID_ARGUMENT
+    assert fwd(dk=130) == N.LA_ERR_UNSUPPORTED
+    assert fwd(b=0) == fwd(t=0) == N.LA_OK  # nothing to do
+    if not torch.cuda.is_available():
+        assert fwd() == N.LA_ERR_NO_DEVICE
+    assert lib.la_decay_step(p, s, p, s, p, s, p, None, s, p, 1, 2, 64, 64, 1, 1.0, None) == \
+        N.LA_ERR_INVALID_ARGUMENT
+    assert lib.la_decay_step(p, s, p, s, p, s, p, p, s, p, 0, 2, 64, 64, 1, 1.0, None) == N.LA_OK
+
+
+# --------------------------------------------------------------------- GPU
+WIDTHS = [(16, 64), (64, 64), (128, 128), (64, 128), (40, 72), (128, 8), (57, 33), (1, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [1, 2, 63, 64, 65, 127, 128, 129, 300])
+def test_lengths(t, dtype):
+    q, k, v, g, state = make(2, 3, t, 64, 64, dtype, seed=t)
+    check_forward(q, k, v, g, 0.125, state)
+    check_forward(q, k, v, g, 0.125, None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dk,dv", WIDTHS)
+def test_widths(dk, dv, dtype):
+    q, k, v, g, state = make(2, 5, 261, dk, dv, dtype, "bthd", seed=dk + dv)
+    check_forward(q, k, v, g, 1.0 / math.sqrt(dk), state)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["bthd", "sliced", "odd"])
+def test_layouts(layout, dtype):
+    q, k, v, g, state = make(2, 3, 200, 64, 64, dtype, layout)
+    out, end = check_forward(q, k, v, g, 0.125, state)
+    plain = ops.decay_attention(*(x.contiguous() for x in (q, k, v)), g, scale=0.125,
+                                initial_state=state, return_state=True)
+    assert torch.equal(out, plain[0]) and torch.equal(end, plain[1])
+    if layout == "bthd":
+        assert out.transpose(1, 2).is_contiguous()
+    # a broadcast head
+    one = q[:, :1].expand(-1, 3, -1, -1)
+    a = ops.decay_attention(one, k, v, g, scale=0.125)
+    assert torch.equal(a, ops.decay_attention(one.contiguous(), k, v, g, scale=0.125))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,segments", [(1000, 2), (1000, 3), (1024, 8), (2049, 5)])
+def test_segments(t, segments, dtype):
+    q, k, v, g, state = make(1, 4, t, 64, 128, dtype, seed=segments)
+    check_forward(q, k, v, g, 0.125, state, segments)
+    check_forward(q, k, v, g, 0.125, None, segments)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decays(dtype):
+    """No decay, none of the past, and everything between; an infinite decay is
+    the limit of a large one."""
+    q, k, v, _, state = make(1, 6, 333, 64, 64, dtype)
+    g = torch.tensor([0.0, -1e-4, -0.1, -3.0, -90.0, -200.0], device="cuda")
+    check_forward(q, k, v, g, 0.125, state)
+    g[4:] = float("-inf")
+    out, end = ops.decay_attention(q, k, v, g, scale=0.125, initial_state=state, return_state=True)
+    assert torch.isfinite(out).all()
+    near = torch.tensor([0.0, -1e-4, -0.1, -3.0, -200.0, -200.0], device="cuda")
+    same = ops.decay_attention(q, k, v, near, scale=0.125, initial_state=state, return_state=True)
+    assert torch.equal(out, same[0]) and torch.equal(end, same[1])
+
+
+@gpu
+def test_empty_and_zero_tokens():
+    q, k, v, g, state = make(2, 3, 0, 16, 64, torch.bfloat16)
+    out, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)
+    assert out.shape == (2, 3, 0, 64) and torch.equal(end, state)
+    _, end = T.decay_linear_attention(q, k, v, g, return_state=True)
+    assert not end.any()
+    q, k, v, g, state = make(0, 3, 5, 16, 64, torch.bfloat16)
+    assert T.decay_linear_attention(q, k, v, g).shape == (0, 3, 5, 64)
+    s = torch.zeros(0, 3, 16, 64, device="cuda")
+    assert T.decay_linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g, s).shape == (0, 3, 64)
+    q, k, v, g, state = make(1, 2, 0, 16, 64, torch.bfloat16)
+    state.requires_grad_()
+    _, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)
+    assert torch.equal(torch.autograd.grad(end.sum(), state)[0], torch.ones_like(state))
+
+
+@gpu
+def test_long_sequence_many_tiles():
+    """Slow decays over many tiles: the carried state and its power stay exact."""
+    q, k, v, g, state = make(1, 2, 20000, 16, 64, torch.float32)
+    g = torch.tensor([-1e-4, -2e-3], device="cuda")
+    check_forward(q, k, v, g, 0.25, state)
+    check_forward(*(x.bfloat16() for x in (q, k, v)), g, 0.25, state)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,dk,dv,segments", [(1, 16, 64, 0), (70, 64, 64, 0), (129, 40, 72, 0),
+                                              (300, 128, 64, 0), (1000, 64, 128, 3),
+                                              (333, 57, 33, 0), (2049, 64, 64, 5)])
+def test_gradients(t, dk, dv, segments, dtype):
+    q, k, v, g, state = make(2, 2, t, dk, dv, dtype, "bthd", seed=t)
+    do = torch.randn(2, 2, t, dv, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    ds = torch.randn(2, 2, dk, dv, generator=torch.Generator().manual_seed(2)).cuda()
+    got = ops.decay_attention_backward(q, k, v, g, do, scale=0.2, initial_state=state, d_state=ds,
+                                       want_d_initial=True, segments=segments)
+
+    def formulas(absolute):
+        leaves = [x.double() for x in (q, k, v, state)]
+        up = [x.double() for x in (do, ds)]
+        if absolute:
+            leaves, up = [x.abs() for x in leaves], [x.abs() for x in up]
+        leaves = [x.requires_grad_() for x in leaves]
+        out, end = definition(*leaves[:3], g, 0.2, leaves[3])
+        return torch.autograd.grad((out, end), leaves, up)
+
+    for i, (x, y, a) in enumerate(zip(got, formulas(False), formulas(True))):
+        kind = torch.float32 if i == 3 else dtype
+        slack = 2.0 ** -17 if i == 3 and dtype == torch.bfloat16 else 0.0
+        assert ((x.double() - y).abs() <= bound(kind, y, a, t, max(dk, dv)) + slack * a).all(), i
+
+
+@gpu
+def test_gradients_against_differences():
+    """The loss is linear in each input alone, so a central difference of any
+    length is the directional derivative, up to the forward pass's rounding."""
+    q, k, v, g, state = make(1, 3, 200, 40, 24, torch.float32)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v, state)]
+    gen = torch.Generator().manual_seed(3)
+    do = torch.randn(1, 3, 200, 24, generator=gen).cuda()
+    ds = torch.randn(1, 3, 40, 24, generator=gen).cuda()
+
+    def loss(*x):
+        out, end = T.decay_linear_attention(*x[:3], g, initial_state=x[3], return_state=True)
+        return (out.double() * do).sum() + (end.double() * ds).sum()
+
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    for i, x in enumerate(leaves):
+        step = torch.randn(x.shape, generator=gen).cuda()
+        up, down = ([y.detach() if j != i else (y + s * step).detach()
+                     for j, y in enumerate(leaves)] for s in (1, -1))
+        high, low = loss(*up), loss(*down)
+        slope = (grads[i].double() * step).sum()
+        # both sides are fp32 sums of these sizes
+        size = high.abs() + low.abs() + (grads[i].double().abs() * step.abs()).sum()
+        assert abs((high - low) / 2 - slope) <= 400 * 2.0 ** -24 * size
+
+
+@gpu
+def test_autograd_needs_and_nones():
+    q, k, v, g, state = make(1, 2, 50, 16, 16, torch.bfloat16)
+    q.requires_grad_()
+    out, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)
+    only = torch.autograd.grad(end.sum(), q, retain_graph=True, allow_unused=True)[0]
+    assert not only.any()  # the final state does not depend on q
+    dq = torch.autograd.grad(out.sum(), q)[0]  # an expanded gradient
+    want = ops.decay_attention_backward(q.detach(), k, v, g, torch.ones_like(out),
+                                        initial_state=state)[0]
+    assert torch.equal(dq, want)
+    with torch.no_grad():
+        assert not T.decay_linear_attention(q, k, v, g).requires_grad
+    out = T.decay_linear_attention(q, k, v, g)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(out.sum(), q, create_graph=True)[0].sum(), q)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,h,dk,dv", [(1, 1, 1, 1), (3, 5, 64, 64), (2, 4, 128, 128),
+                                       (2, 3, 40, 72), (2, 3, 57, 33), (300, 2, 16, 64)])
+def test_step(b, h, dk, dv, dtype):
+    q, k, v, g, state = make(b, h, 1, dk, dv, dtype)
+    q, k, v = (x[:, :, 0] for x in (q, k, v))
+    lam = torch.exp(g.double())[:, None, None]
+    want = lam * state.double() + k.double()[..., None] * v.double()[..., None, :]
+    held = lam * state.double().abs() + (k.double()[..., None] * v.double()[..., None, :]).abs()
+    out_want = (q.double()[..., None, :] @ want).squeeze(-2) * 0.3
+    size = (q.double().abs()[..., None, :] @ held).squeeze(-2) * 0.3
+    before = state.clone()
+    out = T.decay_linear_attention_step(q, k, v, g, state, scale=0.3)
+    assert ((state.double() - want).abs() <= 4 * 2.0 ** -24 * held).all()
+    last = 2.0 ** -8 * out_want.abs() if dtype == torch.bfloat16 else 0.0
+    assert ((out.double() - out_want).abs() <= (dk + 8) * 2.0 ** -24 * size * 1.01 + last).all()
+    # a view of a larger pool, strided vectors: the same bits, the rest untouched
+    pool = torch.full((b + 2, h, dk, dv), 7.0, device="cuda")
+    pool[1:b + 1] = before
+    wide = torch.empty(b, h + 1, dk, dtype=dtype, device="cuda")
+    wide[:, :h] = q
+    again = T.decay_linear_attention_step(wide[:, :h], k, v, g, pool[1:b + 1], scale=0.3)
+    assert torch.equal(out, again) and torch.equal(pool[1:b + 1], state)
+    assert (pool[0] == 7).all() and (pool[b + 1] == 7).all()
+
+
+@gpu
+def test_step_refuses():
+    q, k, v, g, state = make(2, 3, 1, 16, 16, torch.float32)
+    q, k, v = (x[:, :, 0] for x in (q, k, v))
+    for bad in (state[:1].expand(2, -1, -1, -1), state.transpose(2, 3), state[:, :, :8],
+                state.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            T.decay_linear_attention_step(q, k, v, g, bad)
+    with pytest.raises(ValueError):
+        T.decay_linear_attention_step(q, k, v[:1], g, state)
+    with pytest.raises(ValueError, match="state"):
+        T.decay_linear_attention(*(x[:, :, None] for x in (q, k, v)), g, initial_state=state[:1])
+    with pytest.raises(T.LaError):
+        T.decay_linear_attention(*(torch.zeros(1, 3, 4, 160, device="cuda"),) * 3, g)
+    # the state may not be rewritten under a backward pass that needs it
+    q4, k4, v4 = (x[:, :, None].clone().requires_grad_() for x in (q, k, v))
+    out = T.decay_linear_attention(q4, k4, v4, g, initial_state=state)
+    T.decay_linear_attention_step(q, k, v, g, state)
+    with pytest.raises(RuntimeError, match="modified"):
+        out.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_in_pieces_then_tokens(dtype):
+    """A prompt read at once, in pieces, and token by token end in one state."""
+    q, k, v, g, _ = make(2, 4, 300, 64, 64, dtype)
+    whole, end = check_forward(q, k, v, g, 0.125, None)
+    state, outs = None, []
+    for a, b in ((0, 100), (100, 101), (101, 290)):
+        out, state = T.decay_linear_attention(q[:, :, a:b], k[:, :, a:b], v[:, :, a:b], g,
+                                              initial_state=state, return_state=True)
+        outs.append(out)
+    for t in range(290, 300):
+        outs.append(T.decay_linear_attention_step(q[:, :, t], k[:, :, t], v[:, :, t], g,
+                                                  state)[:, :, None])
+    got = torch.cat(outs, 2).double()
+    wide = [x.double() for x in (q, k, v)]
+    s0 = torch.zeros(2, 4, 64, 64, device="cuda", dtype=torch.float64)
+    want, want_end = definition(*wide, g, 0.125, s0)
+    a_out, a_end = definition(*(x.abs() for x in wide), g, 0.125, s0)
+    assert ((got - want).abs() <= bound(dtype, want, a_out, 300, 64)).all()
+    assert ((state.double() - want_end).abs()
+            <= bound(torch.float32, want_end, a_end, 300, 64) + 2.0 ** -17 * a_end).all()
+
+
+@gpu
+def test_repeats_streams_and_graphs():
+    """The same bits on every call, on another stream, and replayed from graphs
+    whose captures share the allocator."""
+    q, k, v, g, state = make(1, 3, 4000, 64, 64, torch.bfloat16)
+    do = torch.randn_like(v)
+
+    def call():
+        return (*ops.decay_attention(q, k, v, g, initial_state=state, return_state=True),
+                *ops.decay_attention_backward(q, k, v, g, do, initial_state=state,
+                                              want_d_initial=True))
+
+    first = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    q0 = q.clone()
+    q.copy_(torch.randn_like(q))
+    for graph, _ in graphs:
+        graph.replay()
+    other = call()
+    q.copy_(q0)
+    assert all(torch.equal(x, y) for x, y in zip(graphs[0][1], other))
+    for graph, _ in reversed(graphs):
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in (second, graphs[0][1], graphs[1][1]):
+        assert all(torch.equal(x, y) for x, y in zip(first, got))
+    assert ops.N.lib().la_take_device_error(None) == 0

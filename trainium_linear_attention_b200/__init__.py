@@ -15,6 +15,9 @@ from .kernels.sliding_attention import nki_sliding_window_attn, ref_sliding_wind
 from .kernels.based_layer import based_layer, ref_based_layer  # noqa: F401
 from .kernels.based_module import (  # noqa: F401
     TrainiumBasedLinearAttention, TrainiumBasedLinearAttentionNKI)
+from .kernels.decay_attention import (  # noqa: F401
+    decay_linear_attention, decay_linear_attention_step, ref_decay_attn)
+from .kernels.rms_norm import ref_rms_norm, rms_norm, rms_norm_fp8  # noqa: F401
 from ._native import LaError  # noqa: F401
 
 __all__ = [
@@ -23,5 +26,7 @@ __all__ = [
     "based_chunked_state", "taylor_feature_map", "chunked_identity_numerator",
     "ref_identity_numerator", "based_chunked_host", "nki_sliding_window_attn",
     "ref_sliding_window_attn", "based_layer", "ref_based_layer",
-    "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI", "LaError",
+    "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI",
+    "decay_linear_attention", "decay_linear_attention_step", "ref_decay_attn",
+    "rms_norm", "rms_norm_fp8", "ref_rms_norm", "LaError",
 ]

@@ -44,6 +44,14 @@ EXPORTED_SYMBOLS = (
     "la_based_chunked_state",
     "la_sliding_window_fwd",
     "la_based_layer_fwd",
+    "la_decay_plan",
+    "la_decay_chunked_fwd",
+    "la_decay_chunked_bwd",
+    "la_decay_step",
+    "la_rms_norm_fwd",
+    "la_rms_norm_fp8",
+    "la_rms_norm_bwd_workspace_size",
+    "la_rms_norm_bwd",
 )
 
 _lock = threading.Lock()
@@ -96,6 +104,26 @@ def _declare(lib) -> None:
     lib.la_based_layer_fwd.argtypes = [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _i64,
                                        _f, _p, _sz, _int, _p]
     lib.la_based_layer_fwd.restype = _int
+    # (pointer, strides) pairs, then the sizes
+    lib.la_decay_plan.argtypes = [_i64] * 5 + [_int, _int, _int, ctypes.POINTER(_int),
+                                               ctypes.POINTER(_sz)]
+    lib.la_decay_plan.restype = _int
+    lib.la_decay_chunked_fwd.argtypes = ([_p] * 9 + [_i64] * 5
+                                         + [_int, _f, _p, _p, _p, _sz, _int, _p])
+    lib.la_decay_chunked_fwd.restype = _int
+    lib.la_decay_chunked_bwd.argtypes = ([_p] * 15 + [_i64] * 5
+                                         + [_int, _f, _p, _p, _p, _p, _sz, _int, _p])
+    lib.la_decay_chunked_bwd.restype = _int
+    lib.la_decay_step.argtypes = [_p] * 10 + [_i64] * 4 + [_int, _f, _p]
+    lib.la_decay_step.restype = _int
+    lib.la_rms_norm_fwd.argtypes = [_p] * 9 + [_i64, _int, _int, _f, _p]
+    lib.la_rms_norm_fwd.restype = _int
+    lib.la_rms_norm_fp8.argtypes = [_p] * 9 + [_i64, _i64, _int, _int, _f, _p]
+    lib.la_rms_norm_fp8.restype = _int
+    lib.la_rms_norm_bwd_workspace_size.argtypes = [_i64, _i64, ctypes.POINTER(_sz)]
+    lib.la_rms_norm_bwd_workspace_size.restype = _int
+    lib.la_rms_norm_bwd.argtypes = [_p] * 11 + [_i64, _int, _int, _p, _sz, _p]
+    lib.la_rms_norm_bwd.restype = _int
 
 
 def lib():

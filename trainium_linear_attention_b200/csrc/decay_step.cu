@@ -1,0 +1,109 @@
+// Single-token form of the decayed linear attention, in place:
+//   S = lambda S + k v^T,   out = scale * q S
+//
+// The state is read and written once (8 bytes per element, against one FMA
+// pair), so memory is the bound, and latency for a few heads.  One CTA takes
+// 32 columns of a head's state: 8 lanes x 16 bytes per row and 32 rows at a
+// time, so each thread has all its (at most 4) 16-byte loads in flight before
+// it uses the first, and a single sequence of 16 heads already spreads over 32
+// to 64 CTAs.  The read-out is summed over a warp's 4 row groups by shuffles
+// and over the 8 warps in shared memory, in a fixed order.
+#include "decay.cuh"
+#include "decay_step.cuh"
+
+namespace la {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kCols = 32;
+constexpr int kRowGroups = 32;
+constexpr int kRows = kDecayMaxWidth / kRowGroups;  // rows per thread, at most
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kThreads)
+decay_step_kernel(const DecayStep p) {
+  __shared__ float part[kThreads / 32][kCols];
+  const int64_t bh = blockIdx.x;
+  const int64_t ib = bh / p.heads, ih = bh % p.heads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.y * kCols + (lane & 7) * 4;
+  const int rg = warp * 4 + (lane >> 3);
+  float *state = p.state + ib * p.state_sb + ih * p.state_sh;
+  const T *q = (const T *)p.q + ib * p.q_sb + ih * p.q_sh;
+  const T *k = (const T *)p.k + ib * p.k_sb + ih * p.k_sh;
+  const T *v = (const T *)p.v + ib * p.v_sb + ih * p.v_sh;
+  float s[kRows][4], qr[kRows], kr[kRows], vc[4];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = rg + kRowGroups * i;
+    const bool in = row < p.dk;
+    if (kVec) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && col < p.dv) x = *(const float4 *)(state + (int64_t)row * p.dv + col);
+      s[i][0] = x.x; s[i][1] = x.y; s[i][2] = x.z; s[i][3] = x.w;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        s[i][x] = in && col + x < p.dv ? state[(int64_t)row * p.dv + col + x] : 0.f;
+    }
+    qr[i] = in ? to_f32(q[row]) : 0.f;
+    kr[i] = in ? to_f32(k[row]) : 0.f;
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) vc[x] = col + x < p.dv ? to_f32(v[col + x]) : 0.f;
+  const float lambda = decay_pow(p.log_decay[ih], 1);
+  float o[4] = {};
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = rg + kRowGroups * i;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      s[i][x] = fmaf(kr[i], vc[x], lambda * s[i][x]);
+      if (row < p.dk) o[x] = fmaf(qr[i], s[i][x], o[x]);
+    }
+    if (row < p.dk) {
+      float *dst = state + (int64_t)row * p.dv + col;
+      if (kVec) {
+        if (col < p.dv) *(float4 *)dst = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (col + x < p.dv) dst[x] = s[i][x];
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    o[x] += __shfl_xor_sync(0xffffffffu, o[x], 8);
+    o[x] += __shfl_xor_sync(0xffffffffu, o[x], 16);
+    if (lane < 8) part[warp][lane * 4 + x] = o[x];
+  }
+  __syncthreads();
+  if (threadIdx.x < kCols) {
+    const int c = blockIdx.y * kCols + threadIdx.x;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) sum += part[w][threadIdx.x];
+    if (c < p.dv) ((T *)p.out)[(ib * p.heads + ih) * p.dv + c] = from_f32<T>(p.scale * sum);
+  }
+}
+
+}  // namespace
+
+int launch_decay_step(const DecayStep &p, int64_t batch, int dtype, cudaStream_t s) {
+  const int64_t bh = batch * p.heads;
+  if (p.dk > kDecayMaxWidth || p.dv > kDecayMaxWidth || bh > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)bh, (unsigned)((p.dv + kCols - 1) / kCols));
+  const bool vec = ((uintptr_t)p.state & 15) == 0 && p.dv % 4 == 0 && p.state_sb % 4 == 0 &&
+                   p.state_sh % 4 == 0;
+  if (dtype == LA_DTYPE_FLOAT32) {
+    if (vec) decay_step_kernel<float, true><<<grid, kThreads, 0, s>>>(p);
+    else decay_step_kernel<float, false><<<grid, kThreads, 0, s>>>(p);
+  } else {
+    if (vec) decay_step_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, s>>>(p);
+    else decay_step_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, s>>>(p);
+  }
+  return check_launch();
+}
+
+}  // namespace la

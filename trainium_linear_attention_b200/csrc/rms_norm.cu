@@ -1,0 +1,596 @@
+// Root-mean-square norm with the residual's addition, its gradient, and the
+// form whose output is held in e4m3 with fp32 scales.
+//
+//   s = x + r,   y = s * rstd * w,   rstd = 1 / sqrt(mean(s^2) + eps)
+//   ds = rstd * (w dy - s rstd^2 mean(w dy s)) + d_sum,   dw = sum_rows dy s rstd
+//   fp8: scale = max(amax |y|, 2^-96) / 448 over a row or a group, e4m3(y / scale)
+//
+// All of it is bound by memory.  A row is held in registers by `TPR` threads
+// (8 per row of 64 up to a whole CTA), `NV` packs of 8 elements each, loaded
+// once with 16-byte loads; the statistics are fp32 sums over shuffles (and
+// shared memory where a row spans warps).  The gradient's CTAs walk the rows
+// with a fixed set of columns per thread, so dw is summed in registers, then
+// over the CTA's row lanes, and a second kernel adds the CTAs' partial rows in
+// a fixed order: no atomics, the same bits every time.
+#include <cuda_fp8.h>
+#include <math.h>
+
+#include "common.cuh"
+
+namespace la {
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr uint32_t kAmaxMinBits = (uint32_t)(127 - 96) << 23;  // 2^-96
+constexpr int64_t kMaxWidth = 16384;
+
+// Rows of a tensor with up to three leading dimensions (strides in elements)
+// and a dense last one.
+struct Rows {
+  const void *p;
+  int64_t s0, s1, s2;
+};
+struct Shape {
+  int64_t rows;
+  uint32_t n1, n2;  // the two inner leading dimensions
+};
+
+__device__ __forceinline__ int64_t row_offset(const Rows &t, const Shape &sh, int64_t row) {
+  if (sh.n2 == sh.rows) return row * t.s2;
+  if (sh.rows <= UINT32_MAX) {  // 32-bit divisions
+    const uint32_t r = (uint32_t)row, outer = r / sh.n2;
+    return (int64_t)(outer / sh.n1) * t.s0 + (int64_t)(outer % sh.n1) * t.s1 +
+           (int64_t)(r % sh.n2) * t.s2;
+  }
+  const int64_t outer = row / sh.n2;
+  return (outer / sh.n1) * t.s0 + (outer % sh.n1) * t.s1 + (row % sh.n2) * t.s2;
+}
+
+// Column of element e of pack i of thread t: packs of 8 neighbours with 16-byte
+// accesses, single elements otherwise.
+template <int TPR, bool kVec>
+__device__ __forceinline__ int column(int t, int i, int e) {
+  return kVec ? (i * TPR + t) * 8 + e : (i * 8 + e) * TPR + t;
+}
+
+template <typename T, int TPR, int NV, bool kVec>
+__device__ __forceinline__ void load_row(float (&x)[NV][8], const T *p, int t, int d) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (kVec) {
+      const int c = column<TPR, true>(t, i, 0);
+      if (c < d) {
+        if constexpr (sizeof(T) == 2) {
+          const uint4 w = *(const uint4 *)(p + c);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[i][2 * e] = __uint_as_float(u[e] << 16);
+            x[i][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+          }
+        } else {
+          const float4 a = *(const float4 *)(p + c), b = *(const float4 *)(p + c + 4);
+          x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+          x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = column<TPR, false>(t, i, e);
+        x[i][e] = c < d ? to_f32(p[c]) : 0.f;
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, int NV, bool kVec>
+__device__ __forceinline__ void store_row(const float (&x)[NV][8], T *p, int t, int d) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (kVec) {
+      const int c = column<TPR, true>(t, i, 0);
+      if (c >= d) continue;
+      if constexpr (sizeof(T) == 2) {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(x[i][2 * e], x[i][2 * e + 1]);
+          u[e] = *(const uint32_t *)&b;
+        }
+        *(uint4 *)(p + c) = make_uint4(u[0], u[1], u[2], u[3]);
+      } else {
+        *(float4 *)(p + c) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+        *(float4 *)(p + c + 4) = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = column<TPR, false>(t, i, e);
+        if (c < d) p[c] = from_f32<T>(x[i][e]);
+      }
+    }
+  }
+}
+
+// The weight row (fp32 or bf16; null: ones).
+template <int TPR, int NV, bool kVec>
+__device__ __forceinline__ void load_weight(float (&w)[NV][8], const void *p, int dtype, int t,
+                                            int d) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[i][e] = 1.f;
+  } else if (dtype == LA_DTYPE_FLOAT32) {
+    load_row<float, TPR, NV, kVec>(w, (const float *)p, t, d);
+  } else {
+    load_row<__nv_bfloat16, TPR, NV, kVec>(w, (const __nv_bfloat16 *)p, t, d);
+  }
+}
+
+struct Add {
+  static __device__ __forceinline__ float zero() { return 0.f; }
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+// Largest of non-negative values by their bits: a NaN (above infinity) stays.
+struct MaxBits {
+  static __device__ __forceinline__ uint32_t zero() { return 0u; }
+  static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+};
+
+// Over the TPR threads of a row; every thread gets the result.  `slot`: shared
+// memory for the warps of a row, one per warp of the CTA.  With TPR > 32 the
+// CTA holds whole rows and every thread takes part.
+template <int TPR, class Op, typename V>
+__device__ __forceinline__ V reduce_row(V x, V *slot) {
+#pragma unroll
+  for (int m = 1; m < (TPR < 32 ? TPR : 32); m <<= 1)
+    x = Op::of(x, __shfl_xor_sync(0xffffffffu, x, m));
+  if constexpr (TPR > 32) {
+    constexpr int kWarps = TPR / 32;
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();  // the slots of the use before are read
+    if ((threadIdx.x & 31) == 0) slot[warp] = x;
+    __syncthreads();
+    const int first = warp / kWarps * kWarps;
+    x = Op::zero();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) x = Op::of(x, slot[first + i]);
+  }
+  return x;
+}
+
+constexpr int threads_of(int tpr) { return tpr > 256 ? tpr : 256; }
+
+struct NormFwd {
+  Rows x, r;              // r.p null: no residual
+  const void *weight;     // null: ones
+  int weight_dtype;
+  void *y;                // output (T, or e4m3), contiguous rows
+  void *sum;              // null, or x + r, contiguous rows
+  float *rstd;            // null, or one per row
+  float *scales;          // fp8: (rows, d / group)
+  Shape sh;
+  int d, group;           // group == d: one scale for the row
+  float eps, inv_d;
+};
+
+template <typename T, int TPR, int NV, bool kVec, bool kFp8>
+__global__ void __launch_bounds__(threads_of(TPR))
+rms_norm_fwd_kernel(const NormFwd p) {
+  constexpr int kRowsPer = threads_of(TPR) / TPR;
+  __shared__ float slot[32];
+  __shared__ uint32_t slot_max[32];
+  const int t = threadIdx.x % TPR;
+  const int64_t row0 = (int64_t)blockIdx.x * kRowsPer + threadIdx.x / TPR;
+  const bool live = row0 < p.sh.rows;
+  const int64_t row = live ? row0 : p.sh.rows - 1;  // idle lanes redo the last row, unstored
+  float s[NV][8];
+  load_row<T, TPR, NV, kVec>(s, (const T *)p.x.p + row_offset(p.x, p.sh, row), t, p.d);
+  if (p.r.p) {
+    float r[NV][8];
+    load_row<T, TPR, NV, kVec>(r, (const T *)p.r.p + row_offset(p.r, p.sh, row), t, p.d);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[i][e] += r[i][e];
+  }
+  float w[NV][8];
+  load_weight<TPR, NV, kVec>(w, p.weight, p.weight_dtype, t, p.d);
+  if (p.sum && live) store_row<T, TPR, NV, kVec>(s, (T *)p.sum + row * p.d, t, p.d);
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sq = fmaf(s[i][e], s[i][e], sq);
+  sq = reduce_row<TPR, Add>(sq, slot);
+  const float rstd = 1.f / sqrtf(fmaf(sq, p.inv_d, p.eps));
+  if (p.rstd && live && t == 0) p.rstd[row] = rstd;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[i][e] = s[i][e] * rstd * w[i][e];
+  if constexpr (!kFp8) {
+    if (live) store_row<T, TPR, NV, kVec>(s, (T *)p.y + row * p.d, t, p.d);
+  } else {
+    uint32_t m[NV], all = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      m[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = column<TPR, kVec>(t, i, e) < p.d;
+        m[i] = MaxBits::of(m[i], in ? __float_as_uint(fabsf(s[i][e])) : 0u);
+      }
+      all = MaxBits::of(all, m[i]);
+    }
+    const bool whole = p.group == p.d;
+    if (whole) {
+      all = reduce_row<TPR, MaxBits>(all, slot_max);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) m[i] = all;
+    } else {  // a group is group / 8 neighbouring lanes of one pack (kVec only)
+      const int lanes = p.group / 8;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        for (int x = 1; x < lanes; x <<= 1)
+          m[i] = MaxBits::of(m[i], __shfl_xor_sync(0xffffffffu, m[i], x));
+    }
+    uint8_t *y = (uint8_t *)p.y + row * p.d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = column<TPR, kVec>(t, i, 0);
+      const float scale = __uint_as_float(MaxBits::of(m[i], kAmaxMinBits)) / kE4m3Max;
+      // one division per group: y * (1 / scale) is within an ulp of y / scale
+      // ahead of the rounding to 4 bits
+      const float inv = 1.f / scale;
+      if (live && (whole ? t == 0 && i == 0 : c < p.d && c % p.group == 0))
+        p.scales[row * (p.d / p.group) + (whole ? 0 : c / p.group)] = scale;
+      uint16_t q[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        q[e] = __nv_cvt_float2_to_fp8x2(make_float2(s[i][2 * e] * inv, s[i][2 * e + 1] * inv),
+                                        __NV_SATFINITE, __NV_E4M3);
+      if (!live) continue;
+      if constexpr (kVec) {
+        if (c < p.d)
+          *(uint2 *)(y + c) = make_uint2(q[0] | ((uint32_t)q[1] << 16),
+                                         q[2] | ((uint32_t)q[3] << 16));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int ce = column<TPR, false>(t, i, e);
+          if (ce < p.d) y[ce] = (uint8_t)(q[e / 2] >> (8 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
+struct NormBwd {
+  Rows s, dy, dsum;     // s: the normed rows (x + r); dsum.p null: none
+  const void *weight;     // null: ones
+  int weight_dtype;
+  const float *rstd;
+  void *ds;             // contiguous rows
+  float *partial;       // null (no dw), or (gridDim.x, d)
+  Shape sh;
+  int d;
+  float inv_d;
+};
+
+template <typename T, int TPR, int NV, bool kVec>
+__global__ void __launch_bounds__(threads_of(TPR))
+rms_norm_bwd_kernel(const NormBwd p) {
+  constexpr int kThreads = threads_of(TPR);
+  constexpr int kRowsPer = kThreads / TPR;
+  __shared__ float slot[32];
+  extern __shared__ float lanes_dw[];  // (kRowsPer - 1, d) with kRowsPer > 1
+  const int t = threadIdx.x % TPR, lane_row = threadIdx.x / TPR;
+  float w[NV][8], dw[NV][8] = {};
+  load_weight<TPR, NV, kVec>(w, p.weight, p.weight_dtype, t, p.d);
+  for (int64_t first = (int64_t)blockIdx.x * kRowsPer; first < p.sh.rows;
+       first += (int64_t)gridDim.x * kRowsPer) {
+    const bool live = first + lane_row < p.sh.rows;
+    const int64_t row = live ? first + lane_row : p.sh.rows - 1;
+    float s[NV][8], g[NV][8];
+    load_row<T, TPR, NV, kVec>(s, (const T *)p.s.p + row_offset(p.s, p.sh, row), t, p.d);
+    load_row<T, TPR, NV, kVec>(g, (const T *)p.dy.p + row_offset(p.dy, p.sh, row), t, p.d);
+    const float rstd = p.rstd[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (live) dw[i][e] = fmaf(g[i][e] * s[i][e], rstd, dw[i][e]);
+        g[i][e] *= w[i][e];
+        dot = fmaf(g[i][e], s[i][e], dot);
+      }
+    dot = reduce_row<TPR, Add>(dot, slot) * p.inv_d;
+    const float c = rstd * rstd * dot;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[i][e] = rstd * (g[i][e] - s[i][e] * c);
+    if (p.dsum.p) {
+      float a[NV][8];
+      load_row<T, TPR, NV, kVec>(a, (const T *)p.dsum.p + row_offset(p.dsum, p.sh, row), t, p.d);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[i][e] += a[i][e];
+    }
+    if (live) store_row<T, TPR, NV, kVec>(g, (T *)p.ds + row * p.d, t, p.d);
+  }
+  if (!p.partial) return;
+  if constexpr (kRowsPer > 1) {
+    if (lane_row > 0) {
+      float *dst = lanes_dw + (int64_t)(lane_row - 1) * p.d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = column<TPR, kVec>(t, i, e);
+          if (c < p.d) dst[c] = dw[i][e];
+        }
+    }
+    __syncthreads();
+  }
+  float *dst = p.partial + (int64_t)blockIdx.x * p.d;
+  for (int c = threadIdx.x; kRowsPer > 1 && c < p.d; c += kThreads) {
+    float sum = 0.f;
+    for (int r = 0; r < kRowsPer - 1; ++r) sum += lanes_dw[(int64_t)r * p.d + c];
+    lanes_dw[c] = sum;  // read by the first row lane below
+  }
+  if constexpr (kRowsPer > 1) __syncthreads();
+  if (lane_row == 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = column<TPR, kVec>(t, i, e);
+        if (c < p.d) dst[c] = dw[i][e] + (kRowsPer > 1 ? lanes_dw[c] : 0.f);
+      }
+  }
+}
+
+// dw = sum of the partial rows: 32 columns x 8 row lanes per CTA.
+template <typename TW>
+__global__ void __launch_bounds__(256)
+rms_norm_dw_kernel(const float *partial, int rows, int d, TW *dw) {
+  __shared__ float part[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+  float sum = 0.f;
+  if (c < d)
+    for (int r = lane; r < rows; r += 8) sum += partial[(int64_t)r * d + c];
+  part[lane][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (lane == 0 && c < d) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += part[i][threadIdx.x];
+    dw[c] = from_f32<TW>(sum);
+  }
+}
+
+// The threads per row and packs per thread for a width: up to 4 packs of 8 per
+// thread (64 bytes in flight), rows of up to 1024 within one warp.  Rows whose
+// width or alignment rules out 16-byte accesses take fewer variants.
+template <class F>
+int by_width(int64_t d, bool vec, F &&f) {
+  if (!vec) {
+    if (d <= 256) return f.template run<32, 1, false>();
+    if (d <= 1024) return f.template run<32, 4, false>();
+    if (d <= 4096) return f.template run<128, 4, false>();
+    return f.template run<512, 4, false>();
+  }
+  if (d <= 64) return f.template run<8, 1, true>();
+  if (d <= 128) return f.template run<16, 1, true>();
+  if (d <= 256) return f.template run<32, 1, true>();
+  if (d <= 512) return f.template run<32, 2, true>();
+  if (d <= 1024) return f.template run<32, 4, true>();
+  if (d <= 2048) return f.template run<128, 2, true>();
+  if (d <= 4096) return f.template run<128, 4, true>();
+  if (d <= 8192) return f.template run<256, 4, true>();
+  return f.template run<512, 4, true>();
+}
+
+// The gradient's CTAs walk the rows: this many per SM at most.
+constexpr int kBwdPerSm = 4;
+
+// One partial row of dw for each CTA, at most.
+size_t partial_bytes(int64_t rows, int64_t d, int sm_count) {
+  return (size_t)min64(rows, (int64_t)sm_count * kBwdPerSm) * (size_t)d * sizeof(float);
+}
+
+bool vec_rows(const Rows &t, int size) {
+  const int64_t pack = 16 / size;
+  return !t.p || (((uintptr_t)t.p & 15) == 0 && t.s0 % pack == 0 && t.s1 % pack == 0 &&
+                  t.s2 % pack == 0);
+}
+bool vec_ptr(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename T, bool kFp8>
+struct FwdLaunch {
+  const NormFwd &p;
+  cudaStream_t s;
+  template <int TPR, int NV, bool kVec>
+  int run() {
+    constexpr int per = threads_of(TPR) / TPR;
+    const int64_t grid = (p.sh.rows + per - 1) / per;
+    if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
+    rms_norm_fwd_kernel<T, TPR, NV, kVec, kFp8><<<(unsigned)grid, threads_of(TPR), 0, s>>>(p);
+    return check_launch();
+  }
+};
+
+template <typename T>
+struct BwdLaunch {
+  const NormBwd &p;
+  int sm_count;
+  int *grid;
+  cudaStream_t s;
+  template <int TPR, int NV, bool kVec>
+  int run() {
+    constexpr int per = threads_of(TPR) / TPR;
+    *grid = (int)min64((p.sh.rows + per - 1) / per, (int64_t)sm_count * kBwdPerSm);
+    const int smem = p.partial ? (per - 1) * p.d * 4 : 0;  // at most 28 KB
+    rms_norm_bwd_kernel<T, TPR, NV, kVec><<<*grid, threads_of(TPR), smem, s>>>(p);
+    return check_launch();
+  }
+};
+
+bool valid_type(int t) { return t == LA_DTYPE_FLOAT32 || t == LA_DTYPE_BFLOAT16; }
+
+// Checks what the entry points share; LA_OK with *empty set where there is
+// nothing to do.
+int check_norm(const int64_t *shape, int64_t d, int dtype, int weight_dtype, Shape *sh,
+               bool *empty) {
+  *empty = false;
+  if (!shape || shape[0] < 0 || shape[1] < 0 || shape[2] < 0 || d < 1)
+    return LA_ERR_INVALID_ARGUMENT;
+  if (!valid_type(dtype) || !valid_type(weight_dtype)) return LA_ERR_INVALID_ARGUMENT;
+  if (d > kMaxWidth) return LA_ERR_UNSUPPORTED;
+  if (shape[0] == 0 || shape[1] == 0 || shape[2] == 0) {
+    *empty = true;
+    return LA_OK;
+  }
+  if (shape[1] > INT32_MAX || shape[2] > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  const int64_t inner = shape[1] * shape[2];
+  if (inner > INT64_MAX / d / 8 / shape[0]) return LA_ERR_UNSUPPORTED;
+  sh->rows = shape[0] * inner;
+  sh->n1 = (uint32_t)shape[1];
+  sh->n2 = (uint32_t)shape[2];
+  DeviceInfo info;
+  const int st = current_device_info(&info);
+  if (st != LA_OK) return st;
+  return info.cc_major == 10 ? LA_OK : LA_ERR_NO_DEVICE;
+}
+
+Rows rows_of(const void *p, const int64_t *s) {
+  Rows r{p, 0, 0, 0};
+  if (p && s) r.s0 = s[0], r.s1 = s[1], r.s2 = s[2];
+  return r;
+}
+
+template <bool kFp8>
+int launch_fwd(const NormFwd &p, int dtype, cudaStream_t s) {
+  const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+  const bool vec = p.d % 8 == 0 && vec_rows(p.x, size) && vec_rows(p.r, size) &&
+                   vec_ptr(p.weight) && vec_ptr(p.y) && vec_ptr(p.sum);
+  if (kFp8 && p.group != p.d && !vec) return LA_ERR_UNSUPPORTED;
+  if (dtype == LA_DTYPE_FLOAT32) return by_width(p.d, vec, FwdLaunch<float, kFp8>{p, s});
+  return by_width(p.d, vec, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
+}
+
+int launch_bwd(const NormBwd &p, int dtype, int sm_count, int *grid, cudaStream_t s) {
+  const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+  const bool vec = p.d % 8 == 0 && vec_rows(p.s, size) && vec_rows(p.dy, size) &&
+                   vec_rows(p.dsum, size) && vec_ptr(p.weight) && vec_ptr(p.ds);
+  if (dtype == LA_DTYPE_FLOAT32) return by_width(p.d, vec, BwdLaunch<float>{p, sm_count, grid, s});
+  return by_width(p.d, vec, BwdLaunch<__nv_bfloat16>{p, sm_count, grid, s});
+}
+
+}  // namespace
+}  // namespace la
+
+using namespace la;
+
+extern "C" {
+
+int la_rms_norm_fwd(const void *x, const int64_t *x_strides, const void *residual,
+                    const int64_t *residual_strides, const void *weight, void *y, void *sum,
+                    float *rstd, const int64_t *shape, int64_t d, int dtype, int weight_dtype,
+                    float eps, void *stream) {
+  NormFwd p{};
+  bool empty;
+  const int st = check_norm(shape, d, dtype, weight_dtype, &p.sh, &empty);
+  if (st != LA_OK || empty) return st;
+  if (!x || !x_strides || !y || (residual && !residual_strides)) return LA_ERR_INVALID_ARGUMENT;
+  p.x = rows_of(x, x_strides);
+  p.r = rows_of(residual, residual_strides);
+  p.weight = weight, p.weight_dtype = weight_dtype, p.y = y, p.sum = sum, p.rstd = rstd;
+  p.d = p.group = (int)d;
+  p.eps = eps;
+  p.inv_d = 1.f / (float)d;
+  return launch_fwd<false>(p, dtype, (cudaStream_t)stream);
+}
+
+int la_rms_norm_fp8(const void *x, const int64_t *x_strides, const void *residual,
+                    const int64_t *residual_strides, const void *weight, void *y, float *scales,
+                    void *sum, const int64_t *shape, int64_t d, int64_t group, int dtype,
+                    int weight_dtype, float eps, void *stream) {
+  NormFwd p{};
+  bool empty;
+  const int st = check_norm(shape, d, dtype, weight_dtype, &p.sh, &empty);
+  if (st != LA_OK) return st;
+  if (group != d && (group < 16 || group > 256 || (group & (group - 1)) || d % group))
+    return LA_ERR_INVALID_ARGUMENT;
+  if (empty) return LA_OK;
+  if (!x || !x_strides || !y || !scales || (residual && !residual_strides))
+    return LA_ERR_INVALID_ARGUMENT;
+  p.x = rows_of(x, x_strides);
+  p.r = rows_of(residual, residual_strides);
+  p.weight = weight, p.weight_dtype = weight_dtype, p.y = y, p.sum = sum, p.scales = scales;
+  p.d = (int)d;
+  p.group = (int)group;
+  p.eps = eps;
+  p.inv_d = 1.f / (float)d;
+  return launch_fwd<true>(p, dtype, (cudaStream_t)stream);
+}
+
+int la_rms_norm_bwd_workspace_size(int64_t rows, int64_t d, size_t *bytes) {
+  if (!bytes || rows < 0 || d < 1) return LA_ERR_INVALID_ARGUMENT;
+  if (d > kMaxWidth) return LA_ERR_UNSUPPORTED;
+  DeviceInfo info;
+  const int st = current_device_info(&info);
+  if (st != LA_OK) return st;
+  *bytes = partial_bytes(rows, d, info.sm_count);
+  return LA_OK;
+}
+
+int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight, const void *d_y,
+                    const int64_t *d_y_strides, const void *d_sum, const int64_t *d_sum_strides,
+                    const float *rstd, void *d_s, void *d_weight, const int64_t *shape, int64_t d,
+                    int dtype, int weight_dtype, void *workspace, size_t workspace_bytes,
+                    void *stream) {
+  NormBwd p{};
+  bool empty;
+  int st = check_norm(shape, d, dtype, weight_dtype, &p.sh, &empty);
+  if (st != LA_OK) return st;
+  cudaStream_t cs = (cudaStream_t)stream;
+  if (empty) {
+    if (!d_weight) return LA_OK;
+    const size_t size = weight_dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+    return cuda_status(cudaMemsetAsync(d_weight, 0, (size_t)d * size, cs));
+  }
+  if (!s || !s_strides || !d_y || !d_y_strides || !rstd || !d_s || (d_sum && !d_sum_strides))
+    return LA_ERR_INVALID_ARGUMENT;
+  DeviceInfo info;
+  if ((st = current_device_info(&info)) != LA_OK) return st;
+  if (d_weight && (!workspace || workspace_bytes < partial_bytes(p.sh.rows, d, info.sm_count) ||
+                   ((uintptr_t)workspace & 15)))
+    return LA_ERR_WORKSPACE;
+  p.s = rows_of(s, s_strides);
+  p.dy = rows_of(d_y, d_y_strides);
+  p.dsum = rows_of(d_sum, d_sum_strides);
+  p.weight = weight, p.weight_dtype = weight_dtype, p.rstd = rstd, p.ds = d_s;
+  p.partial = d_weight ? (float *)workspace : nullptr;
+  p.d = (int)d;
+  p.inv_d = 1.f / (float)d;
+  int grid = 0;
+  st = launch_bwd(p, dtype, info.sm_count, &grid, cs);
+  if (st != LA_OK || !d_weight) return st;
+  const unsigned cols = (unsigned)((d + 31) / 32);
+  if (weight_dtype == LA_DTYPE_FLOAT32)
+    rms_norm_dw_kernel<float><<<cols, 256, 0, cs>>>(p.partial, grid, p.d, (float *)d_weight);
+  else
+    rms_norm_dw_kernel<__nv_bfloat16>
+        <<<cols, 256, 0, cs>>>(p.partial, grid, p.d, (__nv_bfloat16 *)d_weight);
+  return check_launch();
+}
+
+}  // extern "C"

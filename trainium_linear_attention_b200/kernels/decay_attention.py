@@ -1,0 +1,97 @@
+"""Linear attention with a decay for each head: prompts, training, single tokens.
+
+    S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
+
+the recurrence of the reference's chunked kernel (kernels/
+nki_attention_chunked.py:20-113) with identity features and a forgetting
+factor, in the three forms a model needs:
+
+* ``decay_linear_attention(q, k, v, log_decay, ...)`` -- a whole prompt (or the
+  next piece of one), differentiable in q, k, v and the initial state;
+* ``decay_linear_attention_step(q, k, v, log_decay, state, ...)`` -- one token
+  of every sequence, the state updated in place;
+* ``ref_decay_attn(q, k, v, log_decay, ...)`` -- the definition in plain
+  PyTorch, for comparisons only; no CUDA path calls it.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+
+def ref_decay_attn(q, k, v, log_decay, scale=None, initial_state=None):
+    """The dense definition in the inputs' dtype: (output, final state).
+    Materialises the (t, t) weights."""
+    t, d = q.shape[-2:]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    g = log_decay.to(q.dtype).view(-1, 1, 1)
+    i = torch.arange(t, device=q.device, dtype=q.dtype)
+    lag = i[:, None] - i[None, :]
+    weight = torch.where(lag > 0, torch.exp(g * lag.clamp(min=1)), (lag == 0).to(q.dtype))
+    out = (q @ k.transpose(-2, -1) * weight) @ v
+    left = t - 1 - i
+    into = torch.where(left > 0, torch.exp(g * left.clamp(min=1)), torch.ones_like(g * left))
+    state = (k * into.transpose(-2, -1)).transpose(-2, -1) @ v
+    if initial_state is not None:
+        out = out + torch.exp(g * (i[:, None] + 1)) * (q @ initial_state)
+        state = state + (torch.exp(g * t) if t else 1.0) * initial_state
+    return out * scale, state
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, scale, return_state):
+        got = ops.decay_attention(q, k, v, log_decay, scale=scale, initial_state=initial_state,
+                                  return_state=return_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return got
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_state=None):
+        q, k, v, log_decay, initial_state = ctx.saved_tensors
+        if d_out is None and d_state is None:
+            return (None,) * 7
+        if d_out is None:
+            d_out = torch.zeros_like(v)
+        need = ctx.needs_input_grad
+        dq, dk, dv, d0 = ops.decay_attention_backward(
+            q, k, v, log_decay, d_out, scale=ctx.scale, initial_state=initial_state,
+            d_state=d_state, want_d_initial=need[4])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+                None, d0, None, None)
+
+
+def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
+                           return_state=False):
+    """Causal linear attention with a decay for each head on the sm_100a kernels.
+
+    q, k: (b, h, t, d_qk); v: (b, h, t, d_v), float32 or bfloat16, widths up to
+    128, any strides with a dense last dimension (a projection's transposed
+    heads are read in place, and the output is laid out as v).  ``log_decay``:
+    float32 (h,), <= 0, a constant.  ``scale`` defaults to 1/sqrt(d_qk).
+    ``initial_state``: fp32 (b, h, d_qk, d_v), the state before the first
+    token.  Returns (b, h, t, d_v) in q.dtype, or with ``return_state`` also
+    the fp32 state after the last token.  Differentiable once in q, k, v and
+    ``initial_state``."""
+    if torch.is_grad_enabled() and any(
+            isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, initial_state)):
+        return _DecayAttention.apply(q, k, v, log_decay, initial_state, scale, bool(return_state))
+    return ops.decay_attention(q, k, v, log_decay, scale=scale, initial_state=initial_state,
+                               return_state=return_state)
+
+
+def decay_linear_attention_step(q, k, v, log_decay, state, scale=None):
+    """One token of every sequence on the sm_100a kernel.
+
+    q, k: (b, h, d_qk); v: (b, h, d_v).  ``state`` (fp32 (b, h, d_qk, d_v), as
+    ``decay_linear_attention`` returns it) is updated in place.  Returns
+    (b, h, d_v) in q.dtype; no gradient."""
+    return ops.decay_attention_step(q, k, v, log_decay, state, scale=scale)

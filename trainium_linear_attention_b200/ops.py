@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -227,6 +228,314 @@ def based_layer(q, k, v, window_size: int = 64, eps: float = 1e-6, segments: int
             int(segments), _stream_ptr(q.device))
     N.check(st, "la_based_layer_fwd")
     return out
+
+
+# ---- linear attention with a decay for each head ---------------------------------
+_Strides = ctypes.c_int64 * 3
+
+
+def _heads_view(t: torch.Tensor):
+    """``t`` (b, h, t, d) as the kernels read it -- a dense last dimension and,
+    for bf16, 16-byte rows where the width allows them -- and its strides.  A
+    copy is made only where the strides rule that out (or overlap)."""
+    b, h, n, d = t.shape
+    sb, sh, st, sd = t.stride()
+    ok = ((sd == 1 or d == 1) and (sb > 0 or b == 1) and (sh > 0 or h == 1)
+          and (st >= d or n == 1))
+    if ok and d % 8 == 0 and t.dtype == torch.bfloat16:
+        ok = (t.data_ptr() % 16 == 0 and (sb % 8 == 0 or b == 1) and (sh % 8 == 0 or h == 1)
+              and (st % 8 == 0 or n == 1))
+    if not ok:
+        t = t.contiguous()
+        if t.data_ptr() % 16:  # a contiguous view at an odd offset
+            t = t.clone()
+        sb, sh, st, _ = t.stride()
+    # a dimension of one entry has no stride of its own
+    return t, _Strides(sb if b > 1 else h * n * d, sh if h > 1 else n * d, st if n > 1 else d)
+
+
+def _heads_like(t: torch.Tensor, d: int) -> torch.Tensor:
+    """An empty (b, h, t, d) tensor laid out as ``t``: tokens before heads where
+    ``t`` is a transposed projection, else contiguous."""
+    b, h, n, _ = t.shape
+    if h > 1 and n > 1 and t.stride(1) < t.stride(2):
+        return torch.empty((b, n, h, d), dtype=t.dtype, device=t.device).transpose(1, 2)
+    return torch.empty((b, h, n, d), dtype=t.dtype, device=t.device)
+
+
+def _check_decay(q, k, v, log_decay):
+    code = _check_qkv(q, k, v)
+    _check_log_decay(log_decay, q.shape[1], q.device)
+    return code
+
+
+def _check_log_decay(log_decay, heads, device):
+    if not isinstance(log_decay, torch.Tensor):
+        raise TypeError("log_decay must be a torch.Tensor")
+    if (log_decay.dtype != torch.float32 or log_decay.device != device
+            or tuple(log_decay.shape) != (heads,)):
+        raise ValueError(f"log_decay must be float32 ({heads},) on {device}")
+    if log_decay.requires_grad:
+        raise ValueError("log_decay is a constant of the operator: it has no gradient")
+
+
+def _check_state(state, shape, device, name):
+    if not isinstance(state, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if state.dtype != torch.float32 or state.device != device or tuple(state.shape) != shape:
+        raise ValueError(f"{name} must be float32 {shape} on {device}")
+
+
+def _default_scale(scale, d_qk: int) -> float:
+    return 1.0 / math.sqrt(d_qk) if scale is None else float(scale)
+
+
+@functools.lru_cache(maxsize=1024)
+def _decay_plan(batch, heads, seq_len, d_qk, d_v, code, backward, segments, device_index):
+    g = ctypes.c_int(0)
+    ws = ctypes.c_size_t(0)
+    st = N.lib().la_decay_plan(batch, heads, seq_len, d_qk, d_v, code, int(backward), segments,
+                               ctypes.byref(g), ctypes.byref(ws))
+    N.check(st, "la_decay_plan")
+    return g.value, ws.value
+
+
+def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_state: bool = False,
+                    segments: int = 0):
+    """Forward pass of the decayed linear attention (no autograd): the output,
+    or (output, final state fp32 (b, h, d_qk, d_v))."""
+    code = _check_decay(q, k, v, log_decay)
+    b, h, t, d = q.shape
+    dv = v.shape[-1]
+    if initial_state is not None:
+        _check_state(initial_state, (b, h, d, dv), q.device, "initial_state")
+        initial_state = initial_state.contiguous()
+    out = _heads_like(v, dv)
+    final = torch.empty((b, h, d, dv), dtype=torch.float32, device=q.device) if return_state else None
+    log_decay = log_decay.contiguous()
+    (q, qs), (k, ks), (v, vs), (_, os_) = (_heads_view(x) for x in (q, k, v, out))
+    with _on_device(q.device):
+        _, ws_bytes = _decay_plan(b, h, t, d, dv, code, False, int(segments),
+                                  torch.cuda.current_device())
+        workspace = _workspace(ws_bytes, q.device)
+        st = N.lib().la_decay_chunked_fwd(
+            _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(out), os_, _ptr(log_decay), b, h, t, d, dv,
+            code, _default_scale(scale, d), _ptr(initial_state), _ptr(final), _ptr(workspace),
+            ws_bytes, int(segments), _stream_ptr(q.device))
+    N.check(st, "la_decay_chunked_fwd")
+    return (out, final) if return_state else out
+
+
+def decay_attention_backward(q, k, v, log_decay, d_out, scale=None, initial_state=None,
+                             d_state=None, want_d_initial: bool = False, segments: int = 0):
+    """Gradients (dq, dk, dv, d_initial_state or None) of ``decay_attention``
+    for the gradients of its output and (``d_state``) of its final state."""
+    code = _check_decay(q, k, v, log_decay)
+    b, h, t, d = q.shape
+    dv = v.shape[-1]
+    if not isinstance(d_out, torch.Tensor) or d_out.shape != v.shape or d_out.dtype != v.dtype:
+        raise ValueError(f"d_out must be {v.dtype} {tuple(v.shape)}")
+    for name, s in (("initial_state", initial_state), ("d_state", d_state)):
+        if s is not None:
+            _check_state(s, (b, h, d, dv), q.device, name)
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    d_state = None if d_state is None else d_state.contiguous()
+    gq, gk, gv = _heads_like(q, d), _heads_like(k, d), _heads_like(v, dv)
+    g0 = (torch.empty((b, h, d, dv), dtype=torch.float32, device=q.device) if want_d_initial
+          else None)
+    log_decay = log_decay.contiguous()
+    (q, qs), (k, ks), (v, vs), (d_out, ds) = (_heads_view(x) for x in (q, k, v, d_out))
+    (_, gqs), (_, gks), (_, gvs) = (_heads_view(x) for x in (gq, gk, gv))
+    with _on_device(q.device):
+        _, ws_bytes = _decay_plan(b, h, t, d, dv, code, True, int(segments),
+                                  torch.cuda.current_device())
+        workspace = _workspace(ws_bytes, q.device)
+        st = N.lib().la_decay_chunked_bwd(
+            _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(d_out), ds, _ptr(gq), gqs, _ptr(gk), gks,
+            _ptr(gv), gvs, _ptr(log_decay), b, h, t, d, dv, code, _default_scale(scale, d),
+            _ptr(initial_state), _ptr(d_state), _ptr(g0), _ptr(workspace), ws_bytes,
+            int(segments), _stream_ptr(q.device))
+    N.check(st, "la_decay_chunked_bwd")
+    return gq, gk, gv, g0
+
+
+def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
+    """One token of every sequence: q, k (b, h, d_qk), v (b, h, d_v); ``state``
+    fp32 (b, h, d_qk, d_v) is updated in place.  Returns (b, h, d_v)."""
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if x.dim() != 3:
+            raise ValueError(f"{name} must be (batch, heads, dim), got shape {tuple(x.shape)}")
+    code = _check_qkv(q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
+    b, h, d = q.shape
+    dv = v.shape[-1]
+    _check_log_decay(log_decay, h, q.device)
+    _check_state(state, (b, h, d, dv), q.device, "state")
+    if state.requires_grad:
+        raise ValueError("state is updated in place: it may not require a gradient")
+    sb, sh, sr, sc = state.stride()
+    if ((sc != 1 and dv > 1) or (sr != dv and d > 1) or (sh < d * dv and h > 1)
+            or (sb < d * dv and b > 1)):
+        raise ValueError("state needs dense (d_qk, d_v) entries that do not overlap")
+    if b > 1 and h > 1 and not (sb >= sh * (h - 1) + d * dv or sh >= sb * (b - 1) + d * dv):
+        raise ValueError("the states of different sequences overlap")
+    log_decay = log_decay.contiguous()
+    q, k, v = (x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous() for x in (q, k, v))
+    out = torch.empty((b, h, dv), dtype=q.dtype, device=q.device)
+    with _on_device(q.device):
+        st = N.lib().la_decay_step(
+            _ptr(q), _Strides(*q.stride()), _ptr(k), _Strides(*k.stride()), _ptr(v),
+            _Strides(*v.stride()), _ptr(out), _ptr(state), _Strides(sb, sh), _ptr(log_decay),
+            b, h, d, dv, code, _default_scale(scale, d), _stream_ptr(q.device))
+    N.check(st, "la_decay_step")
+    torch.autograd.graph.increment_version(state)
+    return out
+
+
+# ---- root-mean-square norm ---------------------------------------------------------
+_FP8_GROUPS = (16, 32, 64, 128, 256)
+
+
+def _check_rows(x, name, like=None):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} must be (..., d), got shape {tuple(x.shape)}")
+    if x.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor (got {x.device}); "
+                         "this library has no CPU implementation")
+    if like is not None and (x.shape != like.shape or x.dtype != like.dtype
+                             or x.device != like.device):
+        raise ValueError(f"{name} must be {like.dtype} {tuple(like.shape)} on {like.device}")
+    return _dtype_code(x)
+
+
+def _check_norm(x, weight, residual):
+    code = _check_rows(x, "x")
+    if residual is not None:
+        _check_rows(residual, "residual", x)
+    wcode = code
+    if weight is not None:
+        if not isinstance(weight, torch.Tensor):
+            raise TypeError("weight must be a torch.Tensor")
+        wcode = _dtype_code(weight)
+        if tuple(weight.shape) != (x.shape[-1],) or weight.device != x.device:
+            raise ValueError(f"weight must be ({x.shape[-1]},) on {x.device}")
+    return code, wcode
+
+
+def _row_views(*tensors):
+    """The tensors (equal shapes, None allowed) as rows under three leading
+    dimensions: ([tensor], [strides], shape).  Only rows that are not dense, or
+    that more than three leading dimensions address, are copied."""
+    first = next(t for t in tensors if t is not None)
+    lead, d = first.shape[:-1], first.shape[-1]
+    if all(t is None or t.is_contiguous() for t in tensors):
+        shape = _Strides(1, 1, first.numel() // d)
+        strides = _Strides(0, 0, d)
+        return tensors, [strides] * len(tensors), shape
+    if len(lead) > 3:
+        return _row_views(*(None if t is None else t.contiguous() for t in tensors))
+    pad = (1,) * (3 - len(lead))
+    got, strides = [], []
+    for t in tensors:
+        if t is not None and t.stride(-1) != 1 and d > 1:
+            t = t.contiguous()
+        got.append(t)
+        strides.append(None if t is None else _Strides(*((0,) * len(pad) + t.stride()[:-1])))
+    return got, strides, _Strides(*(pad + tuple(lead)))
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, want_rstd: bool = False):
+    """Forward pass of the norm (no autograd): (y, x + residual or None, fp32
+    reciprocal root mean squares per row or None)."""
+    code, wcode = _check_norm(x, weight, residual)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = torch.empty_like(y) if residual is not None else None
+    rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_rstd
+            else None)
+    (x, residual), (xs, rs), shape = _row_views(x, residual)
+    weight = None if weight is None else weight.contiguous()
+    with _on_device(x.device):
+        st = N.lib().la_rms_norm_fwd(
+            _ptr(x), xs, _ptr(residual), rs, _ptr(weight), _ptr(y), _ptr(total), _ptr(rstd), shape,
+            x.shape[-1], code, wcode, float(eps), _stream_ptr(x.device))
+    N.check(st, "la_rms_norm_fwd")
+    return y, total, rstd
+
+
+def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6, group_size: int | None = None):
+    """The norm with its output held in e4m3: (y, scales, x + residual or None),
+    scales fp32 (..., d / group_size), one per row without a group size."""
+    code, wcode = _check_norm(x, weight, residual)
+    d = x.shape[-1]
+    group = d if group_size is None else int(group_size)
+    if group_size is not None and (group not in _FP8_GROUPS or d % group):
+        raise ValueError(f"group_size must be None or one of {_FP8_GROUPS} dividing {d}, "
+                         f"got {group_size}")
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((*x.shape[:-1], d // group), dtype=torch.float32, device=x.device)
+    total = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None
+             else None)
+    (x, residual), (xs, rs), shape = _row_views(x, residual)
+    weight = None if weight is None else weight.contiguous()
+    if group != d:  # whole 16-byte packs per group
+        x, xs = _aligned_rows(x, xs, shape)
+        residual, rs = _aligned_rows(residual, rs, shape)
+        if weight is not None and weight.data_ptr() % 16:
+            weight = weight.clone()
+    with _on_device(x.device):
+        st = N.lib().la_rms_norm_fp8(
+            _ptr(x), xs, _ptr(residual), rs, _ptr(weight), _ptr(y), _ptr(scales), _ptr(total),
+            shape, d, group, code, wcode, float(eps), _stream_ptr(x.device))
+    N.check(st, "la_rms_norm_fp8")
+    return y, scales, total
+
+
+def _aligned_rows(t, strides, shape):
+    """``t`` and its row strides, copied where its rows do not start at 16 bytes."""
+    if t is None:
+        return t, strides
+    pack = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and all(s % pack == 0 for s in strides):
+        return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    d = t.shape[-1]
+    return t, _Strides(shape[1] * shape[2] * d, shape[2] * d, d)
+
+
+def rms_norm_backward(s, weight, rstd, d_y, d_sum=None, want_d_weight: bool = True):
+    """Gradients (of x and of the residual alike, of the weight or None) of
+    ``rms_norm`` from its saved rows ``s`` (x + residual) and ``rstd``."""
+    code, wcode = _check_norm(s, weight, None)
+    _check_rows(d_y, "d_y", s)
+    if d_sum is not None:
+        _check_rows(d_sum, "d_sum", s)
+    d = s.shape[-1]
+    d_s = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    d_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if (
+        want_d_weight and weight is not None) else None
+    (s, d_y, d_sum), (ss, ys, us), shape = _row_views(s, d_y, d_sum)
+    weight = None if weight is None else weight.contiguous()
+    rstd = rstd.contiguous()
+    with _on_device(s.device):
+        ws_bytes = 0 if d_w is None else _norm_workspace(s.numel() // d, d,
+                                                         torch.cuda.current_device())
+        workspace = _workspace(ws_bytes, s.device)
+        st = N.lib().la_rms_norm_bwd(
+            _ptr(s), ss, _ptr(weight), _ptr(d_y), ys, _ptr(d_sum), us, _ptr(rstd), _ptr(d_s),
+            _ptr(d_w), shape, d, code, wcode, _ptr(workspace), ws_bytes, _stream_ptr(s.device))
+    N.check(st, "la_rms_norm_bwd")
+    return d_s, d_w
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(rows, d, device_index):
+    n = ctypes.c_size_t(0)
+    N.check(N.lib().la_rms_norm_bwd_workspace_size(rows, d, ctypes.byref(n)),
+            "la_rms_norm_bwd_workspace_size")
+    return n.value
 
 
 _copy_streams: dict = {}
