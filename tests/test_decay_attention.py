@@ -389,6 +389,25 @@ def test_prompt_in_pieces_then_tokens(dtype):
 
 
 @gpu
+def test_first_call_of_a_thread():
+    """A thread without a CUDA context of its own (as an autograd worker's is),
+    whose allocations come from the cache."""
+    import threading
+
+    q, k, v, g, state = make(1, 3, 400, 64, 64, torch.bfloat16)
+    do = torch.randn_like(v)
+    want = ops.decay_attention_backward(q, k, v, g, do)
+    got = []
+    worker = threading.Thread(target=lambda: got.extend(
+        ops.decay_attention_backward(q, k, v, g, do)))
+    torch.cuda.synchronize()
+    worker.start()
+    worker.join()
+    torch.cuda.synchronize()
+    assert len(got) == 4 and all(torch.equal(x, y) for x, y in zip(got[:3], want))
+
+
+@gpu
 def test_repeats_streams_and_graphs():
     """The same bits on every call, on another stream, and replayed from graphs
     whose captures share the allocator."""

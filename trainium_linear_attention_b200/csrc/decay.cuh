@@ -76,4 +76,10 @@ int launch_decay_state_simt(const DecayCall &c, cudaStream_t s);
 // Outputs (and final states) of every role.
 int launch_decay_output_simt(const DecayCall &c, cudaStream_t s);
 
+// The same on tensor cores: bf16, every tensor of the call as decay_tc_view
+// wants it (16-byte rows), n > 0.
+bool decay_tc_view(const DecayView &x, int width, const DecayCall &c);
+int launch_decay_state_tc(const DecayCall &c, cudaStream_t s);
+int launch_decay_output_tc(const DecayCall &c, cudaStream_t s);
+
 }  // namespace la

@@ -94,8 +94,21 @@ __global__ void decay_running_kernel(const RunningArgs a, const float *log_decay
   }
 }
 
+// bf16 whose rows TMA can address runs on tensor cores.
+bool use_tensor_cores(const DecayCall &c) {
+  if (c.dtype != LA_DTYPE_BFLOAT16 || c.n == 0) return false;
+  for (int r = 0; r < c.roles; ++r) {
+    const DecayRole &f = c.role[r];
+    if (!decay_tc_view(f.a, f.da, c) || !decay_tc_view(f.b, f.da, c) ||
+        !decay_tc_view(f.v, f.dvo, c) || !decay_tc_view(f.out, f.dvo, c))
+      return false;
+  }
+  return true;
+}
+
 int run_decay(DecayCall &call, const DecayRole *state_roles, int n_state_roles,
               const float *const *inits, int64_t d_qk, int64_t d_v, cudaStream_t s) {
+  const bool tc = use_tensor_cores(call);
   if (call.segments > 1) {
     DecayCall pass = call;
     pass.roles = n_state_roles;
@@ -107,7 +120,7 @@ int run_decay(DecayCall &call, const DecayRole *state_roles, int n_state_roles,
       run.len0[r] = state_roles[r].reverse ? call.n - (call.segments - 1) * call.seg_len
                                            : call.seg_len;
     }
-    int st = launch_decay_state_simt(pass, s);
+    int st = tc ? launch_decay_state_tc(pass, s) : launch_decay_state_simt(pass, s);
     if (st != LA_OK) return st;
     const int64_t per_head = d_qk * d_v;
     const dim3 grid((unsigned)((per_head + 255) / 256), (unsigned)(call.batch * call.heads),
@@ -117,7 +130,7 @@ int run_decay(DecayCall &call, const DecayRole *state_roles, int n_state_roles,
     st = check_launch();
     if (st != LA_OK) return st;
   }
-  return launch_decay_output_simt(call, s);
+  return tc ? launch_decay_output_tc(call, s) : launch_decay_output_simt(call, s);
 }
 
 bool null_strides(const int64_t *const *s, int n) {

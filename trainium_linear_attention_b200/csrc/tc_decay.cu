@@ -1,0 +1,652 @@
+// Linear attention with a decay for each head on tcgen05 tensor cores (sm_100a):
+// bf16 q/k/v with widths that are multiples of 8 up to 128.
+//
+// One CTA walks one (role, head, segment, 64 columns of v) in tiles of 128
+// tokens (the roles and the recurrence: decay.cuh).  Per tile, with S the
+// state before it, A, B, V the role's tiles, t a token's place in the walk:
+//
+//   scores = A B^T                       tcgen05 M=128 N=128 K=DK  -> TMEM
+//   P      = intra lambda^(ti-tj) scores, tj <= ti   CUDA cores, bf16 over scores
+//   O1     = A S                         M=128 N=64 K=DK  (S as a bf16 copy in smem)
+//   O2     = P V                         M=128 N=64 K=128 (A = P in TMEM)
+//   out    = inter lambda^(ti+e0) O1 + O2               epilogue, rounded once
+//   V'     = inc lambda^(len-e0-tj) V, as two bf16 terms hi + lo    CUDA cores
+//   U      = B^T [V'hi V'lo]             M=128 N=128 K=128
+//   S      = lambda^len S + U_hi + U_lo  fp32 in registers of the state warps
+//
+// The decay never multiplies an accumulator in TMEM: it is on the rows of P and
+// V' (operands), on O1's rows and on the state's registers, so U, the scores
+// and O2 of a tile depend on the tile alone and only O1 waits for the state.
+// V' as hi + lo carries 16 bits, so the fp32 state is exact to about 2^-18
+// (one bf16 term would leave 2^-9 in a state that decoding continues from);
+// stacked along N the second term costs no further MMA instruction and no
+// second read of B.  The bf16 copy of S and P are rounded once (2^-8, like the
+// output).  With DK = 64, M = 128 holds B^T twice (descriptor stride 0), and
+// the state warps of the upper lanes take the other half of the columns.
+//
+// What bounds it: HBM for long walks of enough heads (a tile moves 64 KB at
+// d = 64 against ~1,300 cycles of tensor work); per-tile latency (the chain
+// U -> S -> copy -> O1 -> out) where few CTAs walk.
+//
+// Warps: 0 TMA; 1 scores, O1 and O2 MMAs (TMEM owner); 2 U MMAs; 4.. state
+// (4 warps at DK = 64, 8 at 128); 8 warps P (two groups, alternate tiles); 4
+// warps V'; 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
+#include "decay.cuh"
+#include "tc_common.cuh"
+#include "tc_kernels.cuh"
+#include "tma_host.cuh"
+
+namespace la {
+namespace {
+using namespace tc;
+
+constexpr int kT = kDecayTile;  // tokens per tile
+constexpr int kBlock = kT * 128;  // bytes of 128 tokens x 64 bf16 columns, 128B-swizzled
+constexpr float kLog2e = 1.4426950408889634f;
+
+// TMEM columns
+constexpr uint32_t kColScores = 0;  // two buffers of 128
+constexpr uint32_t kColU = 256;     // hi 64, lo 64
+constexpr uint32_t kColO1 = 384;
+constexpr uint32_t kColO2 = 448;
+
+template <int DK, bool kStateOnly>
+struct TcLayout {
+  static constexpr int kKBlocks = DK / 64;
+  static constexpr int kStateWarps = DK == 64 ? 4 : 8;
+  static constexpr int kWState = 4;
+  static constexpr int kWP = kWState + kStateWarps;  // first P warp
+  static constexpr int kWV = kStateOnly ? kWP : kWP + 8;
+  static constexpr int kWE = kWV + 4;
+  static constexpr int kWarps = kStateOnly ? kWE : kWE + 4;
+  static constexpr int kThreads = kWarps * 32;
+  // stage: A, B (kKBlocks blocks each), V (one block)
+  static constexpr uint32_t kOffA = 0;
+  static constexpr uint32_t kOffB = kStateOnly ? 0 : kKBlocks * kBlock;
+  static constexpr uint32_t kOffV = kOffB + kKBlocks * kBlock;
+  static constexpr uint32_t kStageBytes = kOffV + kBlock;
+  static constexpr uint32_t kSnapBytes = DK * 128;
+  static constexpr uint32_t kTab = 64;  // lambda^0 .. lambda^31 behind 32 zeros
+  static constexpr uint32_t kFixed = 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + kTab * 4 + 512;
+  static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
+                                     ? 6
+                                     : (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes;
+  static constexpr uint32_t kOffVp = kStages * kStageBytes;     // V' hi, lo
+  static constexpr uint32_t kOffSnap = kOffVp + 2 * kBlock;     // two bf16 copies of S
+  static constexpr uint32_t kOffTab = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
+  static constexpr uint32_t kOffBar = kOffTab + kTab * 4;
+  static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
+  static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
+  static_assert(kSmem > 114 * 1024, "one CTA per SM (all TMEM columns)");
+};
+
+enum Bar {
+  kFull = 0,
+  kEmpty = kFull + 6,
+  kSReady = kEmpty + 6,
+  kPReady = kSReady + 2,
+  kSnapReady = kPReady + 2,
+  kSnapFree = kSnapReady + 2,
+  kVpReady = kSnapFree + 2,
+  kUReady,
+  kUFree,
+  kOReady,
+  kOFree,
+  kDone,
+  kNumBars = kDone + 2
+};
+static_assert(8 * kNumBars + 8 <= 512, "barrier area");
+
+struct TcRole {
+  int a, b, v;  // which tensor map
+  __nv_bfloat16 *out;
+  int64_t ob, oh, ot;
+  const float *seeds;
+  float *states, *final_state;
+  int da, dvo, seed_transposed, reverse;
+  float intra, inter, inc;
+};
+
+struct TcParams {
+  CUtensorMap map[4];
+  TcRole role[kDecayMaxRoles];
+  const float *log_decay;
+  int *err;
+  int64_t heads, n, seg_len;
+  int roles, slices, segments;
+};
+
+__device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *map, uint64_t *bar,
+                                            int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// 2^x by the hardware approximation (relative error ~2^-22); only ahead of a
+// rounding to bf16.
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer() - t0 > kWaitTimeoutNs) return false;
+  return true;
+}
+
+template <int DK, bool kStateOnly>
+__global__ void __launch_bounds__(TcLayout<DK, kStateOnly>::kThreads, 1)
+decay_tc_kernel(const __grid_constant__ TcParams p) {
+  using L = TcLayout<DK, kStateOnly>;
+  constexpr int kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sb = smem_u32(smem);
+  uint64_t *bars = (uint64_t *)(smem + L::kOffBar);
+  uint32_t *tmem_slot = (uint32_t *)(smem + L::kOffBar + 8 * kNumBars);
+  volatile int *abort_flag = (volatile int *)(smem + L::kOffBar + 8 * kNumBars + 4);
+  float *tab = (float *)(smem + L::kOffTab);
+
+  // roles fastest, then slices: CTAs that read the same tokens run together
+  int64_t id = blockIdx.x;
+  const TcRole &role = p.role[id % p.roles];
+  id /= p.roles;
+  const int c0 = (int)(id % p.slices) * kDecaySlice;
+  id /= p.slices;
+  const int order = (int)(id % p.segments);
+  const int64_t bh = id / p.segments;
+  if (c0 >= role.dvo) return;
+  const int ib = (int)(bh / p.heads), ih = (int)(bh % p.heads);
+  const bool rev = role.reverse != 0;
+  const int e0 = rev ? 0 : 1;
+  const int64_t t0 = (int64_t)(rev ? p.segments - 1 - order : order) * p.seg_len;
+  const int64_t t1 = min64(p.n, t0 + p.seg_len);
+  const int tiles = (int)((t1 - t0 + kT - 1) / kT);
+  const bool want_final =
+      kStateOnly || (role.final_state != nullptr && order == p.segments - 1);
+  // tiles whose U is needed: the last one's only for the final state
+  const int updates = want_final ? tiles : (tiles > 0 ? tiles - 1 : 0);
+  const float g = p.log_decay[ih];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // first token and valid tokens of the walk's tile c
+  auto tile_start = [&](int c) { return t0 + (int64_t)(rev ? tiles - 1 - c : c) * kT; };
+  auto tile_len = [&](int c) { return (int)min64(kT, t1 - tile_start(c)); };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNumBars; ++i) {
+      const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 || i == kUFree;
+      const bool per_four = i == kPReady || i == kPReady + 1 || i == kVpReady || i == kOFree;
+      const bool stage_empty = i >= kEmpty && i < kEmpty + 6;
+      mbar_init(&bars[i], per_state_warp ? L::kStateWarps
+                          : per_four     ? 4
+                          : stage_empty  ? (kStateOnly ? 1 : 2)
+                                         : 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (threadIdx.x < L::kTab)
+    tab[threadIdx.x] = (int)threadIdx.x < 32 ? 0.f : decay_pow(g, (int)threadIdx.x - 32);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const CUtensorMap *ma = &p.map[role.a], *mb = &p.map[role.b], *mv = &p.map[role.v];
+      if (!kStateOnly) prefetch_tmap(ma);
+      prefetch_tmap(mb);
+      prefetch_tmap(mv);
+      int c = 0;
+      for (; c < tiles; ++c) {
+        const int s = c % kStages;
+        if (c >= kStages && !mbar_wait(&bars[kEmpty + s], ((c / kStages) - 1) & 1, abort_flag))
+          break;
+        const int y = (int)tile_start(c);
+        uint8_t *st = smem + s * L::kStageBytes;
+        mbar_arrive_expect_tx(&bars[kFull + s], L::kStageBytes);
+#pragma unroll
+        for (int b = 0; b < L::kKBlocks; ++b) {
+          tma_load_4d(st + L::kOffB + b * kBlock, mb, &bars[kFull + s], 64 * b, y, ih, ib);
+          if (!kStateOnly)
+            tma_load_4d(st + L::kOffA + b * kBlock, ma, &bars[kFull + s], 64 * b, y, ih, ib);
+        }
+        tma_load_4d(st + L::kOffV, mv, &bars[kFull + s], c0, y, ih, ib);
+      }
+      // every issued copy must land before the CTA can exit
+      for (int i = c - kStages < 0 ? 0 : c - kStages; i < c; ++i)
+        wait_teardown(&bars[kFull + i % kStages], (i / kStages) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------- scores, A S and P V (one tile ahead)
+    if constexpr (!kStateOnly) {
+      constexpr uint32_t id_s = make_idesc_bf16(128, 128, false, false);
+      constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
+      auto issue_scores = [&](int c) -> bool {
+        const int s = c % kStages;
+        if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint32_t st = sb + s * L::kStageBytes;
+        const uint64_t da = make_sdesc(st + L::kOffA, 16, 1024, kSwizzle128B);
+        const uint64_t db = make_sdesc(st + L::kOffB, 16, 1024, kSwizzle128B);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < DK / 16; ++kk) {  // 32 bytes along the 128-byte rows
+            const uint64_t step = (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2);
+            umma_ss(tmem + kColScores + (c & 1) * 128, da + step, db + step, id_s, kk > 0);
+          }
+          umma_commit(&bars[kSReady + (c & 1)]);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = tiles > 0 && issue_scores(0);
+      for (int c = 0; ok && c < tiles; ++c) {
+        const int s = c % kStages, b = c & 1;
+        // the next tile's scores go first: P of the tile after this one is
+        // formed under this tile's read-out (their buffer was read by P V of
+        // tile c - 1, issued before)
+        if (c + 1 < tiles && !issue_scores(c + 1)) break;
+        if (!mbar_wait_warp(&bars[kSnapReady + b], (c / 2) & 1, abort_flag)) break;
+        if (c > 0 && !mbar_wait_warp(&bars[kOFree], (c - 1) & 1, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t st = sb + s * L::kStageBytes;
+        const uint64_t da = make_sdesc(st + L::kOffA, 16, 1024, kSwizzle128B);
+        const uint64_t ds = make_sdesc(sb + L::kOffSnap + b * L::kSnapBytes, 16, 1024, kSwizzle128B);
+        const uint64_t dv = make_sdesc(st + L::kOffV, 16, 1024, kSwizzle128B);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < DK / 16; ++kk)
+            umma_ss(tmem + kColO1, da + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
+                    ds + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
+          umma_commit(&bars[kSnapFree + b]);
+        }
+        __syncwarp();
+        if (!mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kT / 16; ++kk)
+            umma_ts(tmem + kColO2, tmem + kColScores + b * 128 + 8 * kk,
+                    dv + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
+          umma_commit(&bars[kOReady]);
+          umma_commit(&bars[kEmpty + s]);
+        }
+        __syncwarp();
+      }
+      if (elect_one()) umma_commit(&bars[kDone]);
+      __syncwarp();
+      if (lane == 0) wait_teardown(&bars[kDone], 0);
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ U = B^T V'
+    constexpr uint32_t id_u = make_idesc_bf16(128, 128, true, true);
+    for (int c = 0; c < updates; ++c) {
+      const int s = c % kStages;
+      if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) break;
+      if (!mbar_wait_warp(&bars[kVpReady], c & 1, abort_flag)) break;
+      if (c > 0 && !mbar_wait_warp(&bars[kUFree], (c - 1) & 1, abort_flag)) break;
+      tc_fence_after();
+      // A = B^T: the second 64 rows of M are the next 64 columns (DK = 128), or
+      // the same ones again (DK = 64)
+      const uint64_t da = make_sdesc(sb + s * L::kStageBytes + L::kOffB, DK == 64 ? 0 : kBlock,
+                                     1024, kSwizzle128B);
+      const uint64_t db = make_sdesc(sb + L::kOffVp, kBlock, 1024, kSwizzle128B);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk) {
+          const uint64_t step = (uint64_t)(kk * (2048 >> 4));
+          umma_ss(tmem + kColU, da + step, db + step, id_u, kk > 0);
+        }
+        umma_commit(&bars[kUReady]);
+        umma_commit(&bars[kEmpty + s]);
+      }
+      __syncwarp();
+    }
+    if (elect_one()) umma_commit(&bars[kDone + 1]);
+    __syncwarp();
+    if (lane == 0) wait_teardown(&bars[kDone + 1], 0);
+    __syncwarp();
+  } else if (warp >= L::kWState && warp < L::kWP) {
+    // ------------------------------------------------------------ state
+    // A thread owns 32 columns of one row of S.
+    const int wq = warp & 3;  // TMEM lane quarter
+    const int row = DK == 64 ? (wq & 1) * 32 + lane : wq * 32 + lane;
+    const int half = DK == 64 ? wq >> 1 : (warp - L::kWState) >> 2;
+    const int col = c0 + half * 32;
+    float st[32];
+    const int64_t at = (bh * p.segments + order) * (int64_t)role.da * role.dvo;
+    const bool mine = row < role.da;
+    const int cols = mine ? min(32, role.dvo - col) : 0;  // may be negative
+    {
+      const float *src = nullptr;
+      int64_t step = 1;
+      if (!kStateOnly && role.seeds && mine) {
+        src = role.seeds + at + (role.seed_transposed ? (int64_t)col * role.da + row
+                                                      : (int64_t)row * role.dvo + col);
+        if (role.seed_transposed) step = role.da;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        st[i] = src && i < cols ? *src : 0.f;
+        src += src ? step : 0;
+      }
+    }
+    const uint32_t urow = taddr(tmem, wq * 32, kColU + half * 32);
+    auto write_copy = [&](int b) {
+      const uint32_t dst = sb + L::kOffSnap + b * L::kSnapBytes;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        st_shared_v4(dst + sw128_offset(row, half * 4 + q), pack_bf16(st[8 * q], st[8 * q + 1]),
+                     pack_bf16(st[8 * q + 2], st[8 * q + 3]),
+                     pack_bf16(st[8 * q + 4], st[8 * q + 5]),
+                     pack_bf16(st[8 * q + 6], st[8 * q + 7]));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kSnapReady + b]);
+    };
+    if (!kStateOnly && tiles > 0) write_copy(0);
+    const float keep_full = decay_pow(g, kT);
+    for (int c = 0; c < updates; ++c) {
+      const int len = tile_len(c);
+      const float keep = len == kT ? keep_full : decay_pow(g, len);
+      mbar_wait(&bars[kUReady], c & 1, abort_flag);
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t hi[8], lo[8];
+        tmem_ld8(urow + 8 * q, hi);
+        tmem_ld8(urow + 64 + 8 * q, lo);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          st[8 * q + i] = fmaf(keep, st[8 * q + i], __uint_as_float(hi[i]) + __uint_as_float(lo[i]));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kUFree]);
+      if (!kStateOnly && c + 1 < tiles) {
+        const int b = (c + 1) & 1;
+        if (c > 0) mbar_wait(&bars[kSnapFree + b], ((c - 1) / 2) & 1, abort_flag);
+        __syncwarp();
+        write_copy(b);
+      }
+    }
+    if (want_final) {
+      float *dst = (kStateOnly ? role.states + at
+                               : role.final_state + bh * (int64_t)role.da * role.dvo) +
+                   (int64_t)row * role.dvo + col;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < cols) dst[i] = st[i];
+    }
+  } else if (!kStateOnly && warp >= L::kWP && warp < L::kWV) {
+    // ------------------------------------------------------------ P
+    // Group grp takes the tiles grp, grp + 2, ... (one scores buffer each).
+    const int grp = (warp - L::kWP) >> 2;
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    float g2 = g * kLog2e, intra = role.intra;
+    // lambda^(i-j) over 16 columns j0 + t that are all before (a reversed walk:
+    // after) the row: lambda^(i-j0-15) * lambda^(15-t), or lambda^(j0-i) *
+    // lambda^t -- both powers non-negative, so nothing overflows
+    uint64_t w2[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int n0 = rev ? 2 * t : 15 - 2 * t, n1 = rev ? 2 * t + 1 : 14 - 2 * t;
+      w2[t] = f2pack(tab[32 + n0] * intra, tab[32 + n1] * intra);
+    }
+    const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + grp * 128);
+    for (int c = grp; c < tiles; c += 2) {
+      mbar_wait(&bars[kSReady + grp], (c / 2) & 1, abort_flag);
+      __syncwarp();
+      tc_fence_after();
+      // the 128 weights of a row are the same in every tile; hoisted out of the
+      // loop they would be kept in local memory
+      asm volatile("" : "+f"(g2), "+f"(intra));
+#pragma unroll
+      for (int ch = 0; ch < 8; ++ch) {  // 16 columns each; P lands on columns already read
+        uint32_t pk[8];
+        if (rev ? ch < 2 * wq : ch > 2 * wq + 1) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pk[i] = 0;
+        } else {
+          uint32_t x[16];
+          tmem_ld16(srow0 + 16 * ch, x);
+          tmem_wait_ld();
+          if ((ch >> 1) == wq) {
+            // the diagonal: lambda^lag from the table, zero where lag < 0
+            const int j0 = 16 * (ch & 1);
+            const float *lam = tab + 32 + (rev ? j0 - lane : lane - j0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float f0 = lam[rev ? 2 * i : -2 * i], f1 = lam[rev ? 2 * i + 1 : -2 * i - 1];
+              const float y0 = __uint_as_float(x[2 * i]) * (intra * f0);
+              const float y1 = __uint_as_float(x[2 * i + 1]) * (intra * f1);
+              const int j = j0 + 2 * i;
+              const bool in0 = rev ? j >= lane : j <= lane;
+              const bool in1 = rev ? j + 1 >= lane : j + 1 <= lane;
+              pk[i] = pack_bf16(in0 ? y0 : 0.f, in1 ? y1 : 0.f);
+            }
+          } else {
+            const int j0 = 16 * ch;
+            const float f = ex2_approx((float)(rev ? j0 - r : r - j0 - 15) * g2);
+            const uint64_t f2 = f2pack(f, f);
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              pk[t] = pack_bf16x2(
+                  fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
+                        fmul2(f2, w2[t])));
+          }
+        }
+        tmem_st8(srow0 + 8 * ch, pk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kPReady + grp]);
+    }
+  } else if (warp >= L::kWV && warp < L::kWE) {
+    // ------------------------------------------------------------ V' = hi + lo
+    const int j = (warp - L::kWV) * 32 + lane;  // token of the tile
+    // place in a full tile: forward len - 1 - j, reversed (len - 1 - j mirrored) j + 1
+    const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
+    for (int c = 0; c < updates; ++c) {
+      const int s = c % kStages;
+      const int len = tile_len(c);
+      const float w = rev || len == kT ? w_full : role.inc * decay_pow(g, len - 1 - j);
+      mbar_wait(&bars[kFull + s], (c / kStages) & 1, abort_flag);
+      if (c > 0) mbar_wait(&bars[kUReady], (c - 1) & 1, abort_flag);
+      __syncwarp();
+      const uint32_t src = sb + s * L::kStageBytes + L::kOffV, dst = sb + L::kOffVp;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t off = sw128_offset(j, q);
+        uint32_t x[4], hi[4], lo[4];
+        ld_shared_v4(src + off, x[0], x[1], x[2], x[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y0 = bf16lo(x[i]) * w, y1 = bf16hi(x[i]) * w;
+          hi[i] = pack_bf16(y0, y1);
+          lo[i] = pack_bf16(y0 - bf16lo(hi[i]), y1 - bf16hi(hi[i]));
+        }
+        st_shared_v4(dst + off, hi[0], hi[1], hi[2], hi[3]);
+        st_shared_v4(dst + kBlock + off, lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kVpReady]);
+    }
+  } else if (!kStateOnly && warp >= L::kWE) {
+    // ------------------------------------------------------------ epilogue
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const int gi = lane & 3;
+    const float f_full = role.inter * decay_pow(g, (rev ? kT - 1 - r : r) + e0);
+    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0;
+    const uint32_t orow = taddr(tmem, wq * 32, kColO1);
+    for (int c = 0; c < tiles; ++c) {
+      const int64_t base = tile_start(c);
+      const int len = tile_len(c);
+      const float f = !rev || len == kT ? f_full : role.inter * decay_pow(g, len - 1 - r);
+      const uint64_t f2 = f2pack(f, f);
+      mbar_wait(&bars[kOReady], c & 1, abort_flag);
+      __syncwarp();
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        uint32_t x[16], y[16];
+        tmem_ld16(orow + 16 * h, x);
+        tmem_ld16(orow + (kColO2 - kColO1) + 16 * h, y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[8 * h + i] = pack_bf16x2(
+              ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
+                    f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kOFree]);
+      // 4x4 transpose of 32-byte pieces inside each group of four lanes: the
+      // stores then write whole 128-byte rows
+#pragma unroll
+      for (int mm = 2; mm >= 1; mm >>= 1) {
+        const bool hi = (gi & mm) != 0;
+#pragma unroll
+        for (int kx = 0; kx < 2; ++kx) {
+          const int s0 = mm == 2 ? kx : (kx << 1);
+          const int s1 = s0 | mm;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t send = hi ? w[8 * s0 + i] : w[8 * s1 + i];
+            const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, mm);
+            if (hi) w[8 * s0 + i] = recv;
+            else w[8 * s1 + i] = recv;
+          }
+        }
+      }
+      const int rbase = wq * 32 + (lane & ~3);
+      const int left = role.dvo - c0 - 16 * gi;  // columns of this lane's piece, a multiple of 8
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (rbase + i < len) {
+          uint4 *dst = (uint4 *)(out + (base + rbase + i) * role.ot + 16 * gi);
+          if (left > 0) dst[0] = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+          if (left > 8) dst[1] = make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  // Both issuers have seen their last MMA complete before they get here.
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, kErrTimeout);
+}
+
+// 4-D map (width, tokens, heads, batch) with a 64 x 128 box; outside reads as
+// zero.
+bool make_map(CUtensorMap *map, const DecayView &x, int width, const DecayCall &c) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t one = (cuuint64_t)width * 2;  // a dimension of one entry has no stride
+  cuuint64_t gdim[4] = {(cuuint64_t)width, (cuuint64_t)c.n, (cuuint64_t)c.heads,
+                        (cuuint64_t)c.batch};
+  cuuint64_t gstride[3] = {c.n > 1 ? (cuuint64_t)x.st * 2 : one,
+                           c.heads > 1 ? (cuuint64_t)x.sh * 2 : one,
+                           c.batch > 1 ? (cuuint64_t)x.sb * 2 : one};
+  cuuint32_t box[4] = {64, kT, 1, 1};
+  cuuint32_t estride[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(x.p), gdim, gstride, box,
+            estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DK, bool kStateOnly>
+int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
+  using L = TcLayout<DK, kStateOnly>;
+  auto kernel = decay_tc_kernel<DK, kStateOnly>;
+  if (allow_dynamic_smem((const void *)kernel, (int)L::kSmem) != LA_OK) return LA_ERR_CUDA;
+  kernel<<<(unsigned)grid, L::kThreads, L::kSmem, s>>>(p);
+  return check_launch();
+}
+
+template <bool kStateOnly>
+int launch(const DecayCall &c, cudaStream_t s) {
+  TcParams p;
+  // first: it binds the device's context to a thread that has none yet (an
+  // autograd worker), which encoding a tensor map needs
+  p.err = device_error_word();
+  if (!p.err) return LA_ERR_CUDA;
+  int maps = 0, da = 0, slices = 1;
+  struct {
+    DecayView x;
+    int width;
+  } known[4];
+  auto map_of = [&](const DecayView &x, int width) {
+    for (int i = 0; i < maps; ++i) {
+      const DecayView &y = known[i].x;
+      if (y.p == x.p && y.sb == x.sb && y.sh == x.sh && y.st == x.st && known[i].width == width)
+        return i;
+    }
+    if (maps == 4 || !make_map(&p.map[maps], x, width, c)) return -1;
+    known[maps].x = x;
+    known[maps].width = width;
+    return maps++;
+  };
+  for (int r = 0; r < c.roles; ++r) {
+    const DecayRole &f = c.role[r];
+    TcRole &t = p.role[r];
+    t.a = kStateOnly ? 0 : map_of(f.a, f.da);
+    t.b = map_of(f.b, f.da);
+    t.v = map_of(f.v, f.dvo);
+    if (t.a < 0 || t.b < 0 || t.v < 0) return LA_ERR_CUDA;
+    t.out = (__nv_bfloat16 *)f.out.p;
+    t.ob = f.out.sb, t.oh = f.out.sh, t.ot = f.out.st;
+    t.seeds = f.seeds, t.states = f.states, t.final_state = f.final_state;
+    t.da = f.da, t.dvo = f.dvo;
+    t.seed_transposed = f.seed_transposed, t.reverse = f.reverse;
+    t.intra = f.intra, t.inter = f.inter, t.inc = f.inc;
+    if (f.da > da) da = f.da;
+    const int n = (f.dvo + kDecaySlice - 1) / kDecaySlice;
+    if (n > slices) slices = n;
+  }
+  p.log_decay = c.log_decay;
+  p.heads = c.heads, p.n = c.n, p.seg_len = c.seg_len;
+  p.roles = c.roles, p.slices = slices, p.segments = c.segments;
+  const int64_t grid = c.batch * c.heads * c.segments * slices * c.roles;
+  if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  return da <= 64 ? launch_t<64, kStateOnly>(p, grid, s) : launch_t<128, kStateOnly>(p, grid, s);
+}
+
+}  // namespace
+
+bool decay_tc_view(const DecayView &x, int width, const DecayCall &c) {
+  return width % 8 == 0 && ((uintptr_t)x.p & 15) == 0 &&
+         (c.n <= 1 || (x.st % 8 == 0 && x.st >= width)) &&
+         (c.heads <= 1 || (x.sh % 8 == 0 && x.sh > 0)) &&
+         (c.batch <= 1 || (x.sb % 8 == 0 && x.sb > 0));
+}
+
+int launch_decay_state_tc(const DecayCall &c, cudaStream_t s) { return launch<true>(c, s); }
+int launch_decay_output_tc(const DecayCall &c, cudaStream_t s) { return launch<false>(c, s); }
+
+}  // namespace la
