@@ -66,15 +66,13 @@ struct TcLayout {
   static constexpr uint32_t kOffV = kOffB + kKBlocks * kBlock;
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
-  static constexpr uint32_t kTab = 64;  // lambda^0 .. lambda^31 behind 32 zeros
-  static constexpr uint32_t kFixed = 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + kTab * 4 + 512;
+  static constexpr uint32_t kFixed = 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
   static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
                                      ? 6
                                      : (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes;
   static constexpr uint32_t kOffVp = kStages * kStageBytes;     // V' hi, lo
   static constexpr uint32_t kOffSnap = kOffVp + 2 * kBlock;     // two bf16 copies of S
-  static constexpr uint32_t kOffTab = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
-  static constexpr uint32_t kOffBar = kOffTab + kTab * 4;
+  static constexpr uint32_t kOffBar = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kSmem > 114 * 1024, "one CTA per SM (all TMEM columns)");
@@ -151,7 +149,6 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   uint64_t *bars = (uint64_t *)(smem + L::kOffBar);
   uint32_t *tmem_slot = (uint32_t *)(smem + L::kOffBar + 8 * kNumBars);
   volatile int *abort_flag = (volatile int *)(smem + L::kOffBar + 8 * kNumBars + 4);
-  float *tab = (float *)(smem + L::kOffTab);
 
   // roles fastest, then slices: CTAs that read the same tokens run together
   int64_t id = blockIdx.x;
@@ -191,8 +188,6 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x < L::kTab)
-    tab[threadIdx.x] = (int)threadIdx.x < 32 ? 0.f : decay_pow(g, (int)threadIdx.x - 32);
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -360,6 +355,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     for (int c = 0; c < updates; ++c) {
       const int len = tile_len(c);
       const float keep = len == kT ? keep_full : decay_pow(g, len);
+      const uint64_t keep2 = f2pack(keep, keep);
       mbar_wait(&bars[kUReady], c & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
@@ -370,8 +366,12 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         tmem_ld8(urow + 64 + 8 * q, lo);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          st[8 * q + i] = fmaf(keep, st[8 * q + i], __uint_as_float(hi[i]) + __uint_as_float(lo[i]));
+        for (int i = 0; i < 8; i += 2) {
+          const uint64_t u = fadd2(f2pack(__uint_as_float(hi[i]), __uint_as_float(hi[i + 1])),
+                                   f2pack(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1])));
+          f2unpack(ffma2(keep2, f2pack(st[8 * q + i], st[8 * q + i + 1]), u), st[8 * q + i],
+                   st[8 * q + i + 1]);
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -396,61 +396,68 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // Group grp takes the tiles grp, grp + 2, ... (one scores buffer each).
     const int grp = (warp - L::kWP) >> 2;
     const int wq = warp & 3;
-    const int r = wq * 32 + lane;
-    float g2 = g * kLog2e, intra = role.intra;
-    // lambda^(i-j) over 16 columns j0 + t that are all before (a reversed walk:
+    // finite, so that 0 * g2 = 0 (e^-6900 is zero like e^-inf)
+    const float g2 = fmaxf(g * kLog2e, -1e4f);
+    const uint64_t g22 = f2pack(g2, g2), intra2 = f2pack(role.intra, role.intra);
+    const float toward = rev ? 1.f : -1.f;  // a later column: lag + 1, or - 1
+    // lambda^lag over 16 columns j0 + t that are all before (a reversed walk:
     // after) the row: lambda^(i-j0-15) * lambda^(15-t), or lambda^(j0-i) *
     // lambda^t -- both powers non-negative, so nothing overflows
     uint64_t w2[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int n0 = rev ? 2 * t : 15 - 2 * t, n1 = rev ? 2 * t + 1 : 14 - 2 * t;
-      w2[t] = f2pack(tab[32 + n0] * intra, tab[32 + n1] * intra);
+      w2[t] = f2pack(decay_pow(g, n0) * role.intra, decay_pow(g, n1) * role.intra);
     }
     const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + grp * 128);
     for (int c = grp; c < tiles; c += 2) {
       mbar_wait(&bars[kSReady + grp], (c / 2) & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      // the 128 weights of a row are the same in every tile; hoisted out of the
-      // loop they would be kept in local memory
-      asm volatile("" : "+f"(g2), "+f"(intra));
+      // 16 columns at a time; P lands on columns already read.  Kept rolled:
+      // the warps' roles share one instruction cache.
+#pragma unroll 1
+      for (int ch = 0; ch < 8; ++ch) {
+        const int side = rev ? wq - (ch >> 1) : (ch >> 1) - wq;
+        uint32_t x[16];
+        if (side > 0) {
 #pragma unroll
-      for (int ch = 0; ch < 8; ++ch) {  // 16 columns each; P lands on columns already read
-        uint32_t pk[8];
-        if (rev ? ch < 2 * wq : ch > 2 * wq + 1) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pk[i] = 0;
+          for (int i = 0; i < 8; ++i) x[i] = 0;
         } else {
-          uint32_t x[16];
+          // lag of the row and the first column
+          const int first = (wq * 32 + lane - 16 * ch) * (rev ? -1 : 1);
           tmem_ld16(srow0 + 16 * ch, x);
           tmem_wait_ld();
-          if ((ch >> 1) == wq) {
-            // the diagonal: lambda^lag from the table, zero where lag < 0
-            const int j0 = 16 * (ch & 1);
-            const float *lam = tab + 32 + (rev ? j0 - lane : lane - j0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float f0 = lam[rev ? 2 * i : -2 * i], f1 = lam[rev ? 2 * i + 1 : -2 * i - 1];
-              const float y0 = __uint_as_float(x[2 * i]) * (intra * f0);
-              const float y1 = __uint_as_float(x[2 * i + 1]) * (intra * f1);
-              const int j = j0 + 2 * i;
-              const bool in0 = rev ? j >= lane : j <= lane;
-              const bool in1 = rev ? j + 1 >= lane : j + 1 <= lane;
-              pk[i] = pack_bf16(in0 ? y0 : 0.f, in1 ? y1 : 0.f);
-            }
-          } else {
-            const int j0 = 16 * ch;
-            const float f = ex2_approx((float)(rev ? j0 - r : r - j0 - 15) * g2);
+          if (side < 0) {
+            const float f = ex2_approx((float)(rev ? first : first - 15) * g2);
             const uint64_t f2 = f2pack(f, f);
 #pragma unroll
             for (int t = 0; t < 8; ++t)
-              pk[t] = pack_bf16x2(
+              x[t] = pack_bf16x2(
                   fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
                         fmul2(f2, w2[t])));
+          } else {
+            // the diagonal: each pair its own power, zero where lag < 0
+            const float m = (float)first;
+            const uint64_t m2 = f2pack(m, m), step2 = f2pack(toward, toward);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+              const uint64_t lag = ffma2(step2, f2pack(2.f * t, 2.f * t + 1.f), m2);
+              float l0, l1, e0_, e1_;
+              f2unpack(lag, l0, l1);
+              f2unpack(fmul2(lag, g22), e0_, e1_);
+              e0_ = ex2_approx(l0 < 0.f ? -INFINITY : e0_);
+              e1_ = ex2_approx(l1 < 0.f ? -INFINITY : e1_);
+              const uint64_t y =
+                  fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])), intra2);
+              float y0, y1;
+              f2unpack(y, y0, y1);
+              // (a select, not the product: scores beyond the row may not be finite)
+              x[t] = pack_bf16(l0 < 0.f ? 0.f : y0 * e0_, l1 < 0.f ? 0.f : y1 * e1_);
+            }
           }
         }
-        tmem_st8(srow0 + 8 * ch, pk);
+        tmem_st8(srow0 + 8 * ch, x);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -466,20 +473,21 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const int s = c % kStages;
       const int len = tile_len(c);
       const float w = rev || len == kT ? w_full : role.inc * decay_pow(g, len - 1 - j);
+      const uint64_t w2 = f2pack(w, w), minus2 = f2pack(-1.f, -1.f);
       mbar_wait(&bars[kFull + s], (c / kStages) & 1, abort_flag);
       if (c > 0) mbar_wait(&bars[kUReady], (c - 1) & 1, abort_flag);
       __syncwarp();
       const uint32_t src = sb + s * L::kStageBytes + L::kOffV, dst = sb + L::kOffVp;
-#pragma unroll
+#pragma unroll 2
       for (int q = 0; q < 8; ++q) {
         const uint32_t off = sw128_offset(j, q);
         uint32_t x[4], hi[4], lo[4];
         ld_shared_v4(src + off, x[0], x[1], x[2], x[3]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y0 = bf16lo(x[i]) * w, y1 = bf16hi(x[i]) * w;
-          hi[i] = pack_bf16(y0, y1);
-          lo[i] = pack_bf16(y0 - bf16lo(hi[i]), y1 - bf16hi(hi[i]));
+          const uint64_t y = fmul2(f2pack(bf16lo(x[i]), bf16hi(x[i])), w2);
+          hi[i] = pack_bf16x2(y);
+          lo[i] = pack_bf16x2(ffma2(f2pack(bf16lo(hi[i]), bf16hi(hi[i])), minus2, y));
         }
         st_shared_v4(dst + off, hi[0], hi[1], hi[2], hi[3]);
         st_shared_v4(dst + kBlock + off, lo[0], lo[1], lo[2], lo[3]);
@@ -492,9 +500,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // ------------------------------------------------------------ epilogue
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
-    const int gi = lane & 3;
     const float f_full = role.inter * decay_pow(g, (rev ? kT - 1 - r : r) + e0);
     __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0;
+    // 32-byte stores where every row's pieces are 32-byte aligned
+    const bool wide = ((uintptr_t)out & 31) == 0 && role.ot % 16 == 0;
     const uint32_t orow = taddr(tmem, wq * 32, kColO1);
     for (int c = 0; c < tiles; ++c) {
       const int64_t base = tile_start(c);
@@ -504,48 +513,33 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       mbar_wait(&bars[kOReady], c & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      uint32_t w[32];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
+      const bool live = r < len;
+      __nv_bfloat16 *dst = out + (base + r) * role.ot;
+#pragma unroll 1
+      for (int h = 0; h < 4; ++h, dst += 16) {
         uint32_t x[16], y[16];
         tmem_ld16(orow + 16 * h, x);
         tmem_ld16(orow + (kColO2 - kColO1) + 16 * h, y);
         tmem_wait_ld();
+        if (h == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kOFree]);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          w[8 * h + i] = pack_bf16x2(
+          x[i] = pack_bf16x2(
               ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
                     f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kOFree]);
-      // 4x4 transpose of 32-byte pieces inside each group of four lanes: the
-      // stores then write whole 128-byte rows
-#pragma unroll
-      for (int mm = 2; mm >= 1; mm >>= 1) {
-        const bool hi = (gi & mm) != 0;
-#pragma unroll
-        for (int kx = 0; kx < 2; ++kx) {
-          const int s0 = mm == 2 ? kx : (kx << 1);
-          const int s1 = s0 | mm;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t send = hi ? w[8 * s0 + i] : w[8 * s1 + i];
-            const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, mm);
-            if (hi) w[8 * s0 + i] = recv;
-            else w[8 * s1 + i] = recv;
-          }
-        }
-      }
-      const int rbase = wq * 32 + (lane & ~3);
-      const int left = role.dvo - c0 - 16 * gi;  // columns of this lane's piece, a multiple of 8
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (rbase + i < len) {
-          uint4 *dst = (uint4 *)(out + (base + rbase + i) * role.ot + 16 * gi);
-          if (left > 0) dst[0] = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
-          if (left > 8) dst[1] = make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+        const int left = live ? role.dvo - c0 - 16 * h : 0;  // a multiple of 8
+        if (left >= 16 && wide) {
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+                       "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
+                       "r"(x[6]), "r"(x[7])
+                       : "memory");
+        } else {
+          if (left > 0) *(uint4 *)dst = make_uint4(x[0], x[1], x[2], x[3]);
+          if (left > 8) *(uint4 *)(dst + 8) = make_uint4(x[4], x[5], x[6], x[7]);
         }
       }
     }
