@@ -29,7 +29,7 @@
 // U -> S -> copy -> O1 -> out) where few CTAs walk.
 //
 // Warps: 0 TMA; 1 scores, O1 and O2 MMAs (TMEM owner); 2 U MMAs; 4.. state
-// (4 warps at DK = 64, 8 at 128); 8 warps P (two groups, alternate tiles); 4
+// (4 warps at DK = 64, 8 at 128); 8 warps P; 4
 // warps V'; 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
 #include "decay.cuh"
 #include "tc_common.cuh"
@@ -66,12 +66,14 @@ struct TcLayout {
   static constexpr uint32_t kOffV = kOffB + kKBlocks * kBlock;
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
-  static constexpr uint32_t kFixed = 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
+  static constexpr int kVpBufs = DK == 64 ? 2 : 1;
+  static constexpr uint32_t kFixed =
+      kVpBufs * 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
   static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
                                      ? 6
                                      : (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes;
   static constexpr uint32_t kOffVp = kStages * kStageBytes;     // V' hi, lo
-  static constexpr uint32_t kOffSnap = kOffVp + 2 * kBlock;     // two bf16 copies of S
+  static constexpr uint32_t kOffSnap = kOffVp + kVpBufs * 2 * kBlock;  // two bf16 copies of S
   static constexpr uint32_t kOffBar = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
@@ -86,8 +88,8 @@ enum Bar {
   kSnapReady = kPReady + 2,
   kSnapFree = kSnapReady + 2,
   kVpReady = kSnapFree + 2,
-  kUReady,
-  kUFree,
+  kUReady = kVpReady + 2,  // alternate tiles: V' may run a tile ahead of its readers
+  kUFree = kUReady + 2,
   kOReady,
   kOFree,
   kDone,
@@ -130,6 +132,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+__device__ __forceinline__ uint32_t hfma2_bf16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t hneg2_bf16(uint32_t a) { return a ^ 0x80008000u; }
 
 __device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();
@@ -178,10 +187,12 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
       const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 || i == kUFree;
-      const bool per_four = i == kPReady || i == kPReady + 1 || i == kVpReady || i == kOFree;
+      const bool per_four = i == kVpReady || i == kVpReady + 1 || i == kOFree;
+      const bool per_p_warp = i == kPReady || i == kPReady + 1;
       const bool stage_empty = i >= kEmpty && i < kEmpty + 6;
       mbar_init(&bars[i], per_state_warp ? L::kStateWarps
                           : per_four     ? 4
+                          : per_p_warp   ? 8
                           : stage_empty  ? (kStateOnly ? 1 : 2)
                                          : 1);
     }
@@ -226,6 +237,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     if constexpr (!kStateOnly) {
       constexpr uint32_t id_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
+      const int k_steps = (role.da + 15) / 16;  // the columns beyond are zero
       auto issue_scores = [&](int c) -> bool {
         const int s = c % kStages;
         if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) return false;
@@ -237,7 +249,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk) {  // 32 bytes along the 128-byte rows
             const uint64_t step = (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2);
-            umma_ss(tmem + kColScores + (c & 1) * 128, da + step, db + step, id_s, kk > 0);
+            if (kk < k_steps) umma_ss(tmem + kColScores + (c & 1) * 128, da + step, db + step, id_s, kk > 0);
           }
           umma_commit(&bars[kSReady + (c & 1)]);
         }
@@ -247,10 +259,13 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       bool ok = tiles > 0 && issue_scores(0);
       for (int c = 0; ok && c < tiles; ++c) {
         const int s = c % kStages, b = c & 1;
-        // the next tile's scores go first: P of the tile after this one is
-        // formed under this tile's read-out (their buffer was read by P V of
-        // tile c - 1, issued before)
-        if (c + 1 < tiles && !issue_scores(c + 1)) break;
+        // the next tile's scores go first if its copies have landed: P of the
+        // next tile is formed under this tile's read-out (the buffer was read by
+        // P V of tile c - 1, issued before)
+        const bool early =
+            c + 1 < tiles && __all_sync(0xffffffffu, mbar_test_wait(&bars[kFull + (c + 1) % kStages],
+                                                                    ((c + 1) / kStages) & 1));
+        if (early && !issue_scores(c + 1)) break;
         if (!mbar_wait_warp(&bars[kSnapReady + b], (c / 2) & 1, abort_flag)) break;
         if (c > 0 && !mbar_wait_warp(&bars[kOFree], (c - 1) & 1, abort_flag)) break;
         tc_fence_after();
@@ -261,7 +276,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk)
-            umma_ss(tmem + kColO1, da + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
+            if (kk < k_steps)
+              umma_ss(tmem + kColO1, da + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
                     ds + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
           umma_commit(&bars[kSnapFree + b]);
         }
@@ -271,12 +287,13 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kT / 16; ++kk)
-            umma_ts(tmem + kColO2, tmem + kColScores + b * 128 + 8 * kk,
+            umma_ts(tmem + kColO2, tmem + kColScores + b * 128 + (kk / 4) * 64 + (kk % 4) * 8,
                     dv + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
           umma_commit(&bars[kOReady]);
           umma_commit(&bars[kEmpty + s]);
         }
         __syncwarp();
+        if (c + 1 < tiles && !early && !issue_scores(c + 1)) break;
       }
       if (elect_one()) umma_commit(&bars[kDone]);
       __syncwarp();
@@ -289,21 +306,23 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     for (int c = 0; c < updates; ++c) {
       const int s = c % kStages;
       if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) break;
-      if (!mbar_wait_warp(&bars[kVpReady], c & 1, abort_flag)) break;
+      const int vb = c % L::kVpBufs;
+      if (!mbar_wait_warp(&bars[kVpReady + vb], (c / L::kVpBufs) & 1, abort_flag)) break;
       if (c > 0 && !mbar_wait_warp(&bars[kUFree], (c - 1) & 1, abort_flag)) break;
       tc_fence_after();
       // A = B^T: the second 64 rows of M are the next 64 columns (DK = 128), or
       // the same ones again (DK = 64)
       const uint64_t da = make_sdesc(sb + s * L::kStageBytes + L::kOffB, DK == 64 ? 0 : kBlock,
                                      1024, kSwizzle128B);
-      const uint64_t db = make_sdesc(sb + L::kOffVp, kBlock, 1024, kSwizzle128B);
+      const uint64_t db =
+          make_sdesc(sb + L::kOffVp + vb * 2 * kBlock, kBlock, 1024, kSwizzle128B);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kT / 16; ++kk) {
           const uint64_t step = (uint64_t)(kk * (2048 >> 4));
           umma_ss(tmem + kColU, da + step, db + step, id_u, kk > 0);
         }
-        umma_commit(&bars[kUReady]);
+        umma_commit(&bars[kUReady + (c & 1)]);
         umma_commit(&bars[kEmpty + s]);
       }
       __syncwarp();
@@ -356,7 +375,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const int len = tile_len(c);
       const float keep = len == kT ? keep_full : decay_pow(g, len);
       const uint64_t keep2 = f2pack(keep, keep);
-      mbar_wait(&bars[kUReady], c & 1, abort_flag);
+      mbar_wait(&bars[kUReady + (c & 1)], (c / 2) & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
 #pragma unroll
@@ -393,76 +412,81 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     }
   } else if (!kStateOnly && warp >= L::kWP && warp < L::kWV) {
     // ------------------------------------------------------------ P
-    // Group grp takes the tiles grp, grp + 2, ... (one scores buffer each).
-    const int grp = (warp - L::kWP) >> 2;
+    // Two warps per lane quarter, 64 columns each; P takes the first 32 TMEM
+    // columns of its own half, so no warp writes what another still reads.
+    const int half = (warp - L::kWP) >> 2;
     const int wq = warp & 3;
     // finite, so that 0 * g2 = 0 (e^-6900 is zero like e^-inf)
     const float g2 = fmaxf(g * kLog2e, -1e4f);
-    const uint64_t g22 = f2pack(g2, g2), intra2 = f2pack(role.intra, role.intra);
-    const float toward = rev ? 1.f : -1.f;  // a later column: lag + 1, or - 1
-    // lambda^lag over 16 columns j0 + t that are all before (a reversed walk:
-    // after) the row: lambda^(i-j0-15) * lambda^(15-t), or lambda^(j0-i) *
-    // lambda^t -- both powers non-negative, so nothing overflows
+    const float toward = rev ? 1.f : -1.f;  // the next column: lag + 1, or - 1
+    // lambda^lag over 16 columns j0 + t: lambda^(i-j0-15) * lambda^(15-t), in a
+    // reversed walk lambda^(j0-i) * lambda^t.  Off the diagonal both powers are
+    // non-negative; on it the first reaches -15, which fp32 holds while
+    // |g| <= 4, and the columns with lag < 0 are cut from the packed words.
+    const bool mild = g >= -4.f && g <= 4.f;
     uint64_t w2[8];
+    uint32_t cut[2][8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int n0 = rev ? 2 * t : 15 - 2 * t, n1 = rev ? 2 * t + 1 : 14 - 2 * t;
       w2[t] = f2pack(decay_pow(g, n0) * role.intra, decay_pow(g, n1) * role.intra);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int lag = rev ? 16 * q - lane + 2 * t : lane - 16 * q - 2 * t;
+        cut[q][t] = (lag >= 0 ? 0xFFFFu : 0u) | (lag + (rev ? 1 : -1) >= 0 ? 0xFFFF0000u : 0u);
+      }
     }
-    const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + grp * 128);
-    for (int c = grp; c < tiles; c += 2) {
-      mbar_wait(&bars[kSReady + grp], (c / 2) & 1, abort_flag);
+    for (int c = 0; c < tiles; ++c) {
+      const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + (c & 1) * 128 + half * 64);
+      mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      // 16 columns at a time; P lands on columns already read.  Kept rolled:
+      // 32 columns at a time; P lands on columns already read.  Kept rolled:
       // the warps' roles share one instruction cache.
 #pragma unroll 1
-      for (int ch = 0; ch < 8; ++ch) {
-        const int side = rev ? wq - (ch >> 1) : (ch >> 1) - wq;
-        uint32_t x[16];
-        if (side > 0) {
+      for (int ch = 0; ch < 2; ++ch) {
+        const int side = (2 * half + ch - wq) * (rev ? -1 : 1);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0;
-        } else {
-          // lag of the row and the first column
-          const int first = (wq * 32 + lane - 16 * ch) * (rev ? -1 : 1);
-          tmem_ld16(srow0 + 16 * ch, x);
-          tmem_wait_ld();
-          if (side < 0) {
-            const float f = ex2_approx((float)(rev ? first : first - 15) * g2);
-            const uint64_t f2 = f2pack(f, f);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t x[16];
+          if (side > 0) {
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-              x[t] = pack_bf16x2(
-                  fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
-                        fmul2(f2, w2[t])));
+            for (int i = 0; i < 8; ++i) x[i] = 0;
           } else {
-            // the diagonal: each pair its own power, zero where lag < 0
-            const float m = (float)first;
-            const uint64_t m2 = f2pack(m, m), step2 = f2pack(toward, toward);
+            // lag of the row and the first column
+            const int first = (wq * 32 + lane - 64 * half - 32 * ch - 16 * q) * (rev ? -1 : 1);
+            tmem_ld16(srow0 + 32 * ch + 16 * q, x);
+            tmem_wait_ld();
+            if (side < 0 || mild) {
+              // (below -15 every column is cut)
+              const float f = ex2_approx((float)max(rev ? first : first - 15, -15) * g2);
+              const uint64_t f2 = f2pack(f, f);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-              const uint64_t lag = ffma2(step2, f2pack(2.f * t, 2.f * t + 1.f), m2);
-              float l0, l1, e0_, e1_;
-              f2unpack(lag, l0, l1);
-              f2unpack(fmul2(lag, g22), e0_, e1_);
-              e0_ = ex2_approx(l0 < 0.f ? -INFINITY : e0_);
-              e1_ = ex2_approx(l1 < 0.f ? -INFINITY : e1_);
-              const uint64_t y =
-                  fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])), intra2);
-              float y0, y1;
-              f2unpack(y, y0, y1);
-              // (a select, not the product: scores beyond the row may not be finite)
-              x[t] = pack_bf16(l0 < 0.f ? 0.f : y0 * e0_, l1 < 0.f ? 0.f : y1 * e1_);
+              for (int t = 0; t < 8; ++t)
+                x[t] = pack_bf16x2(
+                    fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
+                          fmul2(f2, w2[t])));
+              if (side == 0) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) x[t] &= cut[q][t];
+              }
+            } else {  // strong decays: each column its own power
+#pragma unroll
+              for (int t = 0; t < 8; ++t) {
+                const float l0 = (float)first + toward * (2 * t), l1 = l0 + toward;
+                x[t] = cut[q][t] &
+                       pack_bf16(__uint_as_float(x[2 * t]) * (role.intra * ex2_approx(l0 * g2)),
+                                 __uint_as_float(x[2 * t + 1]) * (role.intra * ex2_approx(l1 * g2)));
+              }
             }
           }
+          tmem_st8(srow0 + 16 * ch + 8 * q, x);
         }
-        tmem_st8(srow0 + 8 * ch, x);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kPReady + grp]);
+      if (lane == 0) mbar_arrive(&bars[kPReady + (c & 1)]);
     }
   } else if (warp >= L::kWV && warp < L::kWE) {
     // ------------------------------------------------------------ V' = hi + lo
@@ -473,37 +497,48 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const int s = c % kStages;
       const int len = tile_len(c);
       const float w = rev || len == kT ? w_full : role.inc * decay_pow(g, len - 1 - j);
-      const uint64_t w2 = f2pack(w, w), minus2 = f2pack(-1.f, -1.f);
+      // w as two bf16 terms; with x * w_hi rounded to hi, the rest of that
+      // product is a bf16 value and fma gives it exactly: three packed
+      // instructions per two values, off by 2^-17 + 2^-18 at most
+      const uint32_t w_hi = pack_bf16(w, w);
+      const float rest = w - bf16lo(w_hi);
+      const uint32_t w_lo = pack_bf16(rest, rest);
       mbar_wait(&bars[kFull + s], (c / kStages) & 1, abort_flag);
-      if (c > 0) mbar_wait(&bars[kUReady], (c - 1) & 1, abort_flag);
+      // U of the tile that used this buffer before has been formed
+      if (c >= L::kVpBufs) {
+        const int u = c - L::kVpBufs;
+        mbar_wait(&bars[kUReady + (u & 1)], (u / 2) & 1, abort_flag);
+      }
       __syncwarp();
-      const uint32_t src = sb + s * L::kStageBytes + L::kOffV, dst = sb + L::kOffVp;
-#pragma unroll 2
+      const uint32_t src = sb + s * L::kStageBytes + L::kOffV,
+                     dst = sb + L::kOffVp + (c % L::kVpBufs) * 2 * kBlock;
+#pragma unroll 4
       for (int q = 0; q < 8; ++q) {
         const uint32_t off = sw128_offset(j, q);
         uint32_t x[4], hi[4], lo[4];
         ld_shared_v4(src + off, x[0], x[1], x[2], x[3]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint64_t y = fmul2(f2pack(bf16lo(x[i]), bf16hi(x[i])), w2);
-          hi[i] = pack_bf16x2(y);
-          lo[i] = pack_bf16x2(ffma2(f2pack(bf16lo(hi[i]), bf16hi(hi[i])), minus2, y));
+          hi[i] = hmul2_bf16(x[i], w_hi);
+          lo[i] = hfma2_bf16(x[i], w_lo, hfma2_bf16(x[i], w_hi, hneg2_bf16(hi[i])));
         }
         st_shared_v4(dst + off, hi[0], hi[1], hi[2], hi[3]);
         st_shared_v4(dst + kBlock + off, lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kVpReady]);
+      if (lane == 0) mbar_arrive(&bars[kVpReady + c % L::kVpBufs]);
     }
   } else if (!kStateOnly && warp >= L::kWE) {
     // ------------------------------------------------------------ epilogue
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const float f_full = role.inter * decay_pow(g, (rev ? kT - 1 - r : r) + e0);
-    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0;
-    // 32-byte stores where every row's pieces are 32-byte aligned
-    const bool wide = ((uintptr_t)out & 31) == 0 && role.ot % 16 == 0;
+    const int gi = lane & 3;
+    const int left = role.dvo - c0 - 16 * gi;  // columns of this lane's pieces, a multiple of 8
+    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0 + 16 * gi;
+    // 32-byte stores where every piece is whole and 32-byte aligned
+    const bool wide = ((uintptr_t)out & 31) == 0 && role.ot % 16 == 0 && role.dvo % 16 == 0;
     const uint32_t orow = taddr(tmem, wq * 32, kColO1);
     for (int c = 0; c < tiles; ++c) {
       const int64_t base = tile_start(c);
@@ -513,33 +548,59 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       mbar_wait(&bars[kOReady], c & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      const bool live = r < len;
-      __nv_bfloat16 *dst = out + (base + r) * role.ot;
-#pragma unroll 1
-      for (int h = 0; h < 4; ++h, dst += 16) {
+      uint32_t w[32];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
         uint32_t x[16], y[16];
         tmem_ld16(orow + 16 * h, x);
         tmem_ld16(orow + (kColO2 - kColO1) + 16 * h, y);
         tmem_wait_ld();
-        if (h == 3) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kOFree]);
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          x[i] = pack_bf16x2(
+          w[8 * h + i] = pack_bf16x2(
               ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
                     f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
-        const int left = live ? role.dvo - c0 - 16 * h : 0;  // a multiple of 8
-        if (left >= 16 && wide) {
-          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
-                       "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
-                       "r"(x[6]), "r"(x[7])
-                       : "memory");
+      }
+      // O is in registers: its columns are free before the stores
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kOFree]);
+      // 4x4 transpose of 32-byte pieces inside each group of four lanes: a store
+      // instruction then writes eight whole 128-byte rows, not 32 pieces of 32
+      // rows (173 -> 151 us at 64 heads of 128, N = 8192)
+#pragma unroll
+      for (int mm = 2; mm >= 1; mm >>= 1) {
+        const bool hi = (gi & mm) != 0;
+#pragma unroll
+        for (int kx = 0; kx < 2; ++kx) {
+          const int s0 = mm == 2 ? kx : (kx << 1);
+          const int s1 = s0 | mm;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t send = hi ? w[8 * s0 + i] : w[8 * s1 + i];
+            const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, mm);
+            if (hi) w[8 * s0 + i] = recv;
+            else w[8 * s1 + i] = recv;
+          }
+        }
+      }
+      const int first = wq * 32 + (lane & ~3);
+      __nv_bfloat16 *dst = out + (base + first) * role.ot;
+#pragma unroll
+      for (int i = 0; i < 4; ++i, dst += role.ot) {
+        if (first + i >= len) continue;
+        if (wide) {
+          if (left >= 16)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]),
+                         "r"(w[8 * i + 4]), "r"(w[8 * i + 5]), "r"(w[8 * i + 6]),
+                         "r"(w[8 * i + 7])
+                         : "memory");
         } else {
-          if (left > 0) *(uint4 *)dst = make_uint4(x[0], x[1], x[2], x[3]);
-          if (left > 8) *(uint4 *)(dst + 8) = make_uint4(x[4], x[5], x[6], x[7]);
+          if (left > 0) *(uint4 *)dst = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+          if (left > 8)
+            *(uint4 *)(dst + 8) =
+                make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
         }
       }
     }
