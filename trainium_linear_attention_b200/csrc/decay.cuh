@@ -32,13 +32,15 @@ struct DecayView {
 struct DecayRole {
   DecayView a, b, v;
   DecayView out;                 // written; unused by a state pass
-  // state before each segment, in the walk's order: seeds[(bh * segments + o)],
-  // each (da, dvo), or (dvo, da) with seed_transposed; null: zero
-  const float *seeds = nullptr;
-  float *states = nullptr;       // state pass: state of each segment, laid out as seeds
+  const float *init = nullptr;   // null, or the state the walk starts with, per head
+  // What each segment adds to the state, in the walk's order, the last one's
+  // left out: states[bh * segments + o].  Written by a state pass, read by the
+  // output pass, whose segment o starts with
+  //   lambda^(tokens before o) init + sum_{i<o} lambda^(tokens between i and o) states_i.
+  float *states = nullptr;
   float *final_state = nullptr;  // null, or (bh, da, dvo)
   int da = 0, dvo = 0;           // widths of a and b, and of v and out
-  int seed_transposed = 0;
+  int transposed = 0;            // init and states are (dvo, da), else (da, dvo)
   int reverse = 0;
   // factors of the tile's own part of out, of the state's part, and of what
   // enters the state
@@ -71,7 +73,16 @@ __device__ __forceinline__ float decay_pow(float g, int n) {
   return expf(x) * (1.f + lost);
 }
 
-// State of every (head, segment) of each role into role.states.
+// Tokens of the walk's segment o (the ragged one comes last, or first in a
+// reversed walk).
+__host__ __device__ __forceinline__ int segment_tokens(int o, bool reverse, int segments,
+                                                       int64_t seg_len, int64_t n) {
+  const int64_t at = (int64_t)(reverse ? segments - 1 - o : o) * seg_len;
+  return (int)min64(seg_len, n - at);
+}
+
+// States of every (head, segment but the walk's last) of each role into
+// role.states.
 int launch_decay_state_simt(const DecayCall &c, cudaStream_t s);
 // Outputs (and final states) of every role.
 int launch_decay_output_simt(const DecayCall &c, cudaStream_t s);

@@ -1,6 +1,5 @@
 // C entry points of the decayed linear attention: argument checks, the split
-// into segments, and the launches (state of each segment, running states,
-// outputs).
+// into segments, and the launches (state of each segment, outputs).
 #include <math.h>
 
 #include "decay.cuh"
@@ -9,8 +8,7 @@
 namespace la {
 namespace {
 
-// A segment is worth its share of the state pass from this many tokens on.
-constexpr int64_t kMinDecaySegment = 4 * kDecayTile;
+constexpr int64_t kMaxAutoSegments = 64;
 
 int require_device(DeviceInfo *info) {
   const int st = current_device_info(info);
@@ -39,19 +37,49 @@ int fit_segments(int64_t n, int64_t want, int64_t *len) {
   return (int)((n + *len - 1) / *len);
 }
 
-// Segments of each walk: as many as fill the SMs with one wave of CTAs.
-int plan_segments(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, bool backward, int requested,
-                  int sm_count, int64_t *len) {
-  int64_t want = requested;
-  if (want == 0) {
-    const int64_t sq = (d_qk + kDecaySlice - 1) / kDecaySlice;
-    const int64_t sv = (d_v + kDecaySlice - 1) / kDecaySlice;
-    const int64_t ctas = bh * (backward ? 2 * sq + sv : sv);
-    want = ctas > 0 ? sm_count / ctas : 1;
-    const int64_t most = n / kMinDecaySegment;
-    if (want > most) want = most;
+// Segments of each walk: the count with the lowest estimated time.  A split
+// run walks each segment but the last twice (the state pass, then the output)
+// and its later segments start by joining the states before them; an unsplit
+// one leaves SMs idle where there are few heads.
+int plan_segments(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype, bool backward,
+                  int requested, int sm_count, int64_t *len) {
+  if (requested != 0) return fit_segments(n, requested, len);
+  const int64_t sq = (d_qk + kDecaySlice - 1) / kDecaySlice;
+  const int64_t sv = (d_v + kDecaySlice - 1) / kDecaySlice;
+  const int64_t ctas = bh * (backward ? 2 * sq + sv : sv);
+  const int64_t state_ctas = bh * (backward ? 2 * sv : sv);
+  const bool wide = backward ? (d_qk > 64 || d_v > 64) : d_qk > 64;
+  // microseconds per 128 tokens of a CTA's walk (output, state) and per wave
+  // of CTAs (start-up, first loads, drain), measured on a B200; the CUDA-core
+  // kernel holds two CTAs per SM up to 64 columns.  (bf16, d = 64: 64 heads of
+  // 2048 / 4096 / 8192 tokens unsplit 26 / 49 / 89 us, in two segments 29 / 48 /
+  // 82; the gradients of 64 heads of 4096 tokens unsplit 99, in two 104.)
+  const bool simt = dtype == LA_DTYPE_FLOAT32;
+  const double t_out = simt ? (wide ? 36.0 : 24.0) : (wide ? 2.3 : 1.4);
+  const double t_state = simt ? (wide ? 14.0 : 9.0) : (wide ? 1.2 : 0.8);
+  constexpr double kWaveOut = 4.0, kWaveState = 3.0, kSplit = 5.0, kJoin = 0.4;
+  const int64_t slots = sm_count * (simt && !wide ? 2 : 1);
+  const int64_t tiles = (n + kDecayTile - 1) / kDecayTile;
+  int best = 1;
+  int64_t best_len = 0;
+  double best_t = 0.0;
+  for (int64_t want = 1; want <= kMaxAutoSegments && want <= (tiles > 1 ? tiles : 1); ++want) {
+    int64_t l = 0;
+    const int g = fit_segments(n, want, &l);
+    if (g != want) continue;  // the same split as a smaller count
+    const double per_seg = (double)(l / kDecayTile);
+    double t = (double)((ctas * g + slots - 1) / slots) * (kWaveOut + per_seg * t_out);
+    if (g > 1)
+      t += kSplit + kJoin * (g - 1) +
+           (double)((state_ctas * (g - 1) + slots - 1) / slots) * (kWaveState + per_seg * t_state);
+    if (want == 1 || t < best_t) {
+      best = g;
+      best_len = l;
+      best_t = t;
+    }
   }
-  return fit_segments(n, want, len);
+  *len = best_len;
+  return best;
 }
 
 size_t state_bytes(int64_t bh, int segments, int64_t d_qk, int64_t d_v, bool backward) {
@@ -68,32 +96,6 @@ DecayView view(const void *p, const int64_t *strides) {
   return v;
 }
 
-// In place: the state of each segment becomes the state before it,
-//   seed_0 = init,  seed_{o+1} = lambda^len_o seed_o + state_o.
-struct RunningArgs {
-  float *states[2];
-  const float *init[2];
-  int64_t len0[2];  // tokens of the walk's first segment (the ragged one of a reversed walk)
-};
-
-__global__ void decay_running_kernel(const RunningArgs a, const float *log_decay, int64_t heads,
-                                     int segments, int64_t per_head, int64_t seg_len) {
-  const int64_t bh = blockIdx.y;
-  float *s = a.states[blockIdx.z] + bh * segments * per_head;
-  const float *init = a.init[blockIdx.z];
-  const float g = log_decay[bh % heads];
-  const float keep0 = decay_pow(g, (int)a.len0[blockIdx.z]), keep = decay_pow(g, (int)seg_len);
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < per_head;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    float run = init ? init[bh * per_head + i] : 0.f;
-    for (int o = 0; o < segments; ++o) {
-      const float x = s[o * per_head + i];
-      s[o * per_head + i] = run;
-      run = fmaf(o == 0 ? keep0 : keep, run, x);
-    }
-  }
-}
-
 // bf16 whose rows TMA can address runs on tensor cores.
 bool use_tensor_cores(const DecayCall &c) {
   if (c.dtype != LA_DTYPE_BFLOAT16 || c.n == 0) return false;
@@ -106,28 +108,14 @@ bool use_tensor_cores(const DecayCall &c) {
   return true;
 }
 
-int run_decay(DecayCall &call, const DecayRole *state_roles, int n_state_roles,
-              const float *const *inits, int64_t d_qk, int64_t d_v, cudaStream_t s) {
+int run_decay(const DecayCall &call, const DecayRole *state_roles, int n_state_roles,
+              cudaStream_t s) {
   const bool tc = use_tensor_cores(call);
   if (call.segments > 1) {
     DecayCall pass = call;
     pass.roles = n_state_roles;
-    RunningArgs run{};
-    for (int r = 0; r < n_state_roles; ++r) {
-      pass.role[r] = state_roles[r];
-      run.states[r] = state_roles[r].states;
-      run.init[r] = inits[r];
-      run.len0[r] = state_roles[r].reverse ? call.n - (call.segments - 1) * call.seg_len
-                                           : call.seg_len;
-    }
-    int st = tc ? launch_decay_state_tc(pass, s) : launch_decay_state_simt(pass, s);
-    if (st != LA_OK) return st;
-    const int64_t per_head = d_qk * d_v;
-    const dim3 grid((unsigned)((per_head + 255) / 256), (unsigned)(call.batch * call.heads),
-                    (unsigned)n_state_roles);
-    decay_running_kernel<<<grid, 256, 0, s>>>(run, call.log_decay, call.heads, call.segments,
-                                              per_head, call.seg_len);
-    st = check_launch();
+    for (int r = 0; r < n_state_roles; ++r) pass.role[r] = state_roles[r];
+    const int st = tc ? launch_decay_state_tc(pass, s) : launch_decay_state_simt(pass, s);
     if (st != LA_OK) return st;
   }
   return tc ? launch_decay_output_tc(call, s) : launch_decay_output_simt(call, s);
@@ -157,7 +145,7 @@ int la_decay_plan(int64_t batch, int64_t heads, int64_t seq_len, int64_t d_qk, i
   info.sm_count = 1;
   if (segments_requested == 0 && (st = require_device(&info)) != LA_OK) return st;
   int64_t len = 0;
-  *segments_out = plan_segments(batch * heads, seq_len, d_qk, d_v, backward != 0,
+  *segments_out = plan_segments(batch * heads, seq_len, d_qk, d_v, dtype, backward != 0,
                                 segments_requested, info.sm_count, &len);
   *workspace_bytes_out = state_bytes(batch * heads, *segments_out, d_qk, d_v, backward != 0);
   return LA_OK;
@@ -181,7 +169,7 @@ int la_decay_chunked_fwd(const void *q, const int64_t *q_strides, const void *k,
   DeviceInfo info;
   if ((st = require_device(&info)) != LA_OK) return st;
   DecayCall c;
-  c.segments = plan_segments(bh, seq_len, d_qk, d_v, false, segments, info.sm_count, &c.seg_len);
+  c.segments = plan_segments(bh, seq_len, d_qk, d_v, dtype, false, segments, info.sm_count, &c.seg_len);
   const size_t need = state_bytes(bh, c.segments, d_qk, d_v, false);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
     return LA_ERR_WORKSPACE;
@@ -198,12 +186,11 @@ int la_decay_chunked_fwd(const void *q, const int64_t *q_strides, const void *k,
   f.out = view(out, out_strides);
   f.da = (int)d_qk;
   f.dvo = (int)d_v;
-  f.seeds = c.segments > 1 ? (const float *)workspace : init_state;
+  f.init = init_state;
+  f.states = (float *)workspace;
   f.final_state = final_state;
   f.intra = f.inter = scale;
-  DecayRole pass = f;
-  pass.states = (float *)workspace;
-  return run_decay(c, &pass, 1, &init_state, d_qk, d_v, (cudaStream_t)stream);
+  return run_decay(c, &f, 1, (cudaStream_t)stream);
 }
 
 int la_decay_chunked_bwd(const void *q, const int64_t *q_strides, const void *k,
@@ -229,13 +216,12 @@ int la_decay_chunked_bwd(const void *q, const int64_t *q_strides, const void *k,
   DeviceInfo info;
   if ((st = require_device(&info)) != LA_OK) return st;
   DecayCall c;
-  c.segments = plan_segments(bh, seq_len, d_qk, d_v, true, segments, info.sm_count, &c.seg_len);
+  c.segments = plan_segments(bh, seq_len, d_qk, d_v, dtype, true, segments, info.sm_count, &c.seg_len);
   const size_t need = state_bytes(bh, c.segments, d_qk, d_v, true);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
     return LA_ERR_WORKSPACE;
-  float *before = (float *)workspace;  // states before each segment, first token first
-  float *after = before + bh * c.segments * d_qk * d_v;  // and of the reversed walk
-  const bool split = c.segments > 1;
+  float *ahead = (float *)workspace;  // the segments' states, first token first
+  float *back = ahead + (c.segments > 1 ? bh * c.segments * d_qk * d_v : 0);  // last token first
   c.roles = 3;
   c.log_decay = log_decay;
   c.batch = batch;
@@ -247,28 +233,26 @@ int la_decay_chunked_bwd(const void *q, const int64_t *q_strides, const void *k,
   DecayRole &a = c.role[0], &b = c.role[1], &d = c.role[2];
   a.a = G, a.b = V, a.v = K, a.out = view(dq, dq_strides);
   a.da = (int)d_v, a.dvo = (int)d_qk;
-  a.seeds = split ? before : init_state;
-  a.seed_transposed = 1;
+  a.init = init_state, a.states = ahead;
+  a.transposed = 1;
   a.intra = a.inter = scale;
   b.a = K, b.b = Q, b.v = G, b.out = view(dv, dv_strides);
   b.da = (int)d_qk, b.dvo = (int)d_v;
-  b.seeds = split ? after : d_final_state;
+  b.init = d_final_state, b.states = back;
   b.final_state = d_init_state;
   b.reverse = 1;
   b.intra = b.inc = scale;
   d.a = V, d.b = G, d.v = Q, d.out = view(dk, dk_strides);
   d.da = (int)d_v, d.dvo = (int)d_qk;
-  d.seeds = split ? after : d_final_state;
-  d.seed_transposed = 1;
+  d.init = d_final_state, d.states = back;
+  d.transposed = 1;
   d.reverse = 1;
   d.intra = d.inc = scale;
   DecayRole pass[2];
   pass[0].b = K, pass[0].v = V, pass[0].da = (int)d_qk, pass[0].dvo = (int)d_v;
-  pass[0].states = before;
+  pass[0].states = ahead;
   pass[1] = b;
-  pass[1].states = after;
-  const float *inits[2] = {init_state, d_final_state};
-  return run_decay(c, pass, 2, inits, d_qk, d_v, (cudaStream_t)stream);
+  return run_decay(c, pass, 2, (cudaStream_t)stream);
 }
 
 int la_decay_step(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides,

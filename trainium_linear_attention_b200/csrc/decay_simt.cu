@@ -103,18 +103,27 @@ decay_simt_kernel(const __grid_constant__ DecayCall call, int slices) {
   const bool vo = !kStateOnly && vec_ok<T>(role.out, role.dvo);
 
   // state rows ty * kR + r, columns c0 + tx * 4 + x
-  float st[kR][4];
-  const int64_t state_at = (bh * call.segments + order) * (int64_t)role.da * role.dvo;
+  float st[kR][4] = {};
+  const int64_t per_head = (int64_t)role.da * role.dvo;
+  const int64_t state_at = (bh * call.segments + order) * per_head;
+  if (!kStateOnly) {
+    auto add = [&](const float *src, float keep) {
 #pragma unroll
-  for (int r = 0; r < kR; ++r)
+      for (int r = 0; r < kR; ++r)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int row = ty * kR + r, col = c0 + tx * 4 + x;
-      st[r][x] = 0.f;
-      if (!kStateOnly && role.seeds && row < role.da && col < role.dvo)
-        st[r][x] = role.seeds[state_at + (role.seed_transposed ? (int64_t)col * role.da + row
-                                                               : (int64_t)row * role.dvo + col)];
-    }
+        for (int x = 0; x < 4; ++x) {
+          const int row = ty * kR + r, col = c0 + tx * 4 + x;
+          if (row < role.da && col < role.dvo)
+            st[r][x] = fmaf(keep, st[r][x],
+                            src[role.transposed ? (int64_t)col * role.da + row
+                                                : (int64_t)row * role.dvo + col]);
+        }
+    };
+    if (role.init) add(role.init + bh * per_head, 0.f);
+    for (int o = 0; o < order; ++o)
+      add(role.states + (bh * call.segments + o) * per_head,
+          decay_pow(g, segment_tokens(o, rev, call.segments, call.seg_len, call.n)));
+  }
 
   for (int c = 0; c < tiles; ++c) {
     const int64_t base = t0 + (int64_t)(rev ? tiles - 1 - c : c) * kC;
@@ -224,8 +233,7 @@ decay_simt_kernel(const __grid_constant__ DecayCall call, int slices) {
   }
   float *dst = nullptr;
   if (kStateOnly) dst = role.states + state_at;
-  else if (role.final_state && order == call.segments - 1)
-    dst = role.final_state + bh * (int64_t)role.da * role.dvo;
+  else if (role.final_state && order == call.segments - 1) dst = role.final_state + bh * per_head;
   if (dst) {
 #pragma unroll
     for (int r = 0; r < kR; ++r)
@@ -242,7 +250,7 @@ int launch_t(const DecayCall &c, int slices, cudaStream_t s) {
   auto kernel = decay_simt_kernel<T, DK, kStateOnly>;
   const int bytes = SimtLayout<DK>::kFloats * 4;
   if (allow_dynamic_smem((const void *)kernel, bytes) != LA_OK) return LA_ERR_CUDA;
-  const dim3 grid((unsigned)(slices * c.segments), (unsigned)(c.batch * c.heads), c.roles);
+  const dim3 grid((unsigned)(slices * (kStateOnly ? c.segments - 1 : c.segments)), (unsigned)(c.batch * c.heads), c.roles);
   kernel<<<grid, kThreads, bytes, s>>>(c, slices);
   return check_launch();
 }

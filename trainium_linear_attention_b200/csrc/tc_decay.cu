@@ -50,6 +50,8 @@ constexpr uint32_t kColU = 256;     // hi 64, lo 64
 constexpr uint32_t kColO1 = 384;
 constexpr uint32_t kColO2 = 448;
 
+constexpr int kJoinPitch = 65;  // floats per row of a joined state: rows in other banks
+
 template <int DK, bool kStateOnly>
 struct TcLayout {
   static constexpr int kKBlocks = DK / 64;
@@ -66,7 +68,7 @@ struct TcLayout {
   static constexpr uint32_t kOffV = kOffB + kKBlocks * kBlock;
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
-  static constexpr int kVpBufs = DK == 64 ? 2 : 1;
+  static constexpr int kVpBufs = DK == 64 || kStateOnly ? 2 : 1;
   static constexpr uint32_t kFixed =
       kVpBufs * 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
   static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
@@ -76,6 +78,8 @@ struct TcLayout {
   static constexpr uint32_t kOffSnap = kOffVp + kVpBufs * 2 * kBlock;  // two bf16 copies of S
   static constexpr uint32_t kOffBar = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
+  static_assert(kStateOnly || (int)(DK * kJoinPitch * 4) <= kVpBufs * 2 * kBlock + 2 * (int)kSnapBytes,
+                "joined state");
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kSmem > 114 * 1024, "one CTA per SM (all TMEM columns)");
 };
@@ -101,9 +105,9 @@ struct TcRole {
   int a, b, v;  // which tensor map
   __nv_bfloat16 *out;
   int64_t ob, oh, ot;
-  const float *seeds;
+  const float *init;
   float *states, *final_state;
-  int da, dvo, seed_transposed, reverse;
+  int da, dvo, transposed, reverse;
   float intra, inter, inc;
 };
 
@@ -114,6 +118,7 @@ struct TcParams {
   int *err;
   int64_t heads, n, seg_len;
   int roles, slices, segments;
+  int orders;  // segments that this launch walks: all, or all but the last
 };
 
 __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *map, uint64_t *bar,
@@ -165,8 +170,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   id /= p.roles;
   const int c0 = (int)(id % p.slices) * kDecaySlice;
   id /= p.slices;
-  const int order = (int)(id % p.segments);
-  const int64_t bh = id / p.segments;
+  const int order = (int)(id % p.orders);
+  const int64_t bh = id / p.orders;
   if (c0 >= role.dvo) return;
   const int ib = (int)(bh / p.heads), ih = (int)(bh % p.heads);
   const bool rev = role.reverse != 0;
@@ -200,6 +205,51 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
+  // The state that a later segment starts with, joined by the whole CTA in the
+  // space of V' and the copies of S:
+  //   lambda^(tokens so far) init + sum_o lambda^(tokens from o's end on) states_o
+  float *joined = (float *)(smem + L::kOffVp);
+  if (!kStateOnly && order > 0) {
+    constexpr int kEach = (DK * 64 + L::kThreads - 1) / L::kThreads;
+    const int64_t per_head = (int64_t)role.da * role.dvo;
+    // neighbouring threads read neighbouring addresses: columns first, or rows
+    // where the states are stored transposed
+    int64_t at[kEach];
+    float sum[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * L::kThreads;
+      const int row = role.transposed ? i % DK : i / 64, col = role.transposed ? i / DK : i % 64;
+      const bool in = i < DK * 64 && row < role.da && c0 + col < role.dvo;
+      at[e] = !in              ? -1
+              : role.transposed ? (int64_t)(c0 + col) * role.da + row
+                                : (int64_t)row * role.dvo + c0 + col;
+      sum[e] = 0.f;
+    }
+    int after = 0;  // tokens from the end of segment o to this one's start
+    grid_dependency_wait();  // the state pass has written its states
+#pragma unroll 2
+    for (int o = order - 1; o >= 0; --o) {
+      const float keep = decay_pow(g, after);
+      const float *src = role.states + (bh * p.segments + o) * per_head;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (at[e] >= 0) sum[e] = fmaf(keep, __ldcg(src + at[e]), sum[e]);
+      after += segment_tokens(o, rev, p.segments, p.seg_len, p.n);
+    }
+    if (role.init) {
+      const float keep = decay_pow(g, after);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (at[e] >= 0) sum[e] = fmaf(keep, role.init[bh * per_head + at[e]], sum[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * L::kThreads;
+      const int row = role.transposed ? i % DK : i / 64, col = role.transposed ? i / DK : i % 64;
+      if (i < DK * 64) joined[row * kJoinPitch + col] = sum[e];
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -339,22 +389,25 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const int half = DK == 64 ? wq >> 1 : (warp - L::kWState) >> 2;
     const int col = c0 + half * 32;
     float st[32];
-    const int64_t at = (bh * p.segments + order) * (int64_t)role.da * role.dvo;
+    const int64_t per_head = (int64_t)role.da * role.dvo;
     const bool mine = row < role.da;
     const int cols = mine ? min(32, role.dvo - col) : 0;  // may be negative
-    {
-      const float *src = nullptr;
-      int64_t step = 1;
-      if (!kStateOnly && role.seeds && mine) {
-        src = role.seeds + at + (role.seed_transposed ? (int64_t)col * role.da + row
-                                                      : (int64_t)row * role.dvo + col);
-        if (role.seed_transposed) step = role.da;
-      }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        st[i] = src && i < cols ? *src : 0.f;
-        src += src ? step : 0;
-      }
+    for (int i = 0; i < 32; ++i) st[i] = 0.f;
+    if constexpr (kStateOnly) {
+      grid_dependents_launch();
+    } else if (order > 0) {
+      const float *src = joined + row * kJoinPitch + half * 32;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) st[i] = src[i];
+      named_barrier_arrive(1, L::kStateWarps * 32 + 128);  // V' may take the space
+    } else if (role.init) {
+      const int64_t step = role.transposed ? role.da : 1;
+      const float *src = role.init + bh * per_head + (role.transposed ? (int64_t)col * role.da + row
+                                                                      : (int64_t)row * role.dvo + col);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < cols) st[i] = src[i * step];
     }
     const uint32_t urow = taddr(tmem, wq * 32, kColU + half * 32);
     auto write_copy = [&](int b) {
@@ -403,8 +456,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       }
     }
     if (want_final) {
-      float *dst = (kStateOnly ? role.states + at
-                               : role.final_state + bh * (int64_t)role.da * role.dvo) +
+      float *dst = (kStateOnly ? role.states + (bh * p.segments + order) * per_head
+                               : role.final_state + bh * per_head) +
                    (int64_t)row * role.dvo + col;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -493,6 +546,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const int j = (warp - L::kWV) * 32 + lane;  // token of the tile
     // place in a full tile: forward len - 1 - j, reversed (len - 1 - j mirrored) j + 1
     const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
+    if (!kStateOnly && order > 0) named_barrier_sync(1, L::kStateWarps * 32 + 128);
     for (int c = 0; c < updates; ++c) {
       const int s = c % kStages;
       const int len = tile_len(c);
@@ -640,7 +694,19 @@ int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
   using L = TcLayout<DK, kStateOnly>;
   auto kernel = decay_tc_kernel<DK, kStateOnly>;
   if (allow_dynamic_smem((const void *)kernel, (int)L::kSmem) != LA_OK) return LA_ERR_CUDA;
-  kernel<<<(unsigned)grid, L::kThreads, L::kSmem, s>>>(p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(L::kThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = s;
+  // behind a state pass of its own call, whose CTAs let it start early: it waits
+  // where it reads the states
+  cudaLaunchAttribute pdl;
+  pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &pdl;
+  cfg.numAttrs = !kStateOnly && p.segments > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch();
 }
 
@@ -676,9 +742,9 @@ int launch(const DecayCall &c, cudaStream_t s) {
     if (t.a < 0 || t.b < 0 || t.v < 0) return LA_ERR_CUDA;
     t.out = (__nv_bfloat16 *)f.out.p;
     t.ob = f.out.sb, t.oh = f.out.sh, t.ot = f.out.st;
-    t.seeds = f.seeds, t.states = f.states, t.final_state = f.final_state;
+    t.init = f.init, t.states = f.states, t.final_state = f.final_state;
     t.da = f.da, t.dvo = f.dvo;
-    t.seed_transposed = f.seed_transposed, t.reverse = f.reverse;
+    t.transposed = f.transposed, t.reverse = f.reverse;
     t.intra = f.intra, t.inter = f.inter, t.inc = f.inc;
     if (f.da > da) da = f.da;
     const int n = (f.dvo + kDecaySlice - 1) / kDecaySlice;
@@ -687,7 +753,8 @@ int launch(const DecayCall &c, cudaStream_t s) {
   p.log_decay = c.log_decay;
   p.heads = c.heads, p.n = c.n, p.seg_len = c.seg_len;
   p.roles = c.roles, p.slices = slices, p.segments = c.segments;
-  const int64_t grid = c.batch * c.heads * c.segments * slices * c.roles;
+  p.orders = kStateOnly ? c.segments - 1 : c.segments;
+  const int64_t grid = c.batch * c.heads * p.orders * slices * c.roles;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
   return da <= 64 ? launch_t<64, kStateOnly>(p, grid, s) : launch_t<128, kStateOnly>(p, grid, s);
 }

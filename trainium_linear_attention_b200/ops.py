@@ -230,43 +230,54 @@ def based_layer(q, k, v, window_size: int = 64, eps: float = 1e-6, segments: int
     return out
 
 
-# ---- linear attention with a decay for each head ---------------------------------
+# ---- plans ---------------------------------------------------------------------
+# The checks of a call, its strides as the C entry points take them and its
+# workspace depend on shapes, strides, types and devices alone.  They are worked
+# out at the first call of a signature and kept under it, so that a decoding
+# step or a small norm does not spend more time here than on the GPU.  Nothing
+# is kept by a tensor's address or contents.
 _Strides = ctypes.c_int64 * 3
+_MAX_PLANS = 4096
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _heads_view(t: torch.Tensor):
-    """``t`` (b, h, t, d) as the kernels read it -- a dense last dimension and,
-    for bf16, 16-byte rows where the width allows them -- and its strides.  A
-    copy is made only where the strides rule that out (or overlap)."""
+def _sig(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _keep(plans: dict, key, plan):
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
+# ---- linear attention with a decay for each head ---------------------------------
+def _heads_strides(t: torch.Tensor):
+    """Strides of ``t`` (b, h, t, d) as the kernels read it in place -- a dense
+    last dimension, and for bf16 rows of whole 16-byte packs where the width
+    allows them -- or None where they rule that out (or overlap)."""
     b, h, n, d = t.shape
     sb, sh, st, sd = t.stride()
     ok = ((sd == 1 or d == 1) and (sb > 0 or b == 1) and (sh > 0 or h == 1)
           and (st >= d or n == 1))
     if ok and d % 8 == 0 and t.dtype == torch.bfloat16:
-        ok = (t.data_ptr() % 16 == 0 and (sb % 8 == 0 or b == 1) and (sh % 8 == 0 or h == 1)
-              and (st % 8 == 0 or n == 1))
+        ok = (sb % 8 == 0 or b == 1) and (sh % 8 == 0 or h == 1) and (st % 8 == 0 or n == 1)
     if not ok:
-        t = t.contiguous()
-        if t.data_ptr() % 16:  # a contiguous view at an odd offset
-            t = t.clone()
-        sb, sh, st, _ = t.stride()
+        return None
     # a dimension of one entry has no stride of its own
-    return t, _Strides(sb if b > 1 else h * n * d, sh if h > 1 else n * d, st if n > 1 else d)
+    return _Strides(sb if b > 1 else h * n * d, sh if h > 1 else n * d, st if n > 1 else d)
 
 
-def _heads_like(t: torch.Tensor, d: int) -> torch.Tensor:
-    """An empty (b, h, t, d) tensor laid out as ``t``: tokens before heads where
-    ``t`` is a transposed projection, else contiguous."""
-    b, h, n, _ = t.shape
-    if h > 1 and n > 1 and t.stride(1) < t.stride(2):
-        return torch.empty((b, n, h, d), dtype=t.dtype, device=t.device).transpose(1, 2)
-    return torch.empty((b, h, n, d), dtype=t.dtype, device=t.device)
+def _tokens_first(t: torch.Tensor) -> bool:
+    """Whether ``t`` (b, h, t, d) lies as (b, t, h, d): a transposed projection."""
+    return t.shape[1] > 1 and t.shape[2] > 1 and t.stride(1) < t.stride(2)
 
 
-def _check_decay(q, k, v, log_decay):
-    code = _check_qkv(q, k, v)
-    _check_log_decay(log_decay, q.shape[1], q.device)
-    return code
+def _empty_heads(b, h, n, d, dtype, device, tokens_first):
+    if tokens_first:
+        return torch.empty((b, n, h, d), dtype=dtype, device=device).transpose(1, 2)
+    return torch.empty((b, h, n, d), dtype=dtype, device=device)
 
 
 def _check_log_decay(log_decay, heads, device):
@@ -286,43 +297,112 @@ def _check_state(state, shape, device, name):
         raise ValueError(f"{name} must be float32 {shape} on {device}")
 
 
-def _default_scale(scale, d_qk: int) -> float:
-    return 1.0 / math.sqrt(d_qk) if scale is None else float(scale)
+class _DecayPlan:
+    """One signature of the decayed linear attention: sizes, strides, workspace."""
+
+    __slots__ = ("index", "device", "dtype", "sizes", "scale", "pack", "copy", "strides",
+                 "outs", "out_strides", "state_shape", "ws_bytes")
+
+    def __init__(self, q, k, v, log_decay, states, grad, segments):
+        code = _check_qkv(q, k, v)
+        b, h, t, d = q.shape
+        dv = v.shape[-1]
+        _check_log_decay(log_decay, h, q.device)
+        for name, s in states:
+            if s is not None:
+                _check_state(s, (b, h, d, dv), q.device, name)
+        if grad is not None and (not isinstance(grad, torch.Tensor) or grad.shape != v.shape
+                                 or grad.dtype != v.dtype or grad.device != v.device):
+            raise ValueError(f"d_out must be {v.dtype} {tuple(v.shape)} on {v.device}")
+        self.device, self.dtype = q.device, q.dtype
+        self.index = q.device.index
+        self.sizes = (b, h, t, d, dv, code)
+        self.scale = 1.0 / math.sqrt(d)
+        self.state_shape = (b, h, d, dv)
+        read = (q, k, v) if grad is None else (q, k, v, grad)
+        # bf16 rows of whole 16-byte packs have to start at 16 bytes
+        self.pack = tuple(q.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0 for x in read)
+        self.strides = tuple(_heads_strides(x) for x in read)
+        self.copy = any(s is None for s in self.strides)
+        written = (v,) if grad is None else (q, k, v)
+        self.outs = tuple((b, h, t, x.shape[-1], x.dtype, x.device, _tokens_first(x))
+                          for x in written)
+        self.out_strides = tuple(
+            _Strides(h * t * w, w if first else t * w, h * w if first else w)
+            for _, _, _, w, _, _, first in self.outs)
+        n, ws = ctypes.c_int(0), ctypes.c_size_t(0)
+        with _on_device(q.device):
+            st = N.lib().la_decay_plan(*self.sizes, int(grad is not None), segments,
+                                       ctypes.byref(n), ctypes.byref(ws))
+        N.check(st, "la_decay_plan")
+        self.ws_bytes = ws.value
 
 
-@functools.lru_cache(maxsize=1024)
-def _decay_plan(batch, heads, seq_len, d_qk, d_v, code, backward, segments, device_index):
-    g = ctypes.c_int(0)
-    ws = ctypes.c_size_t(0)
-    st = N.lib().la_decay_plan(batch, heads, seq_len, d_qk, d_v, code, int(backward), segments,
-                               ctypes.byref(g), ctypes.byref(ws))
-    N.check(st, "la_decay_plan")
-    return g.value, ws.value
+_decay_plans: dict = {}
+
+
+def _decay_plan(q, k, v, log_decay, initial_state, d_state, grad, segments) -> _DecayPlan:
+    try:
+        key = (_sig(q), _sig(k), _sig(v), _sig(log_decay), _sig(initial_state), _sig(d_state),
+               _sig(grad), segments)
+        plan = _decay_plans.get(key)
+        if plan is not None and not log_decay.requires_grad:
+            return plan
+    except AttributeError:  # not tensors: the checks say which
+        key = None
+    return _keep(_decay_plans, key, _DecayPlan(
+        q, k, v, log_decay, (("initial_state", initial_state), ("d_state", d_state)), grad,
+        segments))
+
+
+def _in_place(x: torch.Tensor, strides, pack: bool) -> torch.Tensor:
+    """``x``, or a copy of it where its layout or address cannot be read in place."""
+    if strides is not None and not (pack and x.data_ptr() & 15):
+        return x
+    x = x.contiguous()
+    return x.clone() if pack and x.data_ptr() & 15 else x  # (a view at an odd offset)
+
+
+def _readable(plan, tensors):
+    """The inputs as the kernels can read them, or None if they already are."""
+    if not plan.copy and not any(p and x.data_ptr() & 15 for p, x in zip(plan.pack, tensors)):
+        return None
+    return [_in_place(x, s, p) for x, s, p in zip(tensors, plan.strides, plan.pack)]
 
 
 def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_state: bool = False,
                     segments: int = 0):
     """Forward pass of the decayed linear attention (no autograd): the output,
     or (output, final state fp32 (b, h, d_qk, d_v))."""
-    code = _check_decay(q, k, v, log_decay)
-    b, h, t, d = q.shape
-    dv = v.shape[-1]
-    if initial_state is not None:
-        _check_state(initial_state, (b, h, d, dv), q.device, "initial_state")
+    plan = _decay_plan(q, k, v, log_decay, initial_state, None, None, segments)
+    again = _readable(plan, (q, k, v))
+    if again is not None:
+        out = decay_attention(*again, log_decay, scale, initial_state, return_state, segments)
+        if _tokens_first(v) == _tokens_first(again[2]):
+            return out
+        y = _empty_heads(*plan.outs[0])
+        y.copy_(out[0] if return_state else out)
+        return (y, out[1]) if return_state else y
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return decay_attention(q, k, v, log_decay, scale, initial_state, return_state,
+                                   segments)
+    out = _empty_heads(*plan.outs[0])
+    final = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
+             if return_state else None)
+    if not log_decay.is_contiguous():
+        log_decay = log_decay.contiguous()
+    if initial_state is not None and not initial_state.is_contiguous():
         initial_state = initial_state.contiguous()
-    out = _heads_like(v, dv)
-    final = torch.empty((b, h, d, dv), dtype=torch.float32, device=q.device) if return_state else None
-    log_decay = log_decay.contiguous()
-    (q, qs), (k, ks), (v, vs), (_, os_) = (_heads_view(x) for x in (q, k, v, out))
-    with _on_device(q.device):
-        _, ws_bytes = _decay_plan(b, h, t, d, dv, code, False, int(segments),
-                                  torch.cuda.current_device())
-        workspace = _workspace(ws_bytes, q.device)
-        st = N.lib().la_decay_chunked_fwd(
-            _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(out), os_, _ptr(log_decay), b, h, t, d, dv,
-            code, _default_scale(scale, d), _ptr(initial_state), _ptr(final), _ptr(workspace),
-            ws_bytes, int(segments), _stream_ptr(q.device))
-    N.check(st, "la_decay_chunked_fwd")
+    workspace = _workspace(plan.ws_bytes, plan.device)
+    qs, ks, vs = plan.strides
+    st = N.lib().la_decay_chunked_fwd(
+        q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), plan.out_strides[0],
+        log_decay.data_ptr(), *plan.sizes, plan.scale if scale is None else float(scale),
+        _ptr(initial_state), _ptr(final), _ptr(workspace), plan.ws_bytes, segments,
+        _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_decay_chunked_fwd")
     return (out, final) if return_state else out
 
 
@@ -330,65 +410,96 @@ def decay_attention_backward(q, k, v, log_decay, d_out, scale=None, initial_stat
                              d_state=None, want_d_initial: bool = False, segments: int = 0):
     """Gradients (dq, dk, dv, d_initial_state or None) of ``decay_attention``
     for the gradients of its output and (``d_state``) of its final state."""
-    code = _check_decay(q, k, v, log_decay)
-    b, h, t, d = q.shape
-    dv = v.shape[-1]
-    if not isinstance(d_out, torch.Tensor) or d_out.shape != v.shape or d_out.dtype != v.dtype:
-        raise ValueError(f"d_out must be {v.dtype} {tuple(v.shape)}")
-    for name, s in (("initial_state", initial_state), ("d_state", d_state)):
-        if s is not None:
-            _check_state(s, (b, h, d, dv), q.device, name)
+    plan = _decay_plan(q, k, v, log_decay, initial_state, d_state, d_out, segments)
+    again = _readable(plan, (q, k, v, d_out))
+    if again is not None:
+        q, k, v, d_out = again
+        return decay_attention_backward(q, k, v, log_decay, d_out, scale, initial_state, d_state,
+                                        want_d_initial, segments)
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return decay_attention_backward(q, k, v, log_decay, d_out, scale, initial_state,
+                                            d_state, want_d_initial, segments)
+    gq, gk, gv = (_empty_heads(*o) for o in plan.outs)
+    g0 = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
+          if want_d_initial else None)
+    log_decay = log_decay.contiguous()
     initial_state = None if initial_state is None else initial_state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
-    gq, gk, gv = _heads_like(q, d), _heads_like(k, d), _heads_like(v, dv)
-    g0 = (torch.empty((b, h, d, dv), dtype=torch.float32, device=q.device) if want_d_initial
-          else None)
-    log_decay = log_decay.contiguous()
-    (q, qs), (k, ks), (v, vs), (d_out, ds) = (_heads_view(x) for x in (q, k, v, d_out))
-    (_, gqs), (_, gks), (_, gvs) = (_heads_view(x) for x in (gq, gk, gv))
-    with _on_device(q.device):
-        _, ws_bytes = _decay_plan(b, h, t, d, dv, code, True, int(segments),
-                                  torch.cuda.current_device())
-        workspace = _workspace(ws_bytes, q.device)
-        st = N.lib().la_decay_chunked_bwd(
-            _ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(d_out), ds, _ptr(gq), gqs, _ptr(gk), gks,
-            _ptr(gv), gvs, _ptr(log_decay), b, h, t, d, dv, code, _default_scale(scale, d),
-            _ptr(initial_state), _ptr(d_state), _ptr(g0), _ptr(workspace), ws_bytes,
-            int(segments), _stream_ptr(q.device))
-    N.check(st, "la_decay_chunked_bwd")
+    workspace = _workspace(plan.ws_bytes, plan.device)
+    qs, ks, vs, ds = plan.strides
+    gqs, gks, gvs = plan.out_strides
+    st = N.lib().la_decay_chunked_bwd(
+        q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, d_out.data_ptr(), ds, gq.data_ptr(),
+        gqs, gk.data_ptr(), gks, gv.data_ptr(), gvs, log_decay.data_ptr(), *plan.sizes,
+        plan.scale if scale is None else float(scale), _ptr(initial_state), _ptr(d_state),
+        _ptr(g0), _ptr(workspace), plan.ws_bytes, segments, _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_decay_chunked_bwd")
     return gq, gk, gv, g0
+
+
+class _StepPlan:
+    """One signature of the single-token form."""
+
+    __slots__ = ("index", "device", "dtype", "sizes", "scale", "out", "strides", "copy")
+
+    def __init__(self, q, k, v, log_decay, state):
+        for name, x in (("q", q), ("k", k), ("v", v)):
+            if not isinstance(x, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if x.dim() != 3:
+                raise ValueError(f"{name} must be (batch, heads, dim), got shape {tuple(x.shape)}")
+        code = _check_qkv(q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
+        b, h, d = q.shape
+        dv = v.shape[-1]
+        _check_log_decay(log_decay, h, q.device)
+        _check_state(state, (b, h, d, dv), q.device, "state")
+        sb, sh, sr, sc = state.stride()
+        if ((sc != 1 and dv > 1) or (sr != dv and d > 1) or (sh < d * dv and h > 1)
+                or (sb < d * dv and b > 1)):
+            raise ValueError("state needs dense (d_qk, d_v) entries that do not overlap")
+        if b > 1 and h > 1 and not (sb >= sh * (h - 1) + d * dv or sh >= sb * (b - 1) + d * dv):
+            raise ValueError("the states of different sequences overlap")
+        self.device, self.dtype, self.index = q.device, q.dtype, q.device.index
+        self.sizes = (b, h, d, dv, code)
+        self.scale = 1.0 / math.sqrt(d)
+        self.out = (b, h, dv)
+        self.copy = any(x.stride(2) != 1 and x.shape[2] > 1 for x in (q, k, v))
+        self.strides = tuple(_Strides(*x.stride()) for x in (q, k, v)) + (_Strides(sb, sh),)
+
+
+_step_plans: dict = {}
 
 
 def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
     """One token of every sequence: q, k (b, h, d_qk), v (b, h, d_v); ``state``
     fp32 (b, h, d_qk, d_v) is updated in place.  Returns (b, h, d_v)."""
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(x, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if x.dim() != 3:
-            raise ValueError(f"{name} must be (batch, heads, dim), got shape {tuple(x.shape)}")
-    code = _check_qkv(q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2))
-    b, h, d = q.shape
-    dv = v.shape[-1]
-    _check_log_decay(log_decay, h, q.device)
-    _check_state(state, (b, h, d, dv), q.device, "state")
+    try:
+        key = (_sig(q), _sig(k), _sig(v), _sig(log_decay), _sig(state))
+        plan = None if log_decay.requires_grad else _step_plans.get(key)
+    except AttributeError:  # not tensors: the checks say which
+        key = plan = None
+    if plan is None:
+        plan = _keep(_step_plans, key, _StepPlan(q, k, v, log_decay, state))
     if state.requires_grad:
         raise ValueError("state is updated in place: it may not require a gradient")
-    sb, sh, sr, sc = state.stride()
-    if ((sc != 1 and dv > 1) or (sr != dv and d > 1) or (sh < d * dv and h > 1)
-            or (sb < d * dv and b > 1)):
-        raise ValueError("state needs dense (d_qk, d_v) entries that do not overlap")
-    if b > 1 and h > 1 and not (sb >= sh * (h - 1) + d * dv or sh >= sb * (b - 1) + d * dv):
-        raise ValueError("the states of different sequences overlap")
-    log_decay = log_decay.contiguous()
-    q, k, v = (x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous() for x in (q, k, v))
-    out = torch.empty((b, h, dv), dtype=q.dtype, device=q.device)
-    with _on_device(q.device):
-        st = N.lib().la_decay_step(
-            _ptr(q), _Strides(*q.stride()), _ptr(k), _Strides(*k.stride()), _ptr(v),
-            _Strides(*v.stride()), _ptr(out), _ptr(state), _Strides(sb, sh), _ptr(log_decay),
-            b, h, d, dv, code, _default_scale(scale, d), _stream_ptr(q.device))
-    N.check(st, "la_decay_step")
+    if plan.copy:
+        return decay_attention_step(q.contiguous(), k.contiguous(), v.contiguous(), log_decay,
+                                    state, scale)
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return decay_attention_step(q, k, v, log_decay, state, scale)
+    if not log_decay.is_contiguous():
+        log_decay = log_decay.contiguous()
+    out = torch.empty(plan.out, dtype=plan.dtype, device=plan.device)
+    qs, ks, vs, ss = plan.strides
+    st = N.lib().la_decay_step(
+        q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), state.data_ptr(), ss,
+        log_decay.data_ptr(), *plan.sizes, plan.scale if scale is None else float(scale),
+        _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_decay_step")
     torch.autograd.graph.increment_version(state)
     return out
 
@@ -411,131 +522,160 @@ def _check_rows(x, name, like=None):
     return _dtype_code(x)
 
 
-def _check_norm(x, weight, residual):
-    code = _check_rows(x, "x")
-    if residual is not None:
-        _check_rows(residual, "residual", x)
-    wcode = code
-    if weight is not None:
-        if not isinstance(weight, torch.Tensor):
-            raise TypeError("weight must be a torch.Tensor")
-        wcode = _dtype_code(weight)
-        if tuple(weight.shape) != (x.shape[-1],) or weight.device != x.device:
-            raise ValueError(f"weight must be ({x.shape[-1]},) on {x.device}")
-    return code, wcode
+class _NormPlan:
+    """One signature of the norm: ``rows`` are the (..., d) tensors it reads,
+    the first of them under ``name``, the others of the same shape and type."""
+
+    __slots__ = ("index", "device", "dtype", "shape", "lead", "d", "codes", "strides", "c_shape",
+                 "copy", "aligned", "weight_copy", "group", "scales_shape", "ws_bytes")
+
+    def __init__(self, rows, names, weight, group_size):
+        x = rows[0]
+        code = _check_rows(x, names[0])
+        for t, name in zip(rows[1:], names[1:]):
+            if t is not None:
+                _check_rows(t, name, x)
+        wcode = code
+        d = x.shape[-1]
+        if weight is not None:
+            if not isinstance(weight, torch.Tensor):
+                raise TypeError("weight must be a torch.Tensor")
+            wcode = _dtype_code(weight)
+            if tuple(weight.shape) != (d,) or weight.device != x.device:
+                raise ValueError(f"weight must be ({d},) on {x.device}")
+        self.group = d if group_size is None else group_size
+        if group_size is not None and (group_size not in _FP8_GROUPS or d % group_size):
+            raise ValueError(f"group_size must be None or one of {_FP8_GROUPS} dividing {d}, "
+                             f"got {group_size}")
+        self.device, self.dtype, self.index = x.device, x.dtype, x.device.index
+        self.shape, self.lead, self.d, self.codes = x.shape, x.shape[:-1], d, (code, wcode)
+        self.scales_shape = (*x.shape[:-1], d // self.group)
+        self.weight_copy = weight is not None and not weight.is_contiguous()
+        lead = x.shape[:-1]
+        if all(t is None or t.is_contiguous() for t in rows):
+            self.c_shape = _Strides(1, 1, x.numel() // d)
+            self.strides = (_Strides(0, 0, d),) * len(rows)
+            self.copy = (False,) * len(rows)
+        else:  # up to three leading dimensions are read in place
+            pad = (1,) * (3 - len(lead))
+            self.copy = tuple(t is not None and (len(lead) > 3 or (t.stride(-1) != 1 and d > 1))
+                              for t in rows)
+            if not any(self.copy):
+                self.c_shape = _Strides(*(pad + tuple(lead)))
+                self.strides = tuple(
+                    None if t is None else _Strides(*((0,) * len(pad) + t.stride()[:-1]))
+                    for t in rows)
+        # scales of groups need rows of whole 16-byte packs
+        self.aligned = self.group != d
+        if self.aligned and not any(self.copy):
+            pack = 16 // x.element_size()
+            self.copy = tuple(t is not None and any(n % pack for n in s)
+                              for t, s in zip(rows, self.strides))
+        n = ctypes.c_size_t(0)
+        with _on_device(x.device):
+            N.check(N.lib().la_rms_norm_bwd_workspace_size(x.numel() // d, d, ctypes.byref(n)),
+                    "la_rms_norm_bwd_workspace_size")
+        self.ws_bytes = n.value
 
 
-def _row_views(*tensors):
-    """The tensors (equal shapes, None allowed) as rows under three leading
-    dimensions: ([tensor], [strides], shape).  Only rows that are not dense, or
-    that more than three leading dimensions address, are copied."""
-    first = next(t for t in tensors if t is not None)
-    lead, d = first.shape[:-1], first.shape[-1]
-    if all(t is None or t.is_contiguous() for t in tensors):
-        shape = _Strides(1, 1, first.numel() // d)
-        strides = _Strides(0, 0, d)
-        return tensors, [strides] * len(tensors), shape
-    if len(lead) > 3:
-        return _row_views(*(None if t is None else t.contiguous() for t in tensors))
-    pad = (1,) * (3 - len(lead))
-    got, strides = [], []
-    for t in tensors:
-        if t is not None and t.stride(-1) != 1 and d > 1:
-            t = t.contiguous()
-        got.append(t)
-        strides.append(None if t is None else _Strides(*((0,) * len(pad) + t.stride()[:-1])))
-    return got, strides, _Strides(*(pad + tuple(lead)))
+_norm_plans: dict = {}
+
+
+def _norm_plan(rows, names, weight, group_size=None) -> _NormPlan:
+    try:
+        key = (*map(_sig, rows), names, _sig(weight), group_size)
+        plan = _norm_plans.get(key)
+    except AttributeError:  # not tensors: the checks say which
+        key = plan = None
+    if plan is None:
+        plan = _keep(_norm_plans, key, _NormPlan(rows, names, weight, group_size))
+    return plan
+
+
+def _norm_inputs(plan, rows, weight):
+    """The rows and the weight as the kernels can read them, or None if they
+    already are."""
+    tensors = (*rows, weight)
+    copies = [*plan.copy, plan.weight_copy]
+    if plan.aligned:
+        copies = [c or (t is not None and t.data_ptr() & 15 != 0)
+                  for c, t in zip(copies, tensors)]
+    if not any(copies):
+        return None
+    return [t.clone(memory_format=torch.contiguous_format) if c else t
+            for c, t in zip(copies, tensors)]
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, want_rstd: bool = False):
     """Forward pass of the norm (no autograd): (y, x + residual or None, fp32
     reciprocal root mean squares per row or None)."""
-    code, wcode = _check_norm(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    plan = _norm_plan((x, residual), ("x", "residual"), weight)
+    again = _norm_inputs(plan, (x, residual), weight)
+    if again is not None:
+        return rms_norm(again[0], again[2], again[1], eps, want_rstd)
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return rms_norm(x, weight, residual, eps, want_rstd)
+    y = torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
     total = torch.empty_like(y) if residual is not None else None
-    rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_rstd
+    rstd = (torch.empty(plan.lead, dtype=torch.float32, device=plan.device) if want_rstd
             else None)
-    (x, residual), (xs, rs), shape = _row_views(x, residual)
-    weight = None if weight is None else weight.contiguous()
-    with _on_device(x.device):
-        st = N.lib().la_rms_norm_fwd(
-            _ptr(x), xs, _ptr(residual), rs, _ptr(weight), _ptr(y), _ptr(total), _ptr(rstd), shape,
-            x.shape[-1], code, wcode, float(eps), _stream_ptr(x.device))
-    N.check(st, "la_rms_norm_fwd")
+    st = N.lib().la_rms_norm_fwd(
+        x.data_ptr(), plan.strides[0], _ptr(residual), plan.strides[1], _ptr(weight), y.data_ptr(),
+        _ptr(total), _ptr(rstd), plan.c_shape, plan.d, *plan.codes, eps, _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_rms_norm_fwd")
     return y, total, rstd
 
 
 def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6, group_size: int | None = None):
     """The norm with its output held in e4m3: (y, scales, x + residual or None),
     scales fp32 (..., d / group_size), one per row without a group size."""
-    code, wcode = _check_norm(x, weight, residual)
-    d = x.shape[-1]
-    group = d if group_size is None else int(group_size)
-    if group_size is not None and (group not in _FP8_GROUPS or d % group):
-        raise ValueError(f"group_size must be None or one of {_FP8_GROUPS} dividing {d}, "
-                         f"got {group_size}")
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((*x.shape[:-1], d // group), dtype=torch.float32, device=x.device)
-    total = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None
-             else None)
-    (x, residual), (xs, rs), shape = _row_views(x, residual)
-    weight = None if weight is None else weight.contiguous()
-    if group != d:  # whole 16-byte packs per group
-        x, xs = _aligned_rows(x, xs, shape)
-        residual, rs = _aligned_rows(residual, rs, shape)
-        if weight is not None and weight.data_ptr() % 16:
-            weight = weight.clone()
-    with _on_device(x.device):
-        st = N.lib().la_rms_norm_fp8(
-            _ptr(x), xs, _ptr(residual), rs, _ptr(weight), _ptr(y), _ptr(scales), _ptr(total),
-            shape, d, group, code, wcode, float(eps), _stream_ptr(x.device))
-    N.check(st, "la_rms_norm_fp8")
+    plan = _norm_plan((x, residual), ("x", "residual"), weight, group_size)
+    again = _norm_inputs(plan, (x, residual), weight)
+    if again is not None:
+        return rms_norm_fp8(again[0], again[2], again[1], eps, group_size)
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return rms_norm_fp8(x, weight, residual, eps, group_size)
+    y = torch.empty(plan.shape, dtype=torch.float8_e4m3fn, device=plan.device)
+    scales = torch.empty(plan.scales_shape, dtype=torch.float32, device=plan.device)
+    total = (torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
+             if residual is not None else None)
+    st = N.lib().la_rms_norm_fp8(
+        x.data_ptr(), plan.strides[0], _ptr(residual), plan.strides[1], _ptr(weight), y.data_ptr(),
+        scales.data_ptr(), _ptr(total), plan.c_shape, plan.d, plan.group, *plan.codes, eps,
+        _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_rms_norm_fp8")
     return y, scales, total
-
-
-def _aligned_rows(t, strides, shape):
-    """``t`` and its row strides, copied where its rows do not start at 16 bytes."""
-    if t is None:
-        return t, strides
-    pack = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and all(s % pack == 0 for s in strides):
-        return t, strides
-    t = t.clone(memory_format=torch.contiguous_format)
-    d = t.shape[-1]
-    return t, _Strides(shape[1] * shape[2] * d, shape[2] * d, d)
 
 
 def rms_norm_backward(s, weight, rstd, d_y, d_sum=None, want_d_weight: bool = True):
     """Gradients (of x and of the residual alike, of the weight or None) of
     ``rms_norm`` from its saved rows ``s`` (x + residual) and ``rstd``."""
-    code, wcode = _check_norm(s, weight, None)
-    _check_rows(d_y, "d_y", s)
-    if d_sum is not None:
-        _check_rows(d_sum, "d_sum", s)
-    d = s.shape[-1]
-    d_s = torch.empty(s.shape, dtype=s.dtype, device=s.device)
-    d_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if (
-        want_d_weight and weight is not None) else None
-    (s, d_y, d_sum), (ss, ys, us), shape = _row_views(s, d_y, d_sum)
-    weight = None if weight is None else weight.contiguous()
+    plan = _norm_plan((s, d_y, d_sum), ("s", "d_y", "d_sum"), weight)
+    again = _norm_inputs(plan, (s, d_y, d_sum), weight)
+    if again is not None:
+        return rms_norm_backward(again[0], again[3], rstd, again[1], again[2], want_d_weight)
+    if plan.index != _get_device():
+        with torch.cuda.device(plan.index):
+            return rms_norm_backward(s, weight, rstd, d_y, d_sum, want_d_weight)
+    if rstd.shape != plan.lead or rstd.dtype != torch.float32 or rstd.device != plan.device:
+        raise ValueError(f"rstd must be float32 {tuple(plan.lead)} on {plan.device}")
     rstd = rstd.contiguous()
-    with _on_device(s.device):
-        ws_bytes = 0 if d_w is None else _norm_workspace(s.numel() // d, d,
-                                                         torch.cuda.current_device())
-        workspace = _workspace(ws_bytes, s.device)
-        st = N.lib().la_rms_norm_bwd(
-            _ptr(s), ss, _ptr(weight), _ptr(d_y), ys, _ptr(d_sum), us, _ptr(rstd), _ptr(d_s),
-            _ptr(d_w), shape, d, code, wcode, _ptr(workspace), ws_bytes, _stream_ptr(s.device))
-    N.check(st, "la_rms_norm_bwd")
+    d_s = torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
+    d_w = workspace = None
+    if want_d_weight and weight is not None:
+        d_w = torch.empty_like(weight)
+        workspace = _workspace(plan.ws_bytes, plan.device)
+    st = N.lib().la_rms_norm_bwd(
+        s.data_ptr(), plan.strides[0], _ptr(weight), d_y.data_ptr(), plan.strides[1], _ptr(d_sum),
+        plan.strides[2], rstd.data_ptr(), d_s.data_ptr(), _ptr(d_w), plan.c_shape, plan.d,
+        *plan.codes, _ptr(workspace), plan.ws_bytes, _stream_ptr(plan.device))
+    if st != N.LA_OK:
+        N.check(st, "la_rms_norm_bwd")
     return d_s, d_w
-
-
-@functools.lru_cache(maxsize=1024)
-def _norm_workspace(rows, d, device_index):
-    n = ctypes.c_size_t(0)
-    N.check(N.lib().la_rms_norm_bwd_workspace_size(rows, d, ctypes.byref(n)),
-            "la_rms_norm_bwd_workspace_size")
-    return n.value
 
 
 _copy_streams: dict = {}
