@@ -16,12 +16,13 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 
 namespace la {
 namespace {
 
 constexpr float kE4m3Max = 448.f;
-constexpr uint32_t kAmaxMinBits = (uint32_t)(127 - 96) << 23;  // 2^-96
+constexpr float kAmaxMin = 1.f / 79228162514264337593543950336.f;  // 2^-96
 constexpr int64_t kMaxWidth = 16384;
 
 // Rows of a tensor with up to three leading dimensions (strides in elements)
@@ -132,21 +133,64 @@ __device__ __forceinline__ void load_weight(float (&w)[NV][8], const void *p, in
   }
 }
 
+// A row as it is loaded, ahead of its use: bf16 packs stay packed.
+template <typename T, int NV, bool kVec>
+struct Held {
+  float x[NV][8];
+  template <int TPR>
+  __device__ __forceinline__ void load(const T *p, int t, int d) {
+    load_row<T, TPR, NV, kVec>(x, p, t, d);
+  }
+  __device__ __forceinline__ void get(float (&y)[NV][8]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[i][e] = x[i][e];
+  }
+};
+template <int NV>
+struct Held<__nv_bfloat16, NV, true> {
+  uint4 x[NV];
+  template <int TPR>
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p, int t, int d) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = column<TPR, true>(t, i, 0);
+      x[i] = c < d ? *(const uint4 *)(p + c) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void get(float (&y)[NV][8]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[i][2 * e] = __uint_as_float(u[e] << 16);
+        y[i][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
 struct Add {
   static __device__ __forceinline__ float zero() { return 0.f; }
   static __device__ __forceinline__ float of(float a, float b) { return a + b; }
 };
-// Largest of non-negative values by their bits: a NaN (above infinity) stays.
-struct MaxBits {
-  static __device__ __forceinline__ uint32_t zero() { return 0u; }
-  static __device__ __forceinline__ uint32_t of(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// The larger of two values; a NaN stays.
+struct Max {
+  static __device__ __forceinline__ float zero() { return 0.f; }
+  static __device__ __forceinline__ float of(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+  }
 };
 
 // Over the TPR threads of a row; every thread gets the result.  `slot`: shared
 // memory for the warps of a row, one per warp of the CTA.  With TPR > 32 the
 // CTA holds whole rows and every thread takes part.
-template <int TPR, class Op, typename V>
-__device__ __forceinline__ V reduce_row(V x, V *slot) {
+template <int TPR, class Op>
+__device__ __forceinline__ float reduce_row(float x, float *slot) {
 #pragma unroll
   for (int m = 1; m < (TPR < 32 ? TPR : 32); m <<= 1)
     x = Op::of(x, __shfl_xor_sync(0xffffffffu, x, m));
@@ -175,7 +219,8 @@ struct NormFwd {
   float *rstd;            // null, or one per row
   float *scales;          // fp8: (rows, d / group)
   Shape sh;
-  int d, group;           // group == d: one scale for the row
+  int d;
+  int group_log2;         // fp8: -1 for one scale per row, else log2 of the group
   float eps, inv_d;
 };
 
@@ -184,7 +229,7 @@ __global__ void __launch_bounds__(threads_of(TPR))
 rms_norm_fwd_kernel(const NormFwd p) {
   constexpr int kRowsPer = threads_of(TPR) / TPR;
   __shared__ float slot[32];
-  __shared__ uint32_t slot_max[32];
+  __shared__ float slot_max[32];
   const int t = threadIdx.x % TPR;
   const int64_t row0 = (int64_t)blockIdx.x * kRowsPer + threadIdx.x / TPR;
   const bool live = row0 < p.sh.rows;
@@ -217,39 +262,39 @@ rms_norm_fwd_kernel(const NormFwd p) {
   if constexpr (!kFp8) {
     if (live) store_row<T, TPR, NV, kVec>(s, (T *)p.y + row * p.d, t, p.d);
   } else {
-    uint32_t m[NV], all = 0;
+    float m[NV], all = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      m[i] = 0;
+    for (int i = 0; i < NV; ++i) {  // (columns beyond d are zero)
+      m[i] = fabsf(s[i][0]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = column<TPR, kVec>(t, i, e) < p.d;
-        m[i] = MaxBits::of(m[i], in ? __float_as_uint(fabsf(s[i][e])) : 0u);
-      }
-      all = MaxBits::of(all, m[i]);
+      for (int e = 1; e < 8; ++e) m[i] = Max::of(m[i], fabsf(s[i][e]));
+      all = Max::of(all, m[i]);
     }
-    const bool whole = p.group == p.d;
+    const bool whole = p.group_log2 < 0;
     if (whole) {
-      all = reduce_row<TPR, MaxBits>(all, slot_max);
+      all = reduce_row<TPR, Max>(all, slot_max);
 #pragma unroll
       for (int i = 0; i < NV; ++i) m[i] = all;
     } else {  // a group is group / 8 neighbouring lanes of one pack (kVec only)
-      const int lanes = p.group / 8;
+      const int lanes = 1 << (p.group_log2 - 3);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         for (int x = 1; x < lanes; x <<= 1)
-          m[i] = MaxBits::of(m[i], __shfl_xor_sync(0xffffffffu, m[i], x));
+          m[i] = Max::of(m[i], __shfl_xor_sync(0xffffffffu, m[i], x));
     }
     uint8_t *y = (uint8_t *)p.y + row * p.d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = column<TPR, kVec>(t, i, 0);
-      const float scale = __uint_as_float(MaxBits::of(m[i], kAmaxMinBits)) / kE4m3Max;
+      const float scale = Max::of(m[i], kAmaxMin) * (1.f / kE4m3Max);
       // one division per group: y * (1 / scale) is within an ulp of y / scale
       // ahead of the rounding to 4 bits
       const float inv = 1.f / scale;
-      if (live && (whole ? t == 0 && i == 0 : c < p.d && c % p.group == 0))
-        p.scales[row * (p.d / p.group) + (whole ? 0 : c / p.group)] = scale;
+      if (whole) {
+        if (live && t == 0 && i == 0) p.scales[row] = scale;
+      } else if (live && c < p.d && (c & ((1 << p.group_log2) - 1)) == 0) {
+        p.scales[row * (p.d >> p.group_log2) + (c >> p.group_log2)] = scale;
+      }
       uint16_t q[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -290,17 +335,36 @@ rms_norm_bwd_kernel(const NormBwd p) {
   constexpr int kRowsPer = kThreads / TPR;
   __shared__ float slot[32];
   extern __shared__ float lanes_dw[];  // (kRowsPer - 1, d) with kRowsPer > 1
+  tc::grid_dependents_launch();        // the sum of dw waits for all of this grid
   const int t = threadIdx.x % TPR, lane_row = threadIdx.x / TPR;
   float w[NV][8], dw[NV][8] = {};
   load_weight<TPR, NV, kVec>(w, p.weight, p.weight_dtype, t, p.d);
-  for (int64_t first = (int64_t)blockIdx.x * kRowsPer; first < p.sh.rows;
-       first += (int64_t)gridDim.x * kRowsPer) {
-    const bool live = first + lane_row < p.sh.rows;
-    const int64_t row = live ? first + lane_row : p.sh.rows - 1;
-    float s[NV][8], g[NV][8];
-    load_row<T, TPR, NV, kVec>(s, (const T *)p.s.p + row_offset(p.s, p.sh, row), t, p.d);
-    load_row<T, TPR, NV, kVec>(g, (const T *)p.dy.p + row_offset(p.dy, p.sh, row), t, p.d);
-    const float rstd = p.rstd[row];
+  // The next row is loaded before this one's sum over the row's threads (not
+  // where 1024 threads leave 64 registers each).
+  constexpr bool kAhead = TPR < 1024;
+  Held<T, NV, kVec> hs, hg, ha;
+  float rstd_next = 0.f;
+  const int64_t stride = (int64_t)gridDim.x * kRowsPer;
+  auto fetch = [&](int64_t first) {
+    // idle lanes redo the last row, unstored
+    const int64_t row = min64(first + lane_row, p.sh.rows - 1);
+    hs.template load<TPR>((const T *)p.s.p + row_offset(p.s, p.sh, row), t, p.d);
+    hg.template load<TPR>((const T *)p.dy.p + row_offset(p.dy, p.sh, row), t, p.d);
+    if (p.dsum.p)
+      ha.template load<TPR>((const T *)p.dsum.p + row_offset(p.dsum, p.sh, row), t, p.d);
+    rstd_next = p.rstd[row];
+  };
+  if (kAhead) fetch((int64_t)blockIdx.x * kRowsPer);
+  for (int64_t first = (int64_t)blockIdx.x * kRowsPer; first < p.sh.rows; first += stride) {
+    const int64_t row = first + lane_row;
+    const bool live = row < p.sh.rows;
+    if (!kAhead) fetch(first);
+    float s[NV][8], g[NV][8], a[NV][8];
+    hs.get(s);
+    hg.get(g);
+    if (p.dsum.p) ha.get(a);
+    const float rstd = rstd_next;
+    if (kAhead && first + stride < p.sh.rows) fetch(first + stride);
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -317,8 +381,6 @@ rms_norm_bwd_kernel(const NormBwd p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[i][e] = rstd * (g[i][e] - s[i][e] * c);
     if (p.dsum.p) {
-      float a[NV][8];
-      load_row<T, TPR, NV, kVec>(a, (const T *)p.dsum.p + row_offset(p.dsum, p.sh, row), t, p.d);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -358,48 +420,86 @@ rms_norm_bwd_kernel(const NormBwd p) {
   }
 }
 
-// dw = sum of the partial rows: 32 columns x 8 row lanes per CTA.
+// dw = sum of the partial rows: 32 columns x 32 row lanes per CTA.
 template <typename TW>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 rms_norm_dw_kernel(const float *partial, int rows, int d, TW *dw) {
-  __shared__ float part[8][32];
+  __shared__ float part[32][33];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+  tc::grid_dependency_wait();  // launched behind the kernel that writes the rows
   float sum = 0.f;
-  if (c < d)
-    for (int r = lane; r < rows; r += 8) sum += partial[(int64_t)r * d + c];
+  if (c < d) {
+#pragma unroll 8
+    for (int r = lane; r < rows; r += 32) sum += partial[(int64_t)r * d + c];
+  }
   part[lane][threadIdx.x & 31] = sum;
   __syncthreads();
-  if (lane == 0 && c < d) {
+  // warp w adds column w over the row lanes
+  sum = part[threadIdx.x & 31][lane];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += part[i][threadIdx.x];
-    dw[c] = from_f32<TW>(sum);
-  }
+  for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  if ((threadIdx.x & 31) == 0 && blockIdx.x * 32 + lane < d)
+    dw[blockIdx.x * 32 + lane] = from_f32<TW>(sum);
 }
 
-// The threads per row and packs per thread for a width: up to 4 packs of 8 per
-// thread (64 bytes in flight), rows of up to 1024 within one warp.  Rows whose
-// width or alignment rules out 16-byte accesses take fewer variants.
+template <typename TW>
+int launch_dw(const float *partial, int rows, int d, void *dw, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((d + 31) / 32));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cudaLaunchAttribute pdl;
+  pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &pdl;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, rms_norm_dw_kernel<TW>, partial, rows, d, (TW *)dw);
+  return check_launch();
+}
+
+// The threads per row and packs per thread for a width.  Few packs keep the
+// registers low enough for many CTAs per SM, whose loads then cover one
+// another's reductions.  Rows whose width or alignment rules out 16-byte
+// accesses take fewer variants.
 template <class F>
-int by_width(int64_t d, bool vec, F &&f) {
-  if (!vec) {
-    if (d <= 256) return f.template run<32, 1, false>();
-    if (d <= 1024) return f.template run<32, 4, false>();
-    if (d <= 4096) return f.template run<128, 4, false>();
-    return f.template run<512, 4, false>();
-  }
+int by_width_odd(int64_t d, F &&f) {
+  if (d <= 256) return f.template run<32, 1, false>();
+  if (d <= 1024) return f.template run<128, 1, false>();
+  if (d <= 4096) return f.template run<256, 2, false>();
+  return f.template run<1024, 2, false>();
+}
+// Forward: rows of up to 1024 within one warp (32768 x 4096 with residual to
+// e4m3: 128 threads x 4 packs 231 us, 256 x 2 ...).
+template <class F>
+int by_width_fwd(int64_t d, bool vec, F &&f) {
+  if (!vec) return by_width_odd(d, f);
   if (d <= 64) return f.template run<8, 1, true>();
   if (d <= 128) return f.template run<16, 1, true>();
   if (d <= 256) return f.template run<32, 1, true>();
   if (d <= 512) return f.template run<32, 2, true>();
   if (d <= 1024) return f.template run<32, 4, true>();
   if (d <= 2048) return f.template run<128, 2, true>();
-  if (d <= 4096) return f.template run<128, 4, true>();
+  if (d <= 4096) return f.template run<256, 2, true>();
   if (d <= 8192) return f.template run<256, 4, true>();
-  return f.template run<512, 4, true>();
+  return f.template run<1024, 2, true>();
+}
+// Gradient: it also holds w and the running dw.
+template <class F>
+int by_width_bwd(int64_t d, bool vec, F &&f) {
+  if (!vec) return by_width_odd(d, f);
+  if (d <= 64) return f.template run<8, 1, true>();
+  if (d <= 128) return f.template run<16, 1, true>();
+  if (d <= 256) return f.template run<32, 1, true>();
+  if (d <= 512) return f.template run<64, 1, true>();
+  if (d <= 1024) return f.template run<128, 1, true>();
+  if (d <= 2048) return f.template run<256, 1, true>();
+  if (d <= 4096) return f.template run<256, 2, true>();
+  if (d <= 8192) return f.template run<512, 2, true>();
+  return f.template run<1024, 2, true>();
 }
 
 // The gradient's CTAs walk the rows: this many per SM at most.
-constexpr int kBwdPerSm = 4;
+constexpr int kBwdPerSm = 8;
 
 // One partial row of dw for each CTA, at most.
 size_t partial_bytes(int64_t rows, int64_t d, int sm_count) {
@@ -436,7 +536,17 @@ struct BwdLaunch {
   template <int TPR, int NV, bool kVec>
   int run() {
     constexpr int per = threads_of(TPR) / TPR;
-    *grid = (int)min64((p.sh.rows + per - 1) / per, (int64_t)sm_count * kBwdPerSm);
+    // one wave of CTAs, each walking many rows
+    static const int per_sm = [] {
+      int n = 0;
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+              &n, rms_norm_bwd_kernel<T, TPR, NV, kVec>, threads_of(TPR), 28 * 1024) != cudaSuccess) {
+        cudaGetLastError();
+        n = 2;
+      }
+      return n < 1 ? 1 : n > kBwdPerSm ? kBwdPerSm : n;
+    }();
+    *grid = (int)min64((p.sh.rows + per - 1) / per, (int64_t)sm_count * per_sm);
     const int smem = p.partial ? (per - 1) * p.d * 4 : 0;  // at most 28 KB
     rms_norm_bwd_kernel<T, TPR, NV, kVec><<<*grid, threads_of(TPR), smem, s>>>(p);
     return check_launch();
@@ -481,17 +591,17 @@ int launch_fwd(const NormFwd &p, int dtype, cudaStream_t s) {
   const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
   const bool vec = p.d % 8 == 0 && vec_rows(p.x, size) && vec_rows(p.r, size) &&
                    vec_ptr(p.weight) && vec_ptr(p.y) && vec_ptr(p.sum);
-  if (kFp8 && p.group != p.d && !vec) return LA_ERR_UNSUPPORTED;
-  if (dtype == LA_DTYPE_FLOAT32) return by_width(p.d, vec, FwdLaunch<float, kFp8>{p, s});
-  return by_width(p.d, vec, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
+  if (kFp8 && p.group_log2 >= 0 && !vec) return LA_ERR_UNSUPPORTED;
+  if (dtype == LA_DTYPE_FLOAT32) return by_width_fwd(p.d, vec, FwdLaunch<float, kFp8>{p, s});
+  return by_width_fwd(p.d, vec, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
 }
 
 int launch_bwd(const NormBwd &p, int dtype, int sm_count, int *grid, cudaStream_t s) {
   const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
   const bool vec = p.d % 8 == 0 && vec_rows(p.s, size) && vec_rows(p.dy, size) &&
                    vec_rows(p.dsum, size) && vec_ptr(p.weight) && vec_ptr(p.ds);
-  if (dtype == LA_DTYPE_FLOAT32) return by_width(p.d, vec, BwdLaunch<float>{p, sm_count, grid, s});
-  return by_width(p.d, vec, BwdLaunch<__nv_bfloat16>{p, sm_count, grid, s});
+  if (dtype == LA_DTYPE_FLOAT32) return by_width_bwd(p.d, vec, BwdLaunch<float>{p, sm_count, grid, s});
+  return by_width_bwd(p.d, vec, BwdLaunch<__nv_bfloat16>{p, sm_count, grid, s});
 }
 
 }  // namespace
@@ -513,7 +623,7 @@ int la_rms_norm_fwd(const void *x, const int64_t *x_strides, const void *residua
   p.x = rows_of(x, x_strides);
   p.r = rows_of(residual, residual_strides);
   p.weight = weight, p.weight_dtype = weight_dtype, p.y = y, p.sum = sum, p.rstd = rstd;
-  p.d = p.group = (int)d;
+  p.d = (int)d;
   p.eps = eps;
   p.inv_d = 1.f / (float)d;
   return launch_fwd<false>(p, dtype, (cudaStream_t)stream);
@@ -536,7 +646,9 @@ int la_rms_norm_fp8(const void *x, const int64_t *x_strides, const void *residua
   p.r = rows_of(residual, residual_strides);
   p.weight = weight, p.weight_dtype = weight_dtype, p.y = y, p.sum = sum, p.scales = scales;
   p.d = (int)d;
-  p.group = (int)group;
+  p.group_log2 = -1;
+  for (int i = 4; group != d && i <= 8; ++i)
+    if (group == (int64_t)1 << i) p.group_log2 = i;
   p.eps = eps;
   p.inv_d = 1.f / (float)d;
   return launch_fwd<true>(p, dtype, (cudaStream_t)stream);
@@ -584,13 +696,8 @@ int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight,
   int grid = 0;
   st = launch_bwd(p, dtype, info.sm_count, &grid, cs);
   if (st != LA_OK || !d_weight) return st;
-  const unsigned cols = (unsigned)((d + 31) / 32);
-  if (weight_dtype == LA_DTYPE_FLOAT32)
-    rms_norm_dw_kernel<float><<<cols, 256, 0, cs>>>(p.partial, grid, p.d, (float *)d_weight);
-  else
-    rms_norm_dw_kernel<__nv_bfloat16>
-        <<<cols, 256, 0, cs>>>(p.partial, grid, p.d, (__nv_bfloat16 *)d_weight);
-  return check_launch();
+  if (weight_dtype == LA_DTYPE_FLOAT32) return launch_dw<float>(p.partial, grid, p.d, d_weight, cs);
+  return launch_dw<__nv_bfloat16>(p.partial, grid, p.d, d_weight, cs);
 }
 
 }  // extern "C"
