@@ -208,7 +208,10 @@ __device__ __forceinline__ float reduce_row(float x, float *slot) {
   return x;
 }
 
-constexpr int threads_of(int tpr) { return tpr > 256 ? tpr : 256; }
+// Threads of a CTA.  Forward: one row per CTA from 128 threads a row on, so that
+// no row waits at another's barrier; gradient: at least 256, fewer partial rows.
+constexpr int fwd_threads(int tpr) { return tpr >= 128 ? tpr : 256; }
+constexpr int bwd_threads(int tpr) { return tpr > 256 ? tpr : 256; }
 
 struct NormFwd {
   Rows x, r;              // r.p null: no residual
@@ -225,9 +228,9 @@ struct NormFwd {
 };
 
 template <typename T, int TPR, int NV, bool kVec, bool kFp8>
-__global__ void __launch_bounds__(threads_of(TPR))
+__global__ void __launch_bounds__(fwd_threads(TPR))
 rms_norm_fwd_kernel(const NormFwd p) {
-  constexpr int kRowsPer = threads_of(TPR) / TPR;
+  constexpr int kRowsPer = fwd_threads(TPR) / TPR;
   __shared__ float slot[32];
   __shared__ float slot_max[32];
   const int t = threadIdx.x % TPR;
@@ -329,9 +332,9 @@ struct NormBwd {
 };
 
 template <typename T, int TPR, int NV, bool kVec>
-__global__ void __launch_bounds__(threads_of(TPR))
+__global__ void __launch_bounds__(bwd_threads(TPR))
 rms_norm_bwd_kernel(const NormBwd p) {
-  constexpr int kThreads = threads_of(TPR);
+  constexpr int kThreads = bwd_threads(TPR);
   constexpr int kRowsPer = kThreads / TPR;
   __shared__ float slot[32];
   extern __shared__ float lanes_dw[];  // (kRowsPer - 1, d) with kRowsPer > 1
@@ -468,8 +471,9 @@ int by_width_odd(int64_t d, F &&f) {
   if (d <= 4096) return f.template run<256, 2, false>();
   return f.template run<1024, 2, false>();
 }
-// Forward: rows of up to 1024 within one warp (32768 x 4096 with residual to
-// e4m3: 128 threads x 4 packs 231 us, 256 x 2 ...).
+// Forward: rows of up to 1024 within one warp (32768 x 4096 with a residual, one
+// row of 128 threads x 4 packs per CTA against 256 x 2: 164 and 171 us, to e4m3
+// 188 and 196).
 template <class F>
 int by_width_fwd(int64_t d, bool vec, F &&f) {
   if (!vec) return by_width_odd(d, f);
@@ -479,7 +483,7 @@ int by_width_fwd(int64_t d, bool vec, F &&f) {
   if (d <= 512) return f.template run<32, 2, true>();
   if (d <= 1024) return f.template run<32, 4, true>();
   if (d <= 2048) return f.template run<128, 2, true>();
-  if (d <= 4096) return f.template run<256, 2, true>();
+  if (d <= 4096) return f.template run<128, 4, true>();
   if (d <= 8192) return f.template run<256, 4, true>();
   return f.template run<1024, 2, true>();
 }
@@ -519,10 +523,10 @@ struct FwdLaunch {
   cudaStream_t s;
   template <int TPR, int NV, bool kVec>
   int run() {
-    constexpr int per = threads_of(TPR) / TPR;
+    constexpr int per = fwd_threads(TPR) / TPR;
     const int64_t grid = (p.sh.rows + per - 1) / per;
     if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
-    rms_norm_fwd_kernel<T, TPR, NV, kVec, kFp8><<<(unsigned)grid, threads_of(TPR), 0, s>>>(p);
+    rms_norm_fwd_kernel<T, TPR, NV, kVec, kFp8><<<(unsigned)grid, fwd_threads(TPR), 0, s>>>(p);
     return check_launch();
   }
 };
@@ -535,12 +539,12 @@ struct BwdLaunch {
   cudaStream_t s;
   template <int TPR, int NV, bool kVec>
   int run() {
-    constexpr int per = threads_of(TPR) / TPR;
+    constexpr int per = bwd_threads(TPR) / TPR;
     // one wave of CTAs, each walking many rows
     static const int per_sm = [] {
       int n = 0;
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-              &n, rms_norm_bwd_kernel<T, TPR, NV, kVec>, threads_of(TPR), 28 * 1024) != cudaSuccess) {
+              &n, rms_norm_bwd_kernel<T, TPR, NV, kVec>, bwd_threads(TPR), 28 * 1024) != cudaSuccess) {
         cudaGetLastError();
         n = 2;
       }
@@ -548,7 +552,7 @@ struct BwdLaunch {
     }();
     *grid = (int)min64((p.sh.rows + per - 1) / per, (int64_t)sm_count * per_sm);
     const int smem = p.partial ? (per - 1) * p.d * 4 : 0;  // at most 28 KB
-    rms_norm_bwd_kernel<T, TPR, NV, kVec><<<*grid, threads_of(TPR), smem, s>>>(p);
+    rms_norm_bwd_kernel<T, TPR, NV, kVec><<<*grid, bwd_threads(TPR), smem, s>>>(p);
     return check_launch();
   }
 };
