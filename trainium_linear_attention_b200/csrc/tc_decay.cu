@@ -28,7 +28,7 @@
 // d = 64 against ~1,300 cycles of tensor work); per-tile latency (the chain
 // U -> S -> copy -> O1 -> out) where few CTAs walk.
 //
-// Warps: 0 TMA; 1 scores, O1 and O2 MMAs (TMEM owner); 2 U MMAs; 4.. state
+// Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state
 // (4 warps at DK = 64, 8 at 128); 8 warps P; 4
 // warps V'; 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
 #include "decay.cuh"
@@ -44,8 +44,9 @@ constexpr int kT = kDecayTile;  // tokens per tile
 constexpr int kBlock = kT * 128;  // bytes of 128 tokens x 64 bf16 columns, 128B-swizzled
 constexpr float kLog2e = 1.4426950408889634f;
 
-// TMEM columns
+// TMEM columns.  P (two bf16 per column) is written over its scores.
 constexpr uint32_t kColScores = 0;  // two buffers of 128
+constexpr uint32_t kP1 = 64;        // P of tokens 64 .. 127 of the tile, in the buffer
 constexpr uint32_t kColU = 256;     // hi 64, lo 64
 constexpr uint32_t kColO1 = 384;
 constexpr uint32_t kColO2 = 448;
@@ -69,6 +70,7 @@ struct TcLayout {
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
   static constexpr int kVpBufs = DK == 64 || kStateOnly ? 2 : 1;
+  static constexpr int kUBufs = kStateOnly ? 2 : 1;
   static constexpr uint32_t kFixed =
       kVpBufs * 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
   static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
@@ -90,14 +92,14 @@ enum Bar {
   kSReady = kEmpty + 6,
   kPReady = kSReady + 2,
   kSnapReady = kPReady + 2,
-  kSnapFree = kSnapReady + 2,
-  kVpReady = kSnapFree + 2,
+  kRead = kSnapReady + 2,  // O1 formed: the copy of S is free
+  kVpReady = kRead + 2,
   kUReady = kVpReady + 2,  // alternate tiles: V' may run a tile ahead of its readers
   kUFree = kUReady + 2,
-  kOReady,
-  kOFree,
-  kDone,
-  kNumBars = kDone + 2
+  kOReady = kUFree + 2,
+  kOFree = kOReady + 2,
+  kDone = kOFree + 2,
+  kNumBars = kDone + 3
 };
 static_assert(8 * kNumBars + 8 <= 512, "barrier area");
 
@@ -145,6 +147,13 @@ __device__ __forceinline__ uint32_t hfma2_bf16(uint32_t a, uint32_t b, uint32_t 
 }
 __device__ __forceinline__ uint32_t hneg2_bf16(uint32_t a) { return a ^ 0x80008000u; }
 
+// The signs of bytes 0 and 2 over the low and the high half of a word.
+__device__ __forceinline__ uint32_t spread_signs(uint32_t x) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %1, 0xAA88;" : "=r"(d) : "r"(x));
+  return d;
+}
+
 __device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();
   while (!mbar_try_wait(bar, parity))
@@ -191,8 +200,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
-      const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 || i == kUFree;
-      const bool per_four = i == kVpReady || i == kVpReady + 1 || i == kOFree;
+      const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 ||
+                                  i == kUFree || i == kUFree + 1;
+      const bool per_four =
+          i == kVpReady || i == kVpReady + 1 || i == kOFree || i == kOFree + 1;
       const bool per_p_warp = i == kPReady || i == kPReady + 1;
       const bool stage_empty = i >= kEmpty && i < kEmpty + 6;
       mbar_init(&bars[i], per_state_warp ? L::kStateWarps
@@ -283,66 +294,63 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         wait_teardown(&bars[kFull + i % kStages], (i / kStages) & 1);
     }
   } else if (warp == 1) {
-    // ------------------------------------- scores, A S and P V (one tile ahead)
+    // ------------------------------------------------------- scores and O1 = A S
+    // Three warps issue MMAs: one instruction of a warp takes ten cycles and more
+    // here, so a tile's 24 to 32 MMAs with their waits are too long for one.
     if constexpr (!kStateOnly) {
       constexpr uint32_t id_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
       const int k_steps = (role.da + 15) / 16;  // the columns beyond are zero
+      const uint64_t a0 = make_sdesc(sb + L::kOffA, 16, 1024, kSwizzle128B);
+      const uint64_t b0 = make_sdesc(sb + L::kOffB, 16, 1024, kSwizzle128B);
+      const uint64_t s0 = make_sdesc(sb + L::kOffSnap, 16, 1024, kSwizzle128B);
+      int ss = 0, sp = 0;  // stage of the next scores and its phase
       auto issue_scores = [&](int c) -> bool {
-        const int s = c % kStages;
-        if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) return false;
+        if (!mbar_wait_warp(&bars[kFull + ss], sp, abort_flag)) return false;
+        // the buffer: P of tile c - 2 has been read by P V
+        if (c >= 2 && !mbar_wait_warp(&bars[kOReady + (c & 1)], ((c - 2) / 2) & 1, abort_flag))
+          return false;
         tc_fence_after();
-        const uint32_t st = sb + s * L::kStageBytes;
-        const uint64_t da = make_sdesc(st + L::kOffA, 16, 1024, kSwizzle128B);
-        const uint64_t db = make_sdesc(st + L::kOffB, 16, 1024, kSwizzle128B);
+        const uint64_t at = (uint64_t)(ss * (L::kStageBytes >> 4));
+        const uint32_t d = tmem + kColScores + (c & 1) * 128;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk) {  // 32 bytes along the 128-byte rows
-            const uint64_t step = (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2);
-            if (kk < k_steps) umma_ss(tmem + kColScores + (c & 1) * 128, da + step, db + step, id_s, kk > 0);
+            const uint64_t step = at + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2);
+            if (kk < k_steps) umma_ss(d, a0 + step, b0 + step, id_s, kk > 0);
           }
           umma_commit(&bars[kSReady + (c & 1)]);
         }
         __syncwarp();
+        if (++ss == kStages) ss = 0, sp ^= 1;
         return true;
       };
       bool ok = tiles > 0 && issue_scores(0);
+      int rs = 0;  // stage of tile c
       for (int c = 0; ok && c < tiles; ++c) {
-        const int s = c % kStages, b = c & 1;
-        // the next tile's scores go first if its copies have landed: P of the
-        // next tile is formed under this tile's read-out (the buffer was read by
-        // P V of tile c - 1, issued before)
+        const int b = c & 1;
+        // the next tile's scores go first if nothing holds them up
         const bool early =
-            c + 1 < tiles && __all_sync(0xffffffffu, mbar_test_wait(&bars[kFull + (c + 1) % kStages],
-                                                                    ((c + 1) / kStages) & 1));
+            c + 1 < tiles &&
+            __all_sync(0xffffffffu,
+                       mbar_test_wait(&bars[kFull + ss], sp) &&
+                           (c == 0 || mbar_test_wait(&bars[kOReady + (b ^ 1)], ((c - 1) / 2) & 1)));
         if (early && !issue_scores(c + 1)) break;
         if (!mbar_wait_warp(&bars[kSnapReady + b], (c / 2) & 1, abort_flag)) break;
-        if (c > 0 && !mbar_wait_warp(&bars[kOFree], (c - 1) & 1, abort_flag)) break;
+        if (c > 0 && !mbar_wait_warp(&bars[kOFree + (b ^ 1)], ((c - 1) / 2) & 1, abort_flag)) break;
         tc_fence_after();
-        const uint32_t st = sb + s * L::kStageBytes;
-        const uint64_t da = make_sdesc(st + L::kOffA, 16, 1024, kSwizzle128B);
-        const uint64_t ds = make_sdesc(sb + L::kOffSnap + b * L::kSnapBytes, 16, 1024, kSwizzle128B);
-        const uint64_t dv = make_sdesc(st + L::kOffV, 16, 1024, kSwizzle128B);
+        const uint64_t at = (uint64_t)(rs * (L::kStageBytes >> 4));
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk)
             if (kk < k_steps)
-              umma_ss(tmem + kColO1, da + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
-                    ds + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
-          umma_commit(&bars[kSnapFree + b]);
+              umma_ss(tmem + kColO1,
+                      a0 + at + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
+                      s0 + (uint64_t)(b * (L::kSnapBytes >> 4) + kk * (2048 >> 4)), id_o, kk > 0);
+          umma_commit(&bars[kRead + b]);
         }
         __syncwarp();
-        if (!mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kT / 16; ++kk)
-            umma_ts(tmem + kColO2, tmem + kColScores + b * 128 + (kk / 4) * 64 + (kk % 4) * 8,
-                    dv + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
-          umma_commit(&bars[kOReady]);
-          umma_commit(&bars[kEmpty + s]);
-        }
-        __syncwarp();
+        if (++rs == kStages) rs = 0;
         if (c + 1 < tiles && !early && !issue_scores(c + 1)) break;
       }
       if (elect_one()) umma_commit(&bars[kDone]);
@@ -353,34 +361,69 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   } else if (warp == 2) {
     // ------------------------------------------------------------ U = B^T V'
     constexpr uint32_t id_u = make_idesc_bf16(128, 128, true, true);
+    // A = B^T: the second 64 rows of M are the next 64 columns (DK = 128), or the
+    // same ones again (DK = 64)
+    const uint64_t a0 = make_sdesc(sb + L::kOffB, DK == 64 ? 0 : kBlock, 1024, kSwizzle128B);
+    const uint64_t b0 = make_sdesc(sb + L::kOffVp, kBlock, 1024, kSwizzle128B);
+    int us = 0, up = 0;  // stage and its phase
     for (int c = 0; c < updates; ++c) {
-      const int s = c % kStages;
-      if (!mbar_wait_warp(&bars[kFull + s], (c / kStages) & 1, abort_flag)) break;
       const int vb = c % L::kVpBufs;
+      if (!mbar_wait_warp(&bars[kFull + us], up, abort_flag)) break;
       if (!mbar_wait_warp(&bars[kVpReady + vb], (c / L::kVpBufs) & 1, abort_flag)) break;
-      if (c > 0 && !mbar_wait_warp(&bars[kUFree], (c - 1) & 1, abort_flag)) break;
+      // the columns: U of tile c - 1 (with two buffers c - 2) is in registers
+      if (c >= L::kUBufs) {
+        const int u = c - L::kUBufs;
+        if (!mbar_wait_warp(&bars[kUFree + (u & 1)], (u / 2) & 1, abort_flag)) break;
+      }
       tc_fence_after();
-      // A = B^T: the second 64 rows of M are the next 64 columns (DK = 128), or
-      // the same ones again (DK = 64)
-      const uint64_t da = make_sdesc(sb + s * L::kStageBytes + L::kOffB, DK == 64 ? 0 : kBlock,
-                                     1024, kSwizzle128B);
-      const uint64_t db =
-          make_sdesc(sb + L::kOffVp + vb * 2 * kBlock, kBlock, 1024, kSwizzle128B);
+      const uint32_t d = tmem + kColU + (c % L::kUBufs) * 128;
+      const uint64_t da = a0 + (uint64_t)(us * (L::kStageBytes >> 4));
+      const uint64_t db = b0 + (uint64_t)(vb * (2 * kBlock >> 4));
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kT / 16; ++kk) {
           const uint64_t step = (uint64_t)(kk * (2048 >> 4));
-          umma_ss(tmem + kColU, da + step, db + step, id_u, kk > 0);
+          umma_ss(d, da + step, db + step, id_u, kk > 0);
         }
         umma_commit(&bars[kUReady + (c & 1)]);
-        umma_commit(&bars[kEmpty + s]);
       }
       __syncwarp();
+      if (++us == kStages) us = 0, up ^= 1;
     }
     if (elect_one()) umma_commit(&bars[kDone + 1]);
     __syncwarp();
     if (lane == 0) wait_teardown(&bars[kDone + 1], 0);
     __syncwarp();
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ O2 = P V
+    if constexpr (!kStateOnly) {
+      constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
+      const uint64_t v0 = make_sdesc(sb + L::kOffV, 16, 1024, kSwizzle128B);
+      int vs = 0, vp = 0;  // stage and its phase
+      for (int c = 0; c < tiles; ++c) {
+        const int b = c & 1;
+        if (!mbar_wait_warp(&bars[kFull + vs], vp, abort_flag)) break;
+        if (!mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
+        // the columns: O2 of tile c - 1 has been read out
+        if (c > 0 && !mbar_wait_warp(&bars[kOFree + (b ^ 1)], ((c - 1) / 2) & 1, abort_flag)) break;
+        tc_fence_after();
+        const uint64_t dv = v0 + (uint64_t)(vs * (L::kStageBytes >> 4));
+        const uint32_t buf = tmem + kColScores + b * 128;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kT / 16; ++kk)
+            umma_ts(tmem + kColO2, buf + (kk / 4) * kP1 + (kk % 4) * 8,
+                    dv + (uint64_t)(kk * (2048 >> 4)), id_o, kk > 0);
+          umma_commit(&bars[kOReady + b]);
+        }
+        __syncwarp();
+        if (++vs == kStages) vs = 0, vp ^= 1;
+      }
+      if (elect_one()) umma_commit(&bars[kDone + 2]);
+      __syncwarp();
+      if (lane == 0) wait_teardown(&bars[kDone + 2], 0);
+      __syncwarp();
+    }
   } else if (warp >= L::kWState && warp < L::kWP) {
     // ------------------------------------------------------------ state
     // A thread owns 32 columns of one row of S.
@@ -409,28 +452,34 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       for (int i = 0; i < 32; ++i)
         if (i < cols) st[i] = src[i * step];
     }
-    const uint32_t urow = taddr(tmem, wq * 32, kColU + half * 32);
-    auto write_copy = [&](int b) {
-      const uint32_t dst = sb + L::kOffSnap + b * L::kSnapBytes;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        st_shared_v4(dst + sw128_offset(row, half * 4 + q), pack_bf16(st[8 * q], st[8 * q + 1]),
-                     pack_bf16(st[8 * q + 2], st[8 * q + 3]),
-                     pack_bf16(st[8 * q + 4], st[8 * q + 5]),
-                     pack_bf16(st[8 * q + 6], st[8 * q + 7]));
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kSnapReady + b]);
-    };
-    if (!kStateOnly && tiles > 0) write_copy(0);
     const float keep_full = decay_pow(g, kT);
-    for (int c = 0; c < updates; ++c) {
+#pragma unroll 1
+    for (int c = 0;; ++c) {
+      if (!kStateOnly && c < tiles) {  // the copy of S that tile c reads
+        const int b = c & 1;
+        if (c >= 2) mbar_wait(&bars[kRead + b], ((c - 2) / 2) & 1, abort_flag);
+        __syncwarp();
+        const uint32_t dst = sb + L::kOffSnap + b * L::kSnapBytes;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          st_shared_v4(dst + sw128_offset(row, half * 4 + q), pack_bf16(st[8 * q], st[8 * q + 1]),
+                       pack_bf16(st[8 * q + 2], st[8 * q + 3]),
+                       pack_bf16(st[8 * q + 4], st[8 * q + 5]),
+                       pack_bf16(st[8 * q + 6], st[8 * q + 7]));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kSnapReady + b]);
+      }
+      if (c >= updates) break;
       const int len = tile_len(c);
       const float keep = len == kT ? keep_full : decay_pow(g, len);
       const uint64_t keep2 = f2pack(keep, keep);
       mbar_wait(&bars[kUReady + (c & 1)], (c / 2) & 1, abort_flag);
+      // B and V of the tile's stage have been read by U (and V')
+      if (warp == L::kWState && lane == 0) mbar_arrive(&bars[kEmpty + c % kStages]);
       __syncwarp();
       tc_fence_after();
+      const uint32_t urow = taddr(tmem, wq * 32, kColU + (c % L::kUBufs) * 128 + half * 32);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t hi[8], lo[8];
@@ -447,13 +496,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kUFree]);
-      if (!kStateOnly && c + 1 < tiles) {
-        const int b = (c + 1) & 1;
-        if (c > 0) mbar_wait(&bars[kSnapFree + b], ((c - 1) / 2) & 1, abort_flag);
-        __syncwarp();
-        write_copy(b);
-      }
+      if (lane == 0) mbar_arrive(&bars[kUFree + (c & 1)]);
     }
     if (want_final) {
       float *dst = (kStateOnly ? role.states + (bh * p.segments + order) * per_head
@@ -471,22 +514,23 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const int wq = warp & 3;
     // finite, so that 0 * g2 = 0 (e^-6900 is zero like e^-inf)
     const float g2 = fmaxf(g * kLog2e, -1e4f);
-    const float toward = rev ? 1.f : -1.f;  // the next column: lag + 1, or - 1
-    // lambda^lag over 16 columns j0 + t: lambda^(i-j0-15) * lambda^(15-t), in a
-    // reversed walk lambda^(j0-i) * lambda^t.  Off the diagonal both powers are
-    // non-negative; on it the first reaches -15, which fp32 holds while
+    const int sign = rev ? -1 : 1;
+    // lambda^lag over 16 columns j0 + t: f = lambda^(i-j0-15) times w = lambda^(15-t),
+    // in a reversed walk lambda^(j0-i) * lambda^t.  Off the diagonal both powers
+    // are non-negative; on it the first reaches -15, which fp32 holds while
     // |g| <= 4, and the columns with lag < 0 are cut from the packed words.
     const bool mild = g >= -4.f && g <= 4.f;
+    const int row_lag = (wq * 32 + lane - 64 * half) * sign;  // lag of the warp's first column
     uint64_t w2[8];
-    uint32_t cut[2][8];
+    uint32_t kept[2] = {0, 0};  // columns with lag >= 0 of the diagonal's two chunks
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int n0 = rev ? 2 * t : 15 - 2 * t, n1 = rev ? 2 * t + 1 : 14 - 2 * t;
       w2[t] = f2pack(decay_pow(g, n0) * role.intra, decay_pow(g, n1) * role.intra);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < 2; ++q) {  // even columns in the low half, odd ones in the high
         const int lag = rev ? 16 * q - lane + 2 * t : lane - 16 * q - 2 * t;
-        cut[q][t] = (lag >= 0 ? 0xFFFFu : 0u) | (lag + (rev ? 1 : -1) >= 0 ? 0xFFFF0000u : 0u);
+        kept[q] |= (lag >= 0 ? 1u << t : 0u) | (lag - sign >= 0 ? 0x10000u << t : 0u);
       }
     }
     for (int c = 0; c < tiles; ++c) {
@@ -494,47 +538,50 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      // 32 columns at a time; P lands on columns already read.  Kept rolled:
-      // the warps' roles share one instruction cache.
+      // 16 columns at a time.  Rolled, like the other loops here: the warps of a
+      // scheduler run six different ones, and where those did not fit its
+      // instruction cache together the kernel took 1.3 times as long.
 #pragma unroll 1
-      for (int ch = 0; ch < 2; ++ch) {
-        const int side = (2 * half + ch - wq) * (rev ? -1 : 1);
+      for (int k = 0; k < 4; ++k) {
+        const int side = (2 * half + (k >> 1) - wq) * sign;
+        uint32_t x[16], pk[8];
+        if (side > 0) {  // beyond the diagonal
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t x[16];
-          if (side > 0) {
+          for (int t = 0; t < 8; ++t) pk[t] = 0;
+        } else {
+          const int lag = row_lag - sign * 16 * k;  // of the first column
+          tmem_ld16(srow0 + 16 * k, x);
+          tmem_wait_ld();
+          if (side < 0 || mild) {
+            // (below -15 every column is cut)
+            const float f = ex2_approx((float)max(rev ? lag : lag - 15, -15) * g2);
+            const uint64_t f2 = f2pack(f, f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0;
-          } else {
-            // lag of the row and the first column
-            const int first = (wq * 32 + lane - 64 * half - 32 * ch - 16 * q) * (rev ? -1 : 1);
-            tmem_ld16(srow0 + 32 * ch + 16 * q, x);
-            tmem_wait_ld();
-            if (side < 0 || mild) {
-              // (below -15 every column is cut)
-              const float f = ex2_approx((float)max(rev ? first : first - 15, -15) * g2);
-              const uint64_t f2 = f2pack(f, f);
+            for (int t = 0; t < 8; ++t)
+              pk[t] = pack_bf16x2(
+                  fmul2(fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
+                              w2[t]),
+                        f2));
+          } else {  // strong decays: each column its own power
+            float l = (float)lag;
 #pragma unroll
-              for (int t = 0; t < 8; ++t)
-                x[t] = pack_bf16x2(
-                    fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
-                          fmul2(f2, w2[t])));
-              if (side == 0) {
-#pragma unroll
-                for (int t = 0; t < 8; ++t) x[t] &= cut[q][t];
-              }
-            } else {  // strong decays: each column its own power
-#pragma unroll
-              for (int t = 0; t < 8; ++t) {
-                const float l0 = (float)first + toward * (2 * t), l1 = l0 + toward;
-                x[t] = cut[q][t] &
-                       pack_bf16(__uint_as_float(x[2 * t]) * (role.intra * ex2_approx(l0 * g2)),
-                                 __uint_as_float(x[2 * t + 1]) * (role.intra * ex2_approx(l1 * g2)));
-              }
+            for (int t = 0; t < 8; ++t) {
+              const float y0 = __uint_as_float(x[2 * t]) * (role.intra * ex2_approx(l * g2));
+              l -= (float)sign;
+              const float y1 = __uint_as_float(x[2 * t + 1]) * (role.intra * ex2_approx(l * g2));
+              l -= (float)sign;
+              pk[t] = pack_bf16(y0, y1);
             }
           }
-          tmem_st8(srow0 + 16 * ch + 8 * q, x);
+          if (side == 0) {
+            // bits t and 16 + t, moved to the sign bits of bytes 0 and 2, spread
+            // over the two halves of the word
+            const uint32_t bits = (k & 1) ? kept[1] : kept[0];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) pk[t] &= spread_signs(bits << (7 - t));
+          }
         }
+        tmem_st8(srow0 + 8 * k, pk);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -566,7 +613,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       __syncwarp();
       const uint32_t src = sb + s * L::kStageBytes + L::kOffV,
                      dst = sb + L::kOffVp + (c % L::kVpBufs) * 2 * kBlock;
-#pragma unroll 4
+#pragma unroll 2
       for (int q = 0; q < 8; ++q) {
         const uint32_t off = sw128_offset(j, q);
         uint32_t x[4], hi[4], lo[4];
@@ -588,80 +635,80 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const float f_full = role.inter * decay_pow(g, (rev ? kT - 1 - r : r) + e0);
-    const int gi = lane & 3;
-    const int left = role.dvo - c0 - 16 * gi;  // columns of this lane's pieces, a multiple of 8
-    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0 + 16 * gi;
+    const int odd = lane & 1;
+    const int row0 = r & ~1;
+    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0 + 16 * odd;
+    const uint32_t o1 = taddr(tmem, wq * 32, kColO1), o2 = taddr(tmem, wq * 32, kColO2);
     // 32-byte stores where every piece is whole and 32-byte aligned
     const bool wide = ((uintptr_t)out & 31) == 0 && role.ot % 16 == 0 && role.dvo % 16 == 0;
-    const uint32_t orow = taddr(tmem, wq * 32, kColO1);
     for (int c = 0; c < tiles; ++c) {
       const int64_t base = tile_start(c);
       const int len = tile_len(c);
       const float f = !rev || len == kT ? f_full : role.inter * decay_pow(g, len - 1 - r);
       const uint64_t f2 = f2pack(f, f);
-      mbar_wait(&bars[kOReady], c & 1, abort_flag);
+      mbar_wait(&bars[kRead + (c & 1)], (c / 2) & 1, abort_flag);
+      mbar_wait(&bars[kOReady + (c & 1)], (c / 2) & 1, abort_flag);
+      // the tile's scores, A S and P V are done with its stage
+      if (wq == 0 && lane == 0) mbar_arrive(&bars[kEmpty + c % kStages]);
       __syncwarp();
       tc_fence_after();
-      uint32_t w[32];
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {  // 32 columns
+        uint32_t w[16];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t x[16], y[16];
-        tmem_ld16(orow + 16 * h, x);
-        tmem_ld16(orow + (kColO2 - kColO1) + 16 * h, y);
-        tmem_wait_ld();
+        for (int q = 0; q < 2; ++q) {
+          uint32_t x[16], y[16];
+          tmem_ld16(o1 + 32 * h + 16 * q, x);
+          tmem_ld16(o2 + 32 * h + 16 * q, y);
+          tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[8 * h + i] = pack_bf16x2(
-              ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
-                    f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
-      }
-      // O is in registers: its columns are free before the stores
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kOFree]);
-      // 4x4 transpose of 32-byte pieces inside each group of four lanes: a store
-      // instruction then writes eight whole 128-byte rows, not 32 pieces of 32
-      // rows (173 -> 151 us at 64 heads of 128, N = 8192)
-#pragma unroll
-      for (int mm = 2; mm >= 1; mm >>= 1) {
-        const bool hi = (gi & mm) != 0;
-#pragma unroll
-        for (int kx = 0; kx < 2; ++kx) {
-          const int s0 = mm == 2 ? kx : (kx << 1);
-          const int s1 = s0 | mm;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t send = hi ? w[8 * s0 + i] : w[8 * s1 + i];
-            const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, mm);
-            if (hi) w[8 * s0 + i] = recv;
-            else w[8 * s1 + i] = recv;
-          }
+          for (int i = 0; i < 8; ++i)
+            w[8 * q + i] = pack_bf16x2(
+                ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
+                      f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
         }
-      }
-      const int first = wq * 32 + (lane & ~3);
-      __nv_bfloat16 *dst = out + (base + first) * role.ot;
+        if (h == 1) {  // O is in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kOFree + (c & 1)]);
+        }
+        // neighbouring lanes exchange 32-byte pieces: a store instruction then
+        // writes 64 bytes of 16 rows, not 32 bytes of 32 (the row-per-lane form
+        // took 173 us where whole pieces took 151: 64 heads of 128, N = 8192)
 #pragma unroll
-      for (int i = 0; i < 4; ++i, dst += role.ot) {
-        if (first + i >= len) continue;
-        if (wide) {
-          if (left >= 16)
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
-                         "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]),
-                         "r"(w[8 * i + 4]), "r"(w[8 * i + 5]), "r"(w[8 * i + 6]),
-                         "r"(w[8 * i + 7])
-                         : "memory");
-        } else {
-          if (left > 0) *(uint4 *)dst = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
-          if (left > 8)
-            *(uint4 *)(dst + 8) =
-                make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t send = odd ? w[i] : w[8 + i];
+          const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, 1);
+          if (odd) w[i] = recv;
+          else w[8 + i] = recv;
+        }
+        // rows (lane & ~1) and + 1, columns 32 h + 16 odd
+        const int left = role.dvo - c0 - 32 * h - 16 * odd;  // a multiple of 8
+        __nv_bfloat16 *dst = out + (base + row0) * role.ot + 32 * h;
+#pragma unroll
+        for (int i = 0; i < 2; ++i, dst += role.ot) {
+          if (row0 + i >= len) continue;
+          if (wide) {
+            if (left >= 16)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
+                           "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]),
+                           "r"(w[8 * i + 3]), "r"(w[8 * i + 4]), "r"(w[8 * i + 5]),
+                           "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                           : "memory");
+          } else {
+            if (left > 0)
+              *(uint4 *)dst = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+            if (left > 8)
+              *(uint4 *)(dst + 8) =
+                  make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+          }
         }
       }
     }
   }
 
   // ---------------------------------------------------------------- teardown
-  // Both issuers have seen their last MMA complete before they get here.
+  // The issuers have seen their last MMA complete before they get here.
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
