@@ -14,7 +14,7 @@ from .kernels.chunked_attention import (  # noqa: F401
 from .kernels.sliding_attention import nki_sliding_window_attn, ref_sliding_window_attn  # noqa: F401
 from .kernels.based_layer import based_layer, ref_based_layer  # noqa: F401
 from .kernels.based_module import (  # noqa: F401
-    TrainiumBasedLinearAttention, TrainiumBasedLinearAttentionNKI)
+    DecayLinearAttention, TrainiumBasedLinearAttention, TrainiumBasedLinearAttentionNKI)
 from .kernels.decay_attention import (  # noqa: F401
     decay_linear_attention, decay_linear_attention_step, ref_decay_attn)
 from .kernels.rms_norm import ref_rms_norm, rms_norm, rms_norm_fp8  # noqa: F401
@@ -27,6 +27,6 @@ __all__ = [
     "ref_identity_numerator", "based_chunked_host", "nki_sliding_window_attn",
     "ref_sliding_window_attn", "based_layer", "ref_based_layer",
     "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI",
-    "decay_linear_attention", "decay_linear_attention_step", "ref_decay_attn",
+    "DecayLinearAttention", "decay_linear_attention", "decay_linear_attention_step", "ref_decay_attn",
     "rms_norm", "rms_norm_fp8", "ref_rms_norm", "LaError",
 ]

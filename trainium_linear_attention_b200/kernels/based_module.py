@@ -9,8 +9,13 @@ wrappers (benchmarks/based_attention_benchmark.py:24-69):
 * ``TrainiumBasedLinearAttentionNKI(dim, heads=8, eps=1e-6, window_size=None)``
   -- the kernel path: ``solution_nki`` (the parallel BASED kernel) as in the
   reference; ``attention="auto"`` uses ``solution`` instead (parallel or
-  chunked by the measured crossover), and ``window_size`` adds the
-  sliding-window term (the full BASED layer, ``based_layer``).
+  chunked by the measured crossover), ``window_size`` adds the
+  sliding-window term (the full BASED layer, ``based_layer``), and
+  ``pre_norm`` puts the root-mean-square norm with the residual stream ahead
+  of the projections (``rms_norm``).
+* ``DecayLinearAttention(dim, heads=8, ...)`` -- the same projections around
+  linear attention with a decay for each head (``decay_linear_attention``) and
+  a norm of each head's output, trainable, with ``step`` for single tokens.
 
 The projections are ``nn.Linear`` layers without bias (cuBLAS GEMMs); the
 attention runs on the library's sm_100a kernels, which fail loudly when the
@@ -24,7 +29,9 @@ import torch
 import torch.nn as nn
 
 from .based_layer import based_layer
+from .decay_attention import decay_linear_attention, decay_linear_attention_step
 from .pytorch_attention import ref_based_attn, solution, solution_nki
+from .rms_norm import rms_norm
 
 
 class _Projections(nn.Module):
@@ -72,11 +79,15 @@ class TrainiumBasedLinearAttentionNKI(_Projections):
     ``attention``: "parallel" (``solution_nki``, the reference's call) or
     "auto" (``solution``).  ``window_size``: if set, the full BASED layer
     (linear attention + sliding-window softmax over the last ``window_size``
-    keys) replaces the linear attention.
+    keys) replaces the linear attention.  ``pre_norm``: the hidden states (plus
+    ``residual``, if given) are normed ahead of the projections; the call then
+    returns (output, residual stream), the second being the sum that the next
+    block adds this block's output to.
     """
 
     def __init__(self, dim: int, heads: int = 8, eps: float = 1e-6,
-                 window_size: int | None = None, attention: str = "parallel"):
+                 window_size: int | None = None, attention: str = "parallel",
+                 pre_norm: bool = False):
         super().__init__(dim, heads, eps)
         if attention not in ("parallel", "auto"):
             raise ValueError("attention must be 'parallel' or 'auto'")
@@ -84,6 +95,15 @@ class TrainiumBasedLinearAttentionNKI(_Projections):
             raise ValueError("window_size must be >= 1")
         self.window_size = window_size
         self.attention = attention
+        self.norm_weight = nn.Parameter(torch.ones(dim)) if pre_norm else None
+
+    def forward(self, hidden_states: torch.Tensor, residual: torch.Tensor | None = None):
+        if self.norm_weight is None:
+            if residual is not None:
+                raise ValueError("residual needs pre_norm=True")
+            return super().forward(hidden_states)
+        normed, stream = _pre_norm(hidden_states, residual, self.norm_weight, self.eps)
+        return super().forward(normed), stream
 
     def _attend(self, q, k, v):
         if self.window_size is not None:
@@ -91,3 +111,70 @@ class TrainiumBasedLinearAttentionNKI(_Projections):
         if self.attention == "auto":
             return solution(q, k, v, eps=self.eps)
         return solution_nki(q, k, v, eps=self.eps)
+
+
+def _pre_norm(hidden_states, residual, weight, eps):
+    """(norm of hidden_states + residual, the sum itself)."""
+    if residual is None:
+        return rms_norm(hidden_states, weight, eps=eps), hidden_states
+    return rms_norm(hidden_states, weight, residual=residual, eps=eps)
+
+
+class DecayLinearAttention(_Projections):
+    """Block of linear attention with a decay for each head, on the sm_100a kernels.
+
+    norm (with the residual stream) -> q, k, v projections -> decayed linear
+    attention -> norm of each head's output -> output projection.  The heads
+    are read as the projections leave them and the heads' norm writes
+    (b, t, dim) rows: no transposed copies.  ``log_decay``: fp32 (heads,), by
+    default the geometric slopes -2^(-8 i / heads), i = 1 .. heads; a buffer,
+    not trained.  The projections and norms are; gradients run through the
+    operators' own backward kernels.
+
+    ``forward(x, residual=None, state=None, return_state=False)`` -> (output,
+    residual stream[, state]) for a prompt, or the next piece of one with
+    ``state``; ``step(x, state, residual=None)`` -> (output, residual stream)
+    for one token per sequence (x: (b, dim)), ``state`` (fp32 (b, heads,
+    head_dim, head_dim), zeros for a new sequence) updated in place.
+    """
+
+    def __init__(self, dim: int, heads: int = 8, eps: float = 1e-6, log_decay=None):
+        super().__init__(dim, heads, eps)
+        self.norm_weight = nn.Parameter(torch.ones(dim))
+        self.head_norm_weight = nn.Parameter(torch.ones(self.head_dim))
+        if log_decay is None:
+            log_decay = -torch.exp2(-8.0 * torch.arange(1, heads + 1) / heads)
+        log_decay = torch.as_tensor(log_decay, dtype=torch.float32).detach().clone()
+        if tuple(log_decay.shape) != (heads,):
+            raise ValueError(f"log_decay must be ({heads},), got {tuple(log_decay.shape)}")
+        self.register_buffer("log_decay", log_decay)
+
+    def _apply(self, fn, recurse=True):
+        # the decay stays fp32 when the module is cast
+        super()._apply(fn, recurse)
+        self.log_decay = self.log_decay.float()
+        return self
+
+    def _finish(self, y: torch.Tensor) -> torch.Tensor:
+        """Heads' norm and output projection of y (..., heads, head_dim)."""
+        y = rms_norm(y, self.head_norm_weight, eps=self.eps)
+        return self.o_proj(y.flatten(-2))
+
+    def forward(self, hidden_states: torch.Tensor, residual: torch.Tensor | None = None,
+                state: torch.Tensor | None = None, return_state: bool = False):
+        x, stream = _pre_norm(hidden_states, residual, self.norm_weight, self.eps)
+        got = decay_linear_attention(
+            self._heads(self.q_proj, x), self._heads(self.k_proj, x), self._heads(self.v_proj, x),
+            self.log_decay, initial_state=state, return_state=return_state)
+        y, end = got if return_state else (got, None)
+        out = self._finish(y.transpose(1, 2))
+        return (out, stream, end) if return_state else (out, stream)
+
+    @torch.no_grad()
+    def step(self, hidden_states: torch.Tensor, state: torch.Tensor,
+             residual: torch.Tensor | None = None):
+        x, stream = _pre_norm(hidden_states, residual, self.norm_weight, self.eps)
+        b = x.shape[0]
+        q, k, v = (p(x).view(b, self.num_heads, self.head_dim)
+                   for p in (self.q_proj, self.k_proj, self.v_proj))
+        return self._finish(decay_linear_attention_step(q, k, v, self.log_decay, state)), stream

@@ -301,7 +301,7 @@ class _DecayPlan:
     """One signature of the decayed linear attention: sizes, strides, workspace."""
 
     __slots__ = ("index", "device", "dtype", "sizes", "scale", "pack", "copy", "strides",
-                 "outs", "out_strides", "state_shape", "ws_bytes")
+                 "outs", "out_strides", "state_shape", "ws_bytes", "pad")
 
     def __init__(self, q, k, v, log_decay, states, grad, segments):
         code = _check_qkv(q, k, v)
@@ -322,6 +322,9 @@ class _DecayPlan:
         read = (q, k, v) if grad is None else (q, k, v, grad)
         # bf16 rows of whole 16-byte packs have to start at 16 bytes
         self.pack = tuple(q.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0 for x in read)
+        # widths that no 16-byte pack divides are widened with zeros for the
+        # tensor-core kernel (the CUDA-core one takes them as they are)
+        self.pad = (-d % 8, -dv % 8) if q.dtype == torch.bfloat16 and (d % 8 or dv % 8) else None
         self.strides = tuple(_heads_strides(x) for x in read)
         self.copy = any(s is None for s in self.strides)
         written = (v,) if grad is None else (q, k, v)
@@ -370,11 +373,33 @@ def _readable(plan, tensors):
     return [_in_place(x, s, p) for x, s, p in zip(tensors, plan.strides, plan.pack)]
 
 
+def _widen(x, by, rows_by=0):
+    """``x`` with ``by`` more zero columns (and ``rows_by`` more rows)."""
+    return None if x is None else torch.nn.functional.pad(x, (0, by, 0, rows_by))
+
+
+def _narrowed(outs, tensors):
+    """The leading columns of ``tensors`` laid out as the plan's outputs."""
+    got = []
+    for o, x in zip(outs, tensors):
+        y = _empty_heads(*o)
+        got.append(y.copy_(x[..., :o[3]]))
+    return got
+
+
 def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_state: bool = False,
                     segments: int = 0):
     """Forward pass of the decayed linear attention (no autograd): the output,
     or (output, final state fp32 (b, h, d_qk, d_v))."""
     plan = _decay_plan(q, k, v, log_decay, initial_state, None, None, segments)
+    if plan.pad is not None:
+        a, b = plan.pad
+        out, final = decay_attention(_widen(q, a), _widen(k, a), _widen(v, b), log_decay,
+                                     plan.scale if scale is None else scale,
+                                     _widen(initial_state, b, a), True, segments)
+        out, = _narrowed(plan.outs, (out,))
+        _, _, d, dv = plan.state_shape
+        return (out, final[:, :, :d, :dv].contiguous()) if return_state else out
     again = _readable(plan, (q, k, v))
     if again is not None:
         out = decay_attention(*again, log_decay, scale, initial_state, return_state, segments)
@@ -411,6 +436,15 @@ def decay_attention_backward(q, k, v, log_decay, d_out, scale=None, initial_stat
     """Gradients (dq, dk, dv, d_initial_state or None) of ``decay_attention``
     for the gradients of its output and (``d_state``) of its final state."""
     plan = _decay_plan(q, k, v, log_decay, initial_state, d_state, d_out, segments)
+    if plan.pad is not None:
+        a, b = plan.pad
+        *grads, g0 = decay_attention_backward(
+            _widen(q, a), _widen(k, a), _widen(v, b), log_decay, _widen(d_out, b),
+            plan.scale if scale is None else scale, _widen(initial_state, b, a),
+            _widen(d_state, b, a), want_d_initial, segments)
+        _, _, d, dv = plan.state_shape
+        return (*_narrowed(plan.outs, grads),
+                None if g0 is None else g0[:, :, :d, :dv].contiguous())
     again = _readable(plan, (q, k, v, d_out))
     if again is not None:
         q, k, v, d_out = again
