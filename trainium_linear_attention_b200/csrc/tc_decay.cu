@@ -145,14 +145,6 @@ __device__ __forceinline__ uint32_t hfma2_bf16(uint32_t a, uint32_t b, uint32_t 
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-__device__ __forceinline__ uint32_t hneg2_bf16(uint32_t a) { return a ^ 0x80008000u; }
-
-// The signs of bytes 0 and 2 over the low and the high half of a word.
-__device__ __forceinline__ uint32_t spread_signs(uint32_t x) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %1, 0xAA88;" : "=r"(d) : "r"(x));
-  return d;
-}
 
 __device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();
@@ -473,7 +465,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       if (c >= updates) break;
       const int len = tile_len(c);
       const float keep = len == kT ? keep_full : decay_pow(g, len);
-      const uint64_t keep2 = f2pack(keep, keep);
+      const uint64_t keep2 = f2pack(keep, keep), minus2 = f2pack(-1.f, -1.f);
       mbar_wait(&bars[kUReady + (c & 1)], (c / 2) & 1, abort_flag);
       // B and V of the tile's stage have been read by U (and V')
       if (warp == L::kWState && lane == 0) mbar_arrive(&bars[kEmpty + c % kStages]);
@@ -488,8 +480,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const uint64_t u = fadd2(f2pack(__uint_as_float(hi[i]), __uint_as_float(hi[i + 1])),
-                                   f2pack(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1])));
+          const uint64_t u =
+              ffma2(f2pack(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1])), minus2,
+                    f2pack(__uint_as_float(hi[i]), __uint_as_float(hi[i + 1])));
           f2unpack(ffma2(keep2, f2pack(st[8 * q + i], st[8 * q + i + 1]), u), st[8 * q + i],
                    st[8 * q + i + 1]);
         }
@@ -522,35 +515,42 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const bool mild = g >= -4.f && g <= 4.f;
     const int row_lag = (wq * 32 + lane - 64 * half) * sign;  // lag of the warp's first column
     uint64_t w2[8];
-    uint32_t kept[2] = {0, 0};  // columns with lag >= 0 of the diagonal's two chunks
+    uint32_t cut[2][8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int n0 = rev ? 2 * t : 15 - 2 * t, n1 = rev ? 2 * t + 1 : 14 - 2 * t;
       w2[t] = f2pack(decay_pow(g, n0) * role.intra, decay_pow(g, n1) * role.intra);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {  // even columns in the low half, odd ones in the high
+      for (int q = 0; q < 2; ++q) {
         const int lag = rev ? 16 * q - lane + 2 * t : lane - 16 * q - 2 * t;
-        kept[q] |= (lag >= 0 ? 1u << t : 0u) | (lag - sign >= 0 ? 0x10000u << t : 0u);
+        cut[q][t] = (lag >= 0 ? 0xFFFFu : 0u) | (lag - sign >= 0 ? 0xFFFF0000u : 0u);
       }
     }
+    // the warp's two blocks of 32 columns: before, on or beyond the diagonal
+    const int side0 = (2 * half - wq) * sign, side1 = (2 * half + 1 - wq) * sign;
     for (int c = 0; c < tiles; ++c) {
       const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + (c & 1) * 128 + half * 64);
       mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
       __syncwarp();
       tc_fence_after();
-      // 16 columns at a time.  Rolled, like the other loops here: the warps of a
-      // scheduler run six different ones, and where those did not fit its
-      // instruction cache together the kernel took 1.3 times as long.
+      // Rolled, like the other loops here: the warps of a scheduler run six
+      // different ones, and where those did not fit its instruction cache
+      // together the kernel took 1.3 times as long.
 #pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        const int side = (2 * half + (k >> 1) - wq) * sign;
-        uint32_t x[16], pk[8];
+      for (int ch = 0; ch < 2; ++ch) {
+        const int side = ch ? side1 : side0;
         if (side > 0) {  // beyond the diagonal
+          uint32_t z[16];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) pk[t] = 0;
-        } else {
-          const int lag = row_lag - sign * 16 * k;  // of the first column
-          tmem_ld16(srow0 + 16 * k, x);
+          for (int i = 0; i < 16; ++i) z[i] = 0;
+          tmem_st16(srow0 + 16 * ch, z);
+          continue;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int lag = row_lag - sign * (32 * ch + 16 * q);  // of the first column
+          uint32_t x[16], pk[8];
+          tmem_ld16(srow0 + 32 * ch + 16 * q, x);
           tmem_wait_ld();
           if (side < 0 || mild) {
             // (below -15 every column is cut)
@@ -574,14 +574,11 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
             }
           }
           if (side == 0) {
-            // bits t and 16 + t, moved to the sign bits of bytes 0 and 2, spread
-            // over the two halves of the word
-            const uint32_t bits = (k & 1) ? kept[1] : kept[0];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) pk[t] &= spread_signs(bits << (7 - t));
+            for (int t = 0; t < 8; ++t) pk[t] &= cut[q][t];
           }
+          tmem_st8(srow0 + 16 * ch + 8 * q, pk);
         }
-        tmem_st8(srow0 + 8 * k, pk);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -600,10 +597,11 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const float w = rev || len == kT ? w_full : role.inc * decay_pow(g, len - 1 - j);
       // w as two bf16 terms; with x * w_hi rounded to hi, the rest of that
       // product is a bf16 value and fma gives it exactly: three packed
-      // instructions per two values, off by 2^-17 + 2^-18 at most
+      // instructions per two values.  They leave -lo, which the state warps
+      // subtract.
       const uint32_t w_hi = pack_bf16(w, w);
-      const float rest = w - bf16lo(w_hi);
-      const uint32_t w_lo = pack_bf16(rest, rest);
+      const float rest = bf16lo(w_hi) - w;
+      const uint32_t minus_hi = w_hi ^ 0x80008000u, minus_lo = pack_bf16(rest, rest);
       mbar_wait(&bars[kFull + s], (c / kStages) & 1, abort_flag);
       // U of the tile that used this buffer before has been formed
       if (c >= L::kVpBufs) {
@@ -621,7 +619,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           hi[i] = hmul2_bf16(x[i], w_hi);
-          lo[i] = hfma2_bf16(x[i], w_lo, hfma2_bf16(x[i], w_hi, hneg2_bf16(hi[i])));
+          lo[i] = hfma2_bf16(x[i], minus_lo, hfma2_bf16(x[i], minus_hi, hi[i]));
         }
         st_shared_v4(dst + off, hi[0], hi[1], hi[2], hi[3]);
         st_shared_v4(dst + kBlock + off, lo[0], lo[1], lo[2], lo[3]);
