@@ -31,6 +31,8 @@
 // Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state
 // (4 warps at DK = 64, 8 at 128); 8 warps P; 4
 // warps V'; 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
+#include <type_traits>
+
 #include "decay.cuh"
 #include "tc_common.cuh"
 #include "tc_kernels.cuh"
@@ -186,9 +188,11 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   const int updates = want_final ? tiles : (tiles > 0 ? tiles - 1 : 0);
   const float g = p.log_decay[ih];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // first token and valid tokens of the walk's tile c
+  // first token of the walk's tile c; its tokens: 128 but for the ragged tile,
+  // which is the walk's last, in a reversed walk its first
   auto tile_start = [&](int c) { return t0 + (int64_t)(rev ? tiles - 1 - c : c) * kT; };
-  auto tile_len = [&](int c) { return (int)min64(kT, t1 - tile_start(c)); };
+  const int ragged = rev ? 0 : tiles - 1;
+  const int ragged_len = (int)(t1 - t0) - (tiles - 1) * kT;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
@@ -444,7 +448,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       for (int i = 0; i < 32; ++i)
         if (i < cols) st[i] = src[i * step];
     }
-    const float keep_full = decay_pow(g, kT);
+    const float keep_full = decay_pow(g, kT), keep_ragged = decay_pow(g, ragged_len);
+    const uint64_t minus2 = f2pack(-1.f, -1.f);
+    int stage = 0;
 #pragma unroll 1
     for (int c = 0;; ++c) {
       if (!kStateOnly && c < tiles) {  // the copy of S that tile c reads
@@ -463,12 +469,12 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         if (lane == 0) mbar_arrive(&bars[kSnapReady + b]);
       }
       if (c >= updates) break;
-      const int len = tile_len(c);
-      const float keep = len == kT ? keep_full : decay_pow(g, len);
-      const uint64_t keep2 = f2pack(keep, keep), minus2 = f2pack(-1.f, -1.f);
+      const float keep = c == ragged ? keep_ragged : keep_full;
+      const uint64_t keep2 = f2pack(keep, keep);
       mbar_wait(&bars[kUReady + (c & 1)], (c / 2) & 1, abort_flag);
       // B and V of the tile's stage have been read by U (and V')
-      if (warp == L::kWState && lane == 0) mbar_arrive(&bars[kEmpty + c % kStages]);
+      if (warp == L::kWState && lane == 0) mbar_arrive(&bars[kEmpty + stage]);
+      if (++stage == kStages) stage = 0;
       __syncwarp();
       tc_fence_after();
       const uint32_t urow = taddr(tmem, wq * 32, kColU + (c % L::kUBufs) * 128 + half * 32);
@@ -513,6 +519,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // are non-negative; on it the first reaches -15, which fp32 holds while
     // |g| <= 4, and the columns with lag < 0 are cut from the packed words.
     const bool mild = g >= -4.f && g <= 4.f;
+    const int off = rev ? 0 : 15;
     const int row_lag = (wq * 32 + lane - 64 * half) * sign;  // lag of the warp's first column
     uint64_t w2[8];
     uint32_t cut[2][8];
@@ -528,73 +535,79 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     }
     // the warp's two blocks of 32 columns: before, on or beyond the diagonal
     const int side0 = (2 * half - wq) * sign, side1 = (2 * half + 1 - wq) * sign;
-    for (int c = 0; c < tiles; ++c) {
-      const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + (c & 1) * 128 + half * 64);
-      mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
-      __syncwarp();
-      tc_fence_after();
-      // Rolled, like the other loops here: the warps of a scheduler run six
-      // different ones, and where those did not fit its instruction cache
-      // together the kernel took 1.3 times as long.
+    auto walk = [&](auto is_mild) {
+      for (int c = 0; c < tiles; ++c) {
+        const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + (c & 1) * 128 + half * 64);
+        mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
+        __syncwarp();
+        tc_fence_after();
+        // Rolled, like the other loops here: the warps of a scheduler run six
+        // different ones, and where those did not fit its instruction cache
+        // together the kernel took 1.3 times as long.
 #pragma unroll 1
-      for (int ch = 0; ch < 2; ++ch) {
-        const int side = ch ? side1 : side0;
-        if (side > 0) {  // beyond the diagonal
-          uint32_t z[16];
+        for (int ch = 0; ch < 2; ++ch) {
+          const int side = ch ? side1 : side0;
+          if (side > 0) {  // beyond the diagonal
+            uint32_t z[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) z[i] = 0;
-          tmem_st16(srow0 + 16 * ch, z);
-          continue;
-        }
+            for (int i = 0; i < 16; ++i) z[i] = 0;
+            tmem_st16(srow0 + 16 * ch, z);
+            continue;
+          }
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int lag = row_lag - sign * (32 * ch + 16 * q);  // of the first column
-          uint32_t x[16], pk[8];
-          tmem_ld16(srow0 + 32 * ch + 16 * q, x);
-          tmem_wait_ld();
-          if (side < 0 || mild) {
-            // (below -15 every column is cut)
-            const float f = ex2_approx((float)max(rev ? lag : lag - 15, -15) * g2);
-            const uint64_t f2 = f2pack(f, f);
+          for (int q = 0; q < 2; ++q) {
+            const int lag = row_lag - sign * (32 * ch + 16 * q);  // of the first column
+            uint32_t x[16], pk[8];
+            tmem_ld16(srow0 + 32 * ch + 16 * q, x);
+            tmem_wait_ld();
+            if (decltype(is_mild)::value || side < 0) {
+              // (below -15 every column is cut)
+              const float f = ex2_approx((float)max(lag - off, -15) * g2);
+              const uint64_t f2 = f2pack(f, f);
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-              pk[t] = pack_bf16x2(
-                  fmul2(fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
-                              w2[t]),
-                        f2));
-          } else {  // strong decays: each column its own power
-            float l = (float)lag;
+              for (int t = 0; t < 8; ++t)
+                pk[t] = pack_bf16x2(
+                    fmul2(fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
+                                w2[t]),
+                          f2));
+            } else {  // strong decays: each column its own power
+              float l = (float)lag;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-              const float y0 = __uint_as_float(x[2 * t]) * (role.intra * ex2_approx(l * g2));
-              l -= (float)sign;
-              const float y1 = __uint_as_float(x[2 * t + 1]) * (role.intra * ex2_approx(l * g2));
-              l -= (float)sign;
-              pk[t] = pack_bf16(y0, y1);
+              for (int t = 0; t < 8; ++t) {
+                const float y0 = __uint_as_float(x[2 * t]) * (role.intra * ex2_approx(l * g2));
+                l -= (float)sign;
+                const float y1 = __uint_as_float(x[2 * t + 1]) * (role.intra * ex2_approx(l * g2));
+                l -= (float)sign;
+                pk[t] = pack_bf16(y0, y1);
+              }
             }
-          }
-          if (side == 0) {
+            if (side == 0) {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) pk[t] &= cut[q][t];
+              for (int t = 0; t < 8; ++t) pk[t] &= cut[q][t];
+            }
+            tmem_st8(srow0 + 16 * ch + 8 * q, pk);
           }
-          tmem_st8(srow0 + 16 * ch + 8 * q, pk);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kPReady + (c & 1)]);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kPReady + (c & 1)]);
-    }
+    };
+    // (two loops, so that the rare one's code does not lie inside the other)
+    if (mild) walk(std::true_type{});
+    else walk(std::false_type{});
   } else if (warp >= L::kWV && warp < L::kWE) {
     // ------------------------------------------------------------ V' = hi + lo
     const int j = (warp - L::kWV) * 32 + lane;  // token of the tile
-    // place in a full tile: forward len - 1 - j, reversed (len - 1 - j mirrored) j + 1
+    // tokens from this one to the tile's end; in a reversed walk the tile ends at
+    // its first token, and the state there decays once more
     const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
+    const float w_ragged = role.inc * decay_pow(g, rev ? j + 1 : ragged_len - 1 - j);
+    int s = 0, phase = 0, vb = 0;
     if (!kStateOnly && order > 0) named_barrier_sync(1, L::kStateWarps * 32 + 128);
     for (int c = 0; c < updates; ++c) {
-      const int s = c % kStages;
-      const int len = tile_len(c);
-      const float w = rev || len == kT ? w_full : role.inc * decay_pow(g, len - 1 - j);
+      const float w = c == ragged ? w_ragged : w_full;
       // w as two bf16 terms; with x * w_hi rounded to hi, the rest of that
       // product is a bf16 value and fma gives it exactly: three packed
       // instructions per two values.  They leave -lo, which the state warps
@@ -602,7 +615,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const uint32_t w_hi = pack_bf16(w, w);
       const float rest = bf16lo(w_hi) - w;
       const uint32_t minus_hi = w_hi ^ 0x80008000u, minus_lo = pack_bf16(rest, rest);
-      mbar_wait(&bars[kFull + s], (c / kStages) & 1, abort_flag);
+      mbar_wait(&bars[kFull + s], phase, abort_flag);
       // U of the tile that used this buffer before has been formed
       if (c >= L::kVpBufs) {
         const int u = c - L::kVpBufs;
@@ -610,7 +623,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       }
       __syncwarp();
       const uint32_t src = sb + s * L::kStageBytes + L::kOffV,
-                     dst = sb + L::kOffVp + (c % L::kVpBufs) * 2 * kBlock;
+                     dst = sb + L::kOffVp + vb * 2 * kBlock;
 #pragma unroll 2
       for (int q = 0; q < 8; ++q) {
         const uint32_t off = sw128_offset(j, q);
@@ -626,83 +639,97 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kVpReady + c % L::kVpBufs]);
+      if (lane == 0) mbar_arrive(&bars[kVpReady + vb]);
+      if (++s == kStages) s = 0, phase ^= 1;
+      if (++vb == L::kVpBufs) vb = 0;
     }
   } else if (!kStateOnly && warp >= L::kWE) {
     // ------------------------------------------------------------ epilogue
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const float f_full = role.inter * decay_pow(g, (rev ? kT - 1 - r : r) + e0);
+    const float f_ragged = role.inter * decay_pow(g, (rev ? ragged_len - 1 - r : r) + e0);
     const int odd = lane & 1;
     const int row0 = r & ~1;
-    __nv_bfloat16 *out = role.out + ib * role.ob + ih * role.oh + c0 + 16 * odd;
+    const int64_t ot = role.ot;
+    // columns from this lane's first on, a multiple of 8
+    const int columns = role.dvo - c0 - 16 * odd;
+    __nv_bfloat16 *dst = role.out + ib * role.ob + ih * role.oh + (tile_start(0) + row0) * ot + c0 +
+                         16 * odd;
+    const int64_t tile_step = (rev ? -kT : kT) * ot;
     const uint32_t o1 = taddr(tmem, wq * 32, kColO1), o2 = taddr(tmem, wq * 32, kColO2);
-    // 32-byte stores where every piece is whole and 32-byte aligned
-    const bool wide = ((uintptr_t)out & 31) == 0 && role.ot % 16 == 0 && role.dvo % 16 == 0;
-    for (int c = 0; c < tiles; ++c) {
-      const int64_t base = tile_start(c);
-      const int len = tile_len(c);
-      const float f = !rev || len == kT ? f_full : role.inter * decay_pow(g, len - 1 - r);
-      const uint64_t f2 = f2pack(f, f);
-      mbar_wait(&bars[kRead + (c & 1)], (c / 2) & 1, abort_flag);
-      mbar_wait(&bars[kOReady + (c & 1)], (c / 2) & 1, abort_flag);
-      // the tile's scores, A S and P V are done with its stage
-      if (wq == 0 && lane == 0) mbar_arrive(&bars[kEmpty + c % kStages]);
-      __syncwarp();
-      tc_fence_after();
+    auto walk = [&](auto is_wide) {
+      int stage = 0;
+      for (int c = 0; c < tiles; ++c, dst += tile_step) {
+        const int len = c == ragged ? ragged_len : kT;
+        const float f = c == ragged ? f_ragged : f_full;
+        const uint64_t f2 = f2pack(f, f);
+        mbar_wait(&bars[kRead + (c & 1)], (c / 2) & 1, abort_flag);
+        mbar_wait(&bars[kOReady + (c & 1)], (c / 2) & 1, abort_flag);
+        // the tile's scores, A S and P V are done with its stage
+        if (wq == 0 && lane == 0) mbar_arrive(&bars[kEmpty + stage]);
+        if (++stage == kStages) stage = 0;
+        __syncwarp();
+        tc_fence_after();
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {  // 32 columns
-        uint32_t w[16];
+        for (int h = 0; h < 2; ++h) {  // 32 columns
+          uint32_t w[16];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t x[16], y[16];
-          tmem_ld16(o1 + 32 * h + 16 * q, x);
-          tmem_ld16(o2 + 32 * h + 16 * q, y);
-          tmem_wait_ld();
+          for (int q = 0; q < 2; ++q) {
+            uint32_t x[16], y[16];
+            tmem_ld16(o1 + 32 * h + 16 * q, x);
+            tmem_ld16(o2 + 32 * h + 16 * q, y);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[8 * q + i] = pack_bf16x2(
-                ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
-                      f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
-        }
-        if (h == 1) {  // O is in registers
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kOFree + (c & 1)]);
-        }
-        // neighbouring lanes exchange 32-byte pieces: a store instruction then
-        // writes 64 bytes of 16 rows, not 32 bytes of 32 (the row-per-lane form
-        // took 173 us where whole pieces took 151: 64 heads of 128, N = 8192)
+            for (int i = 0; i < 8; ++i)
+              w[8 * q + i] = pack_bf16x2(
+                  ffma2(f2pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2,
+                        f2pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]))));
+          }
+          if (h == 1) {  // O is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[kOFree + (c & 1)]);
+          }
+          // neighbouring lanes exchange 32-byte pieces: a store instruction then
+          // writes 64 bytes of 16 rows, not 32 bytes of 32 (the row-per-lane form
+          // took 173 us where whole pieces took 151: 64 heads of 128, N = 8192)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t send = odd ? w[i] : w[8 + i];
-          const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, 1);
-          if (odd) w[i] = recv;
-          else w[8 + i] = recv;
-        }
-        // rows (lane & ~1) and + 1, columns 32 h + 16 odd
-        const int left = role.dvo - c0 - 32 * h - 16 * odd;  // a multiple of 8
-        __nv_bfloat16 *dst = out + (base + row0) * role.ot + 32 * h;
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t send = odd ? w[i] : w[8 + i];
+            const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, 1);
+            if (odd) w[i] = recv;
+            else w[8 + i] = recv;
+          }
+          const int left = columns - 32 * h;
 #pragma unroll
-        for (int i = 0; i < 2; ++i, dst += role.ot) {
-          if (row0 + i >= len) continue;
-          if (wide) {
-            if (left >= 16)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst),
-                           "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]),
-                           "r"(w[8 * i + 3]), "r"(w[8 * i + 4]), "r"(w[8 * i + 5]),
-                           "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
-                           : "memory");
-          } else {
-            if (left > 0)
-              *(uint4 *)dst = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
-            if (left > 8)
-              *(uint4 *)(dst + 8) =
-                  make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+          for (int i = 0; i < 2; ++i) {
+            if (row0 + i >= len) continue;
+            __nv_bfloat16 *at = dst + 32 * h + i * ot;
+            if constexpr (decltype(is_wide)::value) {
+              if (left >= 16)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at),
+                             "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]),
+                             "r"(w[8 * i + 3]), "r"(w[8 * i + 4]), "r"(w[8 * i + 5]),
+                             "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                             : "memory");
+            } else {
+              if (left > 0)
+                *(uint4 *)at = make_uint4(w[8 * i], w[8 * i + 1], w[8 * i + 2], w[8 * i + 3]);
+              if (left > 8)
+                *(uint4 *)(at + 8) =
+                    make_uint4(w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]);
+            }
           }
         }
       }
-    }
+    };
+    // 32-byte stores where every piece is whole and 32-byte aligned
+    if (((uintptr_t)role.out & 31) == 0 && role.ob % 16 == 0 && role.oh % 16 == 0 &&
+        ot % 16 == 0 && role.dvo % 16 == 0)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
   }
 
   // ---------------------------------------------------------------- teardown
