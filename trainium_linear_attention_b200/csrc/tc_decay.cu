@@ -450,6 +450,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     }
     const float keep_full = decay_pow(g, kT), keep_ragged = decay_pow(g, ragged_len);
     const uint64_t minus2 = f2pack(-1.f, -1.f);
+    const uint32_t copy_row = sb + L::kOffSnap + sw128_offset(row, half * 4);
     int stage = 0;
 #pragma unroll 1
     for (int c = 0;; ++c) {
@@ -457,10 +458,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         const int b = c & 1;
         if (c >= 2) mbar_wait(&bars[kRead + b], ((c - 2) / 2) & 1, abort_flag);
         __syncwarp();
-        const uint32_t dst = sb + L::kOffSnap + b * L::kSnapBytes;
+        const uint32_t dst = copy_row + b * L::kSnapBytes;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          st_shared_v4(dst + sw128_offset(row, half * 4 + q), pack_bf16(st[8 * q], st[8 * q + 1]),
+          st_shared_v4(dst ^ (16 * q), pack_bf16(st[8 * q], st[8 * q + 1]),
                        pack_bf16(st[8 * q + 2], st[8 * q + 3]),
                        pack_bf16(st[8 * q + 4], st[8 * q + 5]),
                        pack_bf16(st[8 * q + 6], st[8 * q + 7]));
@@ -604,6 +605,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // its first token, and the state there decays once more
     const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
     const float w_ragged = role.inc * decay_pow(g, rev ? j + 1 : ragged_len - 1 - j);
+    const uint32_t row = sb + sw128_offset(j, 0);
     int s = 0, phase = 0, vb = 0;
     if (!kStateOnly && order > 0) named_barrier_sync(1, L::kStateWarps * 32 + 128);
     for (int c = 0; c < updates; ++c) {
@@ -622,20 +624,19 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         mbar_wait(&bars[kUReady + (u & 1)], (u / 2) & 1, abort_flag);
       }
       __syncwarp();
-      const uint32_t src = sb + s * L::kStageBytes + L::kOffV,
-                     dst = sb + L::kOffVp + vb * 2 * kBlock;
+      const uint32_t src = row + s * L::kStageBytes + L::kOffV,
+                     dst = row + L::kOffVp + vb * 2 * kBlock;
 #pragma unroll 2
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t off = sw128_offset(j, q);
+      for (uint32_t q = 0; q < 8 * 16; q += 16) {  // a piece of the row: its swizzle is an xor
         uint32_t x[4], hi[4], lo[4];
-        ld_shared_v4(src + off, x[0], x[1], x[2], x[3]);
+        ld_shared_v4(src ^ q, x[0], x[1], x[2], x[3]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           hi[i] = hmul2_bf16(x[i], w_hi);
           lo[i] = hfma2_bf16(x[i], minus_lo, hfma2_bf16(x[i], minus_hi, hi[i]));
         }
-        st_shared_v4(dst + off, hi[0], hi[1], hi[2], hi[3]);
-        st_shared_v4(dst + kBlock + off, lo[0], lo[1], lo[2], lo[3]);
+        st_shared_v4(dst ^ q, hi[0], hi[1], hi[2], hi[3]);
+        st_shared_v4((dst ^ q) + kBlock, lo[0], lo[1], lo[2], lo[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
