@@ -156,7 +156,7 @@ def test_c_entry_points_refuse():
 
 
 # --------------------------------------------------------------------- GPU
-WIDTHS = [(16, 64), (64, 64), (128, 128), (64, 128), (40, 72), (128, 8), (57, 33), (1, 1)]
+WIDTHS = [(16, 64), (24, 32), (32, 128), (64, 64), (128, 128), (64, 128), (40, 72), (128, 8), (57, 33), (1, 1)]
 
 
 @gpu
@@ -248,7 +248,8 @@ def test_long_sequence_many_tiles():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("t,dk,dv,segments", [(1, 16, 64, 0), (70, 64, 64, 0), (129, 40, 72, 0),
                                               (300, 128, 64, 0), (1000, 64, 128, 3),
-                                              (333, 57, 33, 0), (2049, 64, 64, 5)])
+                                              (333, 57, 33, 0), (2049, 64, 64, 5), (700, 24, 32, 3),
+                                              (260, 32, 16, 0)])
 def test_gradients(t, dk, dv, segments, dtype):
     q, k, v, g, state = make(2, 2, t, dk, dv, dtype, "bthd", seed=t)
     do = torch.randn(2, 2, t, dv, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()

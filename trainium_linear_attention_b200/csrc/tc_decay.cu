@@ -57,8 +57,13 @@ constexpr int kJoinPitch = 65;  // floats per row of a joined state: rows in oth
 
 template <int DK, bool kStateOnly>
 struct TcLayout {
-  static constexpr int kKBlocks = DK / 64;
-  static constexpr int kStateWarps = DK == 64 ? 4 : 8;
+  // A and B: blocks of 64 columns (128-byte rows), or one of 32 (64-byte rows)
+  static constexpr int kKBlocks = DK == 32 ? 1 : DK / 64;
+  static constexpr int kKBlock = DK == 32 ? kBlock / 2 : kBlock;
+  static constexpr auto kKSwizzle = DK == 32 ? kSwizzle64B : kSwizzle128B;
+  static constexpr int kKGroup = DK == 32 ? 512 : 1024;  // bytes of 8 tokens
+  static constexpr int kStateWarps = DK == 128 ? 8 : 4;
+  static constexpr int kStateCols = DK == 32 ? 16 : 32;  // columns of S per thread
   static constexpr int kWState = 4;
   static constexpr int kWP = kWState + kStateWarps;  // first P warp
   static constexpr int kWV = kStateOnly ? kWP : kWP + 8;
@@ -67,11 +72,11 @@ struct TcLayout {
   static constexpr int kThreads = kWarps * 32;
   // stage: A, B (kKBlocks blocks each), V (one block)
   static constexpr uint32_t kOffA = 0;
-  static constexpr uint32_t kOffB = kStateOnly ? 0 : kKBlocks * kBlock;
-  static constexpr uint32_t kOffV = kOffB + kKBlocks * kBlock;
+  static constexpr uint32_t kOffB = kStateOnly ? 0 : kKBlocks * kKBlock;
+  static constexpr uint32_t kOffV = kOffB + kKBlocks * kKBlock;
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
-  static constexpr int kVpBufs = DK == 64 || kStateOnly ? 2 : 1;
+  static constexpr int kVpBufs = DK <= 64 || kStateOnly ? 2 : 1;
   static constexpr int kUBufs = kStateOnly ? 2 : 1;
   static constexpr uint32_t kFixed =
       kVpBufs * 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
@@ -105,6 +110,8 @@ enum Bar {
 };
 static_assert(8 * kNumBars + 8 <= 512, "barrier area");
 
+constexpr int kMaxMaps = 8;  // four tensors, in boxes of 64 columns and of 32
+
 struct TcRole {
   int a, b, v;  // which tensor map
   __nv_bfloat16 *out;
@@ -116,7 +123,7 @@ struct TcRole {
 };
 
 struct TcParams {
-  CUtensorMap map[4];
+  CUtensorMap map[kMaxMaps];
   TcRole role[kDecayMaxRoles];
   const float *log_decay;
   int *err;
@@ -279,9 +286,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         mbar_arrive_expect_tx(&bars[kFull + s], L::kStageBytes);
 #pragma unroll
         for (int b = 0; b < L::kKBlocks; ++b) {
-          tma_load_4d(st + L::kOffB + b * kBlock, mb, &bars[kFull + s], 64 * b, y, ih, ib);
+          tma_load_4d(st + L::kOffB + b * L::kKBlock, mb, &bars[kFull + s], 64 * b, y, ih, ib);
           if (!kStateOnly)
-            tma_load_4d(st + L::kOffA + b * kBlock, ma, &bars[kFull + s], 64 * b, y, ih, ib);
+            tma_load_4d(st + L::kOffA + b * L::kKBlock, ma, &bars[kFull + s], 64 * b, y, ih, ib);
         }
         tma_load_4d(st + L::kOffV, mv, &bars[kFull + s], c0, y, ih, ib);
       }
@@ -297,8 +304,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       constexpr uint32_t id_s = make_idesc_bf16(128, 128, false, false);
       constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
       const int k_steps = (role.da + 15) / 16;  // the columns beyond are zero
-      const uint64_t a0 = make_sdesc(sb + L::kOffA, 16, 1024, kSwizzle128B);
-      const uint64_t b0 = make_sdesc(sb + L::kOffB, 16, 1024, kSwizzle128B);
+      const uint64_t a0 = make_sdesc(sb + L::kOffA, 16, L::kKGroup, L::kKSwizzle);
+      const uint64_t b0 = make_sdesc(sb + L::kOffB, 16, L::kKGroup, L::kKSwizzle);
       const uint64_t s0 = make_sdesc(sb + L::kOffSnap, 16, 1024, kSwizzle128B);
       int ss = 0, sp = 0;  // stage of the next scores and its phase
       auto issue_scores = [&](int c) -> bool {
@@ -311,8 +318,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         const uint32_t d = tmem + kColScores + (c & 1) * 128;
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < DK / 16; ++kk) {  // 32 bytes along the 128-byte rows
-            const uint64_t step = at + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2);
+          for (int kk = 0; kk < DK / 16; ++kk) {  // 32 bytes along the rows
+            const uint64_t step = at + (uint64_t)((kk / 4) * (L::kKBlock >> 4) + (kk % 4) * 2);
             if (kk < k_steps) umma_ss(d, a0 + step, b0 + step, id_s, kk > 0);
           }
           umma_commit(&bars[kSReady + (c & 1)]);
@@ -341,7 +348,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
           for (int kk = 0; kk < DK / 16; ++kk)
             if (kk < k_steps)
               umma_ss(tmem + kColO1,
-                      a0 + at + (uint64_t)((kk / 4) * (kBlock >> 4) + (kk % 4) * 2),
+                      a0 + at + (uint64_t)((kk / 4) * (L::kKBlock >> 4) + (kk % 4) * 2),
                       s0 + (uint64_t)(b * (L::kSnapBytes >> 4) + kk * (2048 >> 4)), id_o, kk > 0);
           umma_commit(&bars[kRead + b]);
         }
@@ -357,9 +364,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   } else if (warp == 2) {
     // ------------------------------------------------------------ U = B^T V'
     constexpr uint32_t id_u = make_idesc_bf16(128, 128, true, true);
-    // A = B^T: the second 64 rows of M are the next 64 columns (DK = 128), or the
-    // same ones again (DK = 64)
-    const uint64_t a0 = make_sdesc(sb + L::kOffB, DK == 64 ? 0 : kBlock, 1024, kSwizzle128B);
+    // A = B^T: M's 128 rows are two blocks of 64 columns, or with DK < 128 the
+    // same columns over again
+    const uint64_t a0 =
+        make_sdesc(sb + L::kOffB, DK == 128 ? kBlock : 0, L::kKGroup, L::kKSwizzle);
     const uint64_t b0 = make_sdesc(sb + L::kOffVp, kBlock, 1024, kSwizzle128B);
     int us = 0, up = 0;  // stage and its phase
     for (int c = 0; c < updates; ++c) {
@@ -378,8 +386,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kT / 16; ++kk) {
-          const uint64_t step = (uint64_t)(kk * (2048 >> 4));
-          umma_ss(d, da + step, db + step, id_u, kk > 0);
+          umma_ss(d, da + (uint64_t)(kk * (2 * L::kKGroup >> 4)),
+                  db + (uint64_t)(kk * (2048 >> 4)), id_u, kk > 0);
         }
         umma_commit(&bars[kUReady + (c & 1)]);
       }
@@ -422,35 +430,37 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     }
   } else if (warp >= L::kWState && warp < L::kWP) {
     // ------------------------------------------------------------ state
-    // A thread owns 32 columns of one row of S.
+    // A thread owns kCols columns of one row of S; where TMEM's lanes hold the
+    // rows more than once, each copy's warps take other columns.
+    constexpr int kCols = L::kStateCols;
     const int wq = warp & 3;  // TMEM lane quarter
-    const int row = DK == 64 ? (wq & 1) * 32 + lane : wq * 32 + lane;
-    const int half = DK == 64 ? wq >> 1 : (warp - L::kWState) >> 2;
-    const int col = c0 + half * 32;
-    float st[32];
+    const int row = DK == 32 ? lane : DK == 64 ? (wq & 1) * 32 + lane : wq * 32 + lane;
+    const int part = DK == 32 ? wq : DK == 64 ? wq >> 1 : (warp - L::kWState) >> 2;
+    const int col = c0 + part * kCols;
+    float st[kCols];
     const int64_t per_head = (int64_t)role.da * role.dvo;
     const bool mine = row < role.da;
-    const int cols = mine ? min(32, role.dvo - col) : 0;  // may be negative
+    const int cols = mine ? min(kCols, role.dvo - col) : 0;  // may be negative
 #pragma unroll
-    for (int i = 0; i < 32; ++i) st[i] = 0.f;
+    for (int i = 0; i < kCols; ++i) st[i] = 0.f;
     if constexpr (kStateOnly) {
       grid_dependents_launch();
     } else if (order > 0) {
-      const float *src = joined + row * kJoinPitch + half * 32;
+      const float *src = joined + row * kJoinPitch + part * kCols;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) st[i] = src[i];
+      for (int i = 0; i < kCols; ++i) st[i] = src[i];
       named_barrier_arrive(1, L::kStateWarps * 32 + 128);  // V' may take the space
     } else if (role.init) {
       const int64_t step = role.transposed ? role.da : 1;
       const float *src = role.init + bh * per_head + (role.transposed ? (int64_t)col * role.da + row
                                                                       : (int64_t)row * role.dvo + col);
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < kCols; ++i)
         if (i < cols) st[i] = src[i * step];
     }
     const float keep_full = decay_pow(g, kT), keep_ragged = decay_pow(g, ragged_len);
     const uint64_t minus2 = f2pack(-1.f, -1.f);
-    const uint32_t copy_row = sb + L::kOffSnap + sw128_offset(row, half * 4);
+    const uint32_t copy_row = sb + L::kOffSnap + sw128_offset(row, part * (kCols / 8));
     int stage = 0;
 #pragma unroll 1
     for (int c = 0;; ++c) {
@@ -460,7 +470,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         __syncwarp();
         const uint32_t dst = copy_row + b * L::kSnapBytes;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < kCols / 8; ++q)
           st_shared_v4(dst ^ (16 * q), pack_bf16(st[8 * q], st[8 * q + 1]),
                        pack_bf16(st[8 * q + 2], st[8 * q + 3]),
                        pack_bf16(st[8 * q + 4], st[8 * q + 5]),
@@ -478,9 +488,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       if (++stage == kStages) stage = 0;
       __syncwarp();
       tc_fence_after();
-      const uint32_t urow = taddr(tmem, wq * 32, kColU + (c % L::kUBufs) * 128 + half * 32);
+      const uint32_t urow = taddr(tmem, wq * 32, kColU + (c % L::kUBufs) * 128 + part * kCols);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < kCols / 8; ++q) {
         uint32_t hi[8], lo[8];
         tmem_ld8(urow + 8 * q, hi);
         tmem_ld8(urow + 64 + 8 * q, lo);
@@ -503,7 +513,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
                                : role.final_state + bh * per_head) +
                    (int64_t)row * role.dvo + col;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < kCols; ++i)
         if (i < cols) dst[i] = st[i];
     }
   } else if (!kStateOnly && warp >= L::kWP && warp < L::kWV) {
@@ -744,9 +754,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.err, kErrTimeout);
 }
 
-// 4-D map (width, tokens, heads, batch) with a 64 x 128 box; outside reads as
-// zero.
-bool make_map(CUtensorMap *map, const DecayView &x, int width, const DecayCall &c) {
+// 4-D map (width, tokens, heads, batch) with a box of 64 or 32 columns x 128
+// tokens; outside reads as zero.
+bool make_map(CUtensorMap *map, const DecayView &x, int width, int box_cols, const DecayCall &c) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t one = (cuuint64_t)width * 2;  // a dimension of one entry has no stride
@@ -755,10 +765,11 @@ bool make_map(CUtensorMap *map, const DecayView &x, int width, const DecayCall &
   cuuint64_t gstride[3] = {c.n > 1 ? (cuuint64_t)x.st * 2 : one,
                            c.heads > 1 ? (cuuint64_t)x.sh * 2 : one,
                            c.batch > 1 ? (cuuint64_t)x.sb * 2 : one};
-  cuuint32_t box[4] = {64, kT, 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)box_cols, kT, 1, 1};
   cuuint32_t estride[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(x.p), gdim, gstride, box,
-            estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -793,25 +804,30 @@ int launch(const DecayCall &c, cudaStream_t s) {
   int maps = 0, da = 0, slices = 1;
   struct {
     DecayView x;
-    int width;
-  } known[4];
-  auto map_of = [&](const DecayView &x, int width) {
+    int width, box;
+  } known[kMaxMaps];
+  auto map_of = [&](const DecayView &x, int width, int box) {
     for (int i = 0; i < maps; ++i) {
       const DecayView &y = known[i].x;
-      if (y.p == x.p && y.sb == x.sb && y.sh == x.sh && y.st == x.st && known[i].width == width)
+      if (y.p == x.p && y.sb == x.sb && y.sh == x.sh && y.st == x.st &&
+          known[i].width == width && known[i].box == box)
         return i;
     }
-    if (maps == 4 || !make_map(&p.map[maps], x, width, c)) return -1;
+    if (maps == kMaxMaps || !make_map(&p.map[maps], x, width, box, c)) return -1;
     known[maps].x = x;
     known[maps].width = width;
+    known[maps].box = box;
     return maps++;
   };
+  for (int r = 0; r < c.roles; ++r)
+    if (c.role[r].da > da) da = c.role[r].da;
+  const int box = da <= 32 ? 32 : 64;
   for (int r = 0; r < c.roles; ++r) {
     const DecayRole &f = c.role[r];
     TcRole &t = p.role[r];
-    t.a = kStateOnly ? 0 : map_of(f.a, f.da);
-    t.b = map_of(f.b, f.da);
-    t.v = map_of(f.v, f.dvo);
+    t.a = kStateOnly ? 0 : map_of(f.a, f.da, box);
+    t.b = map_of(f.b, f.da, box);
+    t.v = map_of(f.v, f.dvo, 64);
     if (t.a < 0 || t.b < 0 || t.v < 0) return LA_ERR_CUDA;
     t.out = (__nv_bfloat16 *)f.out.p;
     t.ob = f.out.sb, t.oh = f.out.sh, t.ot = f.out.st;
@@ -819,7 +835,6 @@ int launch(const DecayCall &c, cudaStream_t s) {
     t.da = f.da, t.dvo = f.dvo;
     t.transposed = f.transposed, t.reverse = f.reverse;
     t.intra = f.intra, t.inter = f.inter, t.inc = f.inc;
-    if (f.da > da) da = f.da;
     const int n = (f.dvo + kDecaySlice - 1) / kDecaySlice;
     if (n > slices) slices = n;
   }
@@ -829,6 +844,7 @@ int launch(const DecayCall &c, cudaStream_t s) {
   p.orders = kStateOnly ? c.segments - 1 : c.segments;
   const int64_t grid = c.batch * c.heads * p.orders * slices * c.roles;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  if (da <= 32) return launch_t<32, kStateOnly>(p, grid, s);
   return da <= 64 ? launch_t<64, kStateOnly>(p, grid, s) : launch_t<128, kStateOnly>(p, grid, s);
 }
 
