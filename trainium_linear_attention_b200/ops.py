@@ -236,9 +236,20 @@ def based_layer(q, k, v, window_size: int = 64, eps: float = 1e-6, segments: int
 # out at the first call of a signature and kept under it, so that a decoding
 # step or a small norm does not spend more time here than on the GPU.  Nothing
 # is kept by a tensor's address or contents.
-_Strides = ctypes.c_int64 * 3
+_Int64x3 = ctypes.c_int64 * 3
 _MAX_PLANS = 4096
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+class _Strides(int):
+    """The address of three int64, with the array that holds them: what ctypes
+    converts fastest."""
+
+    def __new__(cls, *values):
+        array = _Int64x3(*values)
+        self = super().__new__(cls, ctypes.addressof(array))
+        self.array = array
+        return self
 
 
 def _sig(t):
@@ -274,7 +285,9 @@ def _tokens_first(t: torch.Tensor) -> bool:
     return t.shape[1] > 1 and t.shape[2] > 1 and t.stride(1) < t.stride(2)
 
 
-def _empty_heads(b, h, n, d, dtype, device, tokens_first):
+def _empty_heads(b, h, n, d, dtype, device, tokens_first, like=None):
+    if like is not None:  # dense, and laid out as wanted
+        return torch.empty_like(like)
     if tokens_first:
         return torch.empty((b, n, h, d), dtype=dtype, device=device).transpose(1, 2)
     return torch.empty((b, h, n, d), dtype=dtype, device=device)
@@ -301,7 +314,7 @@ class _DecayPlan:
     """One signature of the decayed linear attention: sizes, strides, workspace."""
 
     __slots__ = ("index", "device", "dtype", "sizes", "scale", "pack", "copy", "strides",
-                 "outs", "out_strides", "state_shape", "ws_bytes", "pad")
+                 "outs", "dense", "out_strides", "state_shape", "ws_bytes", "pad")
 
     def __init__(self, q, k, v, log_decay, states, grad, segments):
         code = _check_qkv(q, k, v)
@@ -330,6 +343,8 @@ class _DecayPlan:
         written = (v,) if grad is None else (q, k, v)
         self.outs = tuple((b, h, t, x.shape[-1], x.dtype, x.device, _tokens_first(x))
                           for x in written)
+        self.dense = tuple((x.transpose(1, 2) if o[-1] else x).is_contiguous()
+                           for x, o in zip(written, self.outs))
         self.out_strides = tuple(
             _Strides(h * t * w, w if first else t * w, h * w if first else w)
             for _, _, _, w, _, _, first in self.outs)
@@ -368,8 +383,13 @@ def _in_place(x: torch.Tensor, strides, pack: bool) -> torch.Tensor:
 
 def _readable(plan, tensors):
     """The inputs as the kernels can read them, or None if they already are."""
-    if not plan.copy and not any(p and x.data_ptr() & 15 for p, x in zip(plan.pack, tensors)):
-        return None
+    if not plan.copy:
+        odd = 0
+        for p, x in zip(plan.pack, tensors):
+            if p:
+                odd |= x.data_ptr()
+        if not odd & 15:
+            return None
     return [_in_place(x, s, p) for x, s, p in zip(tensors, plan.strides, plan.pack)]
 
 
@@ -412,7 +432,7 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_s
         with torch.cuda.device(plan.index):
             return decay_attention(q, k, v, log_decay, scale, initial_state, return_state,
                                    segments)
-    out = _empty_heads(*plan.outs[0])
+    out = _empty_heads(*plan.outs[0], v if plan.dense[0] else None)
     final = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
              if return_state else None)
     if not log_decay.is_contiguous():
@@ -454,7 +474,8 @@ def decay_attention_backward(q, k, v, log_decay, d_out, scale=None, initial_stat
         with torch.cuda.device(plan.index):
             return decay_attention_backward(q, k, v, log_decay, d_out, scale, initial_state,
                                             d_state, want_d_initial, segments)
-    gq, gk, gv = (_empty_heads(*o) for o in plan.outs)
+    gq, gk, gv = (_empty_heads(*o, x if dense else None)
+                  for o, x, dense in zip(plan.outs, (q, k, v), plan.dense))
     g0 = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
           if want_d_initial else None)
     log_decay = log_decay.contiguous()
@@ -561,7 +582,8 @@ class _NormPlan:
     the first of them under ``name``, the others of the same shape and type."""
 
     __slots__ = ("index", "device", "dtype", "shape", "lead", "d", "codes", "strides", "c_shape",
-                 "copy", "aligned", "weight_copy", "group", "scales_shape", "ws_bytes")
+                 "copy", "aligned", "weight_copy", "as_is", "dense", "group", "scales_shape",
+                 "ws_bytes")
 
     def __init__(self, rows, names, weight, group_size):
         x = rows[0]
@@ -603,8 +625,10 @@ class _NormPlan:
         self.aligned = self.group != d
         if self.aligned and not any(self.copy):
             pack = 16 // x.element_size()
-            self.copy = tuple(t is not None and any(n % pack for n in s)
+            self.copy = tuple(t is not None and any(n % pack for n in s.array)
                               for t, s in zip(rows, self.strides))
+        self.as_is = not any(self.copy) and not self.weight_copy
+        self.dense = x.is_contiguous()
         n = ctypes.c_size_t(0)
         with _on_device(x.device):
             N.check(N.lib().la_rms_norm_bwd_workspace_size(x.numel() // d, d, ctypes.byref(n)),
@@ -629,6 +653,8 @@ def _norm_plan(rows, names, weight, group_size=None) -> _NormPlan:
 def _norm_inputs(plan, rows, weight):
     """The rows and the weight as the kernels can read them, or None if they
     already are."""
+    if plan.as_is and not plan.aligned:
+        return None
     tensors = (*rows, weight)
     copies = [*plan.copy, plan.weight_copy]
     if plan.aligned:
@@ -638,6 +664,13 @@ def _norm_inputs(plan, rows, weight):
         return None
     return [t.clone(memory_format=torch.contiguous_format) if c else t
             for c, t in zip(copies, tensors)]
+
+
+def _empty_rows(plan, like, dtype=None):
+    """An empty contiguous tensor of the rows' shape; ``like`` has that shape."""
+    if plan.dense:
+        return torch.empty_like(like, dtype=dtype)
+    return torch.empty(plan.shape, dtype=dtype or plan.dtype, device=plan.device)
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, want_rstd: bool = False):
@@ -650,7 +683,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, want_rstd: bool =
     if plan.index != _get_device():
         with torch.cuda.device(plan.index):
             return rms_norm(x, weight, residual, eps, want_rstd)
-    y = torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
+    y = _empty_rows(plan, x)
     total = torch.empty_like(y) if residual is not None else None
     rstd = (torch.empty(plan.lead, dtype=torch.float32, device=plan.device) if want_rstd
             else None)
@@ -672,10 +705,9 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6, group_size: i
     if plan.index != _get_device():
         with torch.cuda.device(plan.index):
             return rms_norm_fp8(x, weight, residual, eps, group_size)
-    y = torch.empty(plan.shape, dtype=torch.float8_e4m3fn, device=plan.device)
+    y = _empty_rows(plan, x, torch.float8_e4m3fn)
     scales = torch.empty(plan.scales_shape, dtype=torch.float32, device=plan.device)
-    total = (torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
-             if residual is not None else None)
+    total = _empty_rows(plan, x) if residual is not None else None
     st = N.lib().la_rms_norm_fp8(
         x.data_ptr(), plan.strides[0], _ptr(residual), plan.strides[1], _ptr(weight), y.data_ptr(),
         scales.data_ptr(), _ptr(total), plan.c_shape, plan.d, plan.group, *plan.codes, eps,
@@ -698,7 +730,7 @@ def rms_norm_backward(s, weight, rstd, d_y, d_sum=None, want_d_weight: bool = Tr
     if rstd.shape != plan.lead or rstd.dtype != torch.float32 or rstd.device != plan.device:
         raise ValueError(f"rstd must be float32 {tuple(plan.lead)} on {plan.device}")
     rstd = rstd.contiguous()
-    d_s = torch.empty(plan.shape, dtype=plan.dtype, device=plan.device)
+    d_s = _empty_rows(plan, s)
     d_w = workspace = None
     if want_d_weight and weight is not None:
         d_w = torch.empty_like(weight)
