@@ -367,6 +367,43 @@ def test_step_refuses():
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_left_padded_batch(dtype):
+    """Sequences of different lengths, padded on the left with zero keys, end in
+    their own states and outputs."""
+    q, k, v, g, _ = make(3, 2, 300, 64, 64, dtype)
+    lengths = (300, 131, 1)
+    for i, n in enumerate(lengths):
+        k[i, :, :300 - n] = 0
+    out, end = T.decay_linear_attention(q, k, v, g, scale=0.125, return_state=True)
+    for i, n in enumerate(lengths):
+        one = [x[i:i + 1, :, 300 - n:].double() for x in (q, k, v)]
+        s0 = torch.zeros(1, 2, 64, 64, device="cuda", dtype=torch.float64)
+        want, want_end = definition(*one, g, 0.125, s0)
+        a_out, a_end = definition(*(x.abs() for x in one), g, 0.125, s0)
+        got = out[i:i + 1, :, 300 - n:].double()
+        assert ((got - want).abs() <= bound(dtype, want, a_out, 300, 64)).all()
+        assert ((end[i:i + 1].double() - want_end).abs()
+                <= bound(torch.float32, want_end, a_end, 300, 64) + 2.0 ** -17 * a_end).all()
+
+
+@gpu
+def test_without_gradients():
+    """Inference mode, and a decay that some other code trains."""
+    q, k, v, g, _ = make(2, 3, 9, 16, 16, torch.bfloat16)
+    want = T.decay_linear_attention(q, k, v, g, return_state=True)
+    g = g.clone().requires_grad_()
+    with pytest.raises(ValueError, match="log_decay"):
+        T.decay_linear_attention(q, k, v, g)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            out, state = T.decay_linear_attention(q, k, v, g, return_state=True)
+            assert torch.equal(out, want[0]) and torch.equal(state, want[1])
+            y = T.decay_linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g, state)
+            assert torch.isfinite(y).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_prompt_in_pieces_then_tokens(dtype):
     """A prompt read at once, in pieces, and token by token end in one state."""
     q, k, v, g, _ = make(2, 4, 300, 64, 64, dtype)

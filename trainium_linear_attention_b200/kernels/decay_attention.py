@@ -80,7 +80,15 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     ``initial_state``: fp32 (b, h, d_qk, d_v), the state before the first
     token.  Returns (b, h, t, d_v) in q.dtype, or with ``return_state`` also
     the fp32 state after the last token.  Differentiable once in q, k, v and
-    ``initial_state``."""
+    ``initial_state``.
+
+    Sequences of different lengths in one batch: pad them on the left with zero
+    k (a zero token adds nothing to the zero state, and ends where the others
+    do), or leave out what the right padding returns; a value that is not
+    finite reaches the outputs of its own tile of 128 tokens, so padding should
+    be finite.  bf16 runs on tensor cores: the weights of a tile's values and
+    the state's read-out are rounded to bf16, the state is carried in fp32 and
+    fed with 16-bit products (2^-17)."""
     if torch.is_grad_enabled() and any(
             isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, initial_state)):
         return _DecayAttention.apply(q, k, v, log_decay, initial_state, scale, bool(return_state))

@@ -299,7 +299,7 @@ def _check_log_decay(log_decay, heads, device):
     if (log_decay.dtype != torch.float32 or log_decay.device != device
             or tuple(log_decay.shape) != (heads,)):
         raise ValueError(f"log_decay must be float32 ({heads},) on {device}")
-    if log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay is a constant of the operator: it has no gradient")
 
 
@@ -364,7 +364,7 @@ def _decay_plan(q, k, v, log_decay, initial_state, d_state, grad, segments) -> _
         key = (_sig(q), _sig(k), _sig(v), _sig(log_decay), _sig(initial_state), _sig(d_state),
                _sig(grad), segments)
         plan = _decay_plans.get(key)
-        if plan is not None and not log_decay.requires_grad:
+        if plan is not None and not (log_decay.requires_grad and torch.is_grad_enabled()):
             return plan
     except AttributeError:  # not tensors: the checks say which
         key = None
@@ -532,7 +532,7 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
     fp32 (b, h, d_qk, d_v) is updated in place.  Returns (b, h, d_v)."""
     try:
         key = (_sig(q), _sig(k), _sig(v), _sig(log_decay), _sig(state))
-        plan = None if log_decay.requires_grad else _step_plans.get(key)
+        plan = _step_plans.get(key)
     except AttributeError:  # not tensors: the checks say which
         key = plan = None
     if plan is None:
@@ -555,7 +555,8 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
         _stream_ptr(plan.device))
     if st != N.LA_OK:
         N.check(st, "la_decay_step")
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return out
 
 
