@@ -203,6 +203,44 @@ def test_segments(t, segments, dtype):
 
 
 @gpu
+def test_some_heads_split():
+    """More heads than SMs: whole ones fill a wave, the rest share the next in
+    segments (the default split; seen by its smaller workspace)."""
+    import ctypes
+
+    from trainium_linear_attention_b200 import _native as N
+
+    b, h, t = 4, 16, 4000
+    q, k, v, g, state = make(b, h, t, 64, 64, torch.bfloat16, "bthd")
+    n, ws = ctypes.c_int(0), ctypes.c_size_t(0)
+    assert N.lib().la_decay_plan(b, h, t, 64, 64, 1, 1, 0, ctypes.byref(n), ctypes.byref(ws)) == 0
+    every = 2 * b * h * n.value * 64 * 64 * 4
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert n.value > 1 and 0 < ws.value < every
+    do, ds = torch.randn_like(v), torch.randn_like(state)
+    got = ops.decay_attention_backward(q, k, v, g, do, scale=0.2, initial_state=state, d_state=ds,
+                                       want_d_initial=True)
+    pick = torch.tensor([0, 17, 48, 49, 55, 63], device="cuda")  # whole and split ones
+
+    def heads(x):
+        return x.flatten(0, 1)[pick][None]
+
+    def formulas(absolute):
+        leaves = [heads(x).double() for x in (q, k, v, state)]
+        up = [heads(x).double() for x in (do, ds)]
+        if absolute:
+            leaves, up = [x.abs() for x in leaves], [x.abs() for x in up]
+        leaves = [x.requires_grad_() for x in leaves]
+        out, end = definition(*leaves[:3], g[pick % h], 0.2, leaves[3])
+        return torch.autograd.grad((out, end), leaves, up)
+
+    for i, (x, y, a) in enumerate(zip(got, formulas(False), formulas(True))):
+        kind = torch.float32 if i == 3 else torch.bfloat16
+        slack = 2.0 ** -17 if i == 3 else 0.0
+        assert ((heads(x).double() - y).abs() <= bound(kind, y, a, t, 64) + slack * a).all(), i
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_decays(dtype):
     """No decay, none of the past, and everything between; an infinite decay is

@@ -33,8 +33,8 @@ struct DecayRole {
   DecayView a, b, v;
   DecayView out;                 // written; unused by a state pass
   const float *init = nullptr;   // null, or the state the walk starts with, per head
-  // What each segment adds to the state, in the walk's order, the last one's
-  // left out: states[bh * segments + o].  Written by a state pass, read by the
+  // What each segment of a split head adds to the state, in the walk's order,
+  // the last one's left out: states[(bh - whole) * segments + o].  Written by a state pass, read by the
   // output pass, whose segment o starts with
   //   lambda^(tokens before o) init + sum_{i<o} lambda^(tokens between i and o) states_i.
   float *states = nullptr;
@@ -57,6 +57,9 @@ struct DecayCall {
   int roles = 0;
   const float *log_decay = nullptr;
   int64_t batch = 0, heads = 0, n = 0;
+  // heads [0, whole) of batch x heads are walked by one CTA each, the others in
+  // `segments` segments of seg_len tokens
+  int64_t whole = 0;
   int64_t seg_len = 0;
   int segments = 1;
   int dtype = 0;
@@ -81,8 +84,8 @@ __host__ __device__ __forceinline__ int segment_tokens(int o, bool reverse, int 
   return (int)min64(seg_len, n - at);
 }
 
-// States of every (head, segment but the walk's last) of each role into
-// role.states.
+// States of every (split head, segment but the walk's last) of each role into
+// role.states.  The CUDA-core kernels take no whole heads beside split ones.
 int launch_decay_state_simt(const DecayCall &c, cudaStream_t s);
 // Outputs (and final states) of every role.
 int launch_decay_output_simt(const DecayCall &c, cudaStream_t s);

@@ -37,54 +37,78 @@ int fit_segments(int64_t n, int64_t want, int64_t *len) {
   return (int)((n + *len - 1) / *len);
 }
 
-// Segments of each walk: the count with the lowest estimated time.  A split
-// run walks each segment but the last twice (the state pass, then the output)
-// and its later segments start by joining the states before them; an unsplit
-// one leaves SMs idle where there are few heads.
-int plan_segments(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype, bool backward,
-                  int requested, int sm_count, int64_t *len) {
-  if (requested != 0) return fit_segments(n, requested, len);
+struct DecaySplit {
+  int64_t whole = 0;  // heads walked unsplit
+  int segments = 1;   // of the others
+  int64_t len = 0;    // tokens per segment
+};
+
+// How the heads are split: the choice with the lowest estimated time.  A split
+// head's segments but the last are walked twice (the state pass, then the
+// output) and the later ones start by joining the states before them; unsplit
+// heads leave SMs idle where there are few, or in a last, partial wave of CTAs.
+// So all heads are walked whole, or all in g segments, or as many whole as fill
+// k waves and the rest in g segments that share the SMs of one more.
+DecaySplit plan_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype, bool backward,
+                      int requested, int sm_count) {
+  DecaySplit best;
+  if (requested != 0) {
+    best.segments = fit_segments(n, requested, &best.len);
+    return best;
+  }
   const int64_t sq = (d_qk + kDecaySlice - 1) / kDecaySlice;
   const int64_t sv = (d_v + kDecaySlice - 1) / kDecaySlice;
-  const int64_t ctas = bh * (backward ? 2 * sq + sv : sv);
-  const int64_t state_ctas = bh * (backward ? 2 * sv : sv);
+  const int64_t per_head = backward ? 2 * sq + sv : sv;    // CTAs that walk a head
+  const int64_t state_per_head = backward ? 2 * sv : sv;   // and in a state pass
   const bool wide = backward ? (d_qk > 64 || d_v > 64) : d_qk > 64;
   // microseconds per 128 tokens of a CTA's walk (output, state) and per wave
   // of CTAs (start-up, first loads, drain), measured on a B200; the CUDA-core
   // kernel holds two CTAs per SM up to 64 columns.  (bf16, d = 64: 64 heads of
-  // 2048 / 4096 / 8192 tokens unsplit 26 / 49 / 89 us, in two segments 29 / 48 /
-  // 82; the gradients of 64 heads of 4096 tokens unsplit 99, in two 104.)
+  // 2048 / 4096 / 8192 tokens unsplit 24 / 45 / 82 us, in two segments 28 / 45 /
+  // 76; the gradients of 64 heads of 4096 tokens, 192 CTAs, unsplit 89 us, in
+  // two segments 94.)
   const bool simt = dtype == LA_DTYPE_FLOAT32;
-  const double t_out = simt ? (wide ? 36.0 : 24.0) : (wide ? 2.3 : 1.4);
+  const double t_out = simt ? (wide ? 36.0 : 24.0) : (wide ? 2.1 : 1.3);
   const double t_state = simt ? (wide ? 14.0 : 9.0) : (wide ? 1.2 : 0.8);
   constexpr double kWaveOut = 4.0, kWaveState = 3.0, kSplit = 5.0, kJoin = 0.4;
   const int64_t slots = sm_count * (simt && !wide ? 2 : 1);
   const int64_t tiles = (n + kDecayTile - 1) / kDecayTile;
-  int best = 1;
-  int64_t best_len = 0;
-  double best_t = 0.0;
-  for (int64_t want = 1; want <= kMaxAutoSegments && want <= (tiles > 1 ? tiles : 1); ++want) {
-    int64_t l = 0;
-    const int g = fit_segments(n, want, &l);
-    if (g != want) continue;  // the same split as a smaller count
-    const double per_seg = (double)(l / kDecayTile);
-    double t = (double)((ctas * g + slots - 1) / slots) * (kWaveOut + per_seg * t_out);
-    if (g > 1)
-      t += kSplit + kJoin * (g - 1) +
-           (double)((state_ctas * (g - 1) + slots - 1) / slots) * (kWaveState + per_seg * t_state);
-    if (want == 1 || t < best_t) {
-      best = g;
-      best_len = l;
-      best_t = t;
+  const int64_t most = tiles < 1 ? 1 : tiles < kMaxAutoSegments ? tiles : kMaxAutoSegments;
+  const int64_t full_waves = simt ? 0 : bh * per_head / slots;
+  best.segments = fit_segments(n, 1, &best.len);
+  double best_t = (double)((bh * per_head + slots - 1) / slots) * (kWaveOut + tiles * t_out);
+  for (int64_t waves = 0; waves <= full_waves; ++waves) {
+    const int64_t whole = waves * slots / per_head;
+    if (whole >= bh) break;
+    if (waves > 0 && waves + 2 < full_waves) continue;  // only the last few waves matter
+    const int64_t rest = bh - whole;
+    for (int64_t want = 2; want <= most; ++want) {
+      int64_t l = 0;
+      const int g = fit_segments(n, want, &l);
+      if (g != want) continue;  // the same split as a smaller count
+      const double per_seg = (double)(l / kDecayTile);
+      const double t =
+          waves * (kWaveOut + tiles * t_out) +
+          (double)((rest * per_head * g + slots - 1) / slots) * (kWaveOut + per_seg * t_out) +
+          kSplit + kJoin * (g - 1) +
+          (double)((rest * state_per_head * (g - 1) + slots - 1) / slots) *
+              (kWaveState + per_seg * t_state);
+      if (t < best_t) {
+        best_t = t;
+        best.whole = whole;
+        best.segments = g;
+        best.len = l;
+      }
     }
   }
-  *len = best_len;
   return best;
 }
 
-size_t state_bytes(int64_t bh, int segments, int64_t d_qk, int64_t d_v, bool backward) {
-  if (segments <= 1) return 0;
-  return (size_t)(backward ? 2 : 1) * (size_t)bh * segments * (size_t)d_qk * (size_t)d_v * 4;
+// States of the split heads: of the walk ahead, and of the one back.
+size_t state_bytes(int64_t bh, const DecaySplit &s, int64_t d_qk, int64_t d_v, bool backward) {
+  if (s.segments <= 1) return 0;
+  return (size_t)(backward ? 2 : 1) * (size_t)(bh - s.whole) * s.segments * (size_t)d_qk *
+         (size_t)d_v * 4;
 }
 
 DecayView view(const void *p, const int64_t *strides) {
@@ -111,6 +135,14 @@ bool use_tensor_cores(const DecayCall &c) {
 int run_decay(const DecayCall &call, const DecayRole *state_roles, int n_state_roles,
               cudaStream_t s) {
   const bool tc = use_tensor_cores(call);
+  // (bf16 that TMA cannot address: the plan for tensor cores may leave heads
+  // whole, the CUDA-core kernels walk every head alike)
+  if (!tc && call.whole > 0) {
+    DecayCall same = call;
+    same.whole = 0;
+    same.segments = fit_segments(call.n, 1, &same.seg_len);
+    return launch_decay_output_simt(same, s);
+  }
   if (call.segments > 1) {
     DecayCall pass = call;
     pass.roles = n_state_roles;
@@ -144,10 +176,10 @@ int la_decay_plan(int64_t batch, int64_t heads, int64_t seq_len, int64_t d_qk, i
   DeviceInfo info;
   info.sm_count = 1;
   if (segments_requested == 0 && (st = require_device(&info)) != LA_OK) return st;
-  int64_t len = 0;
-  *segments_out = plan_segments(batch * heads, seq_len, d_qk, d_v, dtype, backward != 0,
-                                segments_requested, info.sm_count, &len);
-  *workspace_bytes_out = state_bytes(batch * heads, *segments_out, d_qk, d_v, backward != 0);
+  const DecaySplit split = plan_split(batch * heads, seq_len, d_qk, d_v, dtype, backward != 0,
+                                      segments_requested, info.sm_count);
+  *segments_out = split.segments;
+  *workspace_bytes_out = state_bytes(batch * heads, split, d_qk, d_v, backward != 0);
   return LA_OK;
 }
 
@@ -169,8 +201,10 @@ int la_decay_chunked_fwd(const void *q, const int64_t *q_strides, const void *k,
   DeviceInfo info;
   if ((st = require_device(&info)) != LA_OK) return st;
   DecayCall c;
-  c.segments = plan_segments(bh, seq_len, d_qk, d_v, dtype, false, segments, info.sm_count, &c.seg_len);
-  const size_t need = state_bytes(bh, c.segments, d_qk, d_v, false);
+  const DecaySplit split =
+      plan_split(bh, seq_len, d_qk, d_v, dtype, false, segments, info.sm_count);
+  c.whole = split.whole, c.segments = split.segments, c.seg_len = split.len;
+  const size_t need = state_bytes(bh, split, d_qk, d_v, false);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
     return LA_ERR_WORKSPACE;
   c.roles = 1;
@@ -216,12 +250,14 @@ int la_decay_chunked_bwd(const void *q, const int64_t *q_strides, const void *k,
   DeviceInfo info;
   if ((st = require_device(&info)) != LA_OK) return st;
   DecayCall c;
-  c.segments = plan_segments(bh, seq_len, d_qk, d_v, dtype, true, segments, info.sm_count, &c.seg_len);
-  const size_t need = state_bytes(bh, c.segments, d_qk, d_v, true);
+  const DecaySplit split =
+      plan_split(bh, seq_len, d_qk, d_v, dtype, true, segments, info.sm_count);
+  c.whole = split.whole, c.segments = split.segments, c.seg_len = split.len;
+  const size_t need = state_bytes(bh, split, d_qk, d_v, true);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
     return LA_ERR_WORKSPACE;
   float *ahead = (float *)workspace;  // the segments' states, first token first
-  float *back = ahead + (c.segments > 1 ? bh * c.segments * d_qk * d_v : 0);  // last token first
+  float *back = ahead + need / (2 * sizeof(float));  // last token first
   c.roles = 3;
   c.log_decay = log_decay;
   c.batch = batch;

@@ -127,9 +127,11 @@ struct TcParams {
   TcRole role[kDecayMaxRoles];
   const float *log_decay;
   int *err;
-  int64_t heads, n, seg_len;
-  int roles, slices, segments;
-  int orders;  // segments that this launch walks: all, or all but the last
+  int64_t heads, n;
+  // heads [0, whole) are walked by one CTA per role and slice, the others in
+  // segments; a state pass walks all but the last of those
+  int64_t whole, seg_len;
+  int roles, slices, segments, orders;
 };
 
 __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *map, uint64_t *bar,
@@ -174,23 +176,29 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   uint32_t *tmem_slot = (uint32_t *)(smem + L::kOffBar + 8 * kNumBars);
   volatile int *abort_flag = (volatile int *)(smem + L::kOffBar + 8 * kNumBars + 4);
 
-  // roles fastest, then slices: CTAs that read the same tokens run together
-  int64_t id = blockIdx.x;
+  // roles fastest, then slices: CTAs that read the same tokens run together;
+  // whole heads first, so that the shorter walks of the split ones end the grid
+  uint32_t id = blockIdx.x;
   const TcRole &role = p.role[id % p.roles];
   id /= p.roles;
   const int c0 = (int)(id % p.slices) * kDecaySlice;
   id /= p.slices;
-  const int order = (int)(id % p.orders);
-  const int64_t bh = id / p.orders;
+  const bool split = kStateOnly || id >= p.whole;
+  if (split && !kStateOnly) id -= (uint32_t)p.whole;
+  const int segments = split ? p.segments : 1;
+  const int order = split ? (int)(id % p.orders) : 0;
+  const int64_t head_at = split ? id / p.orders : 0;  // of the split heads
+  const int64_t bh = split ? p.whole + head_at : id;
+  const int64_t seg_len = split ? p.seg_len : p.n;
   if (c0 >= role.dvo) return;
   const int ib = (int)(bh / p.heads), ih = (int)(bh % p.heads);
   const bool rev = role.reverse != 0;
   const int e0 = rev ? 0 : 1;
-  const int64_t t0 = (int64_t)(rev ? p.segments - 1 - order : order) * p.seg_len;
-  const int64_t t1 = min64(p.n, t0 + p.seg_len);
+  const int64_t t0 = (int64_t)(rev ? segments - 1 - order : order) * seg_len;
+  const int64_t t1 = min64(p.n, t0 + seg_len);
   const int tiles = (int)((t1 - t0 + kT - 1) / kT);
   const bool want_final =
-      kStateOnly || (role.final_state != nullptr && order == p.segments - 1);
+      kStateOnly || (role.final_state != nullptr && order == segments - 1);
   // tiles whose U is needed: the last one's only for the final state
   const int updates = want_final ? tiles : (tiles > 0 ? tiles - 1 : 0);
   const float g = p.log_decay[ih];
@@ -245,11 +253,11 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll 2
     for (int o = order - 1; o >= 0; --o) {
       const float keep = decay_pow(g, after);
-      const float *src = role.states + (bh * p.segments + o) * per_head;
+      const float *src = role.states + (head_at * segments + o) * per_head;
 #pragma unroll
       for (int e = 0; e < kEach; ++e)
         if (at[e] >= 0) sum[e] = fmaf(keep, __ldcg(src + at[e]), sum[e]);
-      after += segment_tokens(o, rev, p.segments, p.seg_len, p.n);
+      after += segment_tokens(o, rev, segments, seg_len, p.n);
     }
     if (role.init) {
       const float keep = decay_pow(g, after);
@@ -509,7 +517,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       if (lane == 0) mbar_arrive(&bars[kUFree + (c & 1)]);
     }
     if (want_final) {
-      float *dst = (kStateOnly ? role.states + (bh * p.segments + order) * per_head
+      float *dst = (kStateOnly ? role.states + (head_at * segments + order) * per_head
                                : role.final_state + bh * per_head) +
                    (int64_t)row * role.dvo + col;
 #pragma unroll
@@ -839,10 +847,13 @@ int launch(const DecayCall &c, cudaStream_t s) {
     if (n > slices) slices = n;
   }
   p.log_decay = c.log_decay;
-  p.heads = c.heads, p.n = c.n, p.seg_len = c.seg_len;
+  p.heads = c.heads, p.n = c.n;
+  p.whole = c.whole, p.seg_len = c.seg_len;
   p.roles = c.roles, p.slices = slices, p.segments = c.segments;
   p.orders = kStateOnly ? c.segments - 1 : c.segments;
-  const int64_t grid = c.batch * c.heads * p.orders * slices * c.roles;
+  const int64_t walks =
+      (kStateOnly ? 0 : c.whole) + (c.batch * c.heads - c.whole) * (int64_t)p.orders;
+  const int64_t grid = walks * slices * c.roles;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
   if (da <= 32) return launch_t<32, kStateOnly>(p, grid, s);
   return da <= 64 ? launch_t<64, kStateOnly>(p, grid, s) : launch_t<128, kStateOnly>(p, grid, s);
