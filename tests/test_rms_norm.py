@@ -61,7 +61,7 @@ def check(x, w, r):
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("d", [1, 7, 8, 64, 65, 100, 128, 256, 264, 512, 1000, 1024, 2048, 2049,
-                               4096, 5000, 8192, 16384])
+                               4096, 5000, 5001, 8192, 9003, 16382, 16384])
 def test_widths(d, dtype):
     for rows in (1, 5, 33):
         x, r, w = make((rows, d), dtype, rows != 5, dtype if rows != 33 else torch.float32, d)
@@ -108,7 +108,10 @@ def test_extremes():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,d,residual", [(1, 64, True), (700, 64, False), (4097, 128, True),
                                              (37, 1000, True), (2500, 1024, True), (65, 2049, True),
-                                             (9, 8192, False), (3, 16384, True), (5000, 7, True)])
+                                             (9, 8192, False), (3, 16384, True), (5000, 7, True),
+                                             (20000, 37, True), (3001, 1279, False),
+                                             (1500, 2297, True), (700, 5002, True),
+                                             (400, 9003, True)])
 def test_gradients(rows, d, residual, dtype):
     x, r, w = make((rows, d), dtype, residual, dtype, rows)
     leaves = [t.requires_grad_() for t in (x, w, r) if t is not None]
@@ -196,7 +199,8 @@ def test_gradient_parts():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,d,group", [(1, 1024, None), (33, 64, 16), (33, 64, 64), (5, 100, None),
                                           (40, 4096, 128), (7, 1000, None), (3, 8192, 256),
-                                          (3, 16384, 32), (65, 96, 32), (9, 16, 16)])
+                                          (3, 16384, 32), (65, 96, 32), (9, 16, 16),
+                                          (50, 77, None), (9, 2297, None), (5, 6001, None)])
 def test_fp8(rows, d, group, dtype):
     x, r, w = make((rows, d), dtype, True, dtype, rows)
     x[0, :group or d] = 0

@@ -47,54 +47,69 @@ __device__ __forceinline__ int64_t row_offset(const Rows &t, const Shape &sh, in
   return (outer / sh.n1) * t.s0 + (outer % sh.n1) * t.s1 + (row % sh.n2) * t.s2;
 }
 
-// Column of element e of pack i of thread t: packs of 8 neighbours with 16-byte
-// accesses, single elements otherwise.
-template <int TPR, bool kVec>
-__device__ __forceinline__ int column(int t, int i, int e) {
-  return kVec ? (i * TPR + t) * 8 + e : (i * 8 + e) * TPR + t;
+// How a row is accessed: single elements (any strides); packs of 8 neighbours by
+// 16 bytes (rows that start at 16 bytes, d a multiple of 8); or, for contiguous
+// rows of any other width, packs of the memory the row lies in: the first pack
+// starts up to 7 elements before the row, and the row's two edge packs are
+// accessed element by element.
+enum Access { kSingle, kPacked, kShifted };
+
+// Elements from the 16-byte boundary before a contiguous row to the row.
+template <typename T, Access kA>
+__device__ __forceinline__ int row_shift(int64_t row, int d) {
+  return kA == kShifted ? (int)((row * d) & (16 / (int)sizeof(T) - 1)) : 0;
 }
 
-template <typename T, int TPR, int NV, bool kVec>
-__device__ __forceinline__ void load_row(float (&x)[NV][8], const T *p, int t, int d) {
+// Column of element e of pack i of thread t.
+template <int TPR, Access kA>
+__device__ __forceinline__ int column(int t, int i, int e, int shift) {
+  return kA == kSingle ? (i * 8 + e) * TPR + t : (i * TPR + t) * 8 + e - shift;
+}
+__device__ __forceinline__ bool inside(int c, int d) { return (unsigned)c < (unsigned)d; }
+// Whether the whole pack at column c is the row's.
+template <Access kA>
+__device__ __forceinline__ bool whole_pack(int c, int d) {
+  return kA == kPacked ? c < d : kA == kShifted && c >= 0 && c + 8 <= d;
+}
+
+__device__ __forceinline__ void unpack(const uint4 &w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __uint_as_float(u[e] << 16);
+    x[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+  }
+}
+
+template <typename T, int TPR, int NV, Access kA>
+__device__ __forceinline__ void load_row(float (&x)[NV][8], const T *p, int t, int d, int shift) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if constexpr (kVec) {
-      const int c = column<TPR, true>(t, i, 0);
-      if (c < d) {
-        if constexpr (sizeof(T) == 2) {
-          const uint4 w = *(const uint4 *)(p + c);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[i][2 * e] = __uint_as_float(u[e] << 16);
-            x[i][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-          }
-        } else {
-          const float4 a = *(const float4 *)(p + c), b = *(const float4 *)(p + c + 4);
-          x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
-          x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
-        }
+    const int c = column<TPR, kA>(t, i, 0, shift);
+    if (whole_pack<kA>(c, d)) {
+      if constexpr (sizeof(T) == 2) {
+        unpack(*(const uint4 *)(p + c), x[i]);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        const float4 a = *(const float4 *)(p + c), b = *(const float4 *)(p + c + 4);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+        x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = column<TPR, false>(t, i, e);
-        x[i][e] = c < d ? to_f32(p[c]) : 0.f;
+        const int ce = column<TPR, kA>(t, i, e, shift);
+        x[i][e] = kA != kPacked && inside(ce, d) ? to_f32(p[ce]) : 0.f;
       }
     }
   }
 }
 
-template <typename T, int TPR, int NV, bool kVec>
-__device__ __forceinline__ void store_row(const float (&x)[NV][8], T *p, int t, int d) {
+template <typename T, int TPR, int NV, Access kA>
+__device__ __forceinline__ void store_row(const float (&x)[NV][8], T *p, int t, int d, int shift) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if constexpr (kVec) {
-      const int c = column<TPR, true>(t, i, 0);
-      if (c >= d) continue;
+    const int c = column<TPR, kA>(t, i, 0, shift);
+    if (whole_pack<kA>(c, d)) {
       if constexpr (sizeof(T) == 2) {
         uint32_t u[4];
 #pragma unroll
@@ -107,39 +122,55 @@ __device__ __forceinline__ void store_row(const float (&x)[NV][8], T *p, int t, 
         *(float4 *)(p + c) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
         *(float4 *)(p + c + 4) = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
       }
-    } else {
+    } else if constexpr (kA != kPacked) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = column<TPR, false>(t, i, e);
-        if (c < d) p[c] = from_f32<T>(x[i][e]);
+        const int ce = column<TPR, kA>(t, i, e, shift);
+        if (inside(ce, d)) p[ce] = from_f32<T>(x[i][e]);
       }
     }
   }
 }
 
-// The weight row (fp32 or bf16; null: ones).
-template <int TPR, int NV, bool kVec>
+// The weight row (fp32 or bf16; null: ones), which starts at 16 bytes whatever
+// the other rows do: by elements where their packs are shifted.
+template <typename TW, int TPR, int NV, Access kA>
+__device__ __forceinline__ void load_weight_as(float (&w)[NV][8], const TW *p, int t, int d,
+                                               int shift) {
+  if constexpr (kA == kShifted) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = column<TPR, kA>(t, i, e, shift);
+        w[i][e] = inside(c, d) ? to_f32(p[c]) : 0.f;
+      }
+  } else {
+    load_row<TW, TPR, NV, kA>(w, p, t, d, 0);
+  }
+}
+template <int TPR, int NV, Access kA>
 __device__ __forceinline__ void load_weight(float (&w)[NV][8], const void *p, int dtype, int t,
-                                            int d) {
+                                            int d, int shift) {
   if (!p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[i][e] = 1.f;
   } else if (dtype == LA_DTYPE_FLOAT32) {
-    load_row<float, TPR, NV, kVec>(w, (const float *)p, t, d);
+    load_weight_as<float, TPR, NV, kA>(w, (const float *)p, t, d, shift);
   } else {
-    load_row<__nv_bfloat16, TPR, NV, kVec>(w, (const __nv_bfloat16 *)p, t, d);
+    load_weight_as<__nv_bfloat16, TPR, NV, kA>(w, (const __nv_bfloat16 *)p, t, d, shift);
   }
 }
 
 // A row as it is loaded, ahead of its use: bf16 packs stay packed.
-template <typename T, int NV, bool kVec>
+template <typename T, int NV, Access kA>
 struct Held {
   float x[NV][8];
   template <int TPR>
-  __device__ __forceinline__ void load(const T *p, int t, int d) {
-    load_row<T, TPR, NV, kVec>(x, p, t, d);
+  __device__ __forceinline__ void load(const T *p, int t, int d, int shift) {
+    load_row<T, TPR, NV, kA>(x, p, t, d, shift);
   }
   __device__ __forceinline__ void get(float (&y)[NV][8]) const {
 #pragma unroll
@@ -148,29 +179,36 @@ struct Held {
       for (int e = 0; e < 8; ++e) y[i][e] = x[i][e];
   }
 };
-template <int NV>
-struct Held<__nv_bfloat16, NV, true> {
+template <int NV, Access kA>
+struct HeldPacks {
   uint4 x[NV];
   template <int TPR>
-  __device__ __forceinline__ void load(const __nv_bfloat16 *p, int t, int d) {
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p, int t, int d, int shift) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column<TPR, true>(t, i, 0);
-      x[i] = c < d ? *(const uint4 *)(p + c) : make_uint4(0, 0, 0, 0);
+      const int c = column<TPR, kA>(t, i, 0, shift);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (whole_pack<kA>(c, d)) {
+        x[i] = *(const uint4 *)(p + c);
+      } else if (kA == kShifted && c > -8 && c < d) {
+        const uint16_t *q = (const uint16_t *)p;
+        auto two = [&](int e) {
+          const uint32_t lo = inside(c + e, d) ? q[c + e] : 0;
+          return lo | (inside(c + e + 1, d) ? (uint32_t)q[c + e + 1] << 16 : 0);
+        };
+        x[i] = make_uint4(two(0), two(2), two(4), two(6));
+      }
     }
   }
   __device__ __forceinline__ void get(float (&y)[NV][8]) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[i][2 * e] = __uint_as_float(u[e] << 16);
-        y[i][2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-      }
-    }
+    for (int i = 0; i < NV; ++i) unpack(x[i], y[i]);
   }
 };
+template <int NV>
+struct Held<__nv_bfloat16, NV, kPacked> : HeldPacks<NV, kPacked> {};
+template <int NV>
+struct Held<__nv_bfloat16, NV, kShifted> : HeldPacks<NV, kShifted> {};
 
 struct Add {
   static __device__ __forceinline__ float zero() { return 0.f; }
@@ -227,7 +265,7 @@ struct NormFwd {
   float eps, inv_d;
 };
 
-template <typename T, int TPR, int NV, bool kVec, bool kFp8>
+template <typename T, int TPR, int NV, Access kA, bool kFp8>
 __global__ void __launch_bounds__(fwd_threads(TPR))
 rms_norm_fwd_kernel(const NormFwd p) {
   constexpr int kRowsPer = fwd_threads(TPR) / TPR;
@@ -237,19 +275,20 @@ rms_norm_fwd_kernel(const NormFwd p) {
   const int64_t row0 = (int64_t)blockIdx.x * kRowsPer + threadIdx.x / TPR;
   const bool live = row0 < p.sh.rows;
   const int64_t row = live ? row0 : p.sh.rows - 1;  // idle lanes redo the last row, unstored
+  const int shift = row_shift<T, kA>(row, p.d);
   float s[NV][8];
-  load_row<T, TPR, NV, kVec>(s, (const T *)p.x.p + row_offset(p.x, p.sh, row), t, p.d);
+  load_row<T, TPR, NV, kA>(s, (const T *)p.x.p + row_offset(p.x, p.sh, row), t, p.d, shift);
   if (p.r.p) {
     float r[NV][8];
-    load_row<T, TPR, NV, kVec>(r, (const T *)p.r.p + row_offset(p.r, p.sh, row), t, p.d);
+    load_row<T, TPR, NV, kA>(r, (const T *)p.r.p + row_offset(p.r, p.sh, row), t, p.d, shift);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[i][e] += r[i][e];
   }
   float w[NV][8];
-  load_weight<TPR, NV, kVec>(w, p.weight, p.weight_dtype, t, p.d);
-  if (p.sum && live) store_row<T, TPR, NV, kVec>(s, (T *)p.sum + row * p.d, t, p.d);
+  load_weight<TPR, NV, kA>(w, p.weight, p.weight_dtype, t, p.d, shift);
+  if (p.sum && live) store_row<T, TPR, NV, kA>(s, (T *)p.sum + row * p.d, t, p.d, shift);
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -263,7 +302,7 @@ rms_norm_fwd_kernel(const NormFwd p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[i][e] = s[i][e] * rstd * w[i][e];
   if constexpr (!kFp8) {
-    if (live) store_row<T, TPR, NV, kVec>(s, (T *)p.y + row * p.d, t, p.d);
+    if (live) store_row<T, TPR, NV, kA>(s, (T *)p.y + row * p.d, t, p.d, shift);
   } else {
     float m[NV], all = 0.f;
 #pragma unroll
@@ -278,7 +317,7 @@ rms_norm_fwd_kernel(const NormFwd p) {
       all = reduce_row<TPR, Max>(all, slot_max);
 #pragma unroll
       for (int i = 0; i < NV; ++i) m[i] = all;
-    } else {  // a group is group / 8 neighbouring lanes of one pack (kVec only)
+    } else {  // a group is group / 8 neighbouring lanes of one pack (packed rows only)
       const int lanes = 1 << (p.group_log2 - 3);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -288,7 +327,7 @@ rms_norm_fwd_kernel(const NormFwd p) {
     uint8_t *y = (uint8_t *)p.y + row * p.d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column<TPR, kVec>(t, i, 0);
+      const int c = column<TPR, kA>(t, i, 0, shift);
       const float scale = Max::of(m[i], kAmaxMin) * (1.f / kE4m3Max);
       // one division per group: y * (1 / scale) is within an ulp of y / scale
       // ahead of the rounding to 4 bits
@@ -304,15 +343,19 @@ rms_norm_fwd_kernel(const NormFwd p) {
         q[e] = __nv_cvt_float2_to_fp8x2(make_float2(s[i][2 * e] * inv, s[i][2 * e + 1] * inv),
                                         __NV_SATFINITE, __NV_E4M3);
       if (!live) continue;
-      if constexpr (kVec) {
-        if (c < p.d)
-          *(uint2 *)(y + c) = make_uint2(q[0] | ((uint32_t)q[1] << 16),
-                                         q[2] | ((uint32_t)q[3] << 16));
-      } else {
+      if (whole_pack<kA>(c, p.d)) {
+        const uint2 u = make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
+        if constexpr (kA == kPacked || sizeof(T) == 2) {
+          *(uint2 *)(y + c) = u;
+        } else {  // packs of 8 at a multiple of 4 values
+          *(uint32_t *)(y + c) = u.x;
+          *(uint32_t *)(y + c + 4) = u.y;
+        }
+      } else if constexpr (kA != kPacked) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int ce = column<TPR, false>(t, i, e);
-          if (ce < p.d) y[ce] = (uint8_t)(q[e / 2] >> (8 * (e & 1)));
+          const int ce = column<TPR, kA>(t, i, e, shift);
+          if (inside(ce, p.d)) y[ce] = (uint8_t)(q[e / 2] >> (8 * (e & 1)));
         }
       }
     }
@@ -331,7 +374,7 @@ struct NormBwd {
   float inv_d;
 };
 
-template <typename T, int TPR, int NV, bool kVec>
+template <typename T, int TPR, int NV, Access kA>
 __global__ void __launch_bounds__(bwd_threads(TPR))
 rms_norm_bwd_kernel(const NormBwd p) {
   constexpr int kThreads = bwd_threads(TPR);
@@ -341,20 +384,25 @@ rms_norm_bwd_kernel(const NormBwd p) {
   tc::grid_dependents_launch();        // the sum of dw waits for all of this grid
   const int t = threadIdx.x % TPR, lane_row = threadIdx.x / TPR;
   float w[NV][8], dw[NV][8] = {};
-  load_weight<TPR, NV, kVec>(w, p.weight, p.weight_dtype, t, p.d);
+  // the rows of a row lane are a multiple of 8 apart where their packs are
+  // shifted, so that its columns stay the same
+  const int shift = row_shift<T, kA>((int64_t)blockIdx.x * kRowsPer + lane_row, p.d);
+  load_weight<TPR, NV, kA>(w, p.weight, p.weight_dtype, t, p.d, shift);
   // The next row is loaded before this one's sum over the row's threads (not
   // where 1024 threads leave 64 registers each).
   constexpr bool kAhead = TPR < 1024;
-  Held<T, NV, kVec> hs, hg, ha;
+  Held<T, NV, kA> hs, hg, ha;
   float rstd_next = 0.f;
   const int64_t stride = (int64_t)gridDim.x * kRowsPer;
   auto fetch = [&](int64_t first) {
-    // idle lanes redo the last row, unstored
-    const int64_t row = min64(first + lane_row, p.sh.rows - 1);
-    hs.template load<TPR>((const T *)p.s.p + row_offset(p.s, p.sh, row), t, p.d);
-    hg.template load<TPR>((const T *)p.dy.p + row_offset(p.dy, p.sh, row), t, p.d);
+    // idle lanes redo the last row, unstored; shifted, a row of their own shift
+    int64_t row = first + lane_row;
+    const int d = kA == kShifted && row >= p.sh.rows ? 0 : p.d;
+    row = min64(row, p.sh.rows - 1);
+    hs.template load<TPR>((const T *)p.s.p + row_offset(p.s, p.sh, row), t, d, shift);
+    hg.template load<TPR>((const T *)p.dy.p + row_offset(p.dy, p.sh, row), t, d, shift);
     if (p.dsum.p)
-      ha.template load<TPR>((const T *)p.dsum.p + row_offset(p.dsum, p.sh, row), t, p.d);
+      ha.template load<TPR>((const T *)p.dsum.p + row_offset(p.dsum, p.sh, row), t, d, shift);
     rstd_next = p.rstd[row];
   };
   if (kAhead) fetch((int64_t)blockIdx.x * kRowsPer);
@@ -389,7 +437,7 @@ rms_norm_bwd_kernel(const NormBwd p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) g[i][e] += a[i][e];
     }
-    if (live) store_row<T, TPR, NV, kVec>(g, (T *)p.ds + row * p.d, t, p.d);
+    if (live) store_row<T, TPR, NV, kA>(g, (T *)p.ds + row * p.d, t, p.d, shift);
   }
   if (!p.partial) return;
   if constexpr (kRowsPer > 1) {
@@ -399,8 +447,8 @@ rms_norm_bwd_kernel(const NormBwd p) {
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int c = column<TPR, kVec>(t, i, e);
-          if (c < p.d) dst[c] = dw[i][e];
+          const int c = column<TPR, kA>(t, i, e, shift);
+          if (inside(c, p.d)) dst[c] = dw[i][e];
         }
     }
     __syncthreads();
@@ -417,8 +465,8 @@ rms_norm_bwd_kernel(const NormBwd p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int c = column<TPR, kVec>(t, i, e);
-        if (c < p.d) dst[c] = dw[i][e] + (kRowsPer > 1 ? lanes_dw[c] : 0.f);
+        const int c = column<TPR, kA>(t, i, e, shift);
+        if (inside(c, p.d)) dst[c] = dw[i][e] + (kRowsPer > 1 ? lanes_dw[c] : 0.f);
       }
   }
 }
@@ -462,44 +510,54 @@ int launch_dw(const float *partial, int rows, int d, void *dw, cudaStream_t s) {
 
 // The threads per row and packs per thread for a width.  Few packs keep the
 // registers low enough for many CTAs per SM, whose loads then cover one
-// another's reductions.  Rows whose width or alignment rules out 16-byte
-// accesses take fewer variants.
+// another's reductions.  Shifted and single-element rows take fewer variants.
 template <class F>
-int by_width_odd(int64_t d, F &&f) {
-  if (d <= 256) return f.template run<32, 1, false>();
-  if (d <= 1024) return f.template run<128, 1, false>();
-  if (d <= 4096) return f.template run<256, 2, false>();
-  return f.template run<1024, 2, false>();
+int by_width_single(int64_t d, F &&f) {
+  if (d <= 256) return f.template run<32, 1, kSingle>();
+  if (d <= 1024) return f.template run<128, 1, kSingle>();
+  if (d <= 4096) return f.template run<256, 2, kSingle>();
+  return f.template run<1024, 2, kSingle>();
+}
+template <class F>
+int by_width_shifted(int64_t d, F &&f) {  // one pack more than the row's own
+  if (d + 8 <= 256) return f.template run<32, 1, kShifted>();
+  if (d + 8 <= 1024) return f.template run<128, 1, kShifted>();
+  if (d + 8 <= 2048) return f.template run<256, 1, kShifted>();
+  if (d + 8 <= 4096) return f.template run<256, 2, kShifted>();
+  if (d + 8 <= 8192) return f.template run<512, 2, kShifted>();
+  return f.template run<1024, 2, kShifted>();
 }
 // Forward: rows of up to 1024 within one warp (32768 x 4096 with a residual, one
 // row of 128 threads x 4 packs per CTA against 256 x 2: 164 and 171 us, to e4m3
 // 188 and 196).
 template <class F>
-int by_width_fwd(int64_t d, bool vec, F &&f) {
-  if (!vec) return by_width_odd(d, f);
-  if (d <= 64) return f.template run<8, 1, true>();
-  if (d <= 128) return f.template run<16, 1, true>();
-  if (d <= 256) return f.template run<32, 1, true>();
-  if (d <= 512) return f.template run<32, 2, true>();
-  if (d <= 1024) return f.template run<32, 4, true>();
-  if (d <= 2048) return f.template run<128, 2, true>();
-  if (d <= 4096) return f.template run<128, 4, true>();
-  if (d <= 8192) return f.template run<256, 4, true>();
-  return f.template run<1024, 2, true>();
+int by_width_fwd(int64_t d, Access access, F &&f) {
+  if (access == kSingle) return by_width_single(d, f);
+  if (access == kShifted) return by_width_shifted(d, f);
+  if (d <= 64) return f.template run<8, 1, kPacked>();
+  if (d <= 128) return f.template run<16, 1, kPacked>();
+  if (d <= 256) return f.template run<32, 1, kPacked>();
+  if (d <= 512) return f.template run<32, 2, kPacked>();
+  if (d <= 1024) return f.template run<32, 4, kPacked>();
+  if (d <= 2048) return f.template run<128, 2, kPacked>();
+  if (d <= 4096) return f.template run<128, 4, kPacked>();
+  if (d <= 8192) return f.template run<256, 4, kPacked>();
+  return f.template run<1024, 2, kPacked>();
 }
 // Gradient: it also holds w and the running dw.
 template <class F>
-int by_width_bwd(int64_t d, bool vec, F &&f) {
-  if (!vec) return by_width_odd(d, f);
-  if (d <= 64) return f.template run<8, 1, true>();
-  if (d <= 128) return f.template run<16, 1, true>();
-  if (d <= 256) return f.template run<32, 1, true>();
-  if (d <= 512) return f.template run<64, 1, true>();
-  if (d <= 1024) return f.template run<128, 1, true>();
-  if (d <= 2048) return f.template run<256, 1, true>();
-  if (d <= 4096) return f.template run<256, 2, true>();
-  if (d <= 8192) return f.template run<512, 2, true>();
-  return f.template run<1024, 2, true>();
+int by_width_bwd(int64_t d, Access access, F &&f) {
+  if (access == kSingle) return by_width_single(d, f);
+  if (access == kShifted) return by_width_shifted(d, f);
+  if (d <= 64) return f.template run<8, 1, kPacked>();
+  if (d <= 128) return f.template run<16, 1, kPacked>();
+  if (d <= 256) return f.template run<32, 1, kPacked>();
+  if (d <= 512) return f.template run<64, 1, kPacked>();
+  if (d <= 1024) return f.template run<128, 1, kPacked>();
+  if (d <= 2048) return f.template run<256, 1, kPacked>();
+  if (d <= 4096) return f.template run<256, 2, kPacked>();
+  if (d <= 8192) return f.template run<512, 2, kPacked>();
+  return f.template run<1024, 2, kPacked>();
 }
 
 // The gradient's CTAs walk the rows: this many per SM at most.
@@ -510,23 +568,40 @@ size_t partial_bytes(int64_t rows, int64_t d, int sm_count) {
   return (size_t)min64(rows, (int64_t)sm_count * kBwdPerSm) * (size_t)d * sizeof(float);
 }
 
-bool vec_rows(const Rows &t, int size) {
+// Whether rows start at 16 bytes; whether they are contiguous from there on.
+bool packed_rows(const Rows &t, int size) {
   const int64_t pack = 16 / size;
   return !t.p || (((uintptr_t)t.p & 15) == 0 && t.s0 % pack == 0 && t.s1 % pack == 0 &&
                   t.s2 % pack == 0);
 }
-bool vec_ptr(const void *p) { return ((uintptr_t)p & 15) == 0; }
+bool plain_rows(const Rows &t, const Shape &sh, int64_t d) {
+  return !t.p || (((uintptr_t)t.p & 15) == 0 && sh.n2 == sh.rows && t.s2 == d);
+}
+bool at16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// The access for inputs a, b, c and contiguous outputs u, v.
+Access access_of(const Shape &sh, int64_t d, int dtype, const Rows &a, const Rows &b, const Rows &c,
+                 const void *weight, const void *u, const void *v) {
+  const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+  if (!at16(u) || !at16(v)) return kSingle;
+  if (d % 8 == 0 && at16(weight) && packed_rows(a, size) && packed_rows(b, size) &&
+      packed_rows(c, size))
+    return kPacked;
+  if (d + 8 <= kMaxWidth && plain_rows(a, sh, d) && plain_rows(b, sh, d) && plain_rows(c, sh, d))
+    return kShifted;
+  return kSingle;
+}
 
 template <typename T, bool kFp8>
 struct FwdLaunch {
   const NormFwd &p;
   cudaStream_t s;
-  template <int TPR, int NV, bool kVec>
+  template <int TPR, int NV, Access kA>
   int run() {
     constexpr int per = fwd_threads(TPR) / TPR;
     const int64_t grid = (p.sh.rows + per - 1) / per;
     if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
-    rms_norm_fwd_kernel<T, TPR, NV, kVec, kFp8><<<(unsigned)grid, fwd_threads(TPR), 0, s>>>(p);
+    rms_norm_fwd_kernel<T, TPR, NV, kA, kFp8><<<(unsigned)grid, fwd_threads(TPR), 0, s>>>(p);
     return check_launch();
   }
 };
@@ -537,22 +612,24 @@ struct BwdLaunch {
   int sm_count;
   int *grid;
   cudaStream_t s;
-  template <int TPR, int NV, bool kVec>
+  template <int TPR, int NV, Access kA>
   int run() {
     constexpr int per = bwd_threads(TPR) / TPR;
     // one wave of CTAs, each walking many rows
     static const int per_sm = [] {
       int n = 0;
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-              &n, rms_norm_bwd_kernel<T, TPR, NV, kVec>, bwd_threads(TPR), 28 * 1024) != cudaSuccess) {
+              &n, rms_norm_bwd_kernel<T, TPR, NV, kA>, bwd_threads(TPR), 28 * 1024) != cudaSuccess) {
         cudaGetLastError();
         n = 2;
       }
       return n < 1 ? 1 : n > kBwdPerSm ? kBwdPerSm : n;
     }();
-    *grid = (int)min64((p.sh.rows + per - 1) / per, (int64_t)sm_count * per_sm);
+    const int64_t groups = (p.sh.rows + per - 1) / per;
+    *grid = (int)min64(groups, (int64_t)sm_count * per_sm);
+    if (kA == kShifted && *grid < groups) *grid = *grid / 8 * 8;  // whole periods of the shift
     const int smem = p.partial ? (per - 1) * p.d * 4 : 0;  // at most 28 KB
-    rms_norm_bwd_kernel<T, TPR, NV, kVec><<<*grid, bwd_threads(TPR), smem, s>>>(p);
+    rms_norm_bwd_kernel<T, TPR, NV, kA><<<*grid, bwd_threads(TPR), smem, s>>>(p);
     return check_launch();
   }
 };
@@ -592,20 +669,18 @@ Rows rows_of(const void *p, const int64_t *s) {
 
 template <bool kFp8>
 int launch_fwd(const NormFwd &p, int dtype, cudaStream_t s) {
-  const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
-  const bool vec = p.d % 8 == 0 && vec_rows(p.x, size) && vec_rows(p.r, size) &&
-                   vec_ptr(p.weight) && vec_ptr(p.y) && vec_ptr(p.sum);
-  if (kFp8 && p.group_log2 >= 0 && !vec) return LA_ERR_UNSUPPORTED;
-  if (dtype == LA_DTYPE_FLOAT32) return by_width_fwd(p.d, vec, FwdLaunch<float, kFp8>{p, s});
-  return by_width_fwd(p.d, vec, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
+  const Access access = access_of(p.sh, p.d, dtype, p.x, p.r, Rows{}, p.weight, p.y, p.sum);
+  if (kFp8 && p.group_log2 >= 0 && access != kPacked) return LA_ERR_UNSUPPORTED;
+  if (dtype == LA_DTYPE_FLOAT32) return by_width_fwd(p.d, access, FwdLaunch<float, kFp8>{p, s});
+  return by_width_fwd(p.d, access, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
 }
 
 int launch_bwd(const NormBwd &p, int dtype, int sm_count, int *grid, cudaStream_t s) {
-  const int size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
-  const bool vec = p.d % 8 == 0 && vec_rows(p.s, size) && vec_rows(p.dy, size) &&
-                   vec_rows(p.dsum, size) && vec_ptr(p.weight) && vec_ptr(p.ds);
-  if (dtype == LA_DTYPE_FLOAT32) return by_width_bwd(p.d, vec, BwdLaunch<float>{p, sm_count, grid, s});
-  return by_width_bwd(p.d, vec, BwdLaunch<__nv_bfloat16>{p, sm_count, grid, s});
+  const Access access =
+      access_of(p.sh, p.d, dtype, p.s, p.dy, p.dsum, p.weight, p.ds, nullptr);
+  if (dtype == LA_DTYPE_FLOAT32)
+    return by_width_bwd(p.d, access, BwdLaunch<float>{p, sm_count, grid, s});
+  return by_width_bwd(p.d, access, BwdLaunch<__nv_bfloat16>{p, sm_count, grid, s});
 }
 
 }  // namespace
