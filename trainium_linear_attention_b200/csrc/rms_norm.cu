@@ -11,7 +11,13 @@
 // shared memory where a row spans warps).  The gradient's CTAs walk the rows
 // with a fixed set of columns per thread, so dw is summed in registers, then
 // over the CTA's row lanes, and a second kernel adds the CTAs' partial rows in
-// a fixed order: no atomics, the same bits every time.
+// a fixed order: no atomics, the same bits every time.  It works on the saved
+// sum, which is rounded to the inputs' type (half a step: 2^-8 in bf16).
+//
+// Measured, bf16 with a residual, of the copy rate (6.5 TB/s): 16384 x 1024 in
+// 23 us (89%), its gradient 26 (80%); 32768 x 4096 in 164 (100%), to e4m3 188
+// (77%: the conversions and group maxima), gradient 193 (86%); 131072 rows of 64
+// in 10.5 us (98%), gradient 15 (69%); 16384 x 1023 (shifted) in 63 us.
 #include <cuda_fp8.h>
 #include <math.h>
 

@@ -17,20 +17,28 @@
 // The decay never multiplies an accumulator in TMEM: it is on the rows of P and
 // V' (operands), on O1's rows and on the state's registers, so U, the scores
 // and O2 of a tile depend on the tile alone and only O1 waits for the state.
-// V' as hi + lo carries 16 bits, so the fp32 state is exact to about 2^-18
-// (one bf16 term would leave 2^-9 in a state that decoding continues from);
-// stacked along N the second term costs no further MMA instruction and no
-// second read of B.  The bf16 copy of S and P are rounded once (2^-8, like the
-// output).  With DK = 64, M = 128 holds B^T twice (descriptor stride 0), and
-// the state warps of the upper lanes take the other half of the columns.
+// Roundings, each once and half a step at most: P and the copy of S to bf16
+// (2^-8, like the output), and V' to the 16 bits of hi + lo (2^-17): with one
+// bf16 term the fp32 state, which decoding continues from, would be off by 2^-8.
+// Stacked along N the second term costs no further MMA and no second read of B;
+// a third would need 64 more TMEM columns than there are.  With DK < 128, M = 128
+// holds B^T more than once (descriptor stride 0), and the state warps of each
+// copy take other columns.
 //
-// What bounds it: HBM for long walks of enough heads (a tile moves 64 KB at
-// d = 64 against ~1,300 cycles of tensor work); per-tile latency (the chain
-// U -> S -> copy -> O1 -> out) where few CTAs walk.
+// What bounds it.  A tile moves 64 KB at d = 64 and its MMAs read ~190 KB of
+// shared memory (~1,500 cycles); with its 24 warps a tile takes 2,300 to 2,600
+// cycles, of which the issue slots (4,800 warp instructions on 4 schedulers)
+// and the chain O1, O2 -> epilogue -> next O2 are the largest parts: 128 heads
+// of 8192 x 64 in 98 us (5.5 TB/s, 84% of the copy rate), of 16 / 64 in 75 us
+// (4.5 TB/s; with 128-byte key rows and three stages 83), 64 heads of 128 in 130
+// us (4.1 TB/s: the two slices of v form P twice).  What that chain is sensitive
+// to is code size: unrolled loops of P alone made it 1.3 times slower, and the
+// code of rare cases inside the loops 5%.  Twice the epilogue or V' warps, O2 in
+// two buffers, and tiles prefetched into L2 were measured and are no faster.
 //
-// Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state
-// (4 warps at DK = 64, 8 at 128); 8 warps P; 4
-// warps V'; 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
+// Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state (8 warps
+// at DK = 128, else 4); 8 warps P; 4 warps V'; 4 warps epilogue.  Every wait is
+// bounded (tc_common.cuh).
 #include <type_traits>
 
 #include "decay.cuh"
