@@ -234,7 +234,7 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
  * with S_{-1} = init_state (zero if null).  The state is fp32 (batch, heads,
  * d_qk, d_v), contiguous; log_decay is fp32 (heads) in device memory, finite
  * and <= 0 or -inf (no memory).  d_qk and d_v are at most 128 and need not be
- * equal.  The reference has no decayed form; the recurrence without decay is
+ * equal; batch * heads is at most 65535 for prompts and their gradients.  The reference has no decayed form; the recurrence without decay is
  * its chunked kernel's (kernels/nki_attention_chunked.py:20-113).
  *
  * q, k, v, out and the gradients are (batch, heads, seq_len, d) with a dense

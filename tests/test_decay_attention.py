@@ -267,6 +267,9 @@ def test_empty_and_zero_tokens():
     assert T.decay_linear_attention(q, k, v, g).shape == (0, 3, 5, 64)
     s = torch.zeros(0, 3, 16, 64, device="cuda")
     assert T.decay_linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g, s).shape == (0, 3, 64)
+    q, k, v, g, state = make(2, 3, 0, 57, 33, torch.bfloat16)  # (widened)
+    out, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)
+    assert out.shape == (2, 3, 0, 33) and torch.equal(end, state)
     q, k, v, g, state = make(1, 2, 0, 16, 64, torch.bfloat16)
     state.requires_grad_()
     _, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)

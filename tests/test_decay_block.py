@@ -57,12 +57,16 @@ def test_block_on_the_cpu_refuses():
     assert sorted(m.state_dict()) == ["head_norm_weight", "k_proj.weight", "log_decay",
                                       "norm_weight", "o_proj.weight", "q_proj.weight",
                                       "v_proj.weight"]
+    before = m.log_decay.clone()
     assert m.to(torch.bfloat16).log_decay.dtype == torch.float32
+    assert torch.equal(m.log_decay, before) and m.norm_weight.dtype == torch.bfloat16
     assert not any(n == "log_decay" for n, _ in m.named_parameters())
     with pytest.raises(ValueError, match="CUDA"):
         m(torch.zeros(1, 3, 64, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="log_decay"):
         T.DecayLinearAttention(64, 4, log_decay=[-1.0])
+    with pytest.raises(ValueError, match="head dim"):
+        T.DecayLinearAttention(512, 2)
     with pytest.raises(ValueError, match="residual"):
         T.TrainiumBasedLinearAttentionNKI(64, 4)(torch.zeros(1, 3, 64), torch.zeros(1, 3, 64))
 

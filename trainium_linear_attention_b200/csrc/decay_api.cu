@@ -49,13 +49,9 @@ struct DecaySplit {
 // heads leave SMs idle where there are few, or in a last, partial wave of CTAs.
 // So all heads are walked whole, or all in g segments, or as many whole as fill
 // k waves and the rest in g segments that share the SMs of one more.
-DecaySplit plan_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype, bool backward,
-                      int requested, int sm_count) {
+DecaySplit estimate_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype,
+                          bool backward, int sm_count) {
   DecaySplit best;
-  if (requested != 0) {
-    best.segments = fit_segments(n, requested, &best.len);
-    return best;
-  }
   const int64_t sq = (d_qk + kDecaySlice - 1) / kDecaySlice;
   const int64_t sv = (d_v + kDecaySlice - 1) / kDecaySlice;
   const int64_t per_head = backward ? 2 * sq + sv : sv;    // CTAs that walk a head
@@ -102,6 +98,31 @@ DecaySplit plan_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtyp
     }
   }
   return best;
+}
+
+DecaySplit plan_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int dtype, bool backward,
+                      int requested, int sm_count) {
+  if (requested != 0) {
+    DecaySplit s;
+    s.segments = fit_segments(n, requested, &s.len);
+    return s;
+  }
+  // the estimate takes some microseconds for a long sequence: the last one of
+  // each kind is kept per thread
+  struct Kept {
+    int64_t sizes[6] = {-1, -1, -1, -1, -1, -1};
+    DecaySplit split;
+  };
+  static thread_local Kept kept[2];
+  Kept &k = kept[backward ? 1 : 0];
+  const int64_t sizes[6] = {bh, n, d_qk, d_v, dtype, sm_count};
+  bool same = true;
+  for (int i = 0; i < 6; ++i) same = same && k.sizes[i] == sizes[i];
+  if (!same) {
+    k.split = estimate_split(bh, n, d_qk, d_v, dtype, backward, sm_count);
+    for (int i = 0; i < 6; ++i) k.sizes[i] = sizes[i];
+  }
+  return k.split;
 }
 
 // States of the split heads: of the walk ahead, and of the one back.

@@ -140,6 +140,8 @@ class DecayLinearAttention(_Projections):
 
     def __init__(self, dim: int, heads: int = 8, eps: float = 1e-6, log_decay=None):
         super().__init__(dim, heads, eps)
+        if self.head_dim > 128:
+            raise ValueError(f"head dim {self.head_dim} > 128")
         self.norm_weight = nn.Parameter(torch.ones(dim))
         self.head_norm_weight = nn.Parameter(torch.ones(self.head_dim))
         if log_decay is None:
@@ -150,9 +152,13 @@ class DecayLinearAttention(_Projections):
         self.register_buffer("log_decay", log_decay)
 
     def _apply(self, fn, recurse=True):
-        # the decay stays fp32 when the module is cast
+        # the decay moves with the module but keeps its fp32 values when that is cast
+        kept = self.log_decay
         super()._apply(fn, recurse)
-        self.log_decay = self.log_decay.float()
+        if kept.is_meta or self.log_decay.is_meta:
+            self.log_decay = self.log_decay.float()
+        else:
+            self.log_decay = kept.to(self.log_decay.device)
         return self
 
     def _finish(self, y: torch.Tensor) -> torch.Tensor:
