@@ -58,16 +58,16 @@ DecaySplit estimate_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int 
   const int64_t state_per_head = backward ? 2 * sv : sv;   // and in a state pass
   const bool wide = backward ? (d_qk > 64 || d_v > 64) : d_qk > 64;
   // microseconds per 128 tokens of a CTA's walk (output, state) and per wave
-  // of CTAs (start-up, first loads, drain), measured on a B200; the CUDA-core
-  // kernel holds two CTAs per SM up to 64 columns.  (bf16, d = 64: 64 heads of
-  // 2048 / 4096 / 8192 tokens unsplit 24 / 45 / 82 us, in two segments 28 / 45 /
-  // 76; the gradients of 64 heads of 4096 tokens, 192 CTAs, unsplit 89 us, in
-  // two segments 94.)
+  // of CTAs (start-up, first loads, drain), measured on a B200.  (bf16, d = 64:
+  // 64 heads of 2048 / 4096 / 8192 tokens unsplit 24 / 45 / 82 us, in two
+  // segments 28 / 45 / 76; the gradients of 64 heads of 4096 tokens, 192 CTAs,
+  // unsplit 89 us, in two segments 94.  fp32: 64 heads of 4096 tokens unsplit
+  // 468 us, in 2 / 4 / 8 segments 324 / 321 / 337.)
   const bool simt = dtype == LA_DTYPE_FLOAT32;
-  const double t_out = simt ? (wide ? 36.0 : 24.0) : (wide ? 2.1 : 1.3);
-  const double t_state = simt ? (wide ? 14.0 : 9.0) : (wide ? 1.2 : 0.8);
+  const double t_out = simt ? (wide ? 25.0 : 14.3) : (wide ? 2.1 : 1.3);
+  const double t_state = simt ? (wide ? 9.0 : 5.1) : (wide ? 1.2 : 0.8);
   constexpr double kWaveOut = 4.0, kWaveState = 3.0, kSplit = 5.0, kJoin = 0.4;
-  const int64_t slots = sm_count * (simt && !wide ? 2 : 1);
+  const int64_t slots = sm_count;  // one CTA per SM
   const int64_t tiles = (n + kDecayTile - 1) / kDecayTile;
   const int64_t most = tiles < 1 ? 1 : tiles < kMaxAutoSegments ? tiles : kMaxAutoSegments;
   const int64_t full_waves = simt ? 0 : bh * per_head / slots;
