@@ -233,6 +233,21 @@ def test_fp8(rows, d, group, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d", [(1184, 1024), (1185, 1024), (2500, 1000), (592, 2048),
+                                    (593, 2040), (1301, 1032), (296, 4096), (297, 4096),
+                                    (701, 2056), (1000, 520), (260, 8200)])
+def test_many_rows(rows, d, dtype):
+    """Around the number of rows from which a thread takes several packs."""
+    x, r, w = make((rows, d), dtype, True, dtype, rows)
+    check(x, w, r)
+    test_gradients(rows, d, True, dtype)
+    test_fp8(rows, d, None, dtype)
+    if d % 128 == 0:
+        test_fp8(rows, d, 128, dtype)
+
+
+@gpu
 def test_fp8_not_finite():
     x = torch.randn(3, 64, device="cuda")
     x[1, 3] = float("nan")

@@ -15,9 +15,10 @@
 // sum, which is rounded to the inputs' type (half a step: 2^-8 in bf16).
 //
 // Measured, bf16 with a residual, of the copy rate (6.5 TB/s): 16384 x 1024 in
-// 23 us (89%), its gradient 26 (80%); 32768 x 4096 in 164 (100%), to e4m3 188
-// (77%: the conversions and group maxima), gradient 193 (86%); 131072 rows of 64
-// in 10.5 us (98%), gradient 15 (69%); 16384 x 1023 (shifted) in 63 us.
+// 23 us (89%), its gradient 22 (94%); 32768 x 4096 in 158 (104%), to e4m3 155
+// (93%), gradient 154 (107%; both upstream gradients were one tensor); 131072
+// rows of 64 in 10.5 us (98%), gradient 15 (69%); 4096 x 16384 in 90 us (92%),
+// gradient 141 (59%: 64 registers a thread spill); 16384 x 1023 (shifted) in 63 us.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -256,6 +257,18 @@ __device__ __forceinline__ float reduce_row(float x, float *slot) {
 // no row waits at another's barrier; gradient: at least 256, fewer partial rows.
 constexpr int fwd_threads(int tpr) { return tpr >= 128 ? tpr : 256; }
 constexpr int bwd_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+// Forward rows of several packs a thread fetch the weight (from the caches) behind
+// the sum of squares instead of holding it over it, and packed ones are kept to 64
+// registers (80 in fp32, which spills more), so that more rows are on their way (0: no
+// limit, better for 32 threads a row in the plain form).  32768 x 4096 in 164 -> 158 us,
+// to e4m3 189 -> 155 us, 167 with 80 registers; 16384 x 4096 in fp32 164 -> 160 and 138
+// -> 130, 143 with 64.  With one pack a thread the later fetch costs more (131072 x 128
+// in 25.5 -> 27.3).
+constexpr bool fwd_late_weight(int tpr, int nv) { return nv > 1 && tpr < 1024; }
+constexpr int fwd_per_sm(int tpr, int nv, Access a, bool fp8, int size) {
+  return a == kPacked && fwd_late_weight(tpr, nv) && (fp8 || tpr > 32)
+             ? (size == 2 ? 1024 : 768) / fwd_threads(tpr) : 0;
+}
 
 struct NormFwd {
   Rows x, r;              // r.p null: no residual
@@ -272,7 +285,7 @@ struct NormFwd {
 };
 
 template <typename T, int TPR, int NV, Access kA, bool kFp8>
-__global__ void __launch_bounds__(fwd_threads(TPR))
+__global__ void __launch_bounds__(fwd_threads(TPR), fwd_per_sm(TPR, NV, kA, kFp8, sizeof(T)))
 rms_norm_fwd_kernel(const NormFwd p) {
   constexpr int kRowsPer = fwd_threads(TPR) / TPR;
   __shared__ float slot[32];
@@ -293,7 +306,7 @@ rms_norm_fwd_kernel(const NormFwd p) {
       for (int e = 0; e < 8; ++e) s[i][e] += r[i][e];
   }
   float w[NV][8];
-  load_weight<TPR, NV, kA>(w, p.weight, p.weight_dtype, t, p.d, shift);
+  if (!fwd_late_weight(TPR, NV)) load_weight<TPR, NV, kA>(w, p.weight, p.weight_dtype, t, p.d, shift);
   if (p.sum && live) store_row<T, TPR, NV, kA>(s, (T *)p.sum + row * p.d, t, p.d, shift);
   float sq = 0.f;
 #pragma unroll
@@ -303,6 +316,7 @@ rms_norm_fwd_kernel(const NormFwd p) {
   sq = reduce_row<TPR, Add>(sq, slot);
   const float rstd = 1.f / sqrtf(fmaf(sq, p.inv_d, p.eps));
   if (p.rstd && live && t == 0) p.rstd[row] = rstd;
+  if (fwd_late_weight(TPR, NV)) load_weight<TPR, NV, kA>(w, p.weight, p.weight_dtype, t, p.d, shift);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -544,11 +558,16 @@ int by_width_fwd(int64_t d, Access access, F &&f) {
   if (d <= 128) return f.template run<16, 1, kPacked>();
   if (d <= 256) return f.template run<32, 1, kPacked>();
   if (d <= 512) return f.template run<32, 2, kPacked>();
-  if (d <= 1024) return f.template run<32, 4, kPacked>();
-  if (d <= 2048) return f.template run<128, 2, kPacked>();
-  if (d <= 4096) return f.template run<128, 4, kPacked>();
+  // Rows that all fit the SMs at once with one pack a thread take that form, the
+  // shortest way through a row: 8 / 1200 rows of 1024 to e4m3 2.9 / 3.9 us against
+  // 4.2 / 5.2; 2400 rows 5.6 either way, 16384 rows 30 against 24.  (The sums of the
+  // two forms are in other orders: a row's last bit may go by the number of rows.)
+  const bool few = d <= 4096 && f.p.sh.rows * ((d + 1023) / 1024) <= f.sm_count * 8;
+  if (d <= 1024) return few ? f.template run<128, 1, kPacked>() : f.template run<32, 4, kPacked>();
+  if (d <= 2048) return few ? f.template run<256, 1, kPacked>() : f.template run<128, 2, kPacked>();
+  if (d <= 4096) return few ? f.template run<512, 1, kPacked>() : f.template run<128, 4, kPacked>();
   if (d <= 8192) return f.template run<256, 4, kPacked>();
-  return f.template run<1024, 2, kPacked>();
+  return f.template run<512, 4, kPacked>();
 }
 // Gradient: it also holds w and the running dw.
 template <class F>
@@ -558,10 +577,10 @@ int by_width_bwd(int64_t d, Access access, F &&f) {
   if (d <= 64) return f.template run<8, 1, kPacked>();
   if (d <= 128) return f.template run<16, 1, kPacked>();
   if (d <= 256) return f.template run<32, 1, kPacked>();
-  if (d <= 512) return f.template run<64, 1, kPacked>();
-  if (d <= 1024) return f.template run<128, 1, kPacked>();
-  if (d <= 2048) return f.template run<256, 1, kPacked>();
-  if (d <= 4096) return f.template run<256, 2, kPacked>();
+  if (d <= 512) return f.template run<32, 2, kPacked>();
+  if (d <= 1024) return f.template run<64, 2, kPacked>();
+  if (d <= 2048) return f.template run<128, 2, kPacked>();
+  if (d <= 4096) return f.template run<128, 4, kPacked>();
   if (d <= 8192) return f.template run<512, 2, kPacked>();
   return f.template run<1024, 2, kPacked>();
 }
@@ -601,6 +620,7 @@ Access access_of(const Shape &sh, int64_t d, int dtype, const Rows &a, const Row
 template <typename T, bool kFp8>
 struct FwdLaunch {
   const NormFwd &p;
+  int sm_count;
   cudaStream_t s;
   template <int TPR, int NV, Access kA>
   int run() {
@@ -677,8 +697,12 @@ template <bool kFp8>
 int launch_fwd(const NormFwd &p, int dtype, cudaStream_t s) {
   const Access access = access_of(p.sh, p.d, dtype, p.x, p.r, Rows{}, p.weight, p.y, p.sum);
   if (kFp8 && p.group_log2 >= 0 && access != kPacked) return LA_ERR_UNSUPPORTED;
-  if (dtype == LA_DTYPE_FLOAT32) return by_width_fwd(p.d, access, FwdLaunch<float, kFp8>{p, s});
-  return by_width_fwd(p.d, access, FwdLaunch<__nv_bfloat16, kFp8>{p, s});
+  DeviceInfo info;
+  const int st = current_device_info(&info);
+  if (st != LA_OK) return st;
+  if (dtype == LA_DTYPE_FLOAT32)
+    return by_width_fwd(p.d, access, FwdLaunch<float, kFp8>{p, info.sm_count, s});
+  return by_width_fwd(p.d, access, FwdLaunch<__nv_bfloat16, kFp8>{p, info.sm_count, s});
 }
 
 int launch_bwd(const NormBwd &p, int dtype, int sm_count, int *grid, cudaStream_t s) {
