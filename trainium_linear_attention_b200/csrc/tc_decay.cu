@@ -37,8 +37,9 @@
 // two buffers, and tiles prefetched into L2 were measured and are no faster.
 //
 // Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state (8 warps
-// at DK = 128, else 4); 8 warps P; 4 warps V'; 4 warps epilogue.  Every wait is
-// bounded (tc_common.cuh).
+// at DK = 128, else 4); 8 warps P; 4 warps V' (the state pass, which has no P and
+// epilogue, 8: 16 heads of 16384 x 64 in 46 us instead of 47, their gradients in 92
+// instead of 95); 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
 #include <type_traits>
 
 #include "decay.cuh"
@@ -75,7 +76,8 @@ struct TcLayout {
   static constexpr int kWState = 4;
   static constexpr int kWP = kWState + kStateWarps;  // first P warp
   static constexpr int kWV = kStateOnly ? kWP : kWP + 8;
-  static constexpr int kWE = kWV + 4;
+  static constexpr int kVWarps = kStateOnly ? 8 : 4;
+  static constexpr int kWE = kWV + kVWarps;
   static constexpr int kWarps = kStateOnly ? kWE : kWE + 4;
   static constexpr int kThreads = kWarps * 32;
   // stage: A, B (kKBlocks blocks each), V (one block)
@@ -221,11 +223,12 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     for (int i = 0; i < kNumBars; ++i) {
       const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 ||
                                   i == kUFree || i == kUFree + 1;
-      const bool per_four =
-          i == kVpReady || i == kVpReady + 1 || i == kOFree || i == kOFree + 1;
+      const bool per_v_warp = i == kVpReady || i == kVpReady + 1;
+      const bool per_four = i == kOFree || i == kOFree + 1;
       const bool per_p_warp = i == kPReady || i == kPReady + 1;
       const bool stage_empty = i >= kEmpty && i < kEmpty + 6;
       mbar_init(&bars[i], per_state_warp ? L::kStateWarps
+                          : per_v_warp   ? L::kVWarps
                           : per_four     ? 4
                           : per_p_warp   ? 8
                           : stage_empty  ? (kStateOnly ? 1 : 2)
@@ -626,7 +629,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     else walk(std::false_type{});
   } else if (warp >= L::kWV && warp < L::kWE) {
     // ------------------------------------------------------------ V' = hi + lo
-    const int j = (warp - L::kWV) * 32 + lane;  // token of the tile
+    const int j = ((warp - L::kWV) & 3) * 32 + lane;  // token of the tile
+    constexpr uint32_t kPart = 512 / L::kVWarps;      // bytes of its row
+    const uint32_t q0 = (uint32_t)((warp - L::kWV) >> 2) * kPart;
     // tokens from this one to the tile's end; in a reversed walk the tile ends at
     // its first token, and the state there decays once more
     const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
@@ -653,7 +658,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const uint32_t src = row + s * L::kStageBytes + L::kOffV,
                      dst = row + L::kOffVp + vb * 2 * kBlock;
 #pragma unroll 2
-      for (uint32_t q = 0; q < 8 * 16; q += 16) {  // a piece of the row: its swizzle is an xor
+      for (uint32_t q = q0; q < q0 + kPart; q += 16) {  // a piece of the row: its swizzle is an xor
         uint32_t x[4], hi[4], lo[4];
         ld_shared_v4(src ^ q, x[0], x[1], x[2], x[3]);
 #pragma unroll
