@@ -43,6 +43,23 @@ def ref_decay_attn(q, k, v, log_decay, scale=None, initial_state=None):
     return out * scale, state
 
 
+def _gradients(ctx, d_out, d_state=None):
+    q, k, v, log_decay, initial_state = ctx.saved_tensors
+    if d_out is None and d_state is None:
+        return (None,) * 7
+    if d_out is None:
+        d_out = torch.zeros_like(v)
+    need = ctx.needs_input_grad
+    dq, dk, dv, d0 = ops.decay_attention_backward(
+        q, k, v, log_decay, d_out, scale=ctx.scale, initial_state=initial_state,
+        d_state=d_state, want_d_initial=need[4])
+    return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
+            None, d0, None, None)
+
+
+_gradients_once = once_differentiable(_gradients)
+
+
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, scale, return_state):
@@ -54,19 +71,11 @@ class _DecayAttention(torch.autograd.Function):
         return got
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out, d_state=None):
-        q, k, v, log_decay, initial_state = ctx.saved_tensors
-        if d_out is None and d_state is None:
-            return (None,) * 7
-        if d_out is None:
-            d_out = torch.zeros_like(v)
-        need = ctx.needs_input_grad
-        dq, dk, dv, d0 = ops.decay_attention_backward(
-            q, k, v, log_decay, d_out, scale=ctx.scale, initial_state=initial_state,
-            d_state=d_state, want_d_initial=need[4])
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
-                None, d0, None, None)
+    def backward(ctx, *grads):
+        # (gradients of gradients are refused; the check costs 4 us elsewhere)
+        if torch.is_grad_enabled():
+            return _gradients_once(ctx, *grads)
+        return _gradients(ctx, *grads)
 
 
 def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,

@@ -25,6 +25,19 @@ def ref_rms_norm(x, weight=None, residual=None, eps=1e-6):
     return (y if weight is None else y * weight), s
 
 
+def _gradients(ctx, d_y, d_sum=None):
+    s, weight, rstd = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    if d_y is None:  # only the sum was used
+        d_w = torch.zeros_like(weight) if need[1] else None
+        return d_sum if need[0] else None, d_w, d_sum if need[2] else None, None
+    d_s, d_w = ops.rms_norm_backward(s, weight, rstd, d_y, d_sum, want_d_weight=need[1])
+    return d_s if need[0] else None, d_w, d_s if need[2] else None, None
+
+
+_gradients_once = once_differentiable(_gradients)
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -34,15 +47,11 @@ class _RmsNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, d_y, d_sum=None):
-        s, weight, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if d_y is None:  # only the sum was used
-            d_w = torch.zeros_like(weight) if need[1] else None
-            return d_sum if need[0] else None, d_w, d_sum if need[2] else None, None
-        d_s, d_w = ops.rms_norm_backward(s, weight, rstd, d_y, d_sum, want_d_weight=need[1])
-        return d_s if need[0] else None, d_w, d_s if need[2] else None, None
+    def backward(ctx, *grads):
+        # (gradients of gradients are refused; the check costs 4 us elsewhere)
+        if torch.is_grad_enabled():
+            return _gradients_once(ctx, *grads)
+        return _gradients(ctx, *grads)
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6):

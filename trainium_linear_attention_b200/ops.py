@@ -263,6 +263,22 @@ def _keep(plans: dict, key, plan):
     return plan
 
 
+_one_element: dict = {}
+
+
+def _proto(shape, dtype, device):
+    """One element (never read) seen as ``shape``: ``torch.empty_like`` of it makes
+    that contiguous tensor in a third of the time of ``torch.empty`` with its
+    shape, type and device (1 against 3 us)."""
+    if 0 in shape:
+        return torch.empty(shape, dtype=dtype, device=device)
+    key = (dtype, device)
+    one = _one_element.get(key)
+    if one is None:
+        one = _one_element[key] = torch.empty((), dtype=dtype, device=device)
+    return one.expand(shape)
+
+
 # ---- linear attention with a decay for each head ---------------------------------
 def _heads_strides(t: torch.Tensor):
     """Strides of ``t`` (b, h, t, d) as the kernels read it in place -- a dense
@@ -285,12 +301,11 @@ def _tokens_first(t: torch.Tensor) -> bool:
     return t.shape[1] > 1 and t.shape[2] > 1 and t.stride(1) < t.stride(2)
 
 
-def _empty_heads(b, h, n, d, dtype, device, tokens_first, like=None):
+def _empty_heads(b, h, n, d, proto, tokens_first, like=None):
     if like is not None:  # dense, and laid out as wanted
         return torch.empty_like(like)
-    if tokens_first:
-        return torch.empty((b, n, h, d), dtype=dtype, device=device).transpose(1, 2)
-    return torch.empty((b, h, n, d), dtype=dtype, device=device)
+    out = torch.empty_like(proto)
+    return out.transpose(1, 2) if tokens_first else out
 
 
 def _check_log_decay(log_decay, heads, device):
@@ -314,7 +329,8 @@ class _DecayPlan:
     """One signature of the decayed linear attention: sizes, strides, workspace."""
 
     __slots__ = ("index", "device", "dtype", "sizes", "scale", "pack", "copy", "strides",
-                 "outs", "dense", "out_strides", "state_shape", "ws_bytes", "pad")
+                 "outs", "dense", "out_strides", "state_shape", "state", "ws_bytes", "workspace",
+                 "pad")
 
     def __init__(self, q, k, v, log_decay, states, grad, segments):
         code = _check_qkv(q, k, v)
@@ -337,23 +353,35 @@ class _DecayPlan:
         self.pack = tuple(q.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0 for x in read)
         # widths that no 16-byte pack divides are widened with zeros for the
         # tensor-core kernel (the CUDA-core one takes them as they are)
-        self.pad = (-d % 8, -dv % 8) if q.dtype == torch.bfloat16 and (d % 8 or dv % 8) else None
+        # but for a few tiles of 64 tokens at 10 us each, which it walks before the
+        # copies are launched: forward / gradients of 4 heads of 55 x 40 / 57 23 / 23
+        # us against 83 / 135, of 64 heads of 1000 x 60 172 / 335 against 91 / 152
+        walks = (b * h * -(-dv // 64) if grad is None
+                 else b * h * (2 * -(-d // 64) + -(-dv // 64)))
+        per_sm = -(-walks // torch.cuda.get_device_properties(q.device).multi_processor_count)
+        self.pad = ((-d % 8, -dv % 8) if q.dtype == torch.bfloat16 and (d % 8 or dv % 8)
+                    and per_sm * -(-t // 64) > 6 else None)
         self.strides = tuple(_heads_strides(x) for x in read)
         self.copy = any(s is None for s in self.strides)
         written = (v,) if grad is None else (q, k, v)
-        self.outs = tuple((b, h, t, x.shape[-1], x.dtype, x.device, _tokens_first(x))
-                          for x in written)
+        self.outs = tuple(
+            (b, h, t, x.shape[-1],
+             _proto((b, t, h, x.shape[-1]) if _tokens_first(x) else (b, h, t, x.shape[-1]),
+                    x.dtype, x.device), _tokens_first(x))
+            for x in written)
         self.dense = tuple((x.transpose(1, 2) if o[-1] else x).is_contiguous()
                            for x, o in zip(written, self.outs))
         self.out_strides = tuple(
             _Strides(h * t * w, w if first else t * w, h * w if first else w)
-            for _, _, _, w, _, _, first in self.outs)
+            for _, _, _, w, _, first in self.outs)
         n, ws = ctypes.c_int(0), ctypes.c_size_t(0)
         with _on_device(q.device):
             st = N.lib().la_decay_plan(*self.sizes, int(grad is not None), segments,
                                        ctypes.byref(n), ctypes.byref(ws))
         N.check(st, "la_decay_plan")
         self.ws_bytes = ws.value
+        self.workspace = _proto((ws.value,), torch.uint8, q.device) if ws.value else None
+        self.state = _proto(self.state_shape, torch.float32, q.device)
 
 
 _decay_plans: dict = {}
@@ -433,13 +461,12 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_s
             return decay_attention(q, k, v, log_decay, scale, initial_state, return_state,
                                    segments)
     out = _empty_heads(*plan.outs[0], v if plan.dense[0] else None)
-    final = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
-             if return_state else None)
+    final = torch.empty_like(plan.state) if return_state else None
     if not log_decay.is_contiguous():
         log_decay = log_decay.contiguous()
     if initial_state is not None and not initial_state.is_contiguous():
         initial_state = initial_state.contiguous()
-    workspace = _workspace(plan.ws_bytes, plan.device)
+    workspace = None if plan.workspace is None else torch.empty_like(plan.workspace)
     qs, ks, vs = plan.strides
     st = N.lib().la_decay_chunked_fwd(
         q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), plan.out_strides[0],
@@ -476,12 +503,11 @@ def decay_attention_backward(q, k, v, log_decay, d_out, scale=None, initial_stat
                                             d_state, want_d_initial, segments)
     gq, gk, gv = (_empty_heads(*o, x if dense else None)
                   for o, x, dense in zip(plan.outs, (q, k, v), plan.dense))
-    g0 = (torch.empty(plan.state_shape, dtype=torch.float32, device=plan.device)
-          if want_d_initial else None)
+    g0 = torch.empty_like(plan.state) if want_d_initial else None
     log_decay = log_decay.contiguous()
     initial_state = None if initial_state is None else initial_state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
-    workspace = _workspace(plan.ws_bytes, plan.device)
+    workspace = None if plan.workspace is None else torch.empty_like(plan.workspace)
     qs, ks, vs, ds = plan.strides
     gqs, gks, gvs = plan.out_strides
     st = N.lib().la_decay_chunked_bwd(
@@ -519,7 +545,7 @@ class _StepPlan:
         self.device, self.dtype, self.index = q.device, q.dtype, q.device.index
         self.sizes = (b, h, d, dv, code)
         self.scale = 1.0 / math.sqrt(d)
-        self.out = (b, h, dv)
+        self.out = _proto((b, h, dv), q.dtype, q.device)
         self.copy = any(x.stride(2) != 1 and x.shape[2] > 1 for x in (q, k, v))
         self.strides = tuple(_Strides(*x.stride()) for x in (q, k, v)) + (_Strides(sb, sh),)
 
@@ -547,7 +573,7 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
             return decay_attention_step(q, k, v, log_decay, state, scale)
     if not log_decay.is_contiguous():
         log_decay = log_decay.contiguous()
-    out = torch.empty(plan.out, dtype=plan.dtype, device=plan.device)
+    out = torch.empty_like(plan.out)
     qs, ks, vs, ss = plan.strides
     st = N.lib().la_decay_step(
         q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), state.data_ptr(), ss,
@@ -583,8 +609,8 @@ class _NormPlan:
     the first of them under ``name``, the others of the same shape and type."""
 
     __slots__ = ("index", "device", "dtype", "shape", "lead", "d", "codes", "strides", "c_shape",
-                 "copy", "aligned", "weight_copy", "as_is", "dense", "group", "scales_shape",
-                 "ws_bytes")
+                 "copy", "aligned", "weight_copy", "as_is", "dense", "group", "rstd", "scales",
+                 "workspace", "ws_bytes")
 
     def __init__(self, rows, names, weight, group_size):
         x = rows[0]
@@ -606,7 +632,8 @@ class _NormPlan:
                              f"got {group_size}")
         self.device, self.dtype, self.index = x.device, x.dtype, x.device.index
         self.shape, self.lead, self.d, self.codes = x.shape, x.shape[:-1], d, (code, wcode)
-        self.scales_shape = (*x.shape[:-1], d // self.group)
+        self.rstd = _proto(self.lead, torch.float32, x.device)
+        self.scales = _proto((*self.lead, d // self.group), torch.float32, x.device)
         self.weight_copy = weight is not None and not weight.is_contiguous()
         lead = x.shape[:-1]
         if all(t is None or t.is_contiguous() for t in rows):
@@ -635,6 +662,7 @@ class _NormPlan:
             N.check(N.lib().la_rms_norm_bwd_workspace_size(x.numel() // d, d, ctypes.byref(n)),
                     "la_rms_norm_bwd_workspace_size")
         self.ws_bytes = n.value
+        self.workspace = _proto((n.value,), torch.uint8, x.device) if n.value else None
 
 
 _norm_plans: dict = {}
@@ -686,8 +714,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-6, want_rstd: bool =
             return rms_norm(x, weight, residual, eps, want_rstd)
     y = _empty_rows(plan, x)
     total = torch.empty_like(y) if residual is not None else None
-    rstd = (torch.empty(plan.lead, dtype=torch.float32, device=plan.device) if want_rstd
-            else None)
+    rstd = torch.empty_like(plan.rstd) if want_rstd else None
     st = N.lib().la_rms_norm_fwd(
         x.data_ptr(), plan.strides[0], _ptr(residual), plan.strides[1], _ptr(weight), y.data_ptr(),
         _ptr(total), _ptr(rstd), plan.c_shape, plan.d, *plan.codes, eps, _stream_ptr(plan.device))
@@ -707,7 +734,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps: float = 1e-6, group_size: i
         with torch.cuda.device(plan.index):
             return rms_norm_fp8(x, weight, residual, eps, group_size)
     y = _empty_rows(plan, x, torch.float8_e4m3fn)
-    scales = torch.empty(plan.scales_shape, dtype=torch.float32, device=plan.device)
+    scales = torch.empty_like(plan.scales)
     total = _empty_rows(plan, x) if residual is not None else None
     st = N.lib().la_rms_norm_fp8(
         x.data_ptr(), plan.strides[0], _ptr(residual), plan.strides[1], _ptr(weight), y.data_ptr(),
@@ -735,7 +762,8 @@ def rms_norm_backward(s, weight, rstd, d_y, d_sum=None, want_d_weight: bool = Tr
     d_w = workspace = None
     if want_d_weight and weight is not None:
         d_w = torch.empty_like(weight)
-        workspace = _workspace(plan.ws_bytes, plan.device)
+        if plan.workspace is not None:
+            workspace = torch.empty_like(plan.workspace)
     st = N.lib().la_rms_norm_bwd(
         s.data_ptr(), plan.strides[0], _ptr(weight), d_y.data_ptr(), plan.strides[1], _ptr(d_sum),
         plan.strides[2], rstd.data_ptr(), d_s.data_ptr(), _ptr(d_w), plan.c_shape, plan.d,
