@@ -351,11 +351,12 @@ class _DecayPlan:
         read = (q, k, v) if grad is None else (q, k, v, grad)
         # bf16 rows of whole 16-byte packs have to start at 16 bytes
         self.pack = tuple(q.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0 for x in read)
-        # widths that no 16-byte pack divides are widened with zeros for the
-        # tensor-core kernel (the CUDA-core one takes them as they are)
-        # but for a few tiles of 64 tokens at 10 us each, which it walks before the
-        # copies are launched: forward / gradients of 4 heads of 55 x 40 / 57 23 / 23
-        # us against 83 / 135, of 64 heads of 1000 x 60 172 / 335 against 91 / 152
+        # Widths that no 16-byte pack divides are widened with zeros for the
+        # tensor-core kernel.  The CUDA-core kernel takes them as they are, at 10 us
+        # per tile of 64 tokens, and has walked a few of those before the copies are
+        # launched: forward / gradients of 4 heads of 55 x 40 / 57 in 23 / 24 us
+        # against 83 / 135 widened, of 64 heads of 1000 x 60 in 173 / 342 against
+        # 83 / 150.
         walks = (b * h * -(-dv // 64) if grad is None
                  else b * h * (2 * -(-d // 64) + -(-dv // 64)))
         per_sm = -(-walks // torch.cuda.get_device_properties(q.device).multi_processor_count)
