@@ -63,7 +63,7 @@ DecaySplit estimate_split(int64_t bh, int64_t n, int64_t d_qk, int64_t d_v, int 
   // segments 28 / 45 / 76; the gradients of 64 heads of 4096 tokens, 192 CTAs,
   // unsplit 89 us, in two segments 94.  fp32: 64 heads of 4096 tokens unsplit
   // 468 us, in 2 / 4 / 8 segments 324 / 321 / 337.)
-  const bool simt = dtype == LA_DTYPE_FLOAT32;
+  const bool simt = dtype == LA_DTYPE_FLOAT32 || d_qk % 8 || d_v % 8;  // (TMA addresses the rest)
   const double t_out = simt ? (wide ? 25.0 : 14.3) : (wide ? 2.1 : 1.3);
   const double t_state = simt ? (wide ? 9.0 : 5.1) : (wide ? 1.2 : 0.8);
   constexpr double kWaveOut = 4.0, kWaveState = 3.0, kSplit = 5.0, kJoin = 0.4;

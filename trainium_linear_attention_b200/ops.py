@@ -353,15 +353,17 @@ class _DecayPlan:
         self.pack = tuple(q.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0 for x in read)
         # Widths that no 16-byte pack divides are widened with zeros for the
         # tensor-core kernel.  The CUDA-core kernel takes them as they are, at 10 us
-        # per tile of 64 tokens, and has walked a few of those before the copies are
-        # launched: forward / gradients of 4 heads of 55 x 40 / 57 in 23 / 24 us
-        # against 83 / 135 widened, of 64 heads of 1000 x 60 in 173 / 342 against
-        # 83 / 150.
-        walks = (b * h * -(-dv // 64) if grad is None
+        # per tile of 64 tokens and SM, and has walked a few of those before the
+        # copies are launched: forward / gradients of 4 heads of 55 x 40 / 57 in 23 /
+        # 24 us against 83 / 135 widened, of 32 heads of 500 x 60 in 52 / 93 against
+        # 87 / 137, of 64 heads of 1000 x 60 in 138 / 321 against 85 / 150, of one head
+        # of 32768 x 60 in 155 / 205 against 89 / 140.
+        walks = (b * h * -(-dv // 64) * (1 if d <= 64 else 2) if grad is None
                  else b * h * (2 * -(-d // 64) + -(-dv // 64)))
-        per_sm = -(-walks // torch.cuda.get_device_properties(q.device).multi_processor_count)
+        few = t <= 4096 and walks * -(-t // 64) <= 6 * torch.cuda.get_device_properties(
+            q.device).multi_processor_count
         self.pad = ((-d % 8, -dv % 8) if q.dtype == torch.bfloat16 and (d % 8 or dv % 8)
-                    and per_sm * -(-t // 64) > 6 else None)
+                    and not few else None)
         self.strides = tuple(_heads_strides(x) for x in read)
         self.copy = any(s is None for s in self.strides)
         written = (v,) if grad is None else (q, k, v)
