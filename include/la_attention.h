@@ -234,8 +234,9 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
  * with S_{-1} = init_state (zero if null).  The state is fp32 (batch, heads,
  * d_qk, d_v), contiguous; log_decay is fp32 (heads) in device memory, finite
  * and <= 0 or -inf (no memory).  d_qk and d_v are at most 128 and need not be
- * equal; batch * heads is at most 65535 for prompts and their gradients.  The reference has no decayed form; the recurrence without decay is
- * its chunked kernel's (kernels/nki_attention_chunked.py:20-113).
+ * equal; batch * heads is at most 65535 for prompts and their gradients.  The
+ * reference has no decayed form; the recurrence without decay is its chunked
+ * kernel's (kernels/nki_attention_chunked.py:20-113).
  *
  * q, k, v, out and the gradients are (batch, heads, seq_len, d) with a dense
  * last dimension and any strides {batch, heads, seq_len} (in elements), so a
@@ -244,7 +245,8 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
  *
  * segments: each head's sequence is split into this many segments walked by
  * different CTAs (0 = let the library choose); more than one needs the
- * workspace (256-byte aligned) that la_decay_plan reports.  A value that is
+ * workspace (256-byte aligned) that la_decay_plan reports, which for two of the
+ * library's own choice may be none.  A value that is
  * not finite reaches every output of its own 128-token tile, and what the
  * recurrence carries it to.
  * ------------------------------------------------------------------------- */

@@ -9,12 +9,14 @@ bf16 inputs the weights that multiply v and the state that multiplies q are
 rounded once to bf16 (half a step: 2^-8), and so is the output.
 """
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import trainium_linear_attention_b200 as T
+from trainium_linear_attention_b200 import _native as N
 from trainium_linear_attention_b200 import ops
 
 gpu = pytest.mark.gpu
@@ -311,6 +313,36 @@ def test_gradients(t, dk, dv, segments, dtype):
         kind = torch.float32 if i == 3 else dtype
         slack = 2.0 ** -17 if i == 3 and dtype == torch.bfloat16 else 0.0
         assert ((x.double() - y).abs() <= bound(kind, y, a, t, max(dk, dv)) + slack * a).all(), i
+
+
+@gpu
+@pytest.mark.parametrize("heads,t,dk,dv,backward", [
+    (48, 1024, 64, 64, False), (24, 1000, 64, 64, False), (30, 1023, 128, 128, False),
+    (50, 300, 32, 16, False), (40, 1300, 16, 64, False), (16, 1001, 64, 64, True),
+    (16, 1024, 32, 24, True), (20, 129, 64, 64, True)])
+def test_two_parts(heads, t, dk, dv, backward):
+    """Few heads are walked in two parts without a state pass: the same steps as
+    one walk, and so the same bits."""
+    q, k, v, g, state = make(1, heads, t, dk, dv, torch.bfloat16, "bthd", seed=t)
+    n, size = ctypes.c_int(0), ctypes.c_size_t(1)
+    assert N.lib().la_decay_plan(1, heads, t, dk, dv, N.LA_DTYPE_BFLOAT16, int(backward), 0,
+                                 ctypes.byref(n), ctypes.byref(size)) == N.LA_OK
+    assert (n.value, size.value) == (2, 0)
+    if backward:
+        do = torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).to(v.dtype).cuda()
+        ds = torch.randn(state.shape, generator=torch.Generator().manual_seed(2)).cuda()
+
+        def run(segments):
+            return ops.decay_attention_backward(q, k, v, g, do, initial_state=state, d_state=ds,
+                                                want_d_initial=True, segments=segments)
+    else:
+        check_forward(q, k, v, g, 0.125, state)
+
+        def run(segments):
+            return ops.decay_attention(q, k, v, g, initial_state=state, return_state=True,
+                                       segments=segments)
+    for x, y in zip(run(0), run(1)):
+        assert torch.equal(x, y)
 
 
 @gpu

@@ -62,6 +62,11 @@ struct DecayCall {
   int64_t whole = 0;
   int64_t seg_len = 0;
   int segments = 1;
+  // Tensor-core kernel: with `lead` > 0 every head is walked in two parts (segments
+  // = 2) without a state pass or a workspace: the outputs of the walk's first `lead`
+  // tiles by one CTA, those of the others by a second one that walks the first
+  // tiles for the state alone.
+  int lead = 0;
   int dtype = 0;
 };
 

@@ -141,6 +141,7 @@ struct TcParams {
   // heads [0, whole) are walked by one CTA per role and slice, the others in
   // segments; a state pass walks all but the last of those
   int64_t whole, seg_len;
+  int lead;  // 0, or the tiles of the first of two parts (decay.cuh)
   int roles, slices, segments, orders;
 };
 
@@ -174,7 +175,7 @@ __device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
   return true;
 }
 
-template <int DK, bool kStateOnly>
+template <int DK, bool kStateOnly, bool kLead>
 __global__ void __launch_bounds__(TcLayout<DK, kStateOnly>::kThreads, 1)
 decay_tc_kernel(const __grid_constant__ TcParams p) {
   using L = TcLayout<DK, kStateOnly>;
@@ -204,12 +205,19 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   const int ib = (int)(bh / p.heads), ih = (int)(bh % p.heads);
   const bool rev = role.reverse != 0;
   const int e0 = rev ? 0 : 1;
-  const int64_t t0 = (int64_t)(rev ? segments - 1 - order : order) * seg_len;
-  const int64_t t1 = min64(p.n, t0 + seg_len);
+  // two parts without a state pass: a kernel of its own, since its few instructions
+  // more made the other walks 2 to 4% slower
+  const int pre = kLead && order > 0 ? p.lead : 0;  // tiles walked for the state alone
+  const bool joins = !kStateOnly && !kLead && order > 0;
+  const int64_t part = (int64_t)p.lead * kT;
+  const int64_t t0 = !kLead ? (int64_t)(rev ? segments - 1 - order : order) * seg_len
+                     : rev && order == 0 ? (p.n + kT - 1) / kT * kT - part : 0;
+  const int64_t t1 = !kLead ? min64(p.n, t0 + seg_len) : rev || order > 0 ? p.n : part;
   const int tiles = (int)((t1 - t0 + kT - 1) / kT);
   const bool want_final =
       kStateOnly || (role.final_state != nullptr && order == segments - 1);
   // tiles whose U is needed: the last one's only for the final state
+  const int outs = tiles - pre;  // tiles of the output
   const int updates = want_final ? tiles : (tiles > 0 ? tiles - 1 : 0);
   const float g = p.log_decay[ih];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -242,7 +250,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   // space of V' and the copies of S:
   //   lambda^(tokens so far) init + sum_o lambda^(tokens from o's end on) states_o
   float *joined = (float *)(smem + L::kOffVp);
-  if (!kStateOnly && order > 0) {
+  if (joins) {
     constexpr int kEach = (DK * 64 + L::kThreads - 1) / L::kThreads;
     const int64_t per_head = (int64_t)role.da * role.dvo;
     // neighbouring threads read neighbouring addresses: columns first, or rows
@@ -302,11 +310,13 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
           break;
         const int y = (int)tile_start(c);
         uint8_t *st = smem + s * L::kStageBytes;
-        mbar_arrive_expect_tx(&bars[kFull + s], L::kStageBytes);
+        const bool with_a = !kStateOnly && (!kLead || c >= pre);
+        mbar_arrive_expect_tx(&bars[kFull + s],
+                              kStateOnly || with_a ? L::kStageBytes : L::kStageBytes - L::kOffB);
 #pragma unroll
         for (int b = 0; b < L::kKBlocks; ++b) {
           tma_load_4d(st + L::kOffB + b * L::kKBlock, mb, &bars[kFull + s], 64 * b, y, ih, ib);
-          if (!kStateOnly)
+          if (with_a)
             tma_load_4d(st + L::kOffA + b * L::kKBlock, ma, &bars[kFull + s], 64 * b, y, ih, ib);
         }
         tma_load_4d(st + L::kOffV, mv, &bars[kFull + s], c0, y, ih, ib);
@@ -326,7 +336,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const uint64_t a0 = make_sdesc(sb + L::kOffA, 16, L::kKGroup, L::kKSwizzle);
       const uint64_t b0 = make_sdesc(sb + L::kOffB, 16, L::kKGroup, L::kKSwizzle);
       const uint64_t s0 = make_sdesc(sb + L::kOffSnap, 16, 1024, kSwizzle128B);
-      int ss = 0, sp = 0;  // stage of the next scores and its phase
+      int ss = pre % kStages, sp = (pre / kStages) & 1;  // stage of the next scores, its phase
       auto issue_scores = [&](int c) -> bool {
         if (!mbar_wait_warp(&bars[kFull + ss], sp, abort_flag)) return false;
         // the buffer: P of tile c - 2 has been read by P V
@@ -347,13 +357,16 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         if (++ss == kStages) ss = 0, sp ^= 1;
         return true;
       };
-      bool ok = tiles > 0 && issue_scores(0);
-      int rs = 0;  // stage of tile c
-      for (int c = 0; ok && c < tiles; ++c) {
+      // behind tiles walked for the state alone a stage's phase tells the first tile
+      // from those before it only once they are done: when the state is ready
+      bool ok = outs > 0 &&
+                (!kLead || pre == 0 || mbar_wait_warp(&bars[kSnapReady], 0, abort_flag)) && issue_scores(0);
+      int rs = pre % kStages;  // stage of tile c
+      for (int c = 0; ok && c < outs; ++c) {
         const int b = c & 1;
         // the next tile's scores go first if nothing holds them up
         const bool early =
-            c + 1 < tiles &&
+            c + 1 < outs &&
             __all_sync(0xffffffffu,
                        mbar_test_wait(&bars[kFull + ss], sp) &&
                            (c == 0 || mbar_test_wait(&bars[kOReady + (b ^ 1)], ((c - 1) / 2) & 1)));
@@ -373,7 +386,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
         }
         __syncwarp();
         if (++rs == kStages) rs = 0;
-        if (c + 1 < tiles && !early && !issue_scores(c + 1)) break;
+        if (c + 1 < outs && !early && !issue_scores(c + 1)) break;
       }
       if (elect_one()) umma_commit(&bars[kDone]);
       __syncwarp();
@@ -422,11 +435,13 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     if constexpr (!kStateOnly) {
       constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, true);
       const uint64_t v0 = make_sdesc(sb + L::kOffV, 16, 1024, kSwizzle128B);
-      int vs = 0, vp = 0;  // stage and its phase
-      for (int c = 0; c < tiles; ++c) {
+      int vs = pre % kStages, vp = (pre / kStages) & 1;  // stage and its phase
+      for (int c = 0; c < outs; ++c) {
         const int b = c & 1;
+        // (with tiles before the output's P first: it is behind the scores)
+        if (kLead && !mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
         if (!mbar_wait_warp(&bars[kFull + vs], vp, abort_flag)) break;
-        if (!mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
+        if (!kLead && !mbar_wait_warp(&bars[kPReady + b], (c / 2) & 1, abort_flag)) break;
         // the columns: O2 of tile c - 1 has been read out
         if (c > 0 && !mbar_wait_warp(&bars[kOFree + (b ^ 1)], ((c - 1) / 2) & 1, abort_flag)) break;
         tc_fence_after();
@@ -464,7 +479,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     for (int i = 0; i < kCols; ++i) st[i] = 0.f;
     if constexpr (kStateOnly) {
       grid_dependents_launch();
-    } else if (order > 0) {
+    } else if (joins) {
       const float *src = joined + row * kJoinPitch + part * kCols;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) st[i] = src[i];
@@ -483,9 +498,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     int stage = 0;
 #pragma unroll 1
     for (int c = 0;; ++c) {
-      if (!kStateOnly && c < tiles) {  // the copy of S that tile c reads
-        const int b = c & 1;
-        if (c >= 2) mbar_wait(&bars[kRead + b], ((c - 2) / 2) & 1, abort_flag);
+      if (!kStateOnly && (!kLead || c >= pre) && c < tiles) {  // the copy of S that tile c reads
+        const int at = c - pre, b = at & 1;
+        if (at >= 2) mbar_wait(&bars[kRead + b], ((at - 2) / 2) & 1, abort_flag);
         __syncwarp();
         const uint32_t dst = copy_row + b * L::kSnapBytes;
 #pragma unroll
@@ -503,7 +518,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const uint64_t keep2 = f2pack(keep, keep);
       mbar_wait(&bars[kUReady + (c & 1)], (c / 2) & 1, abort_flag);
       // B and V of the tile's stage have been read by U (and V')
-      if (warp == L::kWState && lane == 0) mbar_arrive(&bars[kEmpty + stage]);
+      if (warp == L::kWState && lane == 0) {
+        mbar_arrive(&bars[kEmpty + stage]);
+        if (kLead && c < pre) mbar_arrive(&bars[kEmpty + stage]);  // for the epilogue
+      }
       if (++stage == kStages) stage = 0;
       __syncwarp();
       tc_fence_after();
@@ -566,7 +584,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // the warp's two blocks of 32 columns: before, on or beyond the diagonal
     const int side0 = (2 * half - wq) * sign, side1 = (2 * half + 1 - wq) * sign;
     auto walk = [&](auto is_mild) {
-      for (int c = 0; c < tiles; ++c) {
+      for (int c = 0; c < outs; ++c) {
         const uint32_t srow0 = taddr(tmem, wq * 32, kColScores + (c & 1) * 128 + half * 64);
         mbar_wait(&bars[kSReady + (c & 1)], (c / 2) & 1, abort_flag);
         __syncwarp();
@@ -638,7 +656,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const float w_ragged = role.inc * decay_pow(g, rev ? j + 1 : ragged_len - 1 - j);
     const uint32_t row = sb + sw128_offset(j, 0);
     int s = 0, phase = 0, vb = 0;
-    if (!kStateOnly && order > 0) named_barrier_sync(1, L::kStateWarps * 32 + 128);
+    if (joins) named_barrier_sync(1, L::kStateWarps * 32 + 128);
     for (int c = 0; c < updates; ++c) {
       const float w = c == ragged ? w_ragged : w_full;
       // w as two bf16 terms; with x * w_hi rounded to hi, the rest of that
@@ -686,15 +704,15 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const int64_t ot = role.ot;
     // columns from this lane's first on, a multiple of 8
     const int columns = role.dvo - c0 - 16 * odd;
-    __nv_bfloat16 *dst = role.out + ib * role.ob + ih * role.oh + (tile_start(0) + row0) * ot + c0 +
+    __nv_bfloat16 *dst = role.out + ib * role.ob + ih * role.oh + (tile_start(pre) + row0) * ot + c0 +
                          16 * odd;
     const int64_t tile_step = (rev ? -kT : kT) * ot;
     const uint32_t o1 = taddr(tmem, wq * 32, kColO1), o2 = taddr(tmem, wq * 32, kColO2);
     auto walk = [&](auto is_wide) {
-      int stage = 0;
-      for (int c = 0; c < tiles; ++c, dst += tile_step) {
-        const int len = c == ragged ? ragged_len : kT;
-        const float f = c == ragged ? f_ragged : f_full;
+      int stage = pre % kStages;
+      for (int c = 0; c < outs; ++c, dst += tile_step) {
+        const int len = c + pre == ragged ? ragged_len : kT;
+        const float f = c + pre == ragged ? f_ragged : f_full;
         const uint64_t f2 = f2pack(f, f);
         mbar_wait(&bars[kRead + (c & 1)], (c / 2) & 1, abort_flag);
         mbar_wait(&bars[kOReady + (c & 1)], (c / 2) & 1, abort_flag);
@@ -794,10 +812,10 @@ bool make_map(CUtensorMap *map, const DecayView &x, int width, int box_cols, con
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DK, bool kStateOnly>
+template <int DK, bool kStateOnly, bool kLead>
 int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
   using L = TcLayout<DK, kStateOnly>;
-  auto kernel = decay_tc_kernel<DK, kStateOnly>;
+  auto kernel = decay_tc_kernel<DK, kStateOnly, kLead>;
   if (allow_dynamic_smem((const void *)kernel, (int)L::kSmem) != LA_OK) return LA_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
@@ -810,7 +828,7 @@ int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
   pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &pdl;
-  cfg.numAttrs = !kStateOnly && p.segments > 1 ? 1 : 0;
+  cfg.numAttrs = !kStateOnly && !kLead && p.segments > 1 ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch();
 }
@@ -861,15 +879,23 @@ int launch(const DecayCall &c, cudaStream_t s) {
   }
   p.log_decay = c.log_decay;
   p.heads = c.heads, p.n = c.n;
-  p.whole = c.whole, p.seg_len = c.seg_len;
+  p.whole = c.whole, p.seg_len = c.seg_len, p.lead = c.lead;
   p.roles = c.roles, p.slices = slices, p.segments = c.segments;
   p.orders = kStateOnly ? c.segments - 1 : c.segments;
   const int64_t walks =
       (kStateOnly ? 0 : c.whole) + (c.batch * c.heads - c.whole) * (int64_t)p.orders;
   const int64_t grid = walks * slices * c.roles;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
-  if (da <= 32) return launch_t<32, kStateOnly>(p, grid, s);
-  return da <= 64 ? launch_t<64, kStateOnly>(p, grid, s) : launch_t<128, kStateOnly>(p, grid, s);
+  if constexpr (!kStateOnly) {
+    if (c.lead > 0) {
+      if (da <= 32) return launch_t<32, false, true>(p, grid, s);
+      return da <= 64 ? launch_t<64, false, true>(p, grid, s)
+                      : launch_t<128, false, true>(p, grid, s);
+    }
+  }
+  if (da <= 32) return launch_t<32, kStateOnly, false>(p, grid, s);
+  return da <= 64 ? launch_t<64, kStateOnly, false>(p, grid, s)
+                  : launch_t<128, kStateOnly, false>(p, grid, s);
 }
 
 }  // namespace
