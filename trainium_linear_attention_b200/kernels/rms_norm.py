@@ -61,7 +61,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     (up to three leading dimensions are read in place); weight: (d,) fp32 or
     bf16, or None for ones; d <= 16384.  Statistics in fp32.  Returns y
     (contiguous, in x.dtype), or with ``residual`` the pair (y, x + residual),
-    where y is normed from the unrounded sum.  Differentiable once."""
+    where y is normed from the unrounded sum.  Differentiable once.  The same
+    call gives the same bits; a row's last bit may go by the number of rows."""
     if torch.is_grad_enabled() and any(
             isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, residual)):
         return _RmsNorm.apply(x, weight, residual, float(eps))
