@@ -205,6 +205,21 @@ def test_segments(t, segments, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("segments", [2, 3, 8])
+@pytest.mark.parametrize("dk,dv", [(128, 64), (128, 128), (64, 128)])
+def test_segments_of_wide_heads(dk, dv, segments):
+    """Keys or values of 128: the joined state's last two rows lie where the copies
+    of the state are written, and every row counts (a large state, slow decays)."""
+    q, k, v, _, state = make(2, 4, 2000, dk, dv, torch.bfloat16, "bthd", seed=segments)
+    g = torch.tensor([0.0, -1e-4, -1e-3, -1e-2], device="cuda")
+    first = check_forward(q, k, v, g, dk ** -0.5, 40 * state, segments)
+    again = ops.decay_attention(q, k, v, g, scale=dk ** -0.5, initial_state=40 * state,
+                                return_state=True, segments=segments)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+    test_gradients(2000, dk, dv, segments, torch.bfloat16)
+
+
+@gpu
 def test_some_heads_split():
     """More heads than SMs: whole ones fill a wave, the rest share the next in
     segments (the default split; seen by its smaller workspace)."""

@@ -97,7 +97,11 @@ struct TcLayout {
   static constexpr uint32_t kOffSnap = kOffVp + kVpBufs * 2 * kBlock;  // two bf16 copies of S
   static constexpr uint32_t kOffBar = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
-  static_assert(kStateOnly || (int)(DK * kJoinPitch * 4) <= kVpBufs * 2 * kBlock + 2 * (int)kSnapBytes,
+  static constexpr int kJoinBytes = DK * kJoinPitch * 4;  // a joined state, from kOffVp on
+  // Whether it reaches beyond V' into the copies of S, as with DK = 128 its last two
+  // rows do: a state warp then may write its copy only once all have read theirs.
+  static constexpr bool kJoinOverCopies = kJoinBytes > kVpBufs * 2 * kBlock;
+  static_assert(kStateOnly || kJoinBytes <= kVpBufs * 2 * kBlock + 2 * (int)kSnapBytes,
                 "joined state");
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kSmem > 114 * 1024, "one CTA per SM (all TMEM columns)");
@@ -483,7 +487,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const float *src = joined + row * kJoinPitch + part * kCols;
 #pragma unroll
       for (int i = 0; i < kCols; ++i) st[i] = src[i];
-      named_barrier_arrive(1, L::kStateWarps * 32 + 128);  // V' may take the space
+      // V' may take the space, and the copies of S what lies in theirs
+      if constexpr (L::kJoinOverCopies) named_barrier_sync(1, L::kStateWarps * 32 + L::kVWarps * 32);
+      else named_barrier_arrive(1, L::kStateWarps * 32 + L::kVWarps * 32);
     } else if (role.init) {
       const int64_t step = role.transposed ? role.da : 1;
       const float *src = role.init + bh * per_head + (role.transposed ? (int64_t)col * role.da + row
@@ -656,7 +662,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const float w_ragged = role.inc * decay_pow(g, rev ? j + 1 : ragged_len - 1 - j);
     const uint32_t row = sb + sw128_offset(j, 0);
     int s = 0, phase = 0, vb = 0;
-    if (joins) named_barrier_sync(1, L::kStateWarps * 32 + 128);
+    if (joins) named_barrier_sync(1, L::kStateWarps * 32 + L::kVWarps * 32);
     for (int c = 0; c < updates; ++c) {
       const float w = c == ragged ? w_ragged : w_full;
       // w as two bf16 terms; with x * w_hi rounded to hi, the rest of that
