@@ -124,6 +124,19 @@ def test_refusals():
         ops._check_state(state.double(), (1, 2, 16, 16), q.device, "state")
 
 
+def test_trained_decay_is_refused():
+    """Also where other inputs are trained: inside an autograd function gradients
+    are off, so the check has to come before it."""
+    q, k, v, g, state = make(1, 2, 8, 16, 16, torch.float32, device="cpu")
+    g.requires_grad_()
+    for i in range(4):
+        inputs = [x.clone().requires_grad_(i == j) for j, x in enumerate((q, k, v, state))]
+        with pytest.raises(ValueError, match="log_decay"):
+            T.decay_linear_attention(*inputs[:3], g, initial_state=inputs[3])
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        T.decay_linear_attention(q, k, v, g)  # the decay itself is accepted
+
+
 def test_c_entry_points_refuse():
     import ctypes
 

@@ -85,7 +85,8 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     q, k: (b, h, t, d_qk); v: (b, h, t, d_v), float32 or bfloat16, widths up to
     128, any strides with a dense last dimension (a projection's transposed
     heads are read in place, and the output is laid out as v).  ``log_decay``:
-    float32 (h,), <= 0, a constant.  ``scale`` defaults to 1/sqrt(d_qk).
+    float32 (h,), <= 0, a constant (one that requires a gradient is refused
+    where gradients are recorded).  ``scale`` defaults to 1/sqrt(d_qk).
     ``initial_state``: fp32 (b, h, d_qk, d_v), the state before the first
     token.  Returns (b, h, t, d_v) in q.dtype, or with ``return_state`` also
     the fp32 state after the last token.  Differentiable once in q, k, v and
@@ -100,6 +101,7 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     fed with 16-bit products (2^-17)."""
     if torch.is_grad_enabled() and any(
             isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, initial_state)):
+        ops._check_constant(log_decay)  # (gradients are off inside the function)
         return _DecayAttention.apply(q, k, v, log_decay, initial_state, scale, bool(return_state))
     return ops.decay_attention(q, k, v, log_decay, scale=scale, initial_state=initial_state,
                                return_state=return_state)

@@ -314,7 +314,12 @@ def _check_log_decay(log_decay, heads, device):
     if (log_decay.dtype != torch.float32 or log_decay.device != device
             or tuple(log_decay.shape) != (heads,)):
         raise ValueError(f"log_decay must be float32 ({heads},) on {device}")
-    if log_decay.requires_grad and torch.is_grad_enabled():
+    _check_constant(log_decay)
+
+
+def _check_constant(log_decay):
+    if (isinstance(log_decay, torch.Tensor) and log_decay.requires_grad
+            and torch.is_grad_enabled()):
         raise ValueError("log_decay is a constant of the operator: it has no gradient")
 
 
