@@ -306,6 +306,34 @@ def test_empty_and_zero_tokens():
     assert torch.equal(torch.autograd.grad(end.sum(), state)[0], torch.ones_like(state))
 
 
+def test_empty_inputs_have_no_strides():
+    """A tensor without elements is contiguous whatever its strides say: a copy
+    does not change them, so they are not looked at."""
+    for shape in ((2, 3, 0, 16), (0, 3, 5, 16), (2, 0, 5, 16)):
+        for x in (torch.zeros(1).expand(shape), torch.zeros(1).bfloat16().expand(shape),
+                  torch.zeros(shape[0], shape[1], shape[3], shape[2]).transpose(2, 3)):
+            assert ops._heads_strides(x) is not None
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,h,t", [(2, 3, 0), (0, 3, 5), (2, 0, 5)])
+def test_empty_inputs_of_any_strides(b, h, t, dtype):
+    one = torch.zeros(1, dtype=dtype, device="cuda")
+    g = torch.zeros(h, device="cuda")
+    state = torch.ones(b, h, 16, 64, device="cuda")
+    q, v = one.expand(b, h, t, 16), one.expand(b, h, t, 64)
+    out, end = T.decay_linear_attention(q, q, v, g, initial_state=state, return_state=True)
+    assert out.shape == (b, h, t, 64) and torch.equal(end, state)
+    leaves = [torch.zeros(x.shape, dtype=dtype, device="cuda", requires_grad=True)
+              for x in (q, q, v)]
+    T.decay_linear_attention(*leaves, g).sum().backward()  # an expanded gradient
+    assert all(x.grad.shape == x.shape for x in leaves)
+    if t:
+        qs, vs = one.expand(b, h, 16), torch.zeros(b, 64, h, dtype=dtype, device="cuda").transpose(1, 2)
+        assert T.decay_linear_attention_step(qs, qs, vs, g, state).shape == (b, h, 64)
+
+
 @gpu
 def test_long_sequence_many_tiles():
     """Slow decays over many tiles: the carried state and its power stay exact."""

@@ -285,6 +285,8 @@ def _heads_strides(t: torch.Tensor):
     last dimension, and for bf16 rows of whole 16-byte packs where the width
     allows them -- or None where they rule that out (or overlap)."""
     b, h, n, d = t.shape
+    if t.numel() == 0:  # contiguous whatever its strides are: a copy would not change them
+        return _Strides(h * n * d, n * d, d)
     sb, sh, st, sd = t.stride()
     ok = ((sd == 1 or d == 1) and (sb > 0 or b == 1) and (sh > 0 or h == 1)
           and (st >= d or n == 1))
@@ -554,7 +556,7 @@ class _StepPlan:
         self.sizes = (b, h, d, dv, code)
         self.scale = 1.0 / math.sqrt(d)
         self.out = _proto((b, h, dv), q.dtype, q.device)
-        self.copy = any(x.stride(2) != 1 and x.shape[2] > 1 for x in (q, k, v))
+        self.copy = any(x.stride(2) != 1 and x.shape[2] > 1 and x.numel() > 0 for x in (q, k, v))
         self.strides = tuple(_Strides(*x.stride()) for x in (q, k, v)) + (_Strides(sb, sh),)
 
 
