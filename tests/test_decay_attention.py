@@ -545,6 +545,20 @@ def test_without_gradients():
 
 
 @gpu
+def test_step_refuses_a_trained_decay_always():
+    """Also after the same call without gradients, whose checks are kept."""
+    q, k, v, g, state = make(1, 2, 1, 16, 24, torch.float32)
+    q, k, v = (x[:, :, 0] for x in (q, k, v))
+    g.requires_grad_()
+    with torch.no_grad():
+        T.decay_linear_attention_step(q, k, v, g, state)
+    before = state.clone()
+    with pytest.raises(ValueError, match="log_decay"):
+        T.decay_linear_attention_step(q, k, v, g, state)
+    assert torch.equal(state, before)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_prompt_in_pieces_then_tokens(dtype):
     """A prompt read at once, in pieces, and token by token end in one state."""

@@ -573,6 +573,7 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None) -> torch.Tensor:
         key = plan = None
     if plan is None:
         plan = _keep(_step_plans, key, _StepPlan(q, k, v, log_decay, state))
+    _check_constant(log_decay)
     if state.requires_grad:
         raise ValueError("state is updated in place: it may not require a gradient")
     if plan.copy:
