@@ -14,6 +14,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import trainium_linear_attention_b200 as T
 from trainium_linear_attention_b200 import _native as N
@@ -135,6 +136,21 @@ def test_trained_decay_is_refused():
             T.decay_linear_attention(*inputs[:3], g, initial_state=inputs[3])
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
         T.decay_linear_attention(q, k, v, g)  # the decay itself is accepted
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor requires no gradient; its tangent may not be lost."""
+    q, k, v, g, state = make(1, 2, 8, 16, 16, torch.float32, device="cpu")
+    calls = [(q, k, v, g, state), tuple(x[:, :, 0] for x in (q, k, v)) + (g, state)]
+    with forward_ad.dual_level():
+        for call, args in zip((lambda q, k, v, g, s: T.decay_linear_attention(
+                q, k, v, g, initial_state=s), T.decay_linear_attention_step), calls):
+            for i, x in enumerate(args):
+                dual = forward_ad.make_dual(x, torch.ones_like(x))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args[:i], dual, *args[i + 1:])
+            with pytest.raises(ValueError, match="CUDA"):
+                call(*args)  # none of them dual
 
 
 def test_c_entry_points_refuse():

@@ -9,6 +9,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import trainium_linear_attention_b200 as T
 from trainium_linear_attention_b200 import _native as N
@@ -292,6 +293,19 @@ def test_refusals():
     y, s = T.ref_rms_norm(x.double(), torch.ones(64).double(), x.double(), EPS)
     assert torch.allclose(s, 2 * x.double()) and torch.allclose(
         y.square().mean(-1), torch.ones(4).double(), rtol=1e-4)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor requires no gradient; its tangent may not be lost."""
+    args = make((4, 64), torch.float32, True, torch.float32, device="cpu")
+    with forward_ad.dual_level():
+        for call in (T.rms_norm, T.rms_norm_fp8):
+            for i, x in enumerate(args):
+                x, r, w = (*args[:i], forward_ad.make_dual(x, torch.ones_like(x)), *args[i + 1:])
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(x, w, r)
+            with pytest.raises(ValueError, match="CUDA"):
+                call(args[0], args[2], args[1])  # none of them dual
 
 
 @gpu

@@ -89,8 +89,8 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     where gradients are recorded).  ``scale`` defaults to 1/sqrt(d_qk).
     ``initial_state``: fp32 (b, h, d_qk, d_v), the state before the first
     token.  Returns (b, h, t, d_v) in q.dtype, or with ``return_state`` also
-    the fp32 state after the last token.  Differentiable once in q, k, v and
-    ``initial_state``.
+    the fp32 state after the last token.  Differentiable once, backward, in q, k,
+    v and ``initial_state``; forward mode is refused.
 
     Sequences of different lengths in one batch: pad them on the left with zero
     k (a zero token adds nothing to the zero state, and ends where the others
@@ -99,6 +99,7 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     be finite.  bf16 runs on tensor cores: the weights of a tile's values and
     the state's read-out are rounded to bf16, the state is carried in fp32 and
     fed with 16-bit products (2^-17)."""
+    ops.check_tangents(q, k, v, log_decay, initial_state)
     if torch.is_grad_enabled() and any(
             isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, initial_state)):
         ops._check_constant(log_decay)  # (gradients are off inside the function)
@@ -113,4 +114,5 @@ def decay_linear_attention_step(q, k, v, log_decay, state, scale=None):
     q, k: (b, h, d_qk); v: (b, h, d_v).  ``state`` (fp32 (b, h, d_qk, d_v), as
     ``decay_linear_attention`` returns it) is updated in place.  Returns
     (b, h, d_v) in q.dtype; no gradient."""
+    ops.check_tangents(q, k, v, log_decay, state)
     return ops.decay_attention_step(q, k, v, log_decay, state, scale=scale)

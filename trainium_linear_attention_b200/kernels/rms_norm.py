@@ -61,8 +61,10 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     (up to three leading dimensions are read in place); weight: (d,) fp32 or
     bf16, or None for ones; d <= 16384.  Statistics in fp32.  Returns y
     (contiguous, in x.dtype), or with ``residual`` the pair (y, x + residual),
-    where y is normed from the unrounded sum.  Differentiable once.  The same
-    call gives the same bits; a row's last bit may go by the number of rows."""
+    where y is normed from the unrounded sum.  Differentiable once, backward
+    (forward mode is refused).  The same call gives the same bits; a row's last
+    bit may go by the number of rows."""
+    ops.check_tangents(x, weight, residual)
     if torch.is_grad_enabled() and any(
             isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, residual)):
         return _RmsNorm.apply(x, weight, residual, float(eps))
@@ -77,5 +79,6 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-6, group_size=None):
     float8_e4m3fn like x, scales fp32 (..., d / group_size) with y * scale the
     normed value; one scale per row without ``group_size``, else per 16, 32,
     64, 128 or 256 neighbours.  A scale is max(amax, 2^-96) / 448."""
+    ops.check_tangents(x, weight, residual)
     y, scales, total = ops.rms_norm_fp8(x, weight, residual, eps, group_size)
     return (y, scales) if residual is None else (y, scales, total)

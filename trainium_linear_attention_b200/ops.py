@@ -14,6 +14,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -228,6 +229,15 @@ def based_layer(q, k, v, window_size: int = 64, eps: float = 1e-6, segments: int
             int(segments), _stream_ptr(q.device))
     N.check(st, "la_based_layer_fwd")
     return out
+
+
+def check_tangents(*tensors) -> None:
+    """Forward-mode derivatives are refused: a dual tensor requires no gradient, and
+    a kernel given its address would drop the tangent."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (-1 outside of a dual level)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("this operator has no forward-mode derivative")
 
 
 # ---- plans ---------------------------------------------------------------------
