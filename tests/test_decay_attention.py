@@ -303,6 +303,24 @@ def test_decays(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_small_values_under_strong_decays(d):
+    """A token's own weight is one however strong the decay: scores of 1e-21 may not
+    meet a power of it on the way there.  Gradients scale with d_out (a step of
+    bf16 where a sum's last bits change, and what falls below fp32 at 2^-126)."""
+    q, k, v, _, state = make(1, 4, 300, d, 64, torch.bfloat16, seed=d)
+    g = torch.tensor([-3.95, -3.0, -2.0, -1.0], device="cuda")
+    small = 2.0 ** -70
+    check_forward(q * small, k, v, g, 0.125, None)
+    check_forward(q * small, k, v, g, 0.125, state)
+    do = torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).to(v.dtype).cuda()
+    grads = [ops.decay_attention_backward(q, k, v, g, up, scale=0.125)[:3]
+             for up in (do, do * small)]
+    for x, y in zip(*(map(torch.Tensor.double, part) for part in grads)):
+        assert ((y / small - x).abs() <= 2.0 ** -7 * x.abs() + 2.0 ** -40 * x.abs().max()).all()
+
+
+@gpu
 def test_empty_and_zero_tokens():
     q, k, v, g, state = make(2, 3, 0, 16, 64, torch.bfloat16)
     out, end = T.decay_linear_attention(q, k, v, g, initial_state=state, return_state=True)

@@ -571,7 +571,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     // lambda^lag over 16 columns j0 + t: f = lambda^(i-j0-15) times w = lambda^(15-t),
     // in a reversed walk lambda^(j0-i) * lambda^t.  Off the diagonal both powers
     // are non-negative; on it the first reaches -15, which fp32 holds while
-    // |g| <= 4, and the columns with lag < 0 are cut from the packed words.
+    // |g| <= 4, and the columns with lag < 0 are cut from the packed words.  The two
+    // are multiplied before they meet the score, which lambda^15 alone (e^-60) could
+    // take below fp32's range.
     const bool mild = g >= -4.f && g <= 4.f;
     const int off = rev ? 0 : 15;
     const int row_lag = (wq * 32 + lane - 64 * half) * sign;  // lag of the warp's first column
@@ -621,9 +623,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll
               for (int t = 0; t < 8; ++t)
                 pk[t] = pack_bf16x2(
-                    fmul2(fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
-                                w2[t]),
-                          f2));
+                    fmul2(f2pack(__uint_as_float(x[2 * t]), __uint_as_float(x[2 * t + 1])),
+                          fmul2(w2[t], f2)));
             } else {  // strong decays: each column its own power
               float l = (float)lag;
 #pragma unroll
