@@ -449,6 +449,26 @@ def test_odd_widths(b, t, dk, dv):
 
 
 @gpu
+def test_odd_widths_take_their_paths():
+    """Which of test_odd_widths' cases are widened; empty inputs never are."""
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the number of tiles that count as few goes by the SMs")
+    widened = {  # (d_qk, d_v): forward, backward, by (batch, tokens) below
+        (57, 33): ((0, 0, 0, 1, 1), (0, 0, 1, 1, 1)),
+        (20, 100): ((0, 0, 1, 1, 1), (0, 0, 1, 1, 1)),
+        (3, 5): ((0, 0, 0, 1, 1), (0, 0, 1, 1, 1)),
+        (125, 60): ((0, 0, 1, 1, 1), (0, 0, 1, 1, 1))}
+    for (dk, dv), want in widened.items():
+        for i, (b, t) in enumerate([(1, 55), (1, 450), (42, 320), (42, 450), (1, 4097)]):
+            q, k, v, g, _ = make(b, 3, t, dk, dv, torch.bfloat16)
+            for up, pads in zip((None, v), want):
+                plan = ops._decay_plan(q, k, v, g, None, None, up, 0)
+                assert plan.pad == ((-dk % 8, -dv % 8) if pads[i] else None), (dk, dv, b, t)
+    q, k, v, g, _ = make(2, 3, 0, 57, 33, torch.bfloat16)
+    assert ops._decay_plan(q, k, v, g, None, None, None, 0).pad is None
+
+
+@gpu
 def test_gradients_against_differences():
     """The loss is linear in each input alone, so a central difference of any
     length is the directional derivative, up to the forward pass's rounding."""

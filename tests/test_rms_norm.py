@@ -279,6 +279,38 @@ def test_repeats_and_graph():
     assert all(torch.equal(a, b) for a, b in zip(first, call()))
 
 
+@gpu
+def test_streams_and_threads():
+    """The same bits on another stream, and from a thread without a context of its
+    own, forward, backward and to e4m3, while the default stream works too."""
+    import threading
+
+    x, r, w = make((3000, 1024), torch.bfloat16, True, torch.bfloat16)
+    dy, ds = torch.randn_like(x), torch.randn_like(x)
+
+    def call():
+        y, s, rstd = ops.rms_norm(x, w, r, EPS, want_rstd=True)
+        y8, scales, _ = ops.rms_norm_fp8(x, w, r, EPS, 128)
+        return (y, s, rstd, *ops.rms_norm_backward(s, w, rstd, dy, ds), y8.view(torch.uint8),
+                scales)
+
+    first = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    others = []
+    with torch.cuda.stream(side):
+        others.append(call())
+    here = call()
+    torch.cuda.synchronize()
+    worker = threading.Thread(target=lambda: others.append(call()))
+    worker.start()
+    worker.join()
+    torch.cuda.synchronize()
+    assert len(others) == 2
+    for got in (here, *others):
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
 # --------------------------------------------------------------------- CPU
 def test_refusals():
     x = torch.randn(4, 64)
