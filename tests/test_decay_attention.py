@@ -249,6 +249,37 @@ def test_segments_of_wide_heads(dk, dv, segments):
 
 
 @gpu
+@pytest.mark.parametrize("dk,dv", [(16, 64), (64, 64), (64, 128), (128, 128)])
+@pytest.mark.parametrize("t,segments", [(3, 0), (45, 0), (128, 0), (300, 2), (384, 1), (384, 0)])
+def test_final_state_is_held_in_fp32(t, segments, dk, dv):
+    """What decoding goes on from, and its gradient, do not keep bf16's roundings.
+    In units of 2^-24 of the absolute sums: a weight and each tile that carries it 8
+    (expf and its products), the products' split 2 and their sums 16 (8 steps of one
+    rounding, cut), joins 6: 56 for three tiles, so 64.  What decays below 2^-16 may
+    hold two bf16 terms: 2^-14 of it, 2^-30 of what entered."""
+    q, k, v, _, state = make(2, 8, t, dk, dv, torch.bfloat16, "bthd", seed=t)
+    g = torch.tensor([-5.0, -1.0, -0.4, -0.1, -0.03, -0.01, -1e-3, 0.0], device="cuda")
+    do = torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).to(v.dtype).cuda()
+    end = ops.decay_attention(q, k, v, g, initial_state=state, return_state=True,
+                              segments=segments)[1]
+    first = ops.decay_attention_backward(q, k, v, g, do, scale=1.0, initial_state=state,
+                                         d_state=state, want_d_initial=True, segments=segments)[3]
+    i = torch.arange(t, device="cuda")
+    for got, a, b, left in ((end, k, v, t - 1 - i), (first, q, do, i + 1)):
+        a, b = a.double(), b.double()
+        weight = torch.exp(g.double()[:, None] * left)[..., None]
+
+        def total(a, b, s):
+            return (torch.exp(g.double() * t)[:, None, None] * s
+                    + (a * weight).transpose(-1, -2) @ b)
+
+        s = state.double()
+        near = 64 * 2.0 ** -24 * total(a.abs(), b.abs(), s.abs())
+        far = 2.0 ** -30 * (a.abs().transpose(-1, -2) @ b.abs())
+        assert ((got.double() - total(a, b, s)).abs() <= near + far).all()
+
+
+@gpu
 def test_some_heads_split():
     """More heads than SMs: whole ones fill a wave, the rest share the next in
     segments (the default split; seen by its smaller workspace)."""

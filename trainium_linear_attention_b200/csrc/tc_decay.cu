@@ -11,19 +11,28 @@
 //   O2     = P V                         M=128 N=64 K=128 (A = P in TMEM)
 //   out    = inter lambda^(ti+e0) O1 + O2               epilogue, rounded once
 //   V'     = inc lambda^(len-e0-tj) V, as two bf16 terms hi + lo    CUDA cores
-//   U      = B^T [V'hi V'lo]             M=128 N=128 K=128
+//   U      = B^T [V'hi V'lo]             M=128 N=128 K=128 (, a third term N=64)
 //   S      = lambda^len S + U_hi + U_lo  fp32 in registers of the state warps
 //
 // The decay never multiplies an accumulator in TMEM: it is on the rows of P and
 // V' (operands), on O1's rows and on the state's registers, so U, the scores
 // and O2 of a tile depend on the tile alone and only O1 waits for the state.
-// Roundings, each once and half a step at most: P and the copy of S to bf16
-// (2^-8, like the output), and V' to the 16 bits of hi + lo (2^-17): with one
-// bf16 term the fp32 state, which decoding continues from, would be off by 2^-8.
-// Stacked along N the second term costs no further MMA and no second read of B;
-// a third would need 64 more TMEM columns than there are.  With DK < 128, M = 128
-// holds B^T more than once (descriptor stride 0), and the state warps of each
-// copy take other columns.
+// Roundings: P and the copy of S to bf16 (half a step, 2^-8, like the output), and
+// V' to hi + lo: off by 2^-14.8 at most (lo rounds what hi and the weight's own first
+// term leave), 2^-17.8 in the mean square.  That is enough for a state that the
+// outputs read through its bf16 copy, and stacked along N the second term costs no
+// further MMA and no second read of B.  A final state, or its gradient, is asked for
+// in fp32: kernels of their own (kExact) then give V' a third term, added onto the
+// second's columns, in the tiles that have not decayed below 2^-10 by the walk's end
+// (older ones are off by 2^-24.8 of what entered, less than half a step of fp32).
+// The state is then 1e-7 off in the 2-norm, with two terms 4.2e-6, and the fp32
+// formula 2.2e-7.  What it costs: 16 heads of 16384 x 128 in 121 us (two terms
+// 116), 128 heads of 8192 x 64 in 111 (103), 64 heads of 2048 x 64 in 33 (26), 15
+// heads of 1000 x 64 / 128 in 21 (16), where the slow heads take it in every tile.
+// Kept out: the third term in place of hi once that is formed (41 us for 64 heads of
+// 2048), in the same step as the others (35), exact products as four terms (34).
+// With DK < 128, M = 128 holds B^T more than once (descriptor stride 0), and the
+// state warps of each copy take other columns.
 //
 // What bounds it.  A tile moves 64 KB at d = 64 and its MMAs read ~190 KB of
 // shared memory (~1,500 cycles); with its 24 warps a tile takes 2,300 to 2,600
@@ -37,9 +46,10 @@
 // two buffers, and tiles prefetched into L2 were measured and are no faster.
 //
 // Warps: 0 TMA; 1 scores and O1 MMAs (TMEM owner); 2 U; 3 O2; 4.. state (8 warps
-// at DK = 128, else 4); 8 warps P; 4 warps V' (the state pass, which has no P and
-// epilogue, 8: 16 heads of 16384 x 64 in 46 us instead of 47, their gradients in 92
-// instead of 95); 4 warps epilogue.  Every wait is bounded (tc_common.cuh).
+// at DK = 128, else 4); 8 warps P; 4 warps V' (8 in the state pass, which has no P
+// and epilogue: 16 heads of 16384 x 64 in 46 us instead of 47, their gradients in 92
+// instead of 95; 8 with a third term, DK <= 64: 33 us instead of 35); 4 warps
+// epilogue.  Every wait is bounded (tc_common.cuh).
 #include <type_traits>
 
 #include "decay.cuh"
@@ -64,7 +74,7 @@ constexpr uint32_t kColO2 = 448;
 
 constexpr int kJoinPitch = 65;  // floats per row of a joined state: rows in other banks
 
-template <int DK, bool kStateOnly>
+template <int DK, bool kStateOnly, bool kExact>
 struct TcLayout {
   // A and B: blocks of 64 columns (128-byte rows), or one of 32 (64-byte rows)
   static constexpr int kKBlocks = DK == 32 ? 1 : DK / 64;
@@ -76,7 +86,7 @@ struct TcLayout {
   static constexpr int kWState = 4;
   static constexpr int kWP = kWState + kStateWarps;  // first P warp
   static constexpr int kWV = kStateOnly ? kWP : kWP + 8;
-  static constexpr int kVWarps = kStateOnly ? 8 : 4;
+  static constexpr int kVWarps = kStateOnly || (kExact && DK <= 64) ? 8 : 4;
   static constexpr int kWE = kWV + kVWarps;
   static constexpr int kWarps = kStateOnly ? kWE : kWE + 4;
   static constexpr int kThreads = kWarps * 32;
@@ -86,23 +96,35 @@ struct TcLayout {
   static constexpr uint32_t kOffV = kOffB + kKBlocks * kKBlock;
   static constexpr uint32_t kStageBytes = kOffV + kBlock;
   static constexpr uint32_t kSnapBytes = DK * 128;
-  static constexpr int kVpBufs = DK <= 64 || kStateOnly ? 2 : 1;
+  // V': two terms of a tile or, kExact, three; of two tiles where the space allows it
+  static constexpr int kVpBlocks = !kExact ? (DK <= 64 || kStateOnly ? 4 : 2)
+                                   : DK == 32 || (kStateOnly && DK == 64) ? 6
+                                   : DK == 64 || kStateOnly               ? 4
+                                                                          : 3;
+  static constexpr uint32_t kVpBytes = kVpBlocks * kBlock;
+  // Whether tiles of three terms, or of two, alternate between two places, and where
+  // tile c's are.
+  static __device__ __forceinline__ bool vp_two(bool third) {
+    return kVpBlocks == 6 || (kVpBlocks == 4 && !third);
+  }
+  static __device__ __forceinline__ uint32_t vp_at(int c, bool third) {
+    return vp_two(third) ? (c & 1) * (kVpBytes / 2) : 0;
+  }
+  static constexpr int kSnaps = kStateOnly ? 0 : kExact && DK == 128 ? 1 : 2;  // copies of S
   static constexpr int kUBufs = kStateOnly ? 2 : 1;
-  static constexpr uint32_t kFixed =
-      kVpBufs * 2 * kBlock + (kStateOnly ? 0 : 2 * kSnapBytes) + 512;
+  static constexpr uint32_t kFixed = kVpBytes + kSnaps * kSnapBytes + 512;
   static constexpr int kStages = (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes > 6
                                      ? 6
                                      : (227 * 1024 - 1024 - (int)kFixed) / (int)kStageBytes;
-  static constexpr uint32_t kOffVp = kStages * kStageBytes;     // V' hi, lo
-  static constexpr uint32_t kOffSnap = kOffVp + kVpBufs * 2 * kBlock;  // two bf16 copies of S
-  static constexpr uint32_t kOffBar = kOffSnap + (kStateOnly ? 0 : 2 * kSnapBytes);
+  static constexpr uint32_t kOffVp = kStages * kStageBytes;  // V' hi, lo, the third term
+  static constexpr uint32_t kOffSnap = kOffVp + kVpBytes;    // bf16 copies of S
+  static constexpr uint32_t kOffBar = kOffSnap + kSnaps * kSnapBytes;
   static constexpr uint32_t kSmem = kOffBar + 512 + 1024;  // + alignment
   static constexpr int kJoinBytes = DK * kJoinPitch * 4;  // a joined state, from kOffVp on
   // Whether it reaches beyond V' into the copies of S, as with DK = 128 its last two
   // rows do: a state warp then may write its copy only once all have read theirs.
-  static constexpr bool kJoinOverCopies = kJoinBytes > kVpBufs * 2 * kBlock;
-  static_assert(kStateOnly || kJoinBytes <= kVpBufs * 2 * kBlock + 2 * (int)kSnapBytes,
-                "joined state");
+  static constexpr bool kJoinOverCopies = kJoinBytes > (int)kVpBytes;
+  static_assert(kStateOnly || kJoinBytes <= (int)(kVpBytes + kSnaps * kSnapBytes), "joined state");
   static_assert(kStages >= 2 && kSmem <= 227 * 1024, "shared memory budget");
   static_assert(kSmem > 114 * 1024, "one CTA per SM (all TMEM columns)");
 };
@@ -120,7 +142,8 @@ enum Bar {
   kOReady = kUFree + 2,
   kOFree = kOReady + 2,
   kDone = kOFree + 2,
-  kNumBars = kDone + 3
+  kThird = kDone + 3,  // the third term of V', where it has one; alternate tiles
+  kNumBars = kThird + 2
 };
 static_assert(8 * kNumBars + 8 <= 512, "barrier area");
 
@@ -179,10 +202,10 @@ __device__ __forceinline__ bool wait_teardown(uint64_t *bar, uint32_t parity) {
   return true;
 }
 
-template <int DK, bool kStateOnly, bool kLead>
-__global__ void __launch_bounds__(TcLayout<DK, kStateOnly>::kThreads, 1)
+template <int DK, bool kStateOnly, bool kLead, bool kExact>
+__global__ void __launch_bounds__(TcLayout<DK, kStateOnly, kExact>::kThreads, 1)
 decay_tc_kernel(const __grid_constant__ TcParams p) {
-  using L = TcLayout<DK, kStateOnly>;
+  using L = TcLayout<DK, kStateOnly, kExact>;
   constexpr int kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -230,12 +253,23 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   auto tile_start = [&](int c) { return t0 + (int64_t)(rev ? tiles - 1 - c : c) * kT; };
   const int ragged = rev ? 0 : tiles - 1;
   const int ragged_len = (int)(t1 - t0) - (tiles - 1) * kT;
+  // Where the final state is written, the first tile whose V' has three terms: from
+  // there on lambda^(tokens to the walk's end) is above 2^-10.  (The first of two
+  // parts does as a whole walk would, so that its outputs have the same bits.)
+  int third_from = INT32_MAX;
+  if (kExact && role.final_state != nullptr && (want_final || kLead) && g < 0.f) {
+    const int64_t reach = (int64_t)fminf(6.94f / -g, 2e9f);
+    if (!rev)
+      third_from = (int)((max64(0, p.n - kT - t0 - reach) + kT - 1) / kT);
+    else if (reach >= t0)
+      third_from = (int)max64(0, tiles - 1 - (reach - t0) / kT);
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kNumBars; ++i) {
       const bool per_state_warp = i == kSnapReady || i == kSnapReady + 1 ||
                                   i == kUFree || i == kUFree + 1;
-      const bool per_v_warp = i == kVpReady || i == kVpReady + 1;
+      const bool per_v_warp = i == kVpReady || i == kVpReady + 1 || i == kThird || i == kThird + 1;
       const bool per_four = i == kOFree || i == kOFree + 1;
       const bool per_p_warp = i == kPReady || i == kPReady + 1;
       const bool stage_empty = i >= kEmpty && i < kEmpty + 6;
@@ -385,7 +419,8 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
             if (kk < k_steps)
               umma_ss(tmem + kColO1,
                       a0 + at + (uint64_t)((kk / 4) * (L::kKBlock >> 4) + (kk % 4) * 2),
-                      s0 + (uint64_t)(b * (L::kSnapBytes >> 4) + kk * (2048 >> 4)), id_o, kk > 0);
+                      s0 + (uint64_t)(c % L::kSnaps * (L::kSnapBytes >> 4) + kk * (2048 >> 4)), id_o,
+                      kk > 0);
           umma_commit(&bars[kRead + b]);
         }
         __syncwarp();
@@ -407,9 +442,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const uint64_t b0 = make_sdesc(sb + L::kOffVp, kBlock, 1024, kSwizzle128B);
     int us = 0, up = 0;  // stage and its phase
     for (int c = 0; c < updates; ++c) {
-      const int vb = c % L::kVpBufs;
+      const bool third = kExact && c >= third_from;
       if (!mbar_wait_warp(&bars[kFull + us], up, abort_flag)) break;
-      if (!mbar_wait_warp(&bars[kVpReady + vb], (c / L::kVpBufs) & 1, abort_flag)) break;
+      if (!mbar_wait_warp(&bars[kVpReady + (c & 1)], (c / 2) & 1, abort_flag)) break;
       // the columns: U of tile c - 1 (with two buffers c - 2) is in registers
       if (c >= L::kUBufs) {
         const int u = c - L::kUBufs;
@@ -418,16 +453,29 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       tc_fence_after();
       const uint32_t d = tmem + kColU + (c % L::kUBufs) * 128;
       const uint64_t da = a0 + (uint64_t)(us * (L::kStageBytes >> 4));
-      const uint64_t db = b0 + (uint64_t)(vb * (2 * kBlock >> 4));
+      const uint64_t db = b0 + (uint64_t)(L::vp_at(c, third) >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kT / 16; ++kk) {
           umma_ss(d, da + (uint64_t)(kk * (2 * L::kKGroup >> 4)),
                   db + (uint64_t)(kk * (2048 >> 4)), id_u, kk > 0);
         }
-        umma_commit(&bars[kUReady + (c & 1)]);
+        if (!third) umma_commit(&bars[kUReady + (c & 1)]);
       }
       __syncwarp();
+      if (third) {  // onto the second's columns
+        if (!mbar_wait_warp(&bars[kThird + (c & 1)], ((c - third_from) / 2) & 1, abort_flag)) break;
+        tc_fence_after();
+        constexpr uint32_t id_third = make_idesc_bf16(128, 64, true, true);
+        if (elect_one()) {
+#pragma unroll 1
+          for (int kk = 0; kk < kT / 16; ++kk)
+            umma_ss(d + 64, da + (uint64_t)(kk * (2 * L::kKGroup >> 4)),
+                    db + (uint64_t)((2 * kBlock >> 4) + kk * (2048 >> 4)), id_third, true);
+          umma_commit(&bars[kUReady + (c & 1)]);
+        }
+        __syncwarp();
+      }
       if (++us == kStages) us = 0, up ^= 1;
     }
     if (elect_one()) umma_commit(&bars[kDone + 1]);
@@ -505,10 +553,10 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
 #pragma unroll 1
     for (int c = 0;; ++c) {
       if (!kStateOnly && (!kLead || c >= pre) && c < tiles) {  // the copy of S that tile c reads
-        const int at = c - pre, b = at & 1;
-        if (at >= 2) mbar_wait(&bars[kRead + b], ((at - 2) / 2) & 1, abort_flag);
+        const int at = c - pre, b = at & 1, read = at - L::kSnaps;
+        if (read >= 0) mbar_wait(&bars[kRead + (read & 1)], (read / 2) & 1, abort_flag);
         __syncwarp();
-        const uint32_t dst = copy_row + b * L::kSnapBytes;
+        const uint32_t dst = copy_row + (L::kSnaps > 1 ? b * L::kSnapBytes : 0);
 #pragma unroll
         for (int q = 0; q < kCols / 8; ++q)
           st_shared_v4(dst ^ (16 * q), pack_bf16(st[8 * q], st[8 * q + 1]),
@@ -662,7 +710,7 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
     const float w_full = role.inc * decay_pow(g, rev ? j + 1 : kT - 1 - j);
     const float w_ragged = role.inc * decay_pow(g, rev ? j + 1 : ragged_len - 1 - j);
     const uint32_t row = sb + sw128_offset(j, 0);
-    int s = 0, phase = 0, vb = 0;
+    int s = 0, phase = 0;
     if (joins) named_barrier_sync(1, L::kStateWarps * 32 + L::kVWarps * 32);
     for (int c = 0; c < updates; ++c) {
       const float w = c == ragged ? w_ragged : w_full;
@@ -674,14 +722,13 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       const float rest = bf16lo(w_hi) - w;
       const uint32_t minus_hi = w_hi ^ 0x80008000u, minus_lo = pack_bf16(rest, rest);
       mbar_wait(&bars[kFull + s], phase, abort_flag);
-      // U of the tile that used this buffer before has been formed
-      if (c >= L::kVpBufs) {
-        const int u = c - L::kVpBufs;
-        mbar_wait(&bars[kUReady + (u & 1)], (u / 2) & 1, abort_flag);
-      }
+      // U of the tile that used this place before has been formed
+      const bool third = kExact && c >= third_from;
+      const int u = c - (L::vp_two(third) ? 2 : 1);
+      if (u >= 0) mbar_wait(&bars[kUReady + (u & 1)], (u / 2) & 1, abort_flag);
       __syncwarp();
       const uint32_t src = row + s * L::kStageBytes + L::kOffV,
-                     dst = row + L::kOffVp + vb * 2 * kBlock;
+                     dst = row + L::kOffVp + L::vp_at(c, third);
 #pragma unroll 2
       for (uint32_t q = q0; q < q0 + kPart; q += 16) {  // a piece of the row: its swizzle is an xor
         uint32_t x[4], hi[4], lo[4];
@@ -696,9 +743,30 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kVpReady + vb]);
+      if (lane == 0) mbar_arrive(&bars[kVpReady + (c & 1)]);
+      if (third) {
+        // what the two leave of w x (fma: to 2^-32 of it), rounded to bf16, while they
+        // are on their way into U; negative, like lo
+        const uint64_t w2 = f2pack(w, w);
+#pragma unroll 2
+        for (uint32_t q = q0; q < q0 + kPart; q += 16) {
+          uint32_t x[4], hi[4], lo[4];
+          ld_shared_v4(src ^ q, x[0], x[1], x[2], x[3]);
+          ld_shared_v4((dst ^ q) + kBlock, lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            hi[i] = hmul2_bf16(x[i], minus_hi);
+            const uint64_t left = ffma2(f2pack(bf16lo(x[i]), bf16hi(x[i])), w2,
+                                        f2pack(bf16lo(hi[i]), bf16hi(hi[i])));
+            x[i] = pack_bf16x2(fadd2(left, f2pack(bf16lo(lo[i]), bf16hi(lo[i])))) ^ 0x80008000u;
+          }
+          st_shared_v4((dst ^ q) + 2 * kBlock, x[0], x[1], x[2], x[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kThird + (c & 1)]);
+      }
       if (++s == kStages) s = 0, phase ^= 1;
-      if (++vb == L::kVpBufs) vb = 0;
     }
   } else if (!kStateOnly && warp >= L::kWE) {
     // ------------------------------------------------------------ epilogue
@@ -819,10 +887,10 @@ bool make_map(CUtensorMap *map, const DecayView &x, int width, int box_cols, con
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DK, bool kStateOnly, bool kLead>
+template <int DK, bool kStateOnly, bool kLead, bool kExact>
 int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
-  using L = TcLayout<DK, kStateOnly>;
-  auto kernel = decay_tc_kernel<DK, kStateOnly, kLead>;
+  using L = TcLayout<DK, kStateOnly, kExact>;
+  auto kernel = decay_tc_kernel<DK, kStateOnly, kLead, kExact>;
   if (allow_dynamic_smem((const void *)kernel, (int)L::kSmem) != LA_OK) return LA_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
@@ -838,6 +906,13 @@ int launch_t(const TcParams &p, int64_t grid, cudaStream_t s) {
   cfg.numAttrs = !kStateOnly && !kLead && p.segments > 1 ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, p);
   return check_launch();
+}
+
+template <bool kStateOnly, bool kLead, bool kExact>
+int launch_width(const TcParams &p, int da, int64_t grid, cudaStream_t s) {
+  if (da <= 32) return launch_t<32, kStateOnly, kLead, kExact>(p, grid, s);
+  return da <= 64 ? launch_t<64, kStateOnly, kLead, kExact>(p, grid, s)
+                  : launch_t<128, kStateOnly, kLead, kExact>(p, grid, s);
 }
 
 template <bool kStateOnly>
@@ -893,16 +968,15 @@ int launch(const DecayCall &c, cudaStream_t s) {
       (kStateOnly ? 0 : c.whole) + (c.batch * c.heads - c.whole) * (int64_t)p.orders;
   const int64_t grid = walks * slices * c.roles;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  bool exact = false;  // a state is asked for
+  for (int r = 0; r < c.roles; ++r) exact = exact || c.role[r].final_state;
   if constexpr (!kStateOnly) {
-    if (c.lead > 0) {
-      if (da <= 32) return launch_t<32, false, true>(p, grid, s);
-      return da <= 64 ? launch_t<64, false, true>(p, grid, s)
-                      : launch_t<128, false, true>(p, grid, s);
-    }
+    if (c.lead > 0)
+      return exact ? launch_width<false, true, true>(p, da, grid, s)
+                   : launch_width<false, true, false>(p, da, grid, s);
   }
-  if (da <= 32) return launch_t<32, kStateOnly, false>(p, grid, s);
-  return da <= 64 ? launch_t<64, kStateOnly, false>(p, grid, s)
-                  : launch_t<128, kStateOnly, false>(p, grid, s);
+  return exact ? launch_width<kStateOnly, false, true>(p, da, grid, s)
+               : launch_width<kStateOnly, false, false>(p, da, grid, s);
 }
 
 }  // namespace

@@ -97,8 +97,11 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     do), or leave out what the right padding returns; a value that is not
     finite reaches the outputs of its own tile of 128 tokens, so padding should
     be finite.  bf16 runs on tensor cores: the weights of a tile's values and
-    the state's read-out are rounded to bf16, the state is carried in fp32 and
-    fed with 16-bit products (2^-17)."""
+    the state's read-out are rounded to bf16, the state is carried in fp32.  A
+    final state that is returned, and the gradient of ``initial_state``, are
+    exact to fp32; where neither is asked for the state is fed with products of
+    two bf16 terms (2^-14.8 at most, 2^-17.8 in the mean square), so an output's
+    last bit may go by ``return_state``."""
     ops.check_tangents(q, k, v, log_decay, initial_state)
     if torch.is_grad_enabled() and any(
             isinstance(x, torch.Tensor) and x.requires_grad for x in (q, k, v, initial_state)):

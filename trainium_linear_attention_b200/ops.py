@@ -462,12 +462,12 @@ def decay_attention(q, k, v, log_decay, scale=None, initial_state=None, return_s
     plan = _decay_plan(q, k, v, log_decay, initial_state, None, None, segments)
     if plan.pad is not None:
         a, b = plan.pad
-        out, final = decay_attention(_widen(q, a), _widen(k, a), _widen(v, b), log_decay,
-                                     plan.scale if scale is None else scale,
-                                     _widen(initial_state, b, a), True, segments)
-        out, = _narrowed(plan.outs, (out,))
+        got = decay_attention(_widen(q, a), _widen(k, a), _widen(v, b), log_decay,
+                              plan.scale if scale is None else scale,
+                              _widen(initial_state, b, a), return_state, segments)
+        out, = _narrowed(plan.outs, (got[0] if return_state else got,))
         _, _, d, dv = plan.state_shape
-        return (out, final[:, :, :d, :dv].contiguous()) if return_state else out
+        return (out, got[1][:, :, :d, :dv].contiguous()) if return_state else out
     again = _readable(plan, (q, k, v))
     if again is not None:
         out = decay_attention(*again, log_decay, scale, initial_state, return_state, segments)
