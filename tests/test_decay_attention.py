@@ -262,11 +262,11 @@ def test_final_state_is_held_in_fp32(t, segments, dk, dv):
     do = torch.randn(v.shape, generator=torch.Generator().manual_seed(1)).to(v.dtype).cuda()
     end = ops.decay_attention(q, k, v, g, initial_state=state, return_state=True,
                               segments=segments)[1]
-    first = ops.decay_attention_backward(q, k, v, g, do, scale=1.0, initial_state=state,
+    first = ops.decay_attention_backward(q, k, v, g, do, scale=0.3, initial_state=state,
                                          d_state=state, want_d_initial=True, segments=segments)[3]
     i = torch.arange(t, device="cuda")
-    for got, a, b, left in ((end, k, v, t - 1 - i), (first, q, do, i + 1)):
-        a, b = a.double(), b.double()
+    for got, a, b, left, scale in ((end, k, v, t - 1 - i, 1.0), (first, q, do, i + 1, 0.3)):
+        a, b = a.double(), scale * b.double()
         weight = torch.exp(g.double()[:, None] * left)[..., None]
 
         def total(a, b, s):

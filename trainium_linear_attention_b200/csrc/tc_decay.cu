@@ -257,8 +257,9 @@ decay_tc_kernel(const __grid_constant__ TcParams p) {
   // there on lambda^(tokens to the walk's end) is above 2^-10.  (The first of two
   // parts does as a whole walk would, so that its outputs have the same bits.)
   int third_from = INT32_MAX;
-  if (kExact && role.final_state != nullptr && (want_final || kLead) && g < 0.f) {
-    const int64_t reach = (int64_t)fminf(6.94f / -g, 2e9f);
+  if (kExact && role.final_state != nullptr && (want_final || kLead) &&
+      (g != 0.f || role.inc != 1.f)) {  // (weights of one need no more)
+    const int64_t reach = (int64_t)fminf(6.94f / fabsf(g), 2e9f);
     if (!rev)
       third_from = (int)((max64(0, p.n - kT - t0 - reach) + kT - 1) / kT);
     else if (reach >= t0)
