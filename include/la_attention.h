@@ -232,7 +232,7 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
  *   S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T,   out_t = scale * q_t S_t
  *
  * with S_{-1} = init_state (zero if null).  The state is fp32 (batch, heads,
- * d_qk, d_v), contiguous; log_decay is fp32 (heads) in device memory, finite
+ * d_qk, d_v), contiguous, and exact to fp32 where it is written; log_decay is fp32 (heads) in device memory, finite
  * and <= 0 or -inf (no memory).  d_qk and d_v are at most 128 and need not be
  * equal; batch * heads is at most 65535 for prompts and their gradients.  The
  * reference has no decayed form; the recurrence without decay is its chunked
@@ -246,7 +246,10 @@ int la_sliding_window_fwd(const void *q, const void *k, const void *v, void *out
  * segments: each head's sequence is split into this many segments walked by
  * different CTAs (0 = let the library choose); more than one needs the
  * workspace (256-byte aligned) that la_decay_plan reports, which for two of the
- * library's own choice may be none.  A value that is
+ * library's own choice may be none.  bf16 rows that do not start at 16 bytes, or
+ * whose width is no multiple of 8, run on CUDA cores, and unsplit where the
+ * library's choice for tensor cores was two parts or left heads whole: align them,
+ * or ask for segments.  A value that is
  * not finite reaches every output of its own 128-token tile, and what the
  * recurrence carries it to.
  * ------------------------------------------------------------------------- */

@@ -9,7 +9,7 @@
 // to 64 CTAs.  The read-out is summed over a warp's 4 row groups by shuffles
 // and over the 8 warps in shared memory, in a fixed order.  256 sequences of 16
 // heads of 128 x 128: 90 us, 6.0 TB/s (92% of the copy rate); 16 heads of 64 x
-// 64: 2.1 us.
+// 64: 2.3 us.
 #include "decay.cuh"
 #include "decay_step.cuh"
 

@@ -14,11 +14,14 @@
 // a fixed order: no atomics, the same bits every time.  It works on the saved
 // sum, which is rounded to the inputs' type (half a step: 2^-8 in bf16).
 //
-// Measured, bf16 with a residual, of the copy rate (6.5 TB/s): 16384 x 1024 in
-// 23 us (89%), its gradient 22 (94%); 32768 x 4096 in 158 (104%), to e4m3 155
-// (93%), gradient 154 (107%; both upstream gradients were one tensor); 131072
-// rows of 64 in 10.5 us (98%), gradient 15 (69%); 4096 x 16384 in 90 us (92%),
-// gradient 141 (59%: 64 registers a thread spill); 16384 x 1023 (shifted) in 63 us.
+// Measured in a CUDA graph over inputs larger than L2, bf16 with a residual and two
+// upstream gradients, of the copy rate (6.5 TB/s; the last of the output is still in
+// L2): 16384 x 1024 in 24 us (86%), its gradient 28 (75%); 32768 x 4096 in 159
+// (104%), to e4m3 158 (91%), gradient 176 (94%); 131072 rows of 64 in 14.7 us (70%),
+// gradient 18.8 (55%); 4096 x 16384 in 90 us (92%), gradient 150 (55%: 64 registers
+// a thread spill 268 bytes); 16384 x 1023 (shifted) in 63 us, gradient 92.  fp32:
+// 16384 x 4096 in 160 us, to e4m3 128, gradient 175 (94%); 4096 x 16384 in 170,
+// gradient 350 (47%).
 #include <cuda_fp8.h>
 #include <math.h>
 

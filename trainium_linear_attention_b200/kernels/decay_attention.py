@@ -83,8 +83,9 @@ def decay_linear_attention(q, k, v, log_decay, scale=None, initial_state=None,
     """Causal linear attention with a decay for each head on the sm_100a kernels.
 
     q, k: (b, h, t, d_qk); v: (b, h, t, d_v), float32 or bfloat16, widths up to
-    128, any strides with a dense last dimension (a projection's transposed
-    heads are read in place, and the output is laid out as v).  ``log_decay``:
+    128, b * h up to 65535, any strides with a dense last dimension (a
+    projection's transposed heads are read in place, and the output is laid
+    out as v).  ``log_decay``:
     float32 (h,), <= 0, a constant (one that requires a gradient is refused
     where gradients are recorded).  ``scale`` defaults to 1/sqrt(d_qk).
     ``initial_state``: fp32 (b, h, d_qk, d_v), the state before the first
