@@ -593,6 +593,16 @@ def test_step_refuses():
 
 
 @gpu
+def test_widths_of_zero_are_refused():
+    for dk, dv in ((0, 16), (16, 0), (0, 0)):
+        q, k, v, g, state = make(1, 2, 3, dk, dv, torch.float32)
+        with pytest.raises(T.LaError):
+            T.decay_linear_attention(q, k, v, g)
+        with pytest.raises((T.LaError, ValueError)):
+            T.decay_linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], g, state)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_left_padded_batch(dtype):
     """Sequences of different lengths, padded on the left with zero keys, end in

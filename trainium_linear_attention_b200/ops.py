@@ -363,7 +363,7 @@ class _DecayPlan:
         self.device, self.dtype = q.device, q.dtype
         self.index = q.device.index
         self.sizes = (b, h, t, d, dv, code)
-        self.scale = 1.0 / math.sqrt(d)
+        self.scale = 1.0 / math.sqrt(max(d, 1))  # (the library refuses d = 0)
         self.state_shape = (b, h, d, dv)
         read = (q, k, v) if grad is None else (q, k, v, grad)
         # bf16 rows of whole 16-byte packs have to start at 16 bytes
@@ -564,7 +564,7 @@ class _StepPlan:
             raise ValueError("the states of different sequences overlap")
         self.device, self.dtype, self.index = q.device, q.dtype, q.device.index
         self.sizes = (b, h, d, dv, code)
-        self.scale = 1.0 / math.sqrt(d)
+        self.scale = 1.0 / math.sqrt(max(d, 1))  # (the library refuses d = 0)
         self.out = _proto((b, h, dv), q.dtype, q.device)
         self.copy = any(x.stride(2) != 1 and x.shape[2] > 1 and x.numel() > 0 for x in (q, k, v))
         self.strides = tuple(_Strides(*x.stride()) for x in (q, k, v)) + (_Strides(sb, sh),)
