@@ -324,6 +324,129 @@ int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight,
                     int dtype, int weight_dtype, void *workspace, size_t workspace_bytes,
                     void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Gated linear recurrence of each channel of (batch, tokens, channels).
+ *
+ *   h_t = a_t h_{t-1} + beta_t u_t x_t,   out_t = h_t,   s = sigmoid(gate)
+ *   with log_decay (fp32 (channels,), finite and <= 0, in device memory):
+ *     a = exp(log_decay * s), beta = sqrt(1 - a^2);  null: a = s, beta = 1 - s
+ *   u = sigmoid(input_gate), or 1 where that is null
+ *
+ * x, gate, input_gate and d_out have a dense last dimension and strides
+ * {batch, tokens} in elements (>= 0), so slices of one product are read in
+ * place; out and the gradients are contiguous.  States are fp32 (batch,
+ * channels), contiguous, null for zeros (init) or where they are not wanted.
+ * lengths: null, or an int32 or int64 (lengths_bits) for each sequence in
+ * device memory, taken into [0, tokens]: only so many tokens of a sequence are
+ * read, its outputs and gradients behind them are zero, and its final state is
+ * the one after them.  A value that is not finite reaches its channel's
+ * outputs from its own token on.  The reference has no such recurrence;
+ * its chunked kernel's (kernels/nki_attention_chunked.py:20-113) has a matrix for a
+ * state and no gates.
+ * ------------------------------------------------------------------------- */
+/* Bytes of `saved` (what la_recurrence_fwd keeps for the gradient) and of
+ * la_recurrence_bwd's workspace, which only d_log_decay needs. */
+int la_recurrence_plan(int64_t batch, int64_t tokens, int64_t channels, size_t *saved_bytes,
+                       size_t *workspace_bytes);
+
+int la_recurrence_fwd(const void *x, const int64_t *x_strides, const void *gate,
+                      const int64_t *gate_strides, const void *input_gate,
+                      const int64_t *input_strides, const float *log_decay, const float *init_state,
+                      const void *lengths, int lengths_bits, void *out, float *final_state,
+                      float *saved, int64_t batch, int64_t tokens, int64_t channels, int dtype,
+                      void *stream);
+
+/* Gradients for d_out and d_final_state (null: zero).  saved: from the forward
+ * call on the same inputs.  d_log_decay and d_init_state may be null.  At a
+ * log_decay of 0, where beta has no derivative, its gradient is finite and
+ * arbitrary. */
+int la_recurrence_bwd(const void *x, const int64_t *x_strides, const void *gate,
+                      const int64_t *gate_strides, const void *input_gate,
+                      const int64_t *input_strides, const float *log_decay, const float *saved,
+                      const void *lengths, int lengths_bits, const void *d_out,
+                      const int64_t *d_out_strides, const float *d_final_state, void *dx,
+                      void *d_gate, void *d_input_gate, float *d_log_decay, float *d_init_state,
+                      int64_t batch, int64_t tokens, int64_t channels, int dtype, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* One token of every sequence: x, gate, input_gate (batch, channels) with batch
+ * strides; state updated in place, no two sequences' overlapping; out
+ * contiguous. */
+int la_recurrence_step(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
+                       const void *input_gate, int64_t input_stride, const float *log_decay,
+                       float *state, int64_t state_stride, void *out, int64_t batch,
+                       int64_t channels, int dtype, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Causal convolution of each channel with `taps` (2 to 4) weights.
+ *
+ *   z_t = bias + sum_j weight[c][j] x_{t - taps + 1 + j},   out = z, or z sigmoid(z) (silu)
+ *
+ * x, d_out, lengths: as for the recurrence.  weight (channels, taps) and bias
+ * (channels, null: zeros) are fp32 or bf16 by weight_dtype.  init_state: the
+ * taps - 1 tokens before the first, oldest first, (batch, taps - 1, channels)
+ * in x's type, null for zeros; final_state: the last taps - 1 tokens, likewise.
+ * The reference has no convolution.
+ * ------------------------------------------------------------------------- */
+int la_short_conv_fwd(const void *x, const int64_t *x_strides, const void *weight,
+                      const void *bias, int weight_dtype, const void *init_state,
+                      const void *lengths, int lengths_bits, void *out, void *final_state,
+                      int64_t batch, int64_t tokens, int64_t channels, int64_t taps, int silu,
+                      int dtype, void *stream);
+
+/* Bytes of workspace la_short_conv_bwd needs for d_weight or d_bias. */
+int la_short_conv_workspace_size(int64_t batch, int64_t tokens, int64_t channels, int64_t taps,
+                                 size_t *bytes);
+
+/* Gradients for d_out and d_final_state (null: zero); d_weight, d_bias (in
+ * weight_dtype, summed in a fixed order) and d_init_state may be null. */
+int la_short_conv_bwd(const void *x, const int64_t *x_strides, const void *weight,
+                      const void *bias, int weight_dtype, const void *init_state,
+                      const void *lengths, int lengths_bits, const void *d_out,
+                      const int64_t *d_out_strides, const void *d_final_state, void *dx,
+                      void *d_weight, void *d_bias, void *d_init_state, int64_t batch,
+                      int64_t tokens, int64_t channels, int64_t taps, int silu, int dtype,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token of every sequence: state (batch, taps - 1, channels), dense but for
+ * the batch stride, loses its oldest token and gains x. */
+int la_short_conv_step(const void *x, int64_t x_stride, const void *weight, const void *bias,
+                       int weight_dtype, void *state, int64_t state_stride, void *out,
+                       int64_t batch, int64_t channels, int64_t taps, int silu, int dtype,
+                       void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Group norm of each row's channels, in `groups` groups of neighbours of width
+ * channels / groups <= 8192, with an activation or an activated gate:
+ *
+ *   z = (x - mean) / sqrt(var + eps) * weight + bias
+ *   out = act(z), or with a gate z * act(gate);   act: silu, or none
+ *
+ * The statistics are each row's (token's) own, in fp32, var the mean of squared
+ * differences.  x, gate and d_out are rows (shape[0], shape[1], channels) with
+ * a dense last dimension and strides {0, 1} in elements; out and the gradients
+ * are contiguous.  weight (null: ones) and bias (null: zeros), (channels), are
+ * fp32 or bf16 by weight_dtype.  stats (null, or fp32 (rows, groups, 2)) is what
+ * the gradient needs.  The reference has no norm.
+ * ------------------------------------------------------------------------- */
+int la_group_norm_fwd(const void *x, const int64_t *x_strides, const void *gate,
+                      const int64_t *gate_strides, const void *weight, const void *bias,
+                      int weight_dtype, void *out, float *stats, const int64_t *shape,
+                      int64_t channels, int64_t groups, int silu, int dtype, float eps,
+                      void *stream);
+
+/* Bytes of workspace la_group_norm_bwd needs for d_weight or d_bias on this device. */
+int la_group_norm_bwd_workspace_size(int64_t rows, int64_t channels, size_t *bytes);
+
+/* Gradients; d_gate with a gate; d_weight and d_bias (in weight_dtype, summed in
+ * a fixed order) may be null. */
+int la_group_norm_bwd(const void *x, const int64_t *x_strides, const void *gate,
+                      const int64_t *gate_strides, const void *weight, const void *bias,
+                      int weight_dtype, const float *stats, const void *d_out,
+                      const int64_t *d_out_strides, void *dx, void *d_gate, void *d_weight,
+                      void *d_bias, const int64_t *shape, int64_t channels, int64_t groups,
+                      int silu, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

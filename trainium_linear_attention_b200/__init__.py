@@ -17,6 +17,11 @@ from .kernels.based_module import (  # noqa: F401
     DecayLinearAttention, TrainiumBasedLinearAttention, TrainiumBasedLinearAttentionNKI)
 from .kernels.decay_attention import (  # noqa: F401
     decay_linear_attention, decay_linear_attention_step, ref_decay_attn)
+from .kernels.gated_recurrence import (  # noqa: F401
+    gated_recurrence, gated_recurrence_step, ref_gated_recurrence)
+from .kernels.short_conv import causal_conv, causal_conv_step, ref_causal_conv  # noqa: F401
+from .kernels.group_norm import group_norm, ref_group_norm  # noqa: F401
+from .kernels.recurrent_module import GatedRecurrence  # noqa: F401
 from .kernels.rms_norm import ref_rms_norm, rms_norm, rms_norm_fp8  # noqa: F401
 from ._native import LaError  # noqa: F401
 
@@ -28,5 +33,9 @@ __all__ = [
     "ref_sliding_window_attn", "based_layer", "ref_based_layer",
     "TrainiumBasedLinearAttention", "TrainiumBasedLinearAttentionNKI",
     "DecayLinearAttention", "decay_linear_attention", "decay_linear_attention_step", "ref_decay_attn",
-    "rms_norm", "rms_norm_fp8", "ref_rms_norm", "LaError",
+    "rms_norm", "rms_norm_fp8", "ref_rms_norm",
+    "gated_recurrence", "gated_recurrence_step", "ref_gated_recurrence",
+    "causal_conv", "causal_conv_step", "ref_causal_conv", "group_norm", "ref_group_norm",
+    "GatedRecurrence",
+    "LaError",
 ]

@@ -52,6 +52,17 @@ EXPORTED_SYMBOLS = (
     "la_rms_norm_fp8",
     "la_rms_norm_bwd_workspace_size",
     "la_rms_norm_bwd",
+    "la_recurrence_plan",
+    "la_recurrence_fwd",
+    "la_recurrence_bwd",
+    "la_recurrence_step",
+    "la_short_conv_fwd",
+    "la_short_conv_workspace_size",
+    "la_short_conv_bwd",
+    "la_short_conv_step",
+    "la_group_norm_fwd",
+    "la_group_norm_bwd_workspace_size",
+    "la_group_norm_bwd",
 )
 
 _lock = threading.Lock()
@@ -124,6 +135,28 @@ def _declare(lib) -> None:
     lib.la_rms_norm_bwd_workspace_size.restype = _int
     lib.la_rms_norm_bwd.argtypes = [_p] * 11 + [_i64, _int, _int, _p, _sz, _p]
     lib.la_rms_norm_bwd.restype = _int
+    size_out = ctypes.POINTER(_sz)
+    for name, types in (
+            ("la_recurrence_plan", [_i64] * 3 + [size_out] * 2),
+            ("la_recurrence_fwd", [_p] * 9 + [_int] + [_p] * 3 + [_i64] * 3 + [_int, _p]),
+            ("la_recurrence_bwd", ([_p] * 9 + [_int] + [_p] * 8 + [_i64] * 3
+                                   + [_int, _p, _sz, _p])),
+            ("la_recurrence_step", ([_p, _i64] * 3 + [_p, _p, _i64, _p] + [_i64] * 2
+                                    + [_int, _p])),
+            ("la_short_conv_fwd", ([_p] * 4 + [_int, _p, _p, _int, _p, _p] + [_i64] * 4
+                                   + [_int, _int, _p])),
+            ("la_short_conv_workspace_size", [_i64] * 4 + [size_out]),
+            ("la_short_conv_bwd", ([_p] * 4 + [_int, _p, _p, _int] + [_p] * 7 + [_i64] * 4
+                                   + [_int, _int, _p, _sz, _p])),
+            ("la_short_conv_step", ([_p, _i64, _p, _p, _int, _p, _i64, _p] + [_i64] * 3
+                                    + [_int, _int, _p])),
+            ("la_group_norm_fwd", ([_p] * 6 + [_int] + [_p] * 3 + [_i64] * 2
+                                   + [_int, _int, _f, _p])),
+            ("la_group_norm_bwd_workspace_size", [_i64] * 2 + [size_out]),
+            ("la_group_norm_bwd", ([_p] * 6 + [_int] + [_p] * 8 + [_i64] * 2
+                                   + [_int, _int, _p, _sz, _p]))):
+        entry = getattr(lib, name)
+        entry.argtypes, entry.restype = types, _int
 
 
 def lib():

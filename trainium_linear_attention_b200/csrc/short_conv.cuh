@@ -1,0 +1,33 @@
+// Causal convolution of each channel with a few taps: what its launchers take.
+#pragma once
+
+#include "recurrence.cuh"
+
+namespace la {
+
+struct ConvCall {
+  TokenView x, d_out;
+  const void *weight = nullptr;  // (channels, taps), contiguous
+  const void *bias = nullptr;    // null, or (channels)
+  const void *init = nullptr;    // null, or (batch, taps - 1, channels): the tokens before
+  const void *lengths = nullptr;
+  int lengths64 = 0;
+  int64_t batch = 0, tokens = 0;
+  int channels = 0, taps = 0, silu = 0;
+  int weight_dtype = 0;          // of weight and bias
+  // forward
+  void *out = nullptr, *final_state = nullptr;
+  // gradient
+  const void *d_final = nullptr;  // null, or as init
+  void *dx = nullptr, *d_init = nullptr;
+  float *partial = nullptr;       // null, or rows of (channels * taps + channels)
+};
+
+constexpr int kConvMinTaps = 2, kConvMaxTaps = 4;
+
+int launch_conv_fwd(const ConvCall &c, int dtype, cudaStream_t s);
+int launch_conv_bwd(const ConvCall &c, int dtype, cudaStream_t s);
+// Rows of `partial`.
+int64_t conv_partial_rows(int64_t batch, int64_t tokens);
+
+}  // namespace la
