@@ -4,13 +4,14 @@
 //   with a decay:   a = exp(lambda s), beta = sqrt(1 - a^2),   s = sigmoid(gate)
 //   without:        a = s,             beta = 1 - s
 //
-// The kernels hold 1 - a instead of a: it keeps its relative accuracy where a
-// rounds to 1, so that channels with a memory of many thousand tokens forget at
-// their own rate, and beta = sqrt((1 - a)(2 - (1 - a))) needs no difference of
-// near numbers.
+// The kernels hold a - 1 instead of a: it keeps its relative accuracy where a
+// rounds to 1, and beta = sqrt((a - 1)(-1 - a)) needs no difference of near
+// numbers.
 #pragma once
 
 #include "common.cuh"
+#include "tc_common.cuh"
+#include "tma_host.cuh"
 
 namespace la {
 
@@ -43,7 +44,8 @@ struct RecurCall {
   float *partial = nullptr;          // rows of d_log_decay's sums, one per CTA of a channel group
 };
 
-constexpr int kRecurCheck = 64;
+// Tokens from one saved state to the next: those of a forward thread's step.
+constexpr int kRecurCheck = 16;
 constexpr int kRecurThreads = 256;
 constexpr int kRecurMaxCluster = 8;
 
@@ -108,110 +110,131 @@ template <> struct Fn<float> {
   static __device__ __forceinline__ float rsqrt(float x) { return 1.f / sqrtf(x); }
 };
 
-// max that keeps a NaN
+// exp(z) - 1 for z <= 0, to a relative 2^-23: z = n ln 2 + f with |f| <= ln 2 / 2,
+// exp(z) - 1 = 2^n (exp(f) - 1) + (2^n - 1), exp(f) - 1 = f + f^2 q(f).  q is the
+// Chebyshev fit of degree 4 on that interval (1.2e-8 of exp(f) - 1).  On the
+// FMA pipe: the special-function unit is as busy as memory without it.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-
-// exp(z) - 1 for z <= 0, to a relative 2^-23: z = n ln 2 + f with |f| <= ln 2 / 2,
-// exp(z) - 1 = 2^n (exp(f) - 1) + (2^n - 1), exp(f) - 1 = f + f^2 q(f).  q is the
-// Chebyshev fit of degree 4 on that interval (1.2e-8 of exp(f) - 1).  On the
-// FMA pipe: the special-function unit is as busy as memory without it.
 __device__ __forceinline__ float2 expm1_neg(float2 z) {
   z.x = max_nan(z.x, -80.f);  // exp(-80) is far below half an ulp of 1
   z.y = max_nan(z.y, -80.f);
   const float2 magic = two(12582912.f);  // 1.5 * 2^23: the sum's low bits hold n
   const float2 t = __ffma2_rn(z, two(1.4426950408889634f), magic);
   const float2 n = __fadd2_rn(t, two(-12582912.f));
-  float2 f = __ffma2_rn(n, two(-0.693145751953125f), z);
-  f = __ffma2_rn(n, two(-1.42860682e-6f), f);
+  // (ln 2 in one constant: n times its error is 2^-26 n, which 2^n makes small)
+  const float2 f = __ffma2_rn(n, two(-0.69314718055994531f), z);
   float2 q = __ffma2_rn(two(0.0013933685841038823f), f, two(0.008369184099137783f));
   q = __ffma2_rn(q, f, two(0.041666463017463684f));
   q = __ffma2_rn(q, f, two(0.16666504740715027f));
   q = __ffma2_rn(q, f, two(0.5f));
   const float2 p = __ffma2_rn(__fmul2_rn(f, f), q, f);
-  const float2 s = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
-                               __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000));
+  const float2 s = make_float2(__int_as_float(__float_as_int(t.x) * (1 << 23) + 0x3F800000),
+                               __int_as_float(__float_as_int(t.y) * (1 << 23) + 0x3F800000));
   return __ffma2_rn(s, p, __fadd2_rn(s, two(-1.f)));
 }
 
-// sigmoid(g) and 1 - sigmoid(g) from e = exp(-|g|) and 1 / (1 + e): both keep
-// their relative accuracy, and an infinite gate gives 0 and 1 themselves.
-__device__ __forceinline__ void sigmoid_parts(float g, float e, float r, float &s, float &c) {
-  const float small = e * r;
-  s = g < 0.f ? small : r;
-  c = g < 0.f ? r : small;
+// The floor of 1 - a^2 under a root or a division, where it meets a zero.
+constexpr float kBetaFloor = 1e-36f;
+constexpr float kExpMost = 8.5070592e37f;  // 2^126, whose reciprocal is still normal
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float2 min_nan(float2 a, float b) {
+  return make_float2(min_nan(a.x, b), min_nan(a.y, b));
+}
+__device__ __forceinline__ float2 max_nan(float2 a, float b) {
+  return make_float2(max_nan(a.x, b), max_nan(a.y, b));
+}
+template <typename T> __device__ __forceinline__ float2 rcp_two(float2 x) {
+  return make_float2(Fn<T>::rcp(x.x), Fn<T>::rcp(x.y));
+}
+template <typename T> __device__ __forceinline__ float2 rsqrt_two(float2 x) {
+  return make_float2(Fn<T>::rsqrt(x.x), Fn<T>::rsqrt(x.y));
+}
+// exp(-x)
+template <typename T> __device__ __forceinline__ float2 exp_minus(float2 x) {
+  if constexpr (sizeof(T) == 2) {
+    const float2 t = __fmul2_rn(x, two(-1.4426950408889634f));
+    float2 y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(t.y));
+    return y;
+  } else {
+    return make_float2(expf(-x.x), expf(-x.y));
+  }
 }
 
-constexpr float kBetaFloor = 1e-36f;  // of 1 - a^2 under a root or a division
-
 // What a token's gates come to, for two channels.
-struct Gates {
-  float2 s, sc;  // sigmoid(gate) and 1 minus it
-  float2 u, uc;  // of the input gate
+struct Token {
+  float2 am1;  // a - 1
+  float2 bu;   // beta u
+  float2 s;    // sigmoid(gate)
+  float2 sc;   // 1 - s and 1 - u, for the gradient (uc with an input gate)
+  float2 uc;
 };
-template <typename T, bool kInput>
-__device__ __forceinline__ Gates gates_of(float2 g, float2 i) {
-  Gates y;
-  const float egx = Fn<T>::exp(-fabsf(g.x)), egy = Fn<T>::exp(-fabsf(g.y));
+// beta^2 = 1 - a^2 = (a - 1) (-1 - a), without a difference of near numbers, and
+// the same with a floor.
+__device__ __forceinline__ float2 beta_squared(float2 am1, float2 &floored) {
+  const float2 n = __ffma2_rn(am1, two(-1.f), two(-2.f));
+  floored = __ffma2_rn(am1, n, two(kBetaFloor));
+  return __fmul2_rn(am1, n);
+}
+// A closed gate (s = 0; s = 1 without a decay) and a closed input gate (u = 0)
+// give beta u = 0 to the bit, whatever the other is: a masked token changes
+// nothing even where its x is the type's lowest value.
+template <typename T, bool kDecay, bool kInput, bool kGrad>
+__device__ __forceinline__ Token token_of(float2 g, float2 i, float2 lambda) {
+  Token y;
+  float2 eg = exp_minus<T>(g);
+  if constexpr (!kDecay) eg = min_nan(eg, kExpMost);  // 1 - s = e s, and not inf * 0
+  y.s = rcp_two<T>(__fadd2_rn(eg, two(1.f)));
+  if constexpr (!kDecay) y.sc = __fmul2_rn(eg, y.s);
+  else if constexpr (kGrad) y.sc = __fmul2_rn(min_nan(eg, kExpMost), y.s);
+  float2 eu = two(0.f), pu = two(1.f), u = two(1.f);
   if constexpr (kInput) {
-    const float eux = Fn<T>::exp(-fabsf(i.x)), euy = Fn<T>::exp(-fabsf(i.y));
-    const float2 pg = __fadd2_rn(make_float2(egx, egy), two(1.f));
-    const float2 pu = __fadd2_rn(make_float2(eux, euy), two(1.f));
-    float2 rg, ru;
-    if constexpr (sizeof(T) == 2) {  // one reciprocal for both: the product is at most 4
-      const float2 pp = __fmul2_rn(pg, pu);
-      const float2 r = make_float2(Fn<T>::rcp(pp.x), Fn<T>::rcp(pp.y));
-      rg = __fmul2_rn(r, pu);
-      ru = __fmul2_rn(r, pg);
+    eu = exp_minus<T>(i);
+    pu = __fadd2_rn(eu, two(1.f));
+    if constexpr (!kDecay || kGrad) u = rcp_two<T>(pu);
+    if constexpr (kGrad) y.uc = __fmul2_rn(min_nan(eu, kExpMost), u);
+  }
+  if constexpr (kDecay) {
+    y.am1 = expm1_neg(__fmul2_rn(lambda, y.s));
+    float2 w;
+    const float2 v = beta_squared(y.am1, w);
+    if constexpr (kInput && !kGrad) {
+      // one root for both: beta / p = beta^2 / sqrt(beta^2 p^2), p = 1 + exp(-i)
+      y.bu = __fmul2_rn(v, rsqrt_two<T>(__fmul2_rn(w, __fmul2_rn(pu, pu))));
     } else {
-      rg = make_float2(Fn<T>::rcp(pg.x), Fn<T>::rcp(pg.y));
-      ru = make_float2(Fn<T>::rcp(pu.x), Fn<T>::rcp(pu.y));
+      y.bu = __fmul2_rn(v, rsqrt_two<T>(w));
+      if constexpr (kInput) y.bu = __fmul2_rn(y.bu, u);
     }
-    sigmoid_parts(g.x, egx, rg.x, y.s.x, y.sc.x);
-    sigmoid_parts(g.y, egy, rg.y, y.s.y, y.sc.y);
-    sigmoid_parts(i.x, eux, ru.x, y.u.x, y.uc.x);
-    sigmoid_parts(i.y, euy, ru.y, y.u.y, y.uc.y);
   } else {
-    sigmoid_parts(g.x, egx, Fn<T>::rcp(1.f + egx), y.s.x, y.sc.x);
-    sigmoid_parts(g.y, egy, Fn<T>::rcp(1.f + egy), y.s.y, y.sc.y);
+    y.am1 = make_float2(-y.sc.x, -y.sc.y);
+    y.bu = kInput ? __fmul2_rn(y.sc, u) : y.sc;
   }
   return y;
 }
 
-// a - 1, and beta (and, with a decay, beta^2 where the gradient wants it).
-template <typename T, bool kDecay>
-__device__ __forceinline__ void decay_of(const Gates &y, float2 lambda, float2 &am1, float2 &beta,
-                                         float2 &beta2) {
-  if constexpr (kDecay) {
-    am1 = expm1_neg(__fmul2_rn(lambda, y.s));
-    // 1 - a^2 = -(a - 1)(2 + (a - 1)); a gate that forgets nothing adds nothing (0, not 0 * inf)
-    beta2 = __fmul2_rn(make_float2(-am1.x, -am1.y), __fadd2_rn(am1, two(2.f)));
-    beta = __fmul2_rn(beta2, make_float2(Fn<T>::rsqrt(max_nan(beta2.x, kBetaFloor)),
-                                         Fn<T>::rsqrt(max_nan(beta2.y, kBetaFloor))));
-  } else {
-    am1 = make_float2(-y.sc.x, -y.sc.y);
-    beta = y.sc;
-  }
-}
-
 // ---- tiles ------------------------------------------------------------------------
-// Channels that a CTA takes, and how its lanes share a tile: a lane has two
-// channels, a group of CH / 2 lanes ("slot") kL neighbouring tokens, the slots
-// of the CTA neighbouring groups of tokens.
-template <typename T, int CH, int kL>
+// A warp's tile: a lane has two channels and kL neighbouring tokens.  A CTA takes
+// `ch` = 64, 32 or 16 channels; the ch / 2 lanes of a "part" share its tokens, the
+// 64 / ch parts of a warp and the CTA's warps have neighbouring groups of kL.  In
+// shared memory token k of part p lies at (k * parts + p) * ch: lane l finds
+// its two channels at 64 k + 2 l whatever ch is, in other banks than its warp's
+// other lanes.  A warp fetches its own tile and reads no other.
+constexpr int kRecurWarps = kRecurThreads / 32;
+template <typename T, int kL_>
 struct RecurTile {
-  static constexpr int kPairs = CH / 2;
-  static constexpr int kSlots = kRecurThreads / kPairs;
-  static constexpr int kTokens = kSlots * kL;
-  // Rows of 64 bytes: every slot starts 64 bytes on, so that the two slots of a
-  // warp read other banks.
-  static constexpr int kPad = CH * sizeof(T) < 128 ? 64 / sizeof(T) : 0;
-  static constexpr int kElems = kTokens * CH + kSlots * kPad;
-  static constexpr int kBytes = kElems * sizeof(T);
-  static __device__ __forceinline__ int at(int token) { return token * CH + token / kL * kPad; }
+  static constexpr int kL = kL_;
+  static constexpr int kElems = 64 * kL;
+  static constexpr int kBytes = kElems * (int)sizeof(T);
 };
 
 // Bytes that one copy into shared memory moves: the widest that every row's
@@ -237,42 +260,78 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
 }
 
-// Rows [t0, t0 + kTokens) of `row0` (the tensor at this sequence's first token
-// and this CTA's first channel), `width` channels of them, into `tile`; what is
-// outside [0, len) or beyond the width is set to zero and not read.
-template <typename T, int CH, int kL, int kN>
-__device__ __forceinline__ void load_tile_by(T *tile, const T *row0, int64_t st, int64_t t0,
-                                             int64_t len, int width) {
-  using Tile = RecurTile<T, CH, kL>;
+// A warp's tile from the rows of tokens [t0, t0 + 64 / ch * kL) of `row0` (the
+// tensor at this sequence's first token and this CTA's first channel), all of
+// which the sequence has; channels beyond `width` are set to zero and not read.
+template <typename T, int kL, int kN>
+__device__ __forceinline__ void copy_tile_by(T *tile, const T *row0, int64_t st, int t0, int ch,
+                                             int width) {
   constexpr int kPer = kN / (int)sizeof(T);  // elements of a copy
-  constexpr int kRow = CH / kPer;            // copies of a row
-  static_assert(kRecurThreads % kRow == 0 || kRow % kRecurThreads == 0, "whole rows per turn");
-  const int q = threadIdx.x % kRow * kPer;
-  const int left = max(0, min(kN, (width - q) * (int)sizeof(T)));
-  constexpr int kStep = kRecurThreads / kRow;
-  int row = threadIdx.x / kRow;
-  const T *src = row0 + (t0 + row) * st + q;
+  const int lane = threadIdx.x & 31;
 #pragma unroll 4
-  for (; row < Tile::kTokens; row += kStep, src += kStep * st) {
-    const int64_t t = t0 + row;
-    const int bytes = t >= 0 && t < len ? left : 0;
-    T *dst = tile + Tile::at(row) + q;
-    if constexpr (kN < 4) {
-      T v = from_f32<T>(0.f);
-      if (bytes) v = *src;
-      *dst = v;
-    } else {
-      copy_async<kN>((uint32_t)__cvta_generic_to_shared(dst), bytes ? src : row0, bytes);
-    }
+  for (int n = lane; n < 64 * kL / kPer; n += 32) {
+    const int at = n * kPer, k = at / 64, part = at % 64 / ch, q = at % ch;
+    const T *src = row0 + (int64_t)(t0 + part * kL + k) * st + q;
+    const int bytes = max(0, min(kN, (width - q) * (int)sizeof(T)));
+    if constexpr (kN < 4) tile[at] = bytes ? *src : from_f32<T>(0.f);
+    else copy_async<kN>((uint32_t)__cvta_generic_to_shared(tile + at), bytes ? src : row0, bytes);
   }
 }
-template <typename T, int CH, int kL>
-__device__ __forceinline__ void load_tile(T *tile, const T *row0, int64_t st, int64_t t0,
-                                          int64_t len, int width, int copy) {
-  if (copy == 16) load_tile_by<T, CH, kL, 16>(tile, row0, st, t0, len, width);
-  else if (copy == 8) load_tile_by<T, CH, kL, 8>(tile, row0, st, t0, len, width);
-  else if (copy == 4) load_tile_by<T, CH, kL, 4>(tile, row0, st, t0, len, width);
-  else if constexpr (sizeof(T) == 2) load_tile_by<T, CH, kL, 2>(tile, row0, st, t0, len, width);
+template <typename T, int kL>
+__device__ __forceinline__ void copy_tile(T *tile, const T *row0, int64_t st, int t0, int ch,
+                                          int width, int copy) {
+  if (copy == 16) copy_tile_by<T, kL, 16>(tile, row0, st, t0, ch, width);
+  else if (copy == 8) copy_tile_by<T, kL, 8>(tile, row0, st, t0, ch, width);
+  else if (copy == 4) copy_tile_by<T, kL, 4>(tile, row0, st, t0, ch, width);
+  else if constexpr (sizeof(T) == 2) copy_tile_by<T, kL, 2>(tile, row0, st, t0, ch, width);
+}
+// The same for a tile that the sequence ends in, or that lies beside it: tokens
+// outside [0, len) become `outside` and are not read.
+template <typename T, int kL>
+__device__ __forceinline__ void ragged_tile(T *tile, const T *row0, int64_t st, int t0, int len,
+                                            int ch, int width, float outside) {
+  const T none = from_f32<T>(outside);
+#pragma unroll 8
+  for (int at = threadIdx.x & 31; at < 64 * kL; at += 32) {
+    const int t = t0 + at % 64 / ch * kL + at / 64, q = at % ch;
+    T v = none;
+    if (t >= 0 && t < len && q < width) v = row0[(int64_t)t * st + q];
+    tile[at] = v;
+  }
+}
+
+// Over a warp's parts (the lanes `half` = ch / 2 apart): (a, e) becomes the
+// summary of all of them, in token order; returned is that of the parts before
+// the lane's own, (1, 0) for the first.
+struct Summary {
+  float2 a, e;
+};
+__device__ __forceinline__ float2 shuffle_up(float2 v, int by) {
+  return make_float2(__shfl_up_sync(0xffffffffu, v.x, by), __shfl_up_sync(0xffffffffu, v.y, by));
+}
+__device__ __forceinline__ float2 shuffle_down(float2 v, int by) {
+  return make_float2(__shfl_down_sync(0xffffffffu, v.x, by), __shfl_down_sync(0xffffffffu, v.y, by));
+}
+__device__ __forceinline__ float2 shuffle(float2 v, int from) {
+  return make_float2(__shfl_sync(0xffffffffu, v.x, from), __shfl_sync(0xffffffffu, v.y, from));
+}
+template <bool kBackward>  // the other order: the last part first
+__device__ __forceinline__ Summary join_parts(float2 &a, float2 &e, int half, int lane) {
+  Summary own{two(1.f), two(0.f)};
+  if (half == 32) return own;
+  const int at = kBackward ? 31 - lane : lane;
+  for (int d = half; d < 32; d *= 2) {
+    const float2 ao = kBackward ? shuffle_down(a, d) : shuffle_up(a, d);
+    const float2 eo = kBackward ? shuffle_down(e, d) : shuffle_up(e, d);
+    if (at >= d) e = __ffma2_rn(a, eo, e), a = __fmul2_rn(a, ao);
+  }
+  const float2 ao = kBackward ? shuffle_down(a, half) : shuffle_up(a, half);
+  const float2 eo = kBackward ? shuffle_down(e, half) : shuffle_up(e, half);
+  if (at >= half) own = Summary{ao, eo};
+  const int last = kBackward ? lane % half : 32 - half + lane % half;
+  a = shuffle(a, last);
+  e = shuffle(e, last);
+  return own;
 }
 
 // ---- clusters ---------------------------------------------------------------------
@@ -287,15 +346,106 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Into the shared memory of the cluster's CTA `rank`, at this CTA's address `p`.
-__device__ __forceinline__ void store_remote(float4 *p, uint32_t rank, float4 v) {
-  uint32_t at;
+// Into the shared memory of the cluster's CTA `rank`, at this CTA's address `p`,
+// counted there on the mbarrier at this CTA's address `bar`.
+__device__ __forceinline__ void store_remote(float4 *p, uint64_t *bar, uint32_t rank, float4 v) {
+  uint32_t at, on;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                : "=r"(at)
                : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y),
-               "f"(v.z), "f"(v.w)
-               : "memory");
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(on)
+               : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(rank));
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+      ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(on)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int x,
+                                            int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(tc::smem_u32(dst)),
+      "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// What a launch hands its kernel besides the call.
+struct RecurLaunch {
+  int ch;           // channels of a CTA
+  int cluster;      // CTAs along the tokens
+  int copy;         // bytes of a cp.async copy; unused with TMA
+  int *err;         // the library's device error word
+};
+constexpr int kRecurMaps = 4;
+struct RecurMaps {  // (batch, tokens, channels), with boxes of a tile
+  CUtensorMap m[kRecurMaps];
+};
+// Whether TMA can address the tensor: rows at 16 bytes, no broadcast dimension.
+inline bool recur_tma_view(const TokenView &v, const RecurCall &c, int size) {
+  return !v.p || (((uintptr_t)v.p & 15) == 0 && v.st * size % 16 == 0 && v.sb * size % 16 == 0 &&
+                  v.st >= c.channels && (v.sb > 0 || c.batch == 1) &&
+                  v.st < ((int64_t)1 << 32) && v.sb < ((int64_t)1 << 37) && c.batch <= INT32_MAX);
+}
+// (channels, groups of l tokens, tokens of a group, batch), with boxes that fill a
+// warp's tile; for the sequences' whole groups only.
+inline bool recur_map(CUtensorMap *map, const TokenView &v, const RecurCall &c, int dtype, int ch,
+                      int l) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const uint64_t size = dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+  const cuuint64_t st = (cuuint64_t)v.st * size;
+  const cuuint64_t dim[4] = {(cuuint64_t)c.channels, (cuuint64_t)(c.tokens / l), (cuuint64_t)l,
+                             (cuuint64_t)c.batch};
+  const cuuint64_t stride[3] = {st * l, st, c.batch == 1 ? st * l : (cuuint64_t)v.sb * size};
+  const cuuint32_t box[4] = {(cuuint32_t)ch, (cuuint32_t)(64 / ch), (cuuint32_t)l, 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return fn(map, dtype == LA_DTYPE_FLOAT32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            4, const_cast<void *>(v.p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Channels of a CTA and CTAs along the tokens for a size: a CTA for every SM from
+// narrower channel groups, and only then from clusters along the tokens, each of
+// whose CTAs has tokens of its own (l for each of its parts).  A cluster's
+// exchange at every step costs more than an idle SM: 16384 x 2048 in 65 us by 128
+// CTAs of 16 channels, in 86 by 256 in clusters of two; 2048 x 1024 in 12.0 us by 64
+// CTAs, 10.7 by 128 in clusters of two.
+struct RecurShape {
+  int ch, cluster;
+};
+inline RecurShape recur_shape(int64_t batch, int64_t tokens, int channels, int sm_count, int l,
+                              int widest) {
+  RecurShape s{widest, 1};
+  auto ctas = [&] { return batch * ((channels + s.ch - 1) / s.ch) * s.cluster; };
+  while (s.ch > 16 && ctas() < sm_count) s.ch /= 2;
+  while (s.cluster < kRecurMaxCluster && ctas() * 2 <= sm_count &&
+         tokens > (int64_t)s.cluster * (64 / s.ch) * l * kRecurWarps)
+    s.cluster *= 2;
+  return s;
+}
+
+template <class Kernel>
+int launch_clusters(Kernel kernel, const RecurCall &p, const RecurLaunch &l, const RecurMaps &maps,
+                    int smem, cudaStream_t s) {
+  const int64_t grid = p.batch * ((p.channels + l.ch - 1) / l.ch) * l.cluster;
+  if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kRecurThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = l.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = l.cluster > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, p, l, maps);
+  return check_launch();
 }
 
 int launch_recur_fwd(const RecurCall &c, int dtype, cudaStream_t s);

@@ -9,63 +9,88 @@
 //   without: d(gate)_t = H_t (h_{t-1} - u_t x_t) s_t (1 - s_t)
 //   d(initial state) = a_0 H_0
 //
-// The forward pass' tiles, clusters and summaries, walked from the last tile
-// to the first (14 bytes per element in bf16 with both gates, against about
-// 70 instructions).  h is not saved but computed again, in fp32, from the
-// state before each tile that the forward pass left (1/16 byte per element and
-// byte of a float, against two for h rounded to bf16): a thread's summary has
-// both chains, E for the state and R for the gradient, under one product A.
-// d(lambda) is summed over a CTA's tokens and written as one row per CTA; a
-// second kernel adds the rows in a fixed order.
+// The forward pass' tiles, warps and summaries, walked from the last tokens to the
+// first: a summary is (A, R), a H in front = A (a H behind) + R.  14.5 bytes per
+// element in bf16 with both gates, against 75 instructions.  h is not saved but
+// computed again, in fp32, from the state that the forward pass left every 16
+// tokens (a quarter of a byte per element, against two for an h rounded to
+// bf16); those states keep the forward chain out of the walk: with one state per
+// CTA's tile, handed on from warp to warp against the gradient's direction, 4 x
+// 4096 x 1024 took 125 us instead of 72.  d(lambda) is summed over a CTA's tokens
+// and written as one row per CTA; a second kernel adds the rows in a fixed order.
+#include <type_traits>
+
 #include "column_sum.cuh"
 #include "recurrence.cuh"
+#include "tc_kernels.cuh"
 
 namespace la {
 namespace {
 
-constexpr int kL = 8;  // tokens of a thread and step
+constexpr int kL = 8;       // tokens of a thread and step
+constexpr int kStages = 2;   // tiles of a warp
 
-template <typename T, int CH, bool kDecay, bool kInput>
-__global__ void __launch_bounds__(kRecurThreads, 2) recur_bwd_kernel(const RecurCall p,
-                                                                   const int cluster,
-                                                                   const int copy) {
-  using Tile = RecurTile<T, CH, kL>;
-  constexpr int kIn = kInput ? 4 : 3;
-  constexpr int kPairs = Tile::kPairs, kSlots = Tile::kSlots, kTok = Tile::kTokens;
-  static_assert(kTok % kRecurCheck == 0, "tiles start at saved states");
-  extern __shared__ __align__(16) uint8_t smem[];
-  T *tiles = (T *)smem;                                  // [2][kIn][kElems]
-  __shared__ float4 sums[2][kSlots][kPairs];             // (A, A, R, R) of a pair
-  __shared__ float2 sums_e[2][kSlots][kPairs];           // (E, E)
-  __shared__ float4 csums[2][kRecurMaxCluster][kPairs];  // (A, A, R, R) of the cluster's CTAs
+struct Exchange {
+  // What the warp behind hands to each warp: without a cluster a H (in xy), else the
+  // summary (A, A, R, R) of the CTA's tokens behind its own.
+  float4 behind[kRecurWarps][32];
+  float4 csums[2][kRecurMaxCluster][32];  // summaries of the cluster's CTAs
+  float2 sums[kRecurWarps][32];
+  uint64_t full[kStages][kRecurWarps], handed[kRecurWarps], arrived[2];
+  int abort;
+};
+
+template <typename T, bool kDecay, bool kInput, bool kTma>
+__global__ void __launch_bounds__(kRecurThreads, 2)
+recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ RecurMaps maps) {
+  using Tile = RecurTile<T, kL>;
+  constexpr int kIn = kInput ? 4 : 3, kLast = kRecurWarps - 1;
+  static_assert(kRecurCheck == 2 * kL, "every other part starts at a saved state");
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * Tile::kBytes);
 
   column_sum_may_start();
+  const int cluster = l.cluster, ch = l.ch, half = ch / 2, parts = 64 / ch;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int groups = (p.channels + CH - 1) / CH;
-  const int64_t unit = blockIdx.x / cluster;
-  const int64_t ib = unit / groups;
-  const int c0 = (int)(unit % groups) * CH;
-  const int width = min(CH, p.channels - c0);
-  const int64_t len = recur_length(p.lengths, p.lengths64, ib, p.tokens);
-  const int pair = threadIdx.x % kPairs, slot = threadIdx.x / kPairs;
+  const int groups = (p.channels + ch - 1) / ch;
+  const int64_t ib = blockIdx.x / cluster / groups;
+  const int c0 = (int)(blockIdx.x / cluster % groups) * ch;
+  const int width = min(ch, p.channels - c0);
+  const int len = (int)recur_length(p.lengths, p.lengths64, ib, p.tokens);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int pair = lane & (half - 1), part = lane / half;
   const int c = c0 + 2 * pair;
   const bool live = c < p.channels, second = c + 1 < p.channels;
 
-  const T *rows[4] = {(const T *)p.x.p + ib * p.x.sb + c0, (const T *)p.gate.p + ib * p.gate.sb + c0,
-                      (const T *)p.d_out.p + ib * p.d_out.sb + c0,
-                      kInput ? (const T *)p.input_gate.p + ib * p.input_gate.sb + c0 : nullptr};
-  const int64_t st[4] = {p.x.st, p.gate.st, p.d_out.st, p.input_gate.st};
-  const int64_t blocks = (len + kTok - 1) / kTok;
-  const int64_t steps = (blocks + cluster - 1) / cluster;
-  auto block_of = [&](int64_t i) { return blocks - 1 - (i * cluster + rank); };  // < 0: none
-  auto fetch = [&](int64_t i, int buf) {
-    if (i < steps) {
+  T *tiles = (T *)smem + warp * kIn * Tile::kElems;  // [kStages][kRecurWarps][kIn][kElems]
+  constexpr int kStageElems = kRecurWarps * kIn * Tile::kElems;
+  const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
+  const int rows = parts * kL;            // tokens of a warp and step
+  const int block_rows = kRecurWarps * rows;
+  const int blocks = (len + block_rows - 1) / block_rows;
+  const int steps = (blocks + cluster - 1) / cluster;
+  auto source = [&](int n) { return (const T *)views[n]->p + ib * views[n]->sb + c0; };
+  auto block_of = [&](int i) { return blocks - 1 - (i * cluster + rank); };  // < 0: none
+  // Tiles that the sequence fills; the last one is loaded where it is used.
+  auto fetch = [&](int i, int stage) {
+    const int t0 = block_of(i) * block_rows + warp * rows;
+    if (i < steps && t0 >= 0 && t0 + rows <= len) {
+      T *tile = tiles + stage * kStageElems;
+      if constexpr (kTma) {
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(&ex.full[stage][warp], kIn * Tile::kBytes);
 #pragma unroll
-      for (int n = 0; n < kIn; ++n)
-        load_tile<T, CH, kL>(tiles + (buf * kIn + n) * Tile::kElems, rows[n], st[n],
-                             block_of(i) * kTok, len, width, copy);
+          for (int n = 0; n < kIn; ++n)
+            tma_load_4d(tile + n * Tile::kElems, &maps.m[n], &ex.full[stage][warp], c0, t0 / kL,
+                            0, (int)ib);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < kIn; ++n)
+          copy_tile<T, kL>(tile + n * Tile::kElems, source(n), views[n]->st, t0, ch, width, l.copy);
+      }
     }
-    copy_commit();
+    if (!kTma) copy_commit();
   };
 
   float2 lambda = two(0.f), carry = two(0.f), d_lambda = two(0.f);
@@ -76,213 +101,249 @@ __global__ void __launch_bounds__(kRecurThreads, 2) recur_bwd_kernel(const Recur
       carry = make_float2(h[0], second ? h[1] : 0.f);
     }
   }
-  if (cluster > 1) cluster_arrive();
-  fetch(0, 0);
-  fetch(1, 1);
-  if (cluster > 1) cluster_wait();  // the peers run before their shared memory is written
-
-  const bool pairs = p.pairs;
-  const int64_t n_check = (p.tokens + kRecurCheck - 1) / kRecurCheck;
-  const int64_t first = ib * p.tokens * p.channels + c;
-  for (int64_t i = 0; i < steps; ++i) {
-    const int buf = (int)(i & 1);
-    const T *xs = tiles + buf * kIn * Tile::kElems;
-    const T *gs = xs + Tile::kElems, *ds = gs + Tile::kElems, *us = ds + Tile::kElems;
-    const int64_t block = block_of(i);
-    const int64_t t0 = block * kTok + slot * kL;
-    const int inside = block < 0 ? 0 : (int)max64(0, min64(kL, len - t0));
-    float2 start = two(0.f);  // the state before the tile
-    if (block >= 0 && live) {
-      const float *h = p.check + (ib * n_check + block * (kTok / kRecurCheck)) * p.channels + c;
-      start = make_float2(h[0], second ? h[1] : 0.f);
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kRecurWarps; ++w) {
+      for (int j = 0; j < kStages; ++j) tc::mbar_init(&ex.full[j][w], 1);
+      tc::mbar_init(&ex.handed[w], 1);
     }
-    copy_wait<1>();
-    __syncthreads();
-    // bu = beta u; tokens outside the sequence (zero in the tile) keep state and gradient
+    for (int j = 0; j < 2; ++j) tc::mbar_init(&ex.arrived[j], 1);
+    ex.abort = 0;
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  if (cluster > 1) cluster_arrive();
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) fetch(j, j);
+  if (cluster > 1) cluster_wait();  // the peers' barriers are there before they are counted on
+
+  const bool pairs = kTma || p.pairs;
+  const int64_t n_check = (p.tokens + kRecurCheck - 1) / kRecurCheck;
+  const int64_t origin = ib * p.tokens * p.channels + c;
+  // The saved state at or before this thread's tokens of a step; loaded a step ahead.
+  auto saved = [&](int i) {
+    const int t0 = block_of(i) * block_rows + warp * rows + part * kL;
+    if (t0 < 0 || t0 >= len || !live) return two(0.f);
+    const float *v = p.check + (ib * n_check + t0 / kRecurCheck) * p.channels + c;
+    return make_float2(v[0], second ? v[1] : 0.f);
+  };
+  float2 start = saved(0);
+  int stage = 0;
+  uint32_t phases = 0;  // a bit per stage
+  for (int i = 0; i < steps; ++i) {
+    const int buf = i & 1;
+    T *xs = tiles + stage * kStageElems;
+    T *gs = xs + Tile::kElems, *ds = gs + Tile::kElems, *us = ds + Tile::kElems;
+    const int block = block_of(i);
+    const int row0 = block * block_rows + warp * rows, t0 = row0 + part * kL;
+    const bool whole = block >= 0 && row0 + rows <= len;
+    float2 h = start;
+    start = saved(i + 1);
+    if (whole) {
+      if constexpr (kTma) {
+        tc::mbar_wait(&ex.full[stage][warp], phases >> stage & 1, &ex.abort);
+        phases ^= 1u << stage;
+      } else {
+        copy_wait<kStages - 1>();
+      }
+    } else {
+      // tokens outside the sequence keep the state and the gradient
+      ragged_tile<T, kL>(xs, source(0), views[0]->st, row0, len, ch, width, 0.f);
+      ragged_tile<T, kL>(gs, source(1), views[1]->st, row0, len, ch, width,
+                         kDecay ? -INFINITY : INFINITY);
+      ragged_tile<T, kL>(ds, source(2), views[2]->st, row0, len, ch, width, 0.f);
+      if (kInput) ragged_tile<T, kL>(us, source(3), views[3]->st, row0, len, ch, width, 0.f);
+      if (kTma) tc::fence_proxy_async_smem();  // ahead of the next copy into this tile
+    }
+    if (!kTma || !whole) __syncwarp();
     float2 am1[kL], bu[kL], s[kL], sc[kL], uc[kL];
-    float2 sum = two(kDecay ? 0.f : 1.f), e = two(0.f), r = two(0.f);
+    float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f), r = two(0.f);
 #pragma unroll
     for (int k = 0; k < kL; ++k) {
-      const int at = Tile::at(slot * kL + k) + 2 * pair;
-      float2 g = load_two(gs + at);
-      if (k >= inside) g = two(kDecay ? -INFINITY : INFINITY);
-      const Gates y = gates_of<T, kInput>(g, kInput ? load_two(us + at) : two(0.f));
-      float2 beta2;
-      decay_of<T, kDecay>(y, lambda, am1[k], bu[k], beta2);
-      if (kInput) bu[k] = __fmul2_rn(bu[k], y.u), uc[k] = y.uc;
-      s[k] = y.s, sc[k] = y.sc;
+      const int at = 64 * k + 2 * lane;
+      const Token y = token_of<T, kDecay, kInput, true>(
+          load_two(gs + at), kInput ? load_two(us + at) : two(0.f), lambda);
+      am1[k] = y.am1, bu[k] = y.bu, s[k] = y.s, sc[k] = y.sc;
+      if (kInput) uc[k] = y.uc;
       e = __ffma2_rn(bu[k], load_two(xs + at), __ffma2_rn(am1[k], e, e));
-      sum = kDecay ? __fadd2_rn(sum, y.s) : __fmul2_rn(sum, y.s);
+      a = kDecay ? __fadd2_rn(a, y.s) : __fmul2_rn(a, y.s);
     }
 #pragma unroll
     for (int k = kL - 1; k >= 0; --k) {
-      r = __fadd2_rn(r, load_two(ds + Tile::at(slot * kL + k) + 2 * pair));
+      r = __fadd2_rn(r, load_two(ds + 64 * k + 2 * lane));
       r = __ffma2_rn(am1[k], r, r);
     }
     if (kDecay) {
-      sum = __fmul2_rn(sum, lambda);
-      sum = make_float2(Fn<T>::exp(sum.x), Fn<T>::exp(sum.y));
+      a = __fmul2_rn(a, lambda);
+      a = make_float2(Fn<T>::exp(a.x), Fn<T>::exp(a.y));
     }
-    sums[buf][slot][pair] = make_float4(sum.x, sum.y, r.x, r.y);
-    sums_e[buf][slot][pair] = e;
-    __syncthreads();
-
-    float2 h = start, g = carry;  // the state before this thread's tokens, the gradient behind
-    float2 a = two(1.f), a_own = two(1.f), r_own = two(0.f);
-    r = cluster == 1 ? carry : two(0.f);
-#pragma unroll
-    for (int j = kSlots - 1; j >= 0; --j) {
-      if (j == slot) a_own = a, r_own = r;
-      const float4 v = sums[buf][j][pair];
-      r = __ffma2_rn(make_float2(v.x, v.y), r, make_float2(v.z, v.w));
-      a = __fmul2_rn(a, make_float2(v.x, v.y));
+    {  // an odd part's state comes through the part before
+      const float2 ao = shuffle_up(a, half), eo = shuffle_up(e, half);
+      if (part & 1) h = __ffma2_rn(ao, h, eo);
     }
+    const Summary rest = join_parts<true>(a, r, half, lane);
+    float2 g;  // a H of the token behind this thread's
+    const int next = warp == 0 ? kLast : warp - 1;
+    float2 ap = two(1.f), rp = two(0.f);  // of the CTA's warps behind (with a cluster)
     if (cluster == 1) {
-      g = r_own;
-      carry = r;
+      if (warp < kLast || i > 0) {
+        tc::mbar_wait(&ex.handed[warp], (uint32_t)(warp < kLast ? i : i - 1) & 1, &ex.abort);
+        const float4 v = ex.behind[warp][pair];
+        carry = make_float2(v.x, v.y);
+      }
+      g = carry;
+      carry = __ffma2_rn(a, carry, r);
+      if (part == 0) *(float2 *)&ex.behind[next][pair] = carry;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ex.handed[next]);
     } else {
-      if (slot < cluster)
-        store_remote(&csums[buf][rank][pair], (uint32_t)slot, make_float4(a.x, a.y, r.x, r.y));
-      cluster_arrive();
-    }
-    for (int j = 0; j < slot; ++j) {
-      const float4 v = sums[buf][j][pair];
-      h = __ffma2_rn(make_float2(v.x, v.y), h, sums_e[buf][j][pair]);
+      if (warp < kLast) {
+        tc::mbar_wait(&ex.handed[warp], (uint32_t)i & 1, &ex.abort);
+        const float4 v = ex.behind[warp][pair];
+        ap = make_float2(v.x, v.y), rp = make_float2(v.z, v.w);
+      }
+      const float2 at = __fmul2_rn(a, ap), rt = __ffma2_rn(a, rp, r);
+      const float4 sum = make_float4(at.x, at.y, rt.x, rt.y);
+      if (warp > 0) {
+        if (part == 0) ex.behind[next][pair] = sum;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ex.handed[next]);
+      } else {  // the CTA's summary, to all of the cluster
+        if (lane == 0)
+          tc::mbar_arrive_expect_tx(&ex.arrived[buf], cluster * half * sizeof(float4));
+        if (part == 0)
+          for (int j = 0; j < cluster; ++j)
+            store_remote(&ex.csums[buf][rank][pair], &ex.arrived[buf], (uint32_t)j, sum);
+      }
     }
     float2 before[kL];
 #pragma unroll
     for (int k = 0; k < kL; ++k) {
       before[k] = h;
-      const float2 x = load_two(xs + Tile::at(slot * kL + k) + 2 * pair);
+      const float2 x = load_two(xs + 64 * k + 2 * lane);
       h = __ffma2_rn(bu[k], x, __ffma2_rn(am1[k], h, h));
     }
     if (cluster > 1) {
-      cluster_wait();
+      tc::mbar_wait(&ex.arrived[buf], (uint32_t)(i >> 1) & 1, &ex.abort);
       for (int j = 0; j < cluster; ++j) {
         if (j == rank) g = carry;
-        const float4 v = csums[buf][j][pair];
+        const float4 v = ex.csums[buf][j][pair];
         carry = __ffma2_rn(make_float2(v.x, v.y), carry, make_float2(v.z, v.w));
       }
-      g = __ffma2_rn(a_own, g, r_own);
+      g = __ffma2_rn(ap, g, rp);
     }
-    const int64_t o = first + (t0 + kL - 1) * p.channels;
+    g = __ffma2_rn(rest.a, g, rest.e);
+    const int64_t o = origin + (int64_t)t0 * p.channels;
     T *dx = (T *)p.dx + o, *dg = (T *)p.d_gate + o, *di = kInput ? (T *)p.d_input + o : nullptr;
+    auto finish = [&](auto all) {
 #pragma unroll
-    for (int k = kL - 1; k >= 0; --k) {
-      const int at = Tile::at(slot * kL + k) + 2 * pair;
-      const float2 x = load_two(xs + at);
-      const float2 hh = __fadd2_rn(g, load_two(ds + at));
-      g = __ffma2_rn(am1[k], hh, hh);  // a H
-      const float2 dxk = __fmul2_rn(hh, bu[k]);
-      float2 dgk, dik;
-      if constexpr (kInput) dik = __fmul2_rn(__fmul2_rn(dxk, x), uc[k]);
-      if constexpr (kDecay) {
-        float2 beta2 = __fmul2_rn(make_float2(-am1[k].x, -am1[k].y), __fadd2_rn(am1[k], two(2.f)));
-        beta2 = make_float2(Fn<T>::rcp(max_nan(beta2.x, kBetaFloor)),
-                            Fn<T>::rcp(max_nan(beta2.y, kBetaFloor)));
-        // a u x / beta = a (bu x) / beta^2
-        float2 w = __fmul2_rn(__fmul2_rn(bu[k], x), beta2);
-        w = __ffma2_rn(am1[k], w, w);
-        const float2 d_log = __fmul2_rn(g, __fadd2_rn(before[k], make_float2(-w.x, -w.y)));
-        const float2 ds_ = __fmul2_rn(d_log, s[k]);
-        d_lambda = __fadd2_rn(d_lambda, ds_);
-        dgk = __fmul2_rn(__fmul2_rn(ds_, lambda), sc[k]);
-      } else {
-        // bu = (1 - s) u: H (h - u x) s (1 - s) = H s ((1 - s) h - bu x)
-        const float2 bx = __fmul2_rn(bu[k], x);
-        dgk = __fmul2_rn(__fmul2_rn(hh, s[k]),
-                         __ffma2_rn(sc[k], before[k], make_float2(-bx.x, -bx.y)));
+      for (int k = kL - 1; k >= 0; --k) {
+        const int at = 64 * k + 2 * lane;
+        const float2 x = load_two(xs + at);
+        const float2 hh = __fadd2_rn(g, load_two(ds + at));
+        g = __ffma2_rn(am1[k], hh, hh);  // a H
+        const float2 dxk = __fmul2_rn(hh, bu[k]), b = __fmul2_rn(bu[k], x);
+        float2 dgk, dik = two(0.f);
+        if constexpr (kInput) dik = __fmul2_rn(__fmul2_rn(dxk, x), uc[k]);
+        if constexpr (kDecay) {
+          // a u x / beta = a (b / beta^2)
+          float2 w;
+          beta_squared(am1[k], w);
+          w = __fmul2_rn(b, rcp_two<T>(w));
+          w = __ffma2_rn(am1[k], w, w);
+          const float2 d_log = __fmul2_rn(g, __ffma2_rn(w, two(-1.f), before[k]));
+          const float2 ds_ = __fmul2_rn(d_log, s[k]);
+          d_lambda = __fadd2_rn(d_lambda, ds_);
+          dgk = __fmul2_rn(__fmul2_rn(ds_, lambda), sc[k]);
+        } else {
+          // H (h - u x) s (1 - s) = H s ((1 - s) h - b)
+          dgk = __fmul2_rn(__fmul2_rn(hh, s[k]),
+                           __ffma2_rn(b, two(-1.f), __fmul2_rn(sc[k], before[k])));
+        }
+        if (all || (block >= 0 && t0 + k < len)) {
+          const int64_t at_k = (int64_t)k * p.channels;
+          store_two(dx + at_k, dxk, all || pairs, second);
+          store_two(dg + at_k, dgk, all || pairs, second);
+          if constexpr (kInput) store_two(di + at_k, dik, all || pairs, second);
+        }
       }
-      if (live && k < inside) {
-        store_two(dx, dxk, pairs, second);
-        store_two(dg, dgk, pairs, second);
-        if constexpr (kInput) store_two(di, dik, pairs, second);
-      }
-      dx -= p.channels, dg -= p.channels;
-      if (kInput) di -= p.channels;
+    };
+    if (live) {
+      if (pairs && whole) finish(std::true_type{});
+      else finish(std::false_type{});
     }
-    __syncthreads();  // the tile is read
-    fetch(i + 2, buf);
+    __syncwarp();  // the rows are read
+    fetch(i + kStages, stage);
+    if (++stage == kStages) stage = 0;
   }
-  if (p.d_init && rank == 0 && slot == 0 && live)
+  if (p.d_init && rank == 0 && warp == 0 && part == 0 && live)
     store_two(p.d_init + ib * p.channels + c, carry, pairs, second);
-  for (int64_t t = len + rank * kSlots + slot; t < p.tokens && live; t += cluster * kSlots) {
-    const int64_t o = first + t * p.channels;
+  const int slots = kRecurWarps * parts;
+  for (int64_t t = len + rank * slots + warp * parts + part; t < p.tokens && live; t += cluster * slots) {
+    const int64_t o = origin + t * p.channels;
     store_two((T *)p.dx + o, two(0.f), pairs, second);
     store_two((T *)p.d_gate + o, two(0.f), pairs, second);
     if (kInput) store_two((T *)p.d_input + o, two(0.f), pairs, second);
   }
   if (kDecay && p.partial) {
+    for (int d = half; d < 32; d *= 2) {
+      d_lambda.x += __shfl_xor_sync(0xffffffffu, d_lambda.x, d);
+      d_lambda.y += __shfl_xor_sync(0xffffffffu, d_lambda.y, d);
+    }
     __syncthreads();
-    sums_e[0][slot][pair] = d_lambda;
+    if (part == 0) ex.sums[warp][pair] = d_lambda;
     __syncthreads();
-    if (slot == 0 && live) {
+    if (warp == 0 && part == 0 && live) {
       float2 v = two(0.f);
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) v = __fadd2_rn(v, sums_e[0][j][pair]);
-      store_two(p.partial + (ib * cluster + rank) * p.channels + c, v, pairs, second);
+      for (int j = 0; j < kRecurWarps; ++j) v = __fadd2_rn(v, ex.sums[j][pair]);
+      store_two(p.partial + (ib * cluster + rank) * p.channels + c, v, p.channels % 2 == 0, second);
     }
+  }
+  if (ex.abort) {
+    if (l.err) *l.err = tc::kErrTimeout;
+    const uint64_t since = tc::globaltimer();  // copies in flight still write into this CTA
+    while (tc::globaltimer() - since < tc::kWaitTimeoutNs) __nanosleep(1000);
   }
 }
 
-struct Shape {
-  int ch, cluster;
-};
-
-// As in the forward pass: two CTAs per SM, 32 channels where 64 leave SMs idle.
-Shape shape_of(int64_t batch, int64_t tokens, int channels, int sm_count) {
-  auto cluster_for = [&](int ch, int tile) {
-    const int64_t units = batch * ((channels + ch - 1) / ch);
-    int k = 1;
-    while (k < kRecurMaxCluster && units * k * 2 <= 2 * sm_count && tokens > (int64_t)k * tile) k *= 2;
-    return k;
-  };
-  const int wide = cluster_for(64, RecurTile<float, 64, kL>::kTokens);
-  if (batch * ((channels + 63) / 64) * wide <= sm_count && channels > 32)
-    return {32, cluster_for(32, RecurTile<float, 32, kL>::kTokens)};
-  return {64, wide};
+RecurShape shape_of(int64_t batch, int64_t tokens, int channels, int sm_count) {
+  return recur_shape(batch, tokens, channels, sm_count, kL, 32);
 }
 
-template <typename T, int CH, bool kDecay, bool kInput>
-int launch(const RecurCall &p, int cluster, cudaStream_t s) {
-  using Tile = RecurTile<T, CH, kL>;
-  const int smem = 2 * (kInput ? 4 : 3) * Tile::kBytes;
-  auto kernel = recur_bwd_kernel<T, CH, kDecay, kInput>;
+template <typename T, bool kDecay, bool kInput, bool kTma>
+int launch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
+  constexpr int dtype = sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16;
+  constexpr int kIn = kInput ? 4 : 3;
+  const int smem = kStages * kIn * kRecurWarps * RecurTile<T, kL>::kBytes + (int)sizeof(Exchange);
+  auto kernel = recur_bwd_kernel<T, kDecay, kInput, kTma>;
   const int st = allow_dynamic_smem((const void *)kernel, smem);
   if (st != LA_OK) return st;
-  int copy = 16;
-  for (const TokenView *v : {&p.x, &p.gate, &p.d_out, &p.input_gate})
-    if (v->p && copy_bytes(*v, sizeof(T)) < copy) copy = copy_bytes(*v, sizeof(T));
-  const int64_t grid = p.batch * ((p.channels + CH - 1) / CH) * cluster;
-  if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kRecurThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, p, cluster, copy);
-  return check_launch();
+  const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
+  RecurLaunch l{shape.ch, shape.cluster, 16, device_error_word()};
+  RecurMaps maps;
+  for (int n = 0; n < kIn; ++n) {
+    if (kTma && !recur_map(&maps.m[n], *views[n], p, dtype, shape.ch, kL)) return LA_ERR_CUDA;
+    l.copy = min(l.copy, copy_bytes(*views[n], sizeof(T)));
+  }
+  return launch_clusters(kernel, p, l, maps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
-int launch_by_size(const RecurCall &p, const Shape &shape, cudaStream_t s) {
-  if (shape.ch == 32) return launch<T, 32, kDecay, kInput>(p, shape.cluster, s);
-  return launch<T, 64, kDecay, kInput>(p, shape.cluster, s);
+int launch_by_view(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
+  const bool tma = recur_tma_view(p.x, p, sizeof(T)) && recur_tma_view(p.gate, p, sizeof(T)) &&
+                   recur_tma_view(p.d_out, p, sizeof(T)) &&
+                   recur_tma_view(p.input_gate, p, sizeof(T)) && p.pairs && p.tokens >= kL && encode_fn();
+  return tma ? launch<T, kDecay, kInput, true>(p, shape, s)
+             : launch<T, kDecay, kInput, false>(p, shape, s);
 }
 
 template <typename T>
-int launch_typed(const RecurCall &p, const Shape &sh, cudaStream_t s) {
+int launch_typed(const RecurCall &p, const RecurShape &sh, cudaStream_t s) {
   if (p.log_decay)
-    return p.input_gate.p ? launch_by_size<T, true, true>(p, sh, s)
-                          : launch_by_size<T, true, false>(p, sh, s);
-  return p.input_gate.p ? launch_by_size<T, false, true>(p, sh, s)
-                        : launch_by_size<T, false, false>(p, sh, s);
+    return p.input_gate.p ? launch_by_view<T, true, true>(p, sh, s)
+                          : launch_by_view<T, true, false>(p, sh, s);
+  return p.input_gate.p ? launch_by_view<T, false, true>(p, sh, s)
+                        : launch_by_view<T, false, false>(p, sh, s);
 }
 
 }  // namespace
@@ -295,7 +356,7 @@ int launch_recur_bwd(const RecurCall &p, int dtype, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  const Shape sh = shape_of(p.batch, p.tokens, p.channels, info.sm_count);
+  const RecurShape sh = shape_of(p.batch, p.tokens, p.channels, info.sm_count);
   return dtype == LA_DTYPE_FLOAT32 ? launch_typed<float>(p, sh, s)
                                    : launch_typed<__nv_bfloat16>(p, sh, s);
 }

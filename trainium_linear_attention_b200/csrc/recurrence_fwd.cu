@@ -1,61 +1,94 @@
-// Gated linear recurrence: prompts, and single tokens.
+// Gated linear recurrence: prompts.
 //
-// Bound by memory: x and the gates read once, h written once (8 bytes per
-// element in bf16 with both gates), against about 30 instructions.  A sequence
-// of one channel is a chain, so the parallel work is channels x batch, too few
-// for a long prompt: a CTA takes 64 (or 32) channels and, at each step, a tile of
-// neighbouring tokens, and a cluster of up to 8 CTAs along the tokens shares a
-// channel group.  Per step every thread
-//   1. turns kL tokens of two channels into (a - 1, b), kept in registers, and
+// Bound by memory and, nearly as much, by its instructions: x and the gates are
+// read once and h is written once (8 bytes per element in bf16 with both gates),
+// against 35 instructions and 4 of the special-function unit, which does 16 a cycle
+// and SM.  A channel's sequence is a chain, and channels x batch are too few
+// chains for the SMs, so a CTA takes 64, 32 or 16 channels and its lanes and warps
+// neighbouring groups of kL tokens.  A thread
+//   1. turns its tokens of two channels into (a - 1, b), kept in registers, and
 //      folds them to a summary (A, E): h_out = A h_in + E,
-//   2. reads the summaries of the CTA's other threads (shared memory) and of the
-//      cluster's other CTAs (distributed shared memory, one cluster barrier),
-//   3. walks its tokens once more from its own h_in, and writes them.
-// So inputs are read once, nothing waits for another cluster, and the sums have
-// one fixed order.  The tiles are fetched two steps ahead with cp.async.
+//   2. gets h_in: the summaries of the warp's other parts by shuffles, the state
+//      from the warp before, which it hands on to the next one at once,
+//   3. walks its tokens once more from h_in, and writes them.
+// Warps fetch their own tiles by TMA two steps ahead and wait for nothing but
+// them and the warp before: no barrier over the CTA.  With too few channels for the
+// SMs a cluster of up to 8 CTAs along the tokens shares a channel group; its CTAs'
+// summaries cross distributed shared memory once per step.  Inputs that TMA cannot
+// address come by cp.async, or element by element.  The sums have one fixed
+// order.
+//
+// 8 x 32768 x 1024 in 421 us (5.1 TB/s, 78% of the copy rate), 16384 x 2048 in 65
+// (128 CTAs: 63%), 4 x 4096 x 1024 in 35 (58%).  What it took: one barrier-bound form
+// with cp.async 873 us, fewer instructions (one root for beta and u, no selects) 663,
+// TMA 524, the hand-over from warp to warp 451, tiles that any channel width reads
+// without bank conflicts and stores without predicates 421.
 #include "recurrence.cuh"
+#include "tc_kernels.cuh"
 
 namespace la {
 namespace {
 
-constexpr int kL = 16;  // tokens of a thread and step
+constexpr int kL = 16;       // tokens of a thread and step
+constexpr int kStages = 2;   // tiles of a warp
 
-template <typename T, int CH, bool kDecay, bool kInput>
-__global__ void __launch_bounds__(kRecurThreads, 2) recur_fwd_kernel(const RecurCall p,
-                                                                   const int cluster,
-                                                                   const int copy) {
-  using Tile = RecurTile<T, CH, kL>;
-  constexpr int kIn = kInput ? 3 : 2;
-  constexpr int kPairs = Tile::kPairs, kSlots = Tile::kSlots, kTok = Tile::kTokens;
-  extern __shared__ __align__(16) uint8_t smem[];
-  T *tiles = (T *)smem;  // [2][kIn][kElems]
-  __shared__ float4 sums[2][kSlots][kPairs];             // (A, A, E, E) of a pair
-  __shared__ float4 csums[2][kRecurMaxCluster][kPairs];  // of the cluster's CTAs
+struct Exchange {
+  // What the warp before hands to each warp: without a cluster the state (in
+  // xy), else the summary (A, A, E, E) of the CTA's tokens before its own.
+  float4 before[kRecurWarps][32];
+  float4 csums[2][kRecurMaxCluster][32];  // summaries of the cluster's CTAs
+  uint64_t full[kStages][kRecurWarps], handed[kRecurWarps], arrived[2];
+  int abort;
+};
 
+template <typename T, bool kDecay, bool kInput, bool kTma>
+__global__ void __launch_bounds__(kRecurThreads, 2)
+recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ RecurMaps maps) {
+  using Tile = RecurTile<T, kL>;
+  constexpr int kIn = kInput ? 3 : 2, kLast = kRecurWarps - 1;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * Tile::kBytes);
+
+  const int cluster = l.cluster, ch = l.ch, half = ch / 2, parts = 64 / ch;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int groups = (p.channels + CH - 1) / CH;
-  const int64_t unit = blockIdx.x / cluster;
-  const int64_t ib = unit / groups;
-  const int c0 = (int)(unit % groups) * CH;
-  const int width = min(CH, p.channels - c0);
-  const int64_t len = recur_length(p.lengths, p.lengths64, ib, p.tokens);
-  const int pair = threadIdx.x % kPairs, slot = threadIdx.x / kPairs;
+  const int groups = (p.channels + ch - 1) / ch;
+  const int64_t ib = blockIdx.x / cluster / groups;
+  const int c0 = (int)(blockIdx.x / cluster % groups) * ch;
+  const int width = min(ch, p.channels - c0);
+  const int len = (int)recur_length(p.lengths, p.lengths64, ib, p.tokens);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int pair = lane & (half - 1), part = lane / half;
   const int c = c0 + 2 * pair;
   const bool live = c < p.channels, second = c + 1 < p.channels;
 
-  const T *rows[3] = {(const T *)p.x.p + ib * p.x.sb + c0, (const T *)p.gate.p + ib * p.gate.sb + c0,
-                      kInput ? (const T *)p.input_gate.p + ib * p.input_gate.sb + c0 : nullptr};
-  const int64_t st[3] = {p.x.st, p.gate.st, p.input_gate.st};
-  const int64_t step = (int64_t)cluster * kTok;
-  const int64_t steps = (len + step - 1) / step;
-  auto fetch = [&](int64_t i, int buf) {
-    if (i < steps) {
+  T *tiles = (T *)smem + warp * kIn * Tile::kElems;  // [kStages][kRecurWarps][kIn][kElems]
+  constexpr int kStageElems = kRecurWarps * kIn * Tile::kElems;
+  const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
+  const int rows = parts * kL;                      // tokens of a warp and step
+  const int step = cluster * kRecurWarps * rows;    // of all
+  const int steps = (len + step - 1) / step;
+  const int first = (rank * kRecurWarps + warp) * rows;
+  auto source = [&](int n) { return (const T *)views[n]->p + ib * views[n]->sb + c0; };
+  // Tiles that the sequence fills; the last one is loaded where it is used.
+  auto fetch = [&](int i, int stage) {
+    const int t0 = i * step + first;
+    if (t0 + rows <= len) {
+      T *tile = tiles + stage * kStageElems;
+      if constexpr (kTma) {
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(&ex.full[stage][warp], kIn * Tile::kBytes);
 #pragma unroll
-      for (int n = 0; n < kIn; ++n)
-        load_tile<T, CH, kL>(tiles + (buf * kIn + n) * Tile::kElems, rows[n], st[n],
-                             i * step + rank * kTok, len, width, copy);
+          for (int n = 0; n < kIn; ++n)
+            tma_load_4d(tile + n * Tile::kElems, &maps.m[n], &ex.full[stage][warp], c0, t0 / kL,
+                            0, (int)ib);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < kIn; ++n)
+          copy_tile<T, kL>(tile + n * Tile::kElems, source(n), views[n]->st, t0, ch, width, l.copy);
+      }
     }
-    copy_commit();
+    if (!kTma) copy_commit();
   };
 
   float2 lambda = two(0.f), carry = two(0.f);
@@ -66,146 +99,174 @@ __global__ void __launch_bounds__(kRecurThreads, 2) recur_fwd_kernel(const Recur
       carry = make_float2(h[0], second ? h[1] : 0.f);
     }
   }
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kRecurWarps; ++w) {
+      for (int j = 0; j < kStages; ++j) tc::mbar_init(&ex.full[j][w], 1);
+      tc::mbar_init(&ex.handed[w], 1);
+    }
+    for (int j = 0; j < 2; ++j) tc::mbar_init(&ex.arrived[j], 1);
+    ex.abort = 0;
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
   if (cluster > 1) cluster_arrive();
-  fetch(0, 0);
-  fetch(1, 1);
-  if (cluster > 1) cluster_wait();  // the peers run before their shared memory is written
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) fetch(j, j);
+  if (cluster > 1) cluster_wait();  // the peers' barriers are there before they are counted on
 
-  const bool pairs = p.pairs;
+  const bool pairs = kTma || p.pairs;
   T *out = (T *)p.out + ib * p.tokens * p.channels + c;
   const int64_t n_check = (p.tokens + kRecurCheck - 1) / kRecurCheck;
-  for (int64_t i = 0; i < steps; ++i) {
-    const int buf = (int)(i & 1);
-    const T *xs = tiles + buf * kIn * Tile::kElems;
-    const T *gs = xs + Tile::kElems, *us = gs + Tile::kElems;
-    const int64_t t0 = i * step + rank * kTok + slot * kL;
-    copy_wait<1>();
-    __syncthreads();
-    // tokens beyond the sequence (zero in the tile) keep the state: an infinite
-    // gate of the sign that forgets nothing
-    const int inside = (int)max64(0, min64(kL, len - t0));
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int i = 0; i < steps; ++i) {
+    const int buf = i & 1;
+    T *xs = tiles + stage * kStageElems;
+    T *gs = xs + Tile::kElems, *us = gs + Tile::kElems;
+    const int row0 = i * step + first, t0 = row0 + part * kL;
+    const bool whole = row0 + rows <= len;
+    if (whole) {
+      if constexpr (kTma) tc::mbar_wait(&ex.full[stage][warp], phase, &ex.abort);
+      else copy_wait<kStages - 1>();
+    } else {
+      // tokens beyond the sequence keep the state
+      ragged_tile<T, kL>(xs, source(0), views[0]->st, row0, len, ch, width, 0.f);
+      ragged_tile<T, kL>(gs, source(1), views[1]->st, row0, len, ch, width,
+                         kDecay ? -INFINITY : INFINITY);
+      if (kInput) ragged_tile<T, kL>(us, source(2), views[2]->st, row0, len, ch, width, 0.f);
+    }
+    if (!kTma || !whole) __syncwarp();
     float2 am1[kL], b[kL];
-    float2 sum = two(kDecay ? 0.f : 1.f), e = two(0.f);
+    float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f);
 #pragma unroll
     for (int k = 0; k < kL; ++k) {
-      const int at = Tile::at(slot * kL + k) + 2 * pair;
-      float2 g = load_two(gs + at);
-      if (k >= inside) g = two(kDecay ? -INFINITY : INFINITY);
-      const Gates y = gates_of<T, kInput>(g, kInput ? load_two(us + at) : two(0.f));
-      float2 beta, beta2;
-      decay_of<T, kDecay>(y, lambda, am1[k], beta, beta2);
-      if (kInput) beta = __fmul2_rn(beta, y.u);
-      b[k] = __fmul2_rn(beta, load_two(xs + at));
+      const int at = 64 * k + 2 * lane;
+      const Token y = token_of<T, kDecay, kInput, false>(
+          load_two(gs + at), kInput ? load_two(us + at) : two(0.f), lambda);
+      am1[k] = y.am1;
+      b[k] = __fmul2_rn(y.bu, load_two(xs + at));
       e = __fadd2_rn(__ffma2_rn(am1[k], e, e), b[k]);
-      sum = kDecay ? __fadd2_rn(sum, y.s) : __fmul2_rn(sum, y.s);
+      a = kDecay ? __fadd2_rn(a, y.s) : __fmul2_rn(a, y.s);
     }
     if (kDecay) {
-      sum = __fmul2_rn(sum, lambda);
-      sum = make_float2(Fn<T>::exp(sum.x), Fn<T>::exp(sum.y));
+      a = __fmul2_rn(a, lambda);
+      a = make_float2(Fn<T>::exp(a.x), Fn<T>::exp(a.y));
     }
-    sums[buf][slot][pair] = make_float4(sum.x, sum.y, e.x, e.y);
-    __syncthreads();
-    fetch(i + 2, buf);
+    __syncwarp();  // the rows are read
+    fetch(i + kStages, stage);
+    if (++stage == kStages) stage = 0, phase ^= 1;
 
-    float2 h = carry;  // the state before this thread's tokens
+    const Summary own = join_parts<false>(a, e, half, lane);
+    float2 h;  // the state before this thread's tokens
     if (cluster == 1) {
-#pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
-        if (j == slot) h = carry;
-        const float4 v = sums[buf][j][pair];
-        carry = __ffma2_rn(make_float2(v.x, v.y), carry, make_float2(v.z, v.w));
+      if (warp > 0 || i > 0) {
+        tc::mbar_wait(&ex.handed[warp], (uint32_t)(warp > 0 ? i : i - 1) & 1, &ex.abort);
+        const float4 v = ex.before[warp][pair];
+        carry = make_float2(v.x, v.y);
       }
+      h = __ffma2_rn(own.a, carry, own.e);
+      carry = __ffma2_rn(a, carry, e);
+      const int next = warp == kLast ? 0 : warp + 1;
+      if (part == 0) *(float2 *)&ex.before[next][pair] = carry;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ex.handed[next]);
     } else {
-      float2 a = two(1.f), a_own = two(1.f), e_own = two(0.f);
-      e = two(0.f);
-#pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
-        if (j == slot) a_own = a, e_own = e;
-        const float4 v = sums[buf][j][pair];
-        e = __ffma2_rn(make_float2(v.x, v.y), e, make_float2(v.z, v.w));
-        a = __fmul2_rn(a, make_float2(v.x, v.y));
+      float2 ap = two(1.f), ep = two(0.f);  // of the CTA's warps before
+      if (warp > 0) {
+        tc::mbar_wait(&ex.handed[warp], (uint32_t)i & 1, &ex.abort);
+        const float4 v = ex.before[warp][pair];
+        ap = make_float2(v.x, v.y), ep = make_float2(v.z, v.w);
       }
-      if (slot < cluster)
-        store_remote(&csums[buf][rank][pair], (uint32_t)slot, make_float4(a.x, a.y, e.x, e.y));
-      cluster_arrive();
-      cluster_wait();
+      e = __ffma2_rn(a, ep, e);
+      a = __fmul2_rn(a, ap);
+      const float4 sum = make_float4(a.x, a.y, e.x, e.y);
+      if (warp < kLast) {
+        if (part == 0) ex.before[warp + 1][pair] = sum;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ex.handed[warp + 1]);
+      } else {  // the CTA's summary, to all of the cluster
+        if (lane == 0)
+          tc::mbar_arrive_expect_tx(&ex.arrived[buf], cluster * half * sizeof(float4));
+        if (part == 0)
+          for (int j = 0; j < cluster; ++j)
+            store_remote(&ex.csums[buf][rank][pair], &ex.arrived[buf], (uint32_t)j, sum);
+      }
+      tc::mbar_wait(&ex.arrived[buf], (uint32_t)(i >> 1) & 1, &ex.abort);
       for (int j = 0; j < cluster; ++j) {
         if (j == rank) h = carry;
-        const float4 v = csums[buf][j][pair];
+        const float4 v = ex.csums[buf][j][pair];
         carry = __ffma2_rn(make_float2(v.x, v.y), carry, make_float2(v.z, v.w));
       }
-      h = __ffma2_rn(a_own, h, e_own);
+      h = __ffma2_rn(ap, h, ep);
+      h = __ffma2_rn(own.a, h, own.e);
     }
-    if (p.check && live && inside > 0 && (t0 & (kRecurCheck - 1)) == 0)
+    static_assert(kL == kRecurCheck, "every thread saves the state before its tokens");
+    if (p.check && live && t0 < len)
       store_two(p.check + (ib * n_check + t0 / kRecurCheck) * p.channels + c, h, pairs, second);
-    T *dst = out + t0 * p.channels;
+    T *dst = out + (int64_t)t0 * p.channels;
+    if (!live) continue;
+    if (pairs && whole) {
 #pragma unroll
-    for (int k = 0; k < kL; ++k) {
-      h = __fadd2_rn(__ffma2_rn(am1[k], h, h), b[k]);
-      if (live && k < inside) store_two(dst, h, pairs, second);
-      dst += p.channels;
+      for (int k = 0; k < kL; ++k) {
+        h = __fadd2_rn(__ffma2_rn(am1[k], h, h), b[k]);
+        store_two(dst + (int64_t)k * p.channels, h, true, true);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kL; ++k) {
+        h = __fadd2_rn(__ffma2_rn(am1[k], h, h), b[k]);
+        if (t0 + k < len) store_two(dst + (int64_t)k * p.channels, h, pairs, second);
+      }
     }
   }
-  if (p.final_state && rank == 0 && slot == 0 && live)
+  if (p.final_state && rank == 0 && warp == kLast && part == 0 && live)
     store_two(p.final_state + ib * p.channels + c, carry, pairs, second);
   // zeros behind the sequence
-  for (int64_t t = len + rank * kSlots + slot; t < p.tokens && live; t += cluster * kSlots)
+  const int slots = kRecurWarps * parts;
+  for (int64_t t = len + rank * slots + warp * parts + part; t < p.tokens && live; t += cluster * slots)
     store_two(out + t * p.channels, two(0.f), pairs, second);
+  if (ex.abort) {
+    if (l.err) *l.err = tc::kErrTimeout;
+    const uint64_t since = tc::globaltimer();  // copies in flight still write into this CTA
+    while (tc::globaltimer() - since < tc::kWaitTimeoutNs) __nanosleep(1000);
+  }
 }
 
-template <typename T, int CH, bool kDecay, bool kInput>
-int launch(const RecurCall &p, int cluster, cudaStream_t s) {
-  using Tile = RecurTile<T, CH, kL>;
-  const int smem = 2 * (kInput ? 3 : 2) * Tile::kBytes;
-  auto kernel = recur_fwd_kernel<T, CH, kDecay, kInput>;
+template <typename T, bool kDecay, bool kInput, bool kTma>
+int launch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
+  constexpr int dtype = sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16;
+  constexpr int kIn = kInput ? 3 : 2;
+  const int smem = kStages * kIn * kRecurWarps * RecurTile<T, kL>::kBytes + (int)sizeof(Exchange);
+  auto kernel = recur_fwd_kernel<T, kDecay, kInput, kTma>;
   const int st = allow_dynamic_smem((const void *)kernel, smem);
   if (st != LA_OK) return st;
-  int copy = copy_bytes(p.x, sizeof(T)) < copy_bytes(p.gate, sizeof(T)) ? copy_bytes(p.x, sizeof(T))
-                                                                        : copy_bytes(p.gate, sizeof(T));
-  if (kInput && copy_bytes(p.input_gate, sizeof(T)) < copy) copy = copy_bytes(p.input_gate, sizeof(T));
-  const int64_t grid = p.batch * ((p.channels + CH - 1) / CH) * cluster;
-  if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kRecurThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, p, cluster, copy);
-  return check_launch();
+  const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
+  RecurLaunch l{shape.ch, shape.cluster, 16, device_error_word()};
+  RecurMaps maps;
+  for (int n = 0; n < kIn; ++n) {
+    if (kTma && !recur_map(&maps.m[n], *views[n], p, dtype, shape.ch, kL)) return LA_ERR_CUDA;
+    l.copy = min(l.copy, copy_bytes(*views[n], sizeof(T)));
+  }
+  return launch_clusters(kernel, p, l, maps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
-int launch_by_size(const RecurCall &p, cudaStream_t s) {
+int launch_by_view(const RecurCall &p, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  // Two CTAs per SM, by as many CTAs along the tokens as they have tiles for;
-  // 32 channels where that leaves SMs idle.
-  auto cluster_for = [&](int ch, int tokens) {
-    const int64_t units = p.batch * ((p.channels + ch - 1) / ch);
-    int k = 1;
-    while (k < kRecurMaxCluster && units * k * 2 <= 2 * info.sm_count && p.tokens > (int64_t)k * tokens)
-      k *= 2;
-    return k;
-  };
-  const int wide = cluster_for(64, RecurTile<T, 64, kL>::kTokens);
-  const int64_t ctas = p.batch * ((p.channels + 63) / 64) * wide;
-  if (ctas <= info.sm_count && p.channels > 32)
-    return launch<T, 32, kDecay, kInput>(p, cluster_for(32, RecurTile<T, 32, kL>::kTokens), s);
-  return launch<T, 64, kDecay, kInput>(p, wide, s);
+  const RecurShape shape = recur_shape(p.batch, p.tokens, p.channels, info.sm_count, kL, 64);
+  const bool tma = recur_tma_view(p.x, p, sizeof(T)) && recur_tma_view(p.gate, p, sizeof(T)) &&
+                   recur_tma_view(p.input_gate, p, sizeof(T)) && p.pairs && p.tokens >= kL && encode_fn();
+  return tma ? launch<T, kDecay, kInput, true>(p, shape, s)
+             : launch<T, kDecay, kInput, false>(p, shape, s);
 }
 
 template <typename T>
 int launch_typed(const RecurCall &p, cudaStream_t s) {
   if (p.log_decay)
-    return p.input_gate.p ? launch_by_size<T, true, true>(p, s) : launch_by_size<T, true, false>(p, s);
-  return p.input_gate.p ? launch_by_size<T, false, true>(p, s) : launch_by_size<T, false, false>(p, s);
+    return p.input_gate.p ? launch_by_view<T, true, true>(p, s) : launch_by_view<T, true, false>(p, s);
+  return p.input_gate.p ? launch_by_view<T, false, true>(p, s) : launch_by_view<T, false, false>(p, s);
 }
 
 }  // namespace

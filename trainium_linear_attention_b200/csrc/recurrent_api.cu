@@ -45,7 +45,7 @@ int64_t check_rows(int64_t tokens) { return (tokens + kRecurCheck - 1) / kRecurC
 
 int check_sizes(int64_t batch, int64_t tokens, int64_t channels, int dtype) {
   if (batch < 0 || tokens < 0 || channels < 1 || !valid_type(dtype)) return LA_ERR_INVALID_ARGUMENT;
-  if (channels > INT32_MAX / 8 || !fits(batch, tokens, channels)) return LA_ERR_UNSUPPORTED;
+  if (channels > INT32_MAX / 8 || tokens > INT32_MAX / 2 || !fits(batch, tokens, channels)) return LA_ERR_UNSUPPORTED;
   return LA_OK;
 }
 

@@ -53,12 +53,10 @@ __global__ void __launch_bounds__(kThreads) recur_step_kernel(const RecurStep p)
 #pragma unroll
   for (int e = 0; e < kVec; e += 2) {
     const int f = e + 1 < kVec ? e + 1 : e;
-    const Gates y = gates_of<T, kInput>(make_float2(g[e], g[f]), make_float2(u[e], u[f]));
-    float2 am1, beta, beta2;
-    decay_of<T, kDecay>(y, make_float2(lambda[e], lambda[f]), am1, beta, beta2);
-    if (kInput) beta = __fmul2_rn(beta, y.u);
+    const Token y = token_of<T, kDecay, kInput, false>(
+        make_float2(g[e], g[f]), make_float2(u[e], u[f]), make_float2(lambda[e], lambda[f]));
     const float2 old = make_float2(h[e], h[f]);
-    const float2 now = __fadd2_rn(__ffma2_rn(am1, old, old), __fmul2_rn(beta, make_float2(x[e], x[f])));
+    const float2 now = __ffma2_rn(y.bu, make_float2(x[e], x[f]), __ffma2_rn(y.am1, old, old));
     h[e] = now.x;
     if (f != e) h[f] = now.y;
   }
