@@ -40,64 +40,48 @@ struct Exchange {
   int abort;
 };
 
-template <typename T, bool kDecay, bool kInput, bool kTma>
+template <typename T, bool kDecay, bool kInput, Fetch kF>
 __global__ void __launch_bounds__(kRecurThreads, 2)
-recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ RecurMaps maps) {
-  using Tile = RecurTile<T, kL>;
+recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ TileMaps maps) {
   constexpr int kIn = kInput ? 4 : 3, kLast = kRecurWarps - 1;
   static_assert(kRecurCheck == 2 * kL, "every other part starts at a saved state");
   extern __shared__ __align__(1024) uint8_t smem[];
-  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * Tile::kBytes);
-
   column_sum_may_start();
-  const int cluster = l.cluster, ch = l.ch, half = ch / 2, parts = 64 / ch;
+  const int cluster = l.cluster, ch = l.tile.ch, half = ch / 2, parts = 64 / ch;
+  const int channels = p.sizes.channels;
+  const int elems = tile_elems<kF>(kL, ch);
+  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * elems * sizeof(T));
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int groups = (p.channels + ch - 1) / ch;
+  const int groups = (channels + ch - 1) / ch;
   const int64_t ib = blockIdx.x / cluster / groups;
   const int c0 = (int)(blockIdx.x / cluster % groups) * ch;
-  const int width = min(ch, p.channels - c0);
-  const int len = (int)recur_length(p.lengths, p.lengths64, ib, p.tokens);
+  const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.sizes.tokens);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int pair = lane & (half - 1), part = lane / half;
   const int c = c0 + 2 * pair;
-  const bool live = c < p.channels, second = c + 1 < p.channels;
+  const bool live = c < channels, second = c + 1 < channels;
 
-  T *tiles = (T *)smem + warp * kIn * Tile::kElems;  // [kStages][kRecurWarps][kIn][kElems]
-  constexpr int kStageElems = kRecurWarps * kIn * Tile::kElems;
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
+  WarpTiles<T, kL, kIn, kStages, kF> tiles{
+      (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
   const int rows = parts * kL;            // tokens of a warp and step
   const int block_rows = kRecurWarps * rows;
   const int blocks = (len + block_rows - 1) / block_rows;
   const int steps = (blocks + cluster - 1) / cluster;
-  auto source = [&](int n) { return (const T *)views[n]->p + ib * views[n]->sb + c0; };
   auto block_of = [&](int i) { return blocks - 1 - (i * cluster + rank); };  // < 0: none
   // Tiles that the sequence fills; the last one is loaded where it is used.
   auto fetch = [&](int i, int stage) {
     const int t0 = block_of(i) * block_rows + warp * rows;
-    if (i < steps && t0 >= 0 && t0 + rows <= len) {
-      T *tile = tiles + stage * kStageElems;
-      if constexpr (kTma) {
-        if (lane == 0) {
-          tc::mbar_arrive_expect_tx(&ex.full[stage][warp], kIn * Tile::kBytes);
-#pragma unroll
-          for (int n = 0; n < kIn; ++n)
-            tma_load_4d(tile + n * Tile::kElems, &maps.m[n], &ex.full[stage][warp], c0, t0 / kL,
-                            0, (int)ib);
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < kIn; ++n)
-          copy_tile<T, kL>(tile + n * Tile::kElems, source(n), views[n]->st, t0, ch, width, l.copy);
-      }
-    }
-    if (!kTma) copy_commit();
+    if (i < steps && t0 >= 0 && t0 + rows <= len) tiles.fetch(t0, stage);
+    tiles.commit();
   };
 
   float2 lambda = two(0.f), carry = two(0.f), d_lambda = two(0.f);
   if (live) {
     if (kDecay) lambda = make_float2(p.log_decay[c], second ? p.log_decay[c + 1] : 0.f);
     if (p.d_final) {
-      const float *h = p.d_final + ib * p.channels + c;
+      const float *h = p.d_final + ib * channels + c;
       carry = make_float2(h[0], second ? h[1] : 0.f);
     }
   }
@@ -116,45 +100,38 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   for (int j = 0; j < kStages; ++j) fetch(j, j);
   if (cluster > 1) cluster_wait();  // the peers' barriers are there before they are counted on
 
-  const bool pairs = kTma || p.pairs;
-  const int64_t n_check = (p.tokens + kRecurCheck - 1) / kRecurCheck;
-  const int64_t origin = ib * p.tokens * p.channels + c;
+  const bool pairs = kF == Fetch::kTma || p.pairs;
+  const int64_t n_check = (p.sizes.tokens + kRecurCheck - 1) / kRecurCheck;
+  const int64_t origin = ib * p.sizes.tokens * channels + c;
   // The saved state at or before this thread's tokens of a step; loaded a step ahead.
   auto saved = [&](int i) {
     const int t0 = block_of(i) * block_rows + warp * rows + part * kL;
     if (t0 < 0 || t0 >= len || !live) return two(0.f);
-    const float *v = p.check + (ib * n_check + t0 / kRecurCheck) * p.channels + c;
+    const float *v = p.check + (ib * n_check + t0 / kRecurCheck) * channels + c;
     return make_float2(v[0], second ? v[1] : 0.f);
   };
   float2 start = saved(0);
   int stage = 0;
-  uint32_t phases = 0;  // a bit per stage
   for (int i = 0; i < steps; ++i) {
     const int buf = i & 1;
-    T *xs = tiles + stage * kStageElems;
-    T *gs = xs + Tile::kElems, *ds = gs + Tile::kElems, *us = ds + Tile::kElems;
+    const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *ds = tiles.tile(stage, 2),
+            *us = tiles.tile(stage, kIn - 1);
     const int block = block_of(i);
     const int row0 = block * block_rows + warp * rows, t0 = row0 + part * kL;
     const bool whole = block >= 0 && row0 + rows <= len;
     float2 h = start;
     start = saved(i + 1);
     if (whole) {
-      if constexpr (kTma) {
-        tc::mbar_wait(&ex.full[stage][warp], phases >> stage & 1, &ex.abort);
-        phases ^= 1u << stage;
-      } else {
-        copy_wait<kStages - 1>();
-      }
+      tiles.wait(row0, stage, &ex.abort);
     } else {
       // tokens outside the sequence keep the state and the gradient
-      ragged_tile<T, kL>(xs, source(0), views[0]->st, row0, len, ch, width, 0.f);
-      ragged_tile<T, kL>(gs, source(1), views[1]->st, row0, len, ch, width,
-                         kDecay ? -INFINITY : INFINITY);
-      ragged_tile<T, kL>(ds, source(2), views[2]->st, row0, len, ch, width, 0.f);
-      if (kInput) ragged_tile<T, kL>(us, source(3), views[3]->st, row0, len, ch, width, 0.f);
-      if (kTma) tc::fence_proxy_async_smem();  // ahead of the next copy into this tile
+      tiles.load_ragged(row0, len, stage, 0, 0.f);
+      tiles.load_ragged(row0, len, stage, 1, kDecay ? -INFINITY : INFINITY);
+      tiles.load_ragged(row0, len, stage, 2, 0.f);
+      if (kInput) tiles.load_ragged(row0, len, stage, 3, 0.f);
+      if (kF == Fetch::kTma) tc::fence_proxy_async_smem();  // ahead of the next copy into this tile
+      __syncwarp();
     }
-    if (!kTma || !whole) __syncwarp();
     float2 am1[kL], bu[kL], s[kL], sc[kL], uc[kL];
     float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f), r = two(0.f);
 #pragma unroll
@@ -232,7 +209,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
       g = __ffma2_rn(ap, g, rp);
     }
     g = __ffma2_rn(rest.a, g, rest.e);
-    const int64_t o = origin + (int64_t)t0 * p.channels;
+    const int64_t o = origin + (int64_t)t0 * channels;
     T *dx = (T *)p.dx + o, *dg = (T *)p.d_gate + o, *di = kInput ? (T *)p.d_input + o : nullptr;
     auto finish = [&](auto all) {
 #pragma unroll
@@ -260,7 +237,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
                            __ffma2_rn(b, two(-1.f), __fmul2_rn(sc[k], before[k])));
         }
         if (all || (block >= 0 && t0 + k < len)) {
-          const int64_t at_k = (int64_t)k * p.channels;
+          const int64_t at_k = (int64_t)k * channels;
           store_two(dx + at_k, dxk, all || pairs, second);
           store_two(dg + at_k, dgk, all || pairs, second);
           if constexpr (kInput) store_two(di + at_k, dik, all || pairs, second);
@@ -276,10 +253,10 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     if (++stage == kStages) stage = 0;
   }
   if (p.d_init && rank == 0 && warp == 0 && part == 0 && live)
-    store_two(p.d_init + ib * p.channels + c, carry, pairs, second);
+    store_two(p.d_init + ib * channels + c, carry, pairs, second);
   const int slots = kRecurWarps * parts;
-  for (int64_t t = len + rank * slots + warp * parts + part; t < p.tokens && live; t += cluster * slots) {
-    const int64_t o = origin + t * p.channels;
+  for (int64_t t = len + rank * slots + warp * parts + part; t < p.sizes.tokens && live; t += cluster * slots) {
+    const int64_t o = origin + t * channels;
     store_two((T *)p.dx + o, two(0.f), pairs, second);
     store_two((T *)p.d_gate + o, two(0.f), pairs, second);
     if (kInput) store_two((T *)p.d_input + o, two(0.f), pairs, second);
@@ -296,67 +273,62 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
       float2 v = two(0.f);
 #pragma unroll
       for (int j = 0; j < kRecurWarps; ++j) v = __fadd2_rn(v, ex.sums[j][pair]);
-      store_two(p.partial + (ib * cluster + rank) * p.channels + c, v, p.channels % 2 == 0, second);
+      store_two(p.partial + (ib * cluster + rank) * channels + c, v, channels % 2 == 0, second);
     }
   }
   if (ex.abort) {
-    if (l.err) *l.err = tc::kErrTimeout;
+    if (l.tile.err) *l.tile.err = tc::kErrTimeout;
     const uint64_t since = tc::globaltimer();  // copies in flight still write into this CTA
     while (tc::globaltimer() - since < tc::kWaitTimeoutNs) __nanosleep(1000);
   }
 }
 
-RecurShape shape_of(int64_t batch, int64_t tokens, int channels, int sm_count) {
-  return recur_shape(batch, tokens, channels, sm_count, kL, 32);
-}
+RecurShape shape_of(const TokenSizes &z, int sm_count) { return recur_shape(z, sm_count, kL, 32); }
 
-template <typename T, bool kDecay, bool kInput, bool kTma>
-int launch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
-  constexpr int dtype = sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16;
+template <typename T, bool kDecay, bool kInput, Fetch kF>
+int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
   constexpr int kIn = kInput ? 4 : 3;
-  const int smem = kStages * kIn * kRecurWarps * RecurTile<T, kL>::kBytes + (int)sizeof(Exchange);
-  auto kernel = recur_bwd_kernel<T, kDecay, kInput, kTma>;
-  const int st = allow_dynamic_smem((const void *)kernel, smem);
-  if (st != LA_OK) return st;
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
-  RecurLaunch l{shape.ch, shape.cluster, 16, device_error_word()};
-  RecurMaps maps;
-  for (int n = 0; n < kIn; ++n) {
-    if (kTma && !recur_map(&maps.m[n], *views[n], p, dtype, shape.ch, kL)) return LA_ERR_CUDA;
-    l.copy = min(l.copy, copy_bytes(*views[n], sizeof(T)));
-  }
-  return launch_clusters(kernel, p, l, maps, smem, s);
+  TileMaps maps;
+  for (int n = 0; kF == Fetch::kTma && n < kIn; ++n)
+    if (!tile_map(&maps.m[n], *views[n], p.sizes, sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16,
+                  l.tile.ch, kL))
+      return LA_ERR_CUDA;
+  const int smem = kStages * kIn * kRecurWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
+                   (int)sizeof(Exchange);
+  return launch_clusters(recur_bwd_kernel<T, kDecay, kInput, kF>, p, l, maps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
-int launch_by_view(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
-  const bool tma = recur_tma_view(p.x, p, sizeof(T)) && recur_tma_view(p.gate, p, sizeof(T)) &&
-                   recur_tma_view(p.d_out, p, sizeof(T)) &&
-                   recur_tma_view(p.input_gate, p, sizeof(T)) && p.pairs && p.tokens >= kL && encode_fn();
-  return tma ? launch<T, kDecay, kInput, true>(p, shape, s)
-             : launch<T, kDecay, kInput, false>(p, shape, s);
+int launch_by_fetch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
+  RecurLaunch l{{shape.ch, 0, device_error_word()}, shape.cluster};
+  const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
+  const Fetch f = recur_fetch(p, views, 4, sizeof(T), kL, &l.tile.copy);
+  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
+  if constexpr (sizeof(T) == 2) {
+    if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);
+  }
+  return launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
 }
 
 template <typename T>
 int launch_typed(const RecurCall &p, const RecurShape &sh, cudaStream_t s) {
   if (p.log_decay)
-    return p.input_gate.p ? launch_by_view<T, true, true>(p, sh, s)
-                          : launch_by_view<T, true, false>(p, sh, s);
-  return p.input_gate.p ? launch_by_view<T, false, true>(p, sh, s)
-                        : launch_by_view<T, false, false>(p, sh, s);
+    return p.input_gate.p ? launch_by_fetch<T, true, true>(p, sh, s)
+                          : launch_by_fetch<T, true, false>(p, sh, s);
+  return p.input_gate.p ? launch_by_fetch<T, false, true>(p, sh, s)
+                        : launch_by_fetch<T, false, false>(p, sh, s);
 }
 
 }  // namespace
 
-int recur_bwd_rows(int64_t batch, int64_t tokens, int channels, int sm_count) {
-  return shape_of(batch, tokens, channels, sm_count).cluster;
-}
+int recur_bwd_rows(const TokenSizes &z, int sm_count) { return shape_of(z, sm_count).cluster; }
 
 int launch_recur_bwd(const RecurCall &p, int dtype, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  const RecurShape sh = shape_of(p.batch, p.tokens, p.channels, info.sm_count);
+  const RecurShape sh = shape_of(p.sizes, info.sm_count);
   return dtype == LA_DTYPE_FLOAT32 ? launch_typed<float>(p, sh, s)
                                    : launch_typed<__nv_bfloat16>(p, sh, s);
 }

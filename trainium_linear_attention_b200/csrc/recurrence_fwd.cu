@@ -41,61 +41,45 @@ struct Exchange {
   int abort;
 };
 
-template <typename T, bool kDecay, bool kInput, bool kTma>
+template <typename T, bool kDecay, bool kInput, Fetch kF>
 __global__ void __launch_bounds__(kRecurThreads, 2)
-recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ RecurMaps maps) {
-  using Tile = RecurTile<T, kL>;
+recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ TileMaps maps) {
   constexpr int kIn = kInput ? 3 : 2, kLast = kRecurWarps - 1;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * Tile::kBytes);
-
-  const int cluster = l.cluster, ch = l.ch, half = ch / 2, parts = 64 / ch;
+  const int cluster = l.cluster, ch = l.tile.ch, half = ch / 2, parts = 64 / ch;
+  const int channels = p.sizes.channels;
+  const int elems = tile_elems<kF>(kL, ch);
+  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * elems * sizeof(T));
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int groups = (p.channels + ch - 1) / ch;
+  const int groups = (channels + ch - 1) / ch;
   const int64_t ib = blockIdx.x / cluster / groups;
   const int c0 = (int)(blockIdx.x / cluster % groups) * ch;
-  const int width = min(ch, p.channels - c0);
-  const int len = (int)recur_length(p.lengths, p.lengths64, ib, p.tokens);
+  const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.sizes.tokens);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int pair = lane & (half - 1), part = lane / half;
   const int c = c0 + 2 * pair;
-  const bool live = c < p.channels, second = c + 1 < p.channels;
+  const bool live = c < channels, second = c + 1 < channels;
 
-  T *tiles = (T *)smem + warp * kIn * Tile::kElems;  // [kStages][kRecurWarps][kIn][kElems]
-  constexpr int kStageElems = kRecurWarps * kIn * Tile::kElems;
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
+  WarpTiles<T, kL, kIn, kStages, kF> tiles{
+      (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
   const int rows = parts * kL;                      // tokens of a warp and step
   const int step = cluster * kRecurWarps * rows;    // of all
   const int steps = (len + step - 1) / step;
   const int first = (rank * kRecurWarps + warp) * rows;
-  auto source = [&](int n) { return (const T *)views[n]->p + ib * views[n]->sb + c0; };
   // Tiles that the sequence fills; the last one is loaded where it is used.
   auto fetch = [&](int i, int stage) {
     const int t0 = i * step + first;
-    if (t0 + rows <= len) {
-      T *tile = tiles + stage * kStageElems;
-      if constexpr (kTma) {
-        if (lane == 0) {
-          tc::mbar_arrive_expect_tx(&ex.full[stage][warp], kIn * Tile::kBytes);
-#pragma unroll
-          for (int n = 0; n < kIn; ++n)
-            tma_load_4d(tile + n * Tile::kElems, &maps.m[n], &ex.full[stage][warp], c0, t0 / kL,
-                            0, (int)ib);
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < kIn; ++n)
-          copy_tile<T, kL>(tile + n * Tile::kElems, source(n), views[n]->st, t0, ch, width, l.copy);
-      }
-    }
-    if (!kTma) copy_commit();
+    if (t0 + rows <= len) tiles.fetch(t0, stage);
+    tiles.commit();
   };
 
   float2 lambda = two(0.f), carry = two(0.f);
   if (live) {
     if (kDecay) lambda = make_float2(p.log_decay[c], second ? p.log_decay[c + 1] : 0.f);
     if (p.init) {
-      const float *h = p.init + ib * p.channels + c;
+      const float *h = p.init + ib * channels + c;
       carry = make_float2(h[0], second ? h[1] : 0.f);
     }
   }
@@ -114,28 +98,24 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   for (int j = 0; j < kStages; ++j) fetch(j, j);
   if (cluster > 1) cluster_wait();  // the peers' barriers are there before they are counted on
 
-  const bool pairs = kTma || p.pairs;
-  T *out = (T *)p.out + ib * p.tokens * p.channels + c;
-  const int64_t n_check = (p.tokens + kRecurCheck - 1) / kRecurCheck;
+  const bool pairs = kF == Fetch::kTma || p.pairs;
+  T *out = (T *)p.out + ib * p.sizes.tokens * channels + c;
+  const int64_t n_check = (p.sizes.tokens + kRecurCheck - 1) / kRecurCheck;
   int stage = 0;
-  uint32_t phase = 0;
   for (int i = 0; i < steps; ++i) {
     const int buf = i & 1;
-    T *xs = tiles + stage * kStageElems;
-    T *gs = xs + Tile::kElems, *us = gs + Tile::kElems;
+    const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *us = tiles.tile(stage, kIn - 1);
     const int row0 = i * step + first, t0 = row0 + part * kL;
     const bool whole = row0 + rows <= len;
     if (whole) {
-      if constexpr (kTma) tc::mbar_wait(&ex.full[stage][warp], phase, &ex.abort);
-      else copy_wait<kStages - 1>();
+      tiles.wait(row0, stage, &ex.abort);
     } else {
       // tokens beyond the sequence keep the state
-      ragged_tile<T, kL>(xs, source(0), views[0]->st, row0, len, ch, width, 0.f);
-      ragged_tile<T, kL>(gs, source(1), views[1]->st, row0, len, ch, width,
-                         kDecay ? -INFINITY : INFINITY);
-      if (kInput) ragged_tile<T, kL>(us, source(2), views[2]->st, row0, len, ch, width, 0.f);
+      tiles.load_ragged(row0, len, stage, 0, 0.f);
+      tiles.load_ragged(row0, len, stage, 1, kDecay ? -INFINITY : INFINITY);
+      if (kInput) tiles.load_ragged(row0, len, stage, 2, 0.f);
+      __syncwarp();
     }
-    if (!kTma || !whole) __syncwarp();
     float2 am1[kL], b[kL];
     float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f);
 #pragma unroll
@@ -154,7 +134,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     }
     __syncwarp();  // the rows are read
     fetch(i + kStages, stage);
-    if (++stage == kStages) stage = 0, phase ^= 1;
+    if (++stage == kStages) stage = 0;
 
     const Summary own = join_parts<false>(a, e, half, lane);
     float2 h;  // the state before this thread's tokens
@@ -202,71 +182,71 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     }
     static_assert(kL == kRecurCheck, "every thread saves the state before its tokens");
     if (p.check && live && t0 < len)
-      store_two(p.check + (ib * n_check + t0 / kRecurCheck) * p.channels + c, h, pairs, second);
-    T *dst = out + (int64_t)t0 * p.channels;
+      store_two(p.check + (ib * n_check + t0 / kRecurCheck) * channels + c, h, pairs, second);
+    T *dst = out + (int64_t)t0 * channels;
     if (!live) continue;
     if (pairs && whole) {
 #pragma unroll
       for (int k = 0; k < kL; ++k) {
         h = __fadd2_rn(__ffma2_rn(am1[k], h, h), b[k]);
-        store_two(dst + (int64_t)k * p.channels, h, true, true);
+        store_two(dst + (int64_t)k * channels, h, true, true);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kL; ++k) {
         h = __fadd2_rn(__ffma2_rn(am1[k], h, h), b[k]);
-        if (t0 + k < len) store_two(dst + (int64_t)k * p.channels, h, pairs, second);
+        if (t0 + k < len) store_two(dst + (int64_t)k * channels, h, pairs, second);
       }
     }
   }
   if (p.final_state && rank == 0 && warp == kLast && part == 0 && live)
-    store_two(p.final_state + ib * p.channels + c, carry, pairs, second);
+    store_two(p.final_state + ib * channels + c, carry, pairs, second);
   // zeros behind the sequence
   const int slots = kRecurWarps * parts;
-  for (int64_t t = len + rank * slots + warp * parts + part; t < p.tokens && live; t += cluster * slots)
-    store_two(out + t * p.channels, two(0.f), pairs, second);
+  for (int64_t t = len + rank * slots + warp * parts + part; t < p.sizes.tokens && live; t += cluster * slots)
+    store_two(out + t * channels, two(0.f), pairs, second);
   if (ex.abort) {
-    if (l.err) *l.err = tc::kErrTimeout;
+    if (l.tile.err) *l.tile.err = tc::kErrTimeout;
     const uint64_t since = tc::globaltimer();  // copies in flight still write into this CTA
     while (tc::globaltimer() - since < tc::kWaitTimeoutNs) __nanosleep(1000);
   }
 }
 
-template <typename T, bool kDecay, bool kInput, bool kTma>
-int launch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
-  constexpr int dtype = sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16;
+template <typename T, bool kDecay, bool kInput, Fetch kF>
+int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
   constexpr int kIn = kInput ? 3 : 2;
-  const int smem = kStages * kIn * kRecurWarps * RecurTile<T, kL>::kBytes + (int)sizeof(Exchange);
-  auto kernel = recur_fwd_kernel<T, kDecay, kInput, kTma>;
-  const int st = allow_dynamic_smem((const void *)kernel, smem);
-  if (st != LA_OK) return st;
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
-  RecurLaunch l{shape.ch, shape.cluster, 16, device_error_word()};
-  RecurMaps maps;
-  for (int n = 0; n < kIn; ++n) {
-    if (kTma && !recur_map(&maps.m[n], *views[n], p, dtype, shape.ch, kL)) return LA_ERR_CUDA;
-    l.copy = min(l.copy, copy_bytes(*views[n], sizeof(T)));
-  }
-  return launch_clusters(kernel, p, l, maps, smem, s);
+  TileMaps maps;
+  for (int n = 0; kF == Fetch::kTma && n < kIn; ++n)
+    if (!tile_map(&maps.m[n], *views[n], p.sizes, sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16,
+                  l.tile.ch, kL))
+      return LA_ERR_CUDA;
+  const int smem = kStages * kIn * kRecurWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
+                   (int)sizeof(Exchange);
+  return launch_clusters(recur_fwd_kernel<T, kDecay, kInput, kF>, p, l, maps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
-int launch_by_view(const RecurCall &p, cudaStream_t s) {
+int launch_by_fetch(const RecurCall &p, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  const RecurShape shape = recur_shape(p.batch, p.tokens, p.channels, info.sm_count, kL, 64);
-  const bool tma = recur_tma_view(p.x, p, sizeof(T)) && recur_tma_view(p.gate, p, sizeof(T)) &&
-                   recur_tma_view(p.input_gate, p, sizeof(T)) && p.pairs && p.tokens >= kL && encode_fn();
-  return tma ? launch<T, kDecay, kInput, true>(p, shape, s)
-             : launch<T, kDecay, kInput, false>(p, shape, s);
+  const RecurShape shape = recur_shape(p.sizes, info.sm_count, kL, 64);
+  RecurLaunch l{{shape.ch, 0, device_error_word()}, shape.cluster};
+  const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
+  const Fetch f = recur_fetch(p, views, 3, sizeof(T), kL, &l.tile.copy);
+  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
+  if constexpr (sizeof(T) == 2) {
+    if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);
+  }
+  return launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
 }
 
 template <typename T>
 int launch_typed(const RecurCall &p, cudaStream_t s) {
   if (p.log_decay)
-    return p.input_gate.p ? launch_by_view<T, true, true>(p, s) : launch_by_view<T, true, false>(p, s);
-  return p.input_gate.p ? launch_by_view<T, false, true>(p, s) : launch_by_view<T, false, false>(p, s);
+    return p.input_gate.p ? launch_by_fetch<T, true, true>(p, s) : launch_by_fetch<T, true, false>(p, s);
+  return p.input_gate.p ? launch_by_fetch<T, false, true>(p, s) : launch_by_fetch<T, false, false>(p, s);
 }
 
 }  // namespace

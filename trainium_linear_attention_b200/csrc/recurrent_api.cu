@@ -80,7 +80,7 @@ int la_recurrence_plan(int64_t batch, int64_t tokens, int64_t channels, size_t *
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
   *workspace_bytes =
-      (size_t)(batch * recur_bwd_rows(batch, tokens, (int)channels, info.sm_count) * channels) *
+      (size_t)(batch * recur_bwd_rows({batch, tokens, (int)channels}, info.sm_count) * channels) *
       sizeof(float);
   return LA_OK;
 }
@@ -107,7 +107,7 @@ int la_recurrence_fwd(const void *x, const int64_t *x_strides, const void *gate,
   c.input_gate = tokens_of(input_gate, input_strides);
   c.log_decay = log_decay, c.init = init_state;
   c.lengths = lengths, c.lengths64 = lengths_bits == 64;
-  c.batch = batch, c.tokens = tokens, c.channels = (int)channels;
+  c.sizes = {batch, tokens, (int)channels};
   c.check = saved, c.out = out, c.final_state = final_state;
   c.pairs = in_pairs(channels, {out, final_state, saved});
   return launch_recur_fwd(c, dtype, s);
@@ -135,7 +135,7 @@ int la_recurrence_bwd(const void *x, const int64_t *x_strides, const void *gate,
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
-  const int64_t rows = batch * recur_bwd_rows(batch, tokens, (int)channels, info.sm_count);
+  const int64_t rows = batch * recur_bwd_rows({batch, tokens, (int)channels}, info.sm_count);
   if (d_log_decay && (!workspace || ((uintptr_t)workspace & 15) ||
                       workspace_bytes < (size_t)(rows * channels) * sizeof(float)))
     return LA_ERR_WORKSPACE;
@@ -146,7 +146,7 @@ int la_recurrence_bwd(const void *x, const int64_t *x_strides, const void *gate,
   c.d_out = tokens_of(d_out, d_out_strides);
   c.log_decay = log_decay, c.check = const_cast<float *>(saved);
   c.lengths = lengths, c.lengths64 = lengths_bits == 64;
-  c.batch = batch, c.tokens = tokens, c.channels = (int)channels;
+  c.sizes = {batch, tokens, (int)channels};
   c.d_final = d_final_state, c.dx = dx, c.d_gate = d_gate, c.d_input = d_input_gate;
   c.d_init = d_init_state, c.partial = d_log_decay ? (float *)workspace : nullptr;
   c.pairs = in_pairs(channels, {dx, d_gate, d_input_gate, d_init_state});

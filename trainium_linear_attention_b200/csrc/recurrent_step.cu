@@ -91,10 +91,7 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStep p) {
     affine((const __nv_bfloat16 *)p.weight, (const __nv_bfloat16 *)p.bias);
   if (p.silu) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const float s = Fn<T>::exp(-fabsf(z[e])), r = Fn<T>::rcp(1.f + s);
-      z[e] *= z[e] < 0.f ? s * r : r;
-    }
+    for (int e = 0; e < kVec; ++e) z[e] *= sigmoid_two<T>(two(z[e])).x;  // (as the prompts' kernel)
   }
   store<T, kVec>((T *)p.out + ib * p.channels + c, z);
 #pragma unroll

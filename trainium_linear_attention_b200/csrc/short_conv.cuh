@@ -15,6 +15,7 @@ struct ConvCall {
   int64_t batch = 0, tokens = 0;
   int channels = 0, taps = 0, silu = 0;
   int weight_dtype = 0;          // of weight and bias
+  bool wide = false;             // pairs of channels start at their own size (set by the launchers)
   // forward
   void *out = nullptr, *final_state = nullptr;
   // gradient
