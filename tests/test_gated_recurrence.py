@@ -18,7 +18,6 @@ from torch.autograd import forward_ad
 
 import trainium_linear_attention_b200 as T
 from trainium_linear_attention_b200 import _native as N
-from trainium_linear_attention_b200 import ops_recurrent as ops
 
 gpu = pytest.mark.gpu
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}

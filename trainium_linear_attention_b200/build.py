@@ -1,4 +1,4 @@
-"""Build libla_attention.so (sm_100a) in-tree with nvcc.
+"""Build libla_attention.so (sm_100a) in-tree with nvcc, and its torch binding.
 
     python -m trainium_linear_attention_b200.build [--force] [--verbose]
 
@@ -7,8 +7,10 @@ Every ``csrc/*.cu`` is compiled with
 linked into ``trainium_linear_attention_b200/lib/libla_attention.so``.  The
 CUDA runtime is linked statically; the CUDA driver is reached at run time
 through ``cudaGetDriverEntryPoint`` (TMA descriptors), so the library has no
-link-time dependency on ``libcuda``.  Objects are rebuilt only when a source
-or header is newer than they are.
+link-time dependency on ``libcuda``.  ``csrc/torch_binding.cpp`` becomes
+``lib/_la_torch.so`` (g++, torch's headers; it has no kernels and takes the C
+entry points from the library at run time).  Objects are rebuilt only when a
+source or header is newer than they are.
 """
 
 from __future__ import annotations
@@ -19,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -27,6 +30,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "lib" / "libla_attention.so"
+BINDING_SRC = CSRC / "torch_binding.cpp"
+BINDING = PKG / "lib" / "_la_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
@@ -55,8 +60,31 @@ def _compile(src: Path, obj: Path, verbose: bool) -> str:
     return res.stderr if verbose else ""
 
 
+def _build_binding(force: bool) -> None:
+    """Compile the torch binding (no CUDA code: the C++ compiler alone)."""
+    newest = max(BINDING_SRC.stat().st_mtime, (INCLUDE / "la_attention.h").stat().st_mtime)
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest:
+        return
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + str(INCLUDE),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in (root / "include", root / "include/torch/csrc/api/include", cuda / "include",
+                 sysconfig.get_path("include")):
+        cmd += ["-isystem", str(path)]
+    cmd += [str(BINDING_SRC), "-o", str(tmp), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every kernel source and link the shared library; returns its path."""
+    """Compile every kernel source, link the shared library and compile the torch
+    binding; returns the library's path."""
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     hdr = _headers_mtime()
@@ -66,11 +94,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         obj = BUILD / (src.stem + ".o")
         if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, hdr):
             jobs.append((src, obj))
-    if jobs:
-        with cf.ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
-            for out in ex.map(lambda j: _compile(j[0], j[1], verbose), jobs):
-                if out:
-                    print(out, file=sys.stderr)
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(jobs) + 1)) as ex:
+        binding = ex.submit(_build_binding, force)
+        for out in ex.map(lambda j: _compile(j[0], j[1], verbose), jobs):
+            if out:
+                print(out, file=sys.stderr)
+        binding.result()
     objs = [BUILD / (s.stem + ".o") for s in srcs]
     newest = max(o.stat().st_mtime for o in objs)
     if force or jobs or not LIB.exists() or LIB.stat().st_mtime < newest:

@@ -20,9 +20,8 @@ token:
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .. import ops_recurrent as ops
+from .._torch_binding import module
 from ..ops import check_tangents
 
 
@@ -51,40 +50,6 @@ def ref_gated_recurrence(x, gate, log_decay=None, input_gate=None, initial_state
     return torch.cat(outs, 1), h
 
 
-def _gradients(ctx, d_out, d_state=None):
-    x, gate, input_gate, log_decay, lengths, saved = ctx.saved_tensors
-    if d_out is None and d_state is None:
-        return (None,) * 7
-    if d_out is None:
-        d_out = torch.zeros_like(x)
-    need = ctx.needs_input_grad
-    dx, d_gate, d_input, d_log, d_init = ops.gated_recurrence_backward(
-        x, gate, log_decay, input_gate, saved, lengths, d_out, d_state,
-        want_d_decay=need[2], want_d_initial=need[4])
-    return (dx if need[0] else None, d_gate if need[1] else None, d_log,
-            d_input if need[3] else None, d_init, None, None)
-
-
-_gradients_once = once_differentiable(_gradients)
-
-
-class _GatedRecurrence(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gate, log_decay, input_gate, initial_state, lengths, return_state):
-        out, final, saved = ops.gated_recurrence(x, gate, log_decay, input_gate, initial_state,
-                                                 lengths, return_state, want_saved=True)
-        ctx.save_for_backward(x, gate, input_gate, log_decay, lengths, saved)
-        ctx.set_materialize_grads(False)
-        return (out, final) if return_state else out
-
-    @staticmethod
-    def backward(ctx, *grads):
-        # (gradients of gradients are refused; the check costs 4 us elsewhere)
-        if torch.is_grad_enabled():
-            return _gradients_once(ctx, *grads)
-        return _gradients(ctx, *grads)
-
-
 def gated_recurrence(x, gate, log_decay=None, input_gate=None, initial_state=None,
                      return_state=False, lengths=None):
     """The recurrence over a whole prompt on the sm_100a kernels.
@@ -107,14 +72,8 @@ def gated_recurrence(x, gate, log_decay=None, input_gate=None, initial_state=Non
     b with a - 1 to a relative 2^-22: a slow decay is as exact as the state's own
     rounding, half a step a token."""
     check_tangents(x, gate, log_decay, input_gate, initial_state)
-    if torch.is_grad_enabled() and any(
-            isinstance(v, torch.Tensor) and v.requires_grad
-            for v in (x, gate, log_decay, input_gate, initial_state)):
-        return _GatedRecurrence.apply(x, gate, log_decay, input_gate, initial_state, lengths,
-                                      bool(return_state))
-    out, final, _ = ops.gated_recurrence(x, gate, log_decay, input_gate, initial_state, lengths,
-                                         return_state)
-    return (out, final) if return_state else out
+    return module().gated_recurrence(x, gate, log_decay, input_gate, initial_state, lengths,
+                                     bool(return_state))
 
 
 def gated_recurrence_step(x, gate, state, log_decay=None, input_gate=None):
@@ -124,4 +83,4 @@ def gated_recurrence_step(x, gate, state, log_decay=None, input_gate=None):
     ``gated_recurrence`` returns it) is updated in place.  Returns (b, channels)
     in x.dtype; no gradient."""
     check_tangents(x, gate, log_decay, input_gate, state)
-    return ops.gated_recurrence_step(x, gate, state, log_decay, input_gate)
+    return module().gated_recurrence_step(x, gate, state, log_decay, input_gate)

@@ -14,10 +14,11 @@ The statistics are a token's own: a causal model's tokens may not see one anothe
 
 from __future__ import annotations
 
-import torch
-from torch.autograd.function import once_differentiable
+import operator
 
-from .. import ops_recurrent as ops
+import torch
+
+from .._torch_binding import module, silu
 from ..ops import check_tangents
 
 
@@ -32,39 +33,6 @@ def ref_group_norm(x, groups, weight=None, bias=None, gate=None, activation=None
     return act(z) if gate is None else z * act(gate)
 
 
-def _gradients(ctx, d_out):
-    x, weight, bias, gate, stats = ctx.saved_tensors
-    if d_out is None:
-        return (None,) * 7
-    need = ctx.needs_input_grad
-    dx, d_gate, d_weight, d_bias = ops.group_norm_backward(
-        x, ctx.groups, weight, bias, gate, ctx.activation, stats, d_out,
-        want_d_affine=need[2] or need[3])
-    return (dx if need[0] else None, None, d_weight if need[2] else None,
-            d_bias if need[3] else None, d_gate if need[4] else None, None, None)
-
-
-_gradients_once = once_differentiable(_gradients)
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, groups, weight, bias, gate, activation, eps):
-        out, stats = ops.group_norm(x, groups, weight, bias, gate, activation, eps,
-                                    want_stats=True)
-        ctx.save_for_backward(x, weight, bias, gate, stats)
-        ctx.groups, ctx.activation = groups, activation
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    def backward(ctx, *grads):
-        # (gradients of gradients are refused; the check costs 4 us elsewhere)
-        if torch.is_grad_enabled():
-            return _gradients_once(ctx, *grads)
-        return _gradients(ctx, *grads)
-
-
 def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, eps=1e-5):
     """Group norm of the channels of x (..., channels) on the sm_100a kernel.
 
@@ -77,7 +45,5 @@ def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, ep
     (contiguous, in x.dtype).  Differentiable once, backward (forward mode is
     refused); the gradients of weight and bias are summed in a fixed order."""
     check_tangents(x, weight, bias, gate)
-    if torch.is_grad_enabled() and any(
-            isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias, gate)):
-        return _GroupNorm.apply(x, groups, weight, bias, gate, activation, float(eps))
-    return ops.group_norm(x, groups, weight, bias, gate, activation, float(eps))[0]
+    return module().group_norm(x, operator.index(groups), weight, bias, gate, silu(activation),
+                               float(eps))

@@ -16,9 +16,8 @@ based_attention_benchmark.py:24-69) has the projections that it stands behind.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .. import ops_recurrent as ops
+from .._torch_binding import module, silu
 from ..ops import check_tangents
 
 
@@ -38,41 +37,6 @@ def ref_causal_conv(x, weight, bias=None, activation=None, initial_state=None, l
     return torch.where(inside[..., None], y, torch.zeros_like(y)), final
 
 
-def _gradients(ctx, d_out, d_state=None):
-    x, weight, bias, initial_state, lengths = ctx.saved_tensors
-    if d_out is None and d_state is None:
-        return (None,) * 7
-    if d_out is None:
-        d_out = torch.zeros_like(x)
-    need = ctx.needs_input_grad
-    dx, d_weight, d_bias, d_init = ops.causal_conv_backward(
-        x, weight, bias, ctx.activation, initial_state, lengths, d_out, d_state,
-        want_d_weight=need[1] or need[2], want_d_initial=need[4])
-    return (dx if need[0] else None, d_weight if need[1] else None,
-            d_bias if need[2] else None, None, d_init, None, None)
-
-
-_gradients_once = once_differentiable(_gradients)
-
-
-class _CausalConv(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, activation, initial_state, lengths, return_state):
-        out, final = ops.causal_conv(x, weight, bias, activation, initial_state, lengths,
-                                     return_state)
-        ctx.save_for_backward(x, weight, bias, initial_state, lengths)
-        ctx.activation = activation
-        ctx.set_materialize_grads(False)
-        return (out, final) if return_state else out
-
-    @staticmethod
-    def backward(ctx, *grads):
-        # (gradients of gradients are refused; the check costs 4 us elsewhere)
-        if torch.is_grad_enabled():
-            return _gradients_once(ctx, *grads)
-        return _gradients(ctx, *grads)
-
-
 def causal_conv(x, weight, bias=None, activation=None, initial_state=None, return_state=False,
                 lengths=None):
     """Causal convolution of each channel on the sm_100a kernels.
@@ -89,13 +53,8 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, retur
     in x, weight, bias and ``initial_state`` (forward mode is refused); the
     gradients of weight and bias are summed in a fixed order."""
     check_tangents(x, weight, bias, initial_state)
-    if torch.is_grad_enabled() and any(
-            isinstance(v, torch.Tensor) and v.requires_grad
-            for v in (x, weight, bias, initial_state)):
-        return _CausalConv.apply(x, weight, bias, activation, initial_state, lengths,
-                                 bool(return_state))
-    out, final = ops.causal_conv(x, weight, bias, activation, initial_state, lengths, return_state)
-    return (out, final) if return_state else out
+    return module().causal_conv(x, weight, bias, silu(activation), initial_state, lengths,
+                                bool(return_state))
 
 
 def causal_conv_step(x, weight, state, bias=None, activation=None):
@@ -105,4 +64,4 @@ def causal_conv_step(x, weight, state, bias=None, activation=None):
     ``causal_conv`` returns it) loses its oldest token and gains x, in place.
     Returns (b, channels) in x.dtype; no gradient."""
     check_tangents(x, weight, state, bias)
-    return ops.causal_conv_step(x, weight, state, bias, activation)
+    return module().causal_conv_step(x, weight, state, bias, silu(activation))
