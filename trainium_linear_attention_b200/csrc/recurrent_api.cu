@@ -179,7 +179,7 @@ int la_short_conv_workspace_size(int64_t batch, int64_t tokens, int64_t channels
   if (st != LA_OK) return st;
   if (!bytes) return LA_ERR_INVALID_ARGUMENT;
   if (taps < kConvMinTaps || taps > kConvMaxTaps) return LA_ERR_UNSUPPORTED;
-  *bytes = (size_t)(conv_partial_rows(batch, tokens) * channels * (taps + 1)) * sizeof(float);
+  *bytes = (size_t)(conv_partial_rows({batch, tokens, (int)channels}) * channels * (taps + 1)) * sizeof(float);
   return LA_OK;
 }
 
@@ -196,7 +196,7 @@ static int conv_call(ConvCall *c, const void *x, const int64_t *x_strides, const
   c->x = tokens_of(tokens ? x : nullptr, x_strides);
   c->weight = weight, c->bias = bias, c->weight_dtype = weight_dtype, c->init = init_state;
   c->lengths = lengths, c->lengths64 = lengths_bits == 64;
-  c->batch = batch, c->tokens = tokens, c->channels = (int)channels, c->taps = (int)taps;
+  c->sizes = {batch, tokens, (int)channels}, c->taps = (int)taps;
   c->silu = silu != 0;
   DeviceInfo info;
   return check_device(&info);
@@ -234,7 +234,7 @@ int la_short_conv_bwd(const void *x, const int64_t *x_strides, const void *weigh
     return zero(d_bias, channels * size, s);
   }
   if (tokens && (!d_out || !valid_strides(d_out_strides) || !dx)) return LA_ERR_INVALID_ARGUMENT;
-  const int64_t rows = conv_partial_rows(batch, tokens);
+  const int64_t rows = conv_partial_rows({batch, tokens, (int)channels});
   const bool sums = d_weight || d_bias;
   if (sums && (!workspace || ((uintptr_t)workspace & 15) ||
                workspace_bytes < (size_t)(rows * channels * (taps + 1)) * sizeof(float)))
@@ -279,6 +279,7 @@ static int norm_call(GroupNormCall *c, const void *x, const int64_t *x_strides, 
     return LA_ERR_UNSUPPORTED;
   c->rows = shape[0] * shape[1];
   if (!c->rows) return LA_OK;
+  if (c->rows > INT32_MAX / 2) return LA_ERR_UNSUPPORTED;
   if (!x || !valid_strides(x_strides) || (gate && !valid_strides(gate_strides)))
     return LA_ERR_INVALID_ARGUMENT;
   c->n1 = (uint32_t)shape[1];

@@ -6,438 +6,403 @@
 //   dx_t = sum_j w_j dz_{t + taps - 1 - j},  dw_j = sum_t dz_t x_{t - taps + 1 + j}
 //
 // Bound by memory: x read and y written once (4 bytes per element in bf16),
-// the gradient also reads dy (6).  A lane has one or two pairs of neighbouring
-// channels and walks a run of tokens with the taps' window in registers, a batch of
-// tokens ahead on its way; the tokens before a run are read twice, the second
-// time from the caches.  The gradient computes z again instead of keeping it.
-// Its walk meets dz_t once and adds it to the taps' sums that are still open, so
-// that dx, dw and the bias' gradient come from one pass; the sums over tokens are
-// joined over the CTA's warps in shared memory, written as one row per CTA, and
-// the rows added by a second kernel in a fixed order.
+// the gradient also reads dy (6).  A warp takes 64 channels, a pair for each lane,
+// and walks a run of tokens with the taps' window in registers; it fetches its
+// tiles of 16 tokens itself, two ahead, by TMA where the rows allow it (token_tiles.cuh).
+// The tokens before and behind a run are read twice, the second time from the
+// caches.  The gradient computes z again instead of keeping it.  Its walk meets dz_t
+// once and adds it to the taps' sums that are still open, so that dx, dw and the
+// bias' gradient come from one pass; the sums over tokens are joined over the
+// CTA's warps in shared memory, written as one row per CTA, and the rows added by a
+// second kernel in a fixed order.
+#include <type_traits>
+
 #include "column_sum.cuh"
 #include "short_conv.cuh"
+#include "tc_kernels.cuh"
 
 namespace la {
 namespace {
 
-#ifndef CONV_F
-#define CONV_F 4
-#endif
-#ifndef CONV_B
-#define CONV_B 3
-#endif
-#ifndef CONV_FR
-#define CONV_FR 32
-#endif
-#ifndef CONV_BR
-#define CONV_BR 32
-#endif
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBatch = 8;    // tokens whose loads are on their way together
-constexpr int kRest = 4;     // the same where a sequence or a run ends
-constexpr int kFwdRun = CONV_FR;  // tokens of a lane, at most
-constexpr int kBwdRun = CONV_BR;
+constexpr int kL = 16;       // tokens of a tile
+constexpr int kStages = 2;   // tiles of a warp
+// Tokens of a warp's run: many, since a run's ends are read twice and the sums of a
+// gradient's CTA are written once, but fewer where that leaves SMs without a CTA (4
+// x 4096 x 1024 by 256 CTAs of 128-token runs, 512 of 64, 1024 of 32: the gradient
+// in 34, 38 and 39 us, the forward pass in 19 each).  The same for both passes; the
+// workspace's size goes by it.
+constexpr int kMostRun = 128;
+constexpr int64_t kEnoughCtas = 222;  // one and a half for each of a B200's SMs
+int64_t blocks_of(const TokenSizes &z, int run) {
+  return max64(1, (z.tokens + (int64_t)run * kWarps - 1) / ((int64_t)run * kWarps));
+}
+int run_of(const TokenSizes &z) {
+  int run = kMostRun;
+  while (run > kL && z.batch * ((z.channels + 63) / 64) * blocks_of(z, run) < kEnoughCtas) run /= 2;
+  return run;
+}
 
-// NP pairs of neighbouring channels as they lie in memory.
-template <typename T, int NP>
-struct Pack {
-  static constexpr int kWords = NP * (int)sizeof(T) / 2;
-  uint32_t w[kWords];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = 0;
-  }
-  // `wide`: the pack starts at its own size (NP = 1: else by elements, of which the
-  // last may be beyond the row).
-  __device__ __forceinline__ void load(const T *p, bool wide, bool second) {
-    if (NP > 1 || wide) {
-      if constexpr (kWords == 4) {
-        const uint4 v = *(const uint4 *)p;
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-      } else if constexpr (kWords == 2) {
-        const uint2 v = *(const uint2 *)p;
-        w[0] = v.x, w[1] = v.y;
-      } else {
-        w[0] = *(const uint32_t *)p;
-      }
-    } else if constexpr (sizeof(T) == 2) {
-      const uint16_t *q = (const uint16_t *)p;
-      w[0] = q[0] | (second ? (uint32_t)q[1] << 16 : 0);
-    } else {
-      w[0] = ((const uint32_t *)p)[0];
-      w[1] = second ? ((const uint32_t *)p)[1] : 0;
-    }
-  }
-  __device__ __forceinline__ void store(T *p, bool wide, bool second) const {
-    if (NP > 1 || wide) {
-      if constexpr (kWords == 4) *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
-      else if constexpr (kWords == 2) *(uint2 *)p = make_uint2(w[0], w[1]);
-      else *(uint32_t *)p = w[0];
-    } else if constexpr (sizeof(T) == 2) {
-      uint16_t *q = (uint16_t *)p;
-      q[0] = (uint16_t)w[0];
-      if (second) q[1] = (uint16_t)(w[0] >> 16);
-    } else {
-      ((uint32_t *)p)[0] = w[0];
-      if (second) ((uint32_t *)p)[1] = w[1];
-    }
-  }
-  __device__ __forceinline__ float2 get(int i) const {
-    if constexpr (sizeof(T) == 4)
-      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-    else
-      return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
-  }
-  __device__ __forceinline__ void set(int i, float2 v) {
-    if constexpr (sizeof(T) == 4) {
-      w[2 * i] = __float_as_uint(v.x), w[2 * i + 1] = __float_as_uint(v.y);
-    } else {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
-      w[i] = *(const uint32_t *)&b;
-    }
-  }
-};
-
-// A sequence's rows at a lane's channels, with the tokens before it.
-template <typename T, int NP, int kTaps>
+// A pair of a sequence's channels at single tokens, those before the first among them.
+template <typename T, int kTaps>
 struct Row {
   const T *x;
   const T *init;   // null, or the kTaps - 1 rows before
   int64_t st;
   int channels, len;
-  bool wide, second;
-  __device__ __forceinline__ void load(Pack<T, NP> &v, int t) const {
-    v.zero();
-    if (t >= 0) {
-      if (t < len) v.load(x + t * st, wide, second);
-    } else if (init && t >= -(kTaps - 1)) {
-      v.load(init + (int64_t)(t + kTaps - 1) * channels, wide, second);
-    }
+  bool wide, second;  // pairs start at their own size; there is a second channel
+  __device__ __forceinline__ float2 at(const T *p) const {
+    if (wide) return load_two(p);
+    return make_float2(to_f32(p[0]), second ? to_f32(p[1]) : 0.f);
   }
-  __device__ __forceinline__ void load_inside(Pack<T, NP> &v, int t) const {
-    v.load(x + t * st, wide, second);
+  __device__ __forceinline__ float2 load(int t) const {
+    if (t >= 0) return t < len ? at(x + t * st) : two(0.f);
+    return init && t >= -(kTaps - 1) ? at(init + (int64_t)(t + kTaps - 1) * channels) : two(0.f);
   }
 };
 
-template <int NP, int kTaps>
+template <int kTaps>
 struct Weights {
-  float2 w[kTaps][NP], b[NP];
+  float2 w[kTaps], b;
   template <typename TW>
-  __device__ __forceinline__ void load_as(const ConvCall &p, int c) {
+  __device__ __forceinline__ void load_as(const ConvCall &p, int c, bool second) {
     const TW *src = (const TW *)p.weight + (int64_t)c * kTaps;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const bool second = c + 2 * i + 1 < p.channels;
-      if (sizeof(TW) == 2 && second && ((uintptr_t)src & 3) == 0) {  // a pair's in words
-        const uint32_t *words = (const uint32_t *)src + i * kTaps;
-        float v[2 * kTaps];
-#pragma unroll
-        for (int j = 0; j < kTaps; ++j) {
-          const uint32_t u = words[j];
-          v[2 * j] = __uint_as_float(u << 16), v[2 * j + 1] = __uint_as_float(u & 0xFFFF0000u);
-        }
-#pragma unroll
-        for (int j = 0; j < kTaps; ++j) w[j][i] = make_float2(v[j], v[kTaps + j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kTaps; ++j)
-          w[j][i] = make_float2(to_f32(src[2 * i * kTaps + j]),
-                                second ? to_f32(src[(2 * i + 1) * kTaps + j]) : 0.f);
-      }
-      b[i] = two(0.f);
-      if (p.bias) {
-        const TW *bias = (const TW *)p.bias + c + 2 * i;
-        b[i] = make_float2(to_f32(bias[0]), second ? to_f32(bias[1]) : 0.f);
-      }
+    for (int j = 0; j < kTaps; ++j)
+      w[j] = make_float2(to_f32(src[j]), second ? to_f32(src[kTaps + j]) : 0.f);
+    b = two(0.f);
+    if (p.bias) {
+      const TW *bias = (const TW *)p.bias + c;
+      b = make_float2(to_f32(bias[0]), second ? to_f32(bias[1]) : 0.f);
     }
   }
-  __device__ __forceinline__ void load(const ConvCall &p, int c) {
-    if (p.weight_dtype == LA_DTYPE_FLOAT32) load_as<float>(p, c);
-    else load_as<__nv_bfloat16>(p, c);
+  __device__ __forceinline__ void load(const ConvCall &p, int c, bool second) {
+    if (p.weight_dtype == LA_DTYPE_FLOAT32) load_as<float>(p, c, second);
+    else load_as<__nv_bfloat16>(p, c, second);
   }
 };
 
-// A CTA: 32 packs of channels, kWarps runs of tokens.
-template <typename T, int NP, int kTaps, bool kSilu>
-__global__ void __launch_bounds__(kThreads, CONV_F) conv_fwd_kernel(const ConvCall p, const int run,
-                                                          const int columns, const int blocks) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = (blockIdx.x % columns * 32 + lane) * 2 * NP;
-  const int64_t ib = blockIdx.x / columns / blocks;
-  const int t0 = (blockIdx.x / columns % blocks * kWarps + warp) * run;
-  if (c >= p.channels || (t0 >= p.tokens && t0 > 0)) return;
-  const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.tokens);
-  const int end = min(t0 + run, (int)p.tokens);
-  Row<T, NP, kTaps> row;
-  row.x = (const T *)p.x.p + ib * p.x.sb + c;
-  row.init = p.init ? (const T *)p.init + ib * (kTaps - 1) * p.channels + c : nullptr;
-  row.st = p.x.st, row.channels = p.channels, row.len = len;
-  row.wide = p.wide, row.second = c + 1 < p.channels;
-  if (p.final_state && t0 == 0) {
-    T *dst = (T *)p.final_state + ib * (kTaps - 1) * p.channels + c;
-#pragma unroll
-    for (int j = 0; j < kTaps - 1; ++j) {
-      Pack<T, NP> v;
-      row.load(v, len - (kTaps - 1) + j);
-      v.store(dst + (int64_t)j * p.channels, p.wide, row.second);
-    }
+// The warps' mbarriers, behind the tiles.
+struct Bars {
+  uint64_t full[kStages][kWarps];
+  int abort;
+};
+template <int kIn, Fetch kF, typename T>
+__device__ __forceinline__ Bars &start_bars(uint8_t *smem) {
+  Bars &bars = *(Bars *)(smem + kStages * kIn * kWarps * tile_elems<kF>(kL, 64) * sizeof(T));
+  if (threadIdx.x == 0) {
+    for (int j = 0; j < kStages; ++j)
+      for (int w = 0; w < kWarps; ++w) tc::mbar_init(&bars.full[j][w], 1);
+    bars.abort = 0;
+    tc::fence_barrier_init();
   }
-  Weights<NP, kTaps> w;
-  w.load(p, c);
-  float2 x[kTaps][NP];  // the window; the last one is the token's own
-#pragma unroll
-  for (int j = 0; j < kTaps - 1; ++j) {
-    Pack<T, NP> v;
-    row.load(v, t0 - (kTaps - 1) + j);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) x[j + 1][i] = v.get(i);
-  }
-  T *out = (T *)p.out + ib * p.tokens * p.channels + c;
-  auto token = [&](const Pack<T, NP> &in, int t, bool inside) {
-    Pack<T, NP> y;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-#pragma unroll
-      for (int j = 0; j < kTaps - 1; ++j) x[j][i] = x[j + 1][i];
-      x[kTaps - 1][i] = in.get(i);
-      float2 z = w.b[i];
-#pragma unroll
-      for (int j = 0; j < kTaps; ++j) z = __ffma2_rn(w.w[j][i], x[j][i], z);
-      if constexpr (kSilu) z = __fmul2_rn(z, sigmoid_two<T>(z));
-      y.set(i, z);
-    }
-    if (!inside) y.zero();
-    y.store(out + (int64_t)t * p.channels, p.wide, row.second);
-  };
-  int t = t0;
-  const int whole = min(end, len);
-  for (; t + kBatch <= whole; t += kBatch) {
-    Pack<T, NP> in[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) row.load_inside(in[i], t + i);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) token(in[i], t + i, true);
-  }
-  for (; t < end; t += kRest) {
-    Pack<T, NP> in[kRest];
-#pragma unroll
-    for (int i = 0; i < kRest; ++i) row.load(in[i], t + i);
-#pragma unroll
-    for (int i = 0; i < kRest; ++i)
-      if (t + i < end) token(in[i], t + i, t + i < len);
-  }
+  __syncthreads();
+  return bars;
+}
+__device__ __forceinline__ void end_bars(Bars &bars, int *err) {
+  if (!bars.abort) return;
+  if (err) *err = tc::kErrTimeout;
+  const uint64_t since = tc::globaltimer();  // copies in flight still write into this CTA
+  while (tc::globaltimer() - since < tc::kWaitTimeoutNs) __nanosleep(1000);
 }
 
-// A CTA: 32 pairs of channels, kWarps runs of kBwdRun tokens.
-template <typename T, int kTaps, bool kSilu>
-__global__ void __launch_bounds__(kThreads, CONV_B) conv_bwd_kernel(const ConvCall p, const int columns,
-                                                          const int blocks) {
+// A CTA: 64 channels, kWarps runs of `run` tokens (a multiple of kL).
+template <typename T, int kTaps, bool kSilu, Fetch kF>
+__global__ void __launch_bounds__(kThreads, 4)
+conv_fwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ TileMaps maps,
+                const int run, const int columns, const int blocks) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Bars &bars = start_bars<1, kF, T>(smem);
+  const int channels = p.sizes.channels;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x % columns * 64, c = c0 + 2 * lane;
+  const int64_t ib = blockIdx.x / columns / blocks;
+  const int t0 = (blockIdx.x / columns % blocks * kWarps + warp) * run;
+  const int end = min(t0 + run, (int)p.sizes.tokens);
+  const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.sizes.tokens);
+  const int whole = min(end, len);
+  constexpr int kElems = tile_elems<kF>(kL, 64);
+  const TokenView *views[1] = {&p.x};
+  WarpTiles<T, kL, 1, kStages, kF> tiles{
+      (T *)smem + warp * kElems, kWarps * kElems, kElems, &bars.full[0][warp], kWarps, views, maps.m, ib,
+      c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
+  auto fetch = [&](int t, int stage) {
+    if (t + kL <= whole) tiles.fetch(t, stage);
+    tiles.commit();
+  };
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) fetch(t0 + j * kL, j);
+
+  const bool live = c < channels, second = c + 1 < channels;
+  Row<T, kTaps> row{(const T *)p.x.p + ib * p.x.sb + c,
+                    p.init ? (const T *)p.init + ib * (kTaps - 1) * channels + c : nullptr,
+                    p.x.st, channels, live ? len : 0, p.wide_in, second};
+  if (!live) row.init = nullptr;
+  if (p.final_state && t0 == 0 && live) {
+    T *dst = (T *)p.final_state + ib * (kTaps - 1) * channels + c;
+#pragma unroll
+    for (int j = 0; j < kTaps - 1; ++j)
+      store_two(dst + (int64_t)j * channels, row.load(len - (kTaps - 1) + j), p.wide_out, second);
+  }
+  Weights<kTaps> w;
+  w.load(p, live ? c : 0, second);
+  float2 x[kTaps];  // the window; the last one is the token's own
+#pragma unroll
+  for (int j = 0; j < kTaps - 1; ++j) x[j + 1] = row.load(t0 - (kTaps - 1) + j);
+  T *out = (T *)p.out + (ib * p.sizes.tokens + t0) * channels + c;
+  auto token = [&](float2 in) {
+#pragma unroll
+    for (int j = 0; j < kTaps - 1; ++j) x[j] = x[j + 1];
+    x[kTaps - 1] = in;
+    float2 z = w.b;
+#pragma unroll
+    for (int j = 0; j < kTaps; ++j) z = __ffma2_rn(w.w[j], x[j], z);
+    if constexpr (kSilu) z = __fmul2_rn(z, sigmoid_two<T>(z));
+    return z;
+  };
+  int t = t0, stage = 0;
+  for (; t + kL <= whole; t += kL) {
+    tiles.wait(t, stage, &bars.abort);
+    const T *in = tiles.tile(stage, 0) + 2 * lane;
+    if (p.wide_out && live) {
+#pragma unroll
+      for (int k = 0; k < kL; ++k) store_two(out + (int64_t)k * channels, token(load_two(in + 64 * k)), true, true);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kL; ++k) {
+        const float2 y = token(load_two(in + 64 * k));
+        if (live) store_two(out + (int64_t)k * channels, y, false, second);
+      }
+    }
+    out += (int64_t)kL * channels;
+    __syncwarp();  // the tile is read
+    fetch(t + kStages * kL, stage);
+    if (++stage == kStages) stage = 0;
+  }
+  for (; t < end; t += 4) {  // where the sequence or the tensor ends
+    float2 in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in[i] = row.load(t + i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = token(in[i]);
+      if (live && t + i < end)
+        store_two(out + (int64_t)i * channels, t + i < len ? y : two(0.f), p.wide_out, second);
+    }
+    out += (int64_t)4 * channels;
+  }
+  end_bars(bars, l.err);
+}
+
+// The same.
+template <typename T, int kTaps, bool kSilu, Fetch kF>
+__global__ void __launch_bounds__(kThreads, 3)
+conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ TileMaps maps,
+                const int run, const int columns, const int blocks) {
   constexpr int kSums = kTaps + 1;
   __shared__ float2 part[kWarps][kSums][32];
+  extern __shared__ __align__(1024) uint8_t smem[];
   column_sum_may_start();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Bars &bars = start_bars<2, kF, T>(smem);
+  const int channels = p.sizes.channels;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int c0 = blockIdx.x % columns * 64, c = c0 + 2 * lane;
   const int sums_row = blockIdx.x / columns;
   const int64_t ib = sums_row / blocks;
-  const int t0 = (sums_row % blocks * kWarps + warp) * kBwdRun;
+  const int t0 = (sums_row % blocks * kWarps + warp) * run;
+  const int end = min(t0 + run, (int)p.sizes.tokens);
+  const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.sizes.tokens);
   const bool first = t0 == 0;  // also ends the initial state's rows
-  float2 sums[kSums] = {};
-  if (c < p.channels && (t0 < p.tokens || first)) {
-    const int len = (int)sequence_length(p.lengths, p.lengths64, ib, p.tokens);
-    const int end = min(t0 + kBwdRun, (int)p.tokens);
-    Row<T, 1, kTaps> row, dy;
-    row.x = (const T *)p.x.p + ib * p.x.sb + c;
-    row.init = p.init ? (const T *)p.init + ib * (kTaps - 1) * p.channels + c : nullptr;
-    row.st = p.x.st, row.channels = p.channels, row.len = len;
-    row.wide = p.wide, row.second = c + 1 < p.channels;
-    dy = row;
-    dy.x = (const T *)p.d_out.p + ib * p.d_out.sb + c;
-    dy.st = p.d_out.st, dy.init = nullptr;
-    Weights<1, kTaps> w;
-    w.load(p, c);
-    float2 x[kTaps], open[kTaps] = {};  // the window; dx of its tokens so far
-#pragma unroll
-    for (int j = 0; j < kTaps - 1; ++j) {
-      Pack<T, 1> v;
-      row.load(v, t0 - (kTaps - 1) + j);
-      x[j + 1] = v.get(0);
-    }
-    T *dx = (T *)p.dx + ib * p.tokens * p.channels + c;
-    // Takes a token's x and dy; open[0] is then the gradient of the window's oldest.
-    auto token = [&](const Pack<T, 1> &in, const Pack<T, 1> &up, bool inside, bool own) {
-#pragma unroll
-      for (int j = 0; j < kTaps - 1; ++j) x[j] = x[j + 1], open[j] = open[j + 1];
-      x[kTaps - 1] = in.get(0);
-      float2 g = up.get(0);
-      if constexpr (kSilu) {
-        float2 z = w.b[0];
-#pragma unroll
-        for (int j = 0; j < kTaps; ++j) z = __ffma2_rn(w.w[j][0], x[j], z);
-        const float2 s = sigmoid_two<T>(z);
-        // s (1 + z (1 - s)) = s + z s - z s s
-        const float2 zs = __fmul2_rn(z, s);
-        const float2 slope = __fadd2_rn(s, __ffma2_rn(__fmul2_rn(zs, two(-1.f)), s, zs));
-        g = __fmul2_rn(g, slope);
-      }
-      if (!inside) g = two(0.f);
-#pragma unroll
-      for (int j = 0; j < kTaps; ++j) {
-        open[j] = j == kTaps - 1 ? __fmul2_rn(w.w[j][0], g) : __ffma2_rn(w.w[j][0], g, open[j]);
-        if (own) sums[j] = __ffma2_rn(g, x[j], sums[j]);
-      }
-      if (own) sums[kTaps] = __fadd2_rn(sums[kTaps], g);
-    };
-    auto finish = [&](int at) {  // stores open[0], of token `at` (< 0: the initial state's)
-      const int back = at - (len - (kTaps - 1));  // its row of the final state
-      if (p.d_final && back >= 0 && back < kTaps - 1) {
-        Pack<T, 1> v;
-        v.load((const T *)p.d_final + (ib * (kTaps - 1) + back) * p.channels + c, p.wide, row.second);
-        open[0] = __fadd2_rn(open[0], v.get(0));
-      }
-      Pack<T, 1> v;
-      v.set(0, open[0]);
-      if (at >= 0)
-        v.store(dx + (int64_t)at * p.channels, p.wide, row.second);
-      else if (p.d_init)
-        v.store((T *)p.d_init + (ib * (kTaps - 1) + at + kTaps - 1) * p.channels + c, p.wide,
-                row.second);
-    };
-    int t = t0;
-    // Whole batches whose tokens all are the run's own and whose dx all are plain:
-    // not the sequence's first ones, nor those that the final state reaches.
-    const int plain = min(end, p.d_final ? len - (kTaps - 1) : len);
-    for (; !first && t + kBatch <= plain; t += kBatch) {
-      Pack<T, 1> in[kBatch], up[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) row.load_inside(in[i], t + i), dy.load_inside(up[i], t + i);
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        token(in[i], up[i], true, true);
-        if (i >= kTaps - 1 || t > t0) {  // (else the run before stores it)
-          Pack<T, 1> v;
-          v.set(0, open[0]);
-          v.store(dx + (int64_t)(t + i - (kTaps - 1)) * p.channels, p.wide, row.second);
-        }
-      }
-    }
-    for (; t < end + kTaps - 1; t += kRest) {
-      Pack<T, 1> in[kRest], up[kRest];
-#pragma unroll
-      for (int i = 0; i < kRest; ++i) row.load(in[i], t + i), dy.load(up[i], t + i);
-#pragma unroll
-      for (int i = 0; i < kRest; ++i) {
-        if (t + i >= end + kTaps - 1) break;
-        token(in[i], up[i], t + i < len, t + i < min(len, end));
-        const int at = t + i - (kTaps - 1);
-        if (at >= t0 || first) finish(at);
-      }
-    }
-  }
-  if (!p.partial) return;
-#pragma unroll
-  for (int j = 0; j < kSums; ++j) part[warp][j][lane] = sums[j];
-  __syncthreads();
-  float *dst = p.partial + (int64_t)sums_row * p.channels * kSums;
-  for (int i = threadIdx.x; i < kSums * 64; i += kThreads) {
-    const int j = i / 64, channel = c0 + i % 64;
-    if (channel >= p.channels) continue;
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      const float2 v = part[k][j][i % 64 / 2];
-      sum += i & 1 ? v.y : v.x;
-    }
-    if (j < kTaps) dst[(int64_t)channel * kTaps + j] = sum;
-    else dst[(int64_t)p.channels * kTaps + channel] = sum;
-  }
-}
-
-template <typename T, int NP, int kTaps>
-int launch_fwd(const ConvCall &p, cudaStream_t s) {
-  const int columns = (p.channels + 64 * NP - 1) / (64 * NP);
-  int run = kFwdRun;  // shorter runs where long ones leave SMs without a CTA
-  DeviceInfo info;
-  const int st = current_device_info(&info);
-  if (st != LA_OK) return st;
-  while (run > kBatch && p.batch * columns * ((p.tokens + run * kWarps - 1) / (run * kWarps)) <
-                             4 * info.sm_count)
-    run /= 2;
-  const int64_t blocks = max64(1, (p.tokens + run * kWarps - 1) / (run * kWarps));
-  if (blocks > INT32_MAX / p.batch / columns) return LA_ERR_UNSUPPORTED;
-  const unsigned grid = (unsigned)(blocks * p.batch * columns);
-  if (p.silu)
-    conv_fwd_kernel<T, NP, kTaps, true><<<grid, kThreads, 0, s>>>(p, run, columns, (int)blocks);
-  else
-    conv_fwd_kernel<T, NP, kTaps, false><<<grid, kThreads, 0, s>>>(p, run, columns, (int)blocks);
-  return check_launch();
-}
-
-template <typename T, int kTaps>
-int launch_bwd(const ConvCall &p, cudaStream_t s) {
-  const int64_t blocks = conv_partial_rows(1, p.tokens);
-  const int columns = (p.channels + 63) / 64;
-  if (blocks > INT32_MAX / p.batch / columns) return LA_ERR_UNSUPPORTED;
-  const unsigned grid = (unsigned)(blocks * p.batch * columns);
-  if (p.silu) conv_bwd_kernel<T, kTaps, true><<<grid, kThreads, 0, s>>>(p, columns, (int)blocks);
-  else conv_bwd_kernel<T, kTaps, false><<<grid, kThreads, 0, s>>>(p, columns, (int)blocks);
-  return check_launch();
-}
-
-// The widest pack (in bytes, 16 at most) that the channels and every row's start allow.
-int pack_of(const ConvCall &p, bool grad, int size) {
-  uint64_t bits = (uint64_t)p.channels * size;
-  auto at = [&](const void *q) { bits |= (uint64_t)(uintptr_t)q; };
-  auto view = [&](const TokenView &v) {
-    at(v.p);
-    bits |= (uint64_t)(v.sb * (int64_t)size) | (uint64_t)(v.st * (int64_t)size);
+  // Whole tiles: all tokens the run's own, none of their dx reached by the final
+  // state's gradient.
+  const int whole = min(end, p.d_final ? len - (kTaps - 1) : len);
+  constexpr int kElems = tile_elems<kF>(kL, 64);
+  const TokenView *views[2] = {&p.x, &p.d_out};
+  WarpTiles<T, kL, 2, kStages, kF> tiles{
+      (T *)smem + warp * 2 * kElems, kWarps * 2 * kElems, kElems, &bars.full[0][warp], kWarps, views,
+      maps.m, ib, c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
+  auto fetch = [&](int t, int stage) {
+    if (t + kL <= whole) tiles.fetch(t, stage);
+    tiles.commit();
   };
-  view(p.x);
-  at(p.init);
-  if (grad) {
-    view(p.d_out);
-    at(p.dx), at(p.d_init), at(p.d_final);
-  } else {
-    at(p.out), at(p.final_state);
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) fetch(t0 + j * kL, j);
+
+  const bool live = c < channels, second = c + 1 < channels;
+  Row<T, kTaps> row{(const T *)p.x.p + ib * p.x.sb + c,
+                    p.init && live ? (const T *)p.init + ib * (kTaps - 1) * channels + c : nullptr,
+                    p.x.st, channels, live ? len : 0, p.wide_in, second};
+  Row<T, kTaps> dy{(const T *)p.d_out.p + ib * p.d_out.sb + c, nullptr, p.d_out.st, channels,
+                   live ? len : 0, p.wide_in, second};
+  float2 sums[kSums] = {};
+  Weights<kTaps> w;
+  w.load(p, live ? c : 0, second);
+  float2 x[kTaps], open[kTaps] = {};  // the window; dx of its tokens so far
+#pragma unroll
+  for (int j = 0; j < kTaps - 1; ++j) x[j + 1] = row.load(t0 - (kTaps - 1) + j);
+  T *dx = (T *)p.dx + ib * p.sizes.tokens * channels + c;
+  // Takes a token's x and dy; open[0] is then the gradient of the window's oldest.
+  auto token = [&](float2 in, float2 g, auto own) {
+#pragma unroll
+    for (int j = 0; j < kTaps - 1; ++j) x[j] = x[j + 1], open[j] = open[j + 1];
+    x[kTaps - 1] = in;
+    if constexpr (kSilu) {
+      float2 z = w.b;
+#pragma unroll
+      for (int j = 0; j < kTaps; ++j) z = __ffma2_rn(w.w[j], x[j], z);
+      // s (1 + z (1 - s)) = s + z s (1 - s)
+      const float2 s = sigmoid_two<T>(z);
+      g = __fmul2_rn(g, __ffma2_rn(__fmul2_rn(z, s), __ffma2_rn(s, two(-1.f), two(1.f)), s));
+    }
+#pragma unroll
+    for (int j = 0; j < kTaps; ++j) {
+      open[j] = j == kTaps - 1 ? __fmul2_rn(w.w[j], g) : __ffma2_rn(w.w[j], g, open[j]);
+      if (own) sums[j] = __ffma2_rn(g, x[j], sums[j]);
+    }
+    if (own) sums[kTaps] = __fadd2_rn(sums[kTaps], g);
+  };
+  int t = t0, stage = 0;
+  for (; t + kL <= whole; t += kL) {
+    tiles.wait(t, stage, &bars.abort);
+    const T *in = tiles.tile(stage, 0) + 2 * lane, *up = tiles.tile(stage, 1) + 2 * lane;
+    T *dst = dx + (int64_t)(t - (kTaps - 1)) * channels;
+    auto tile = [&](auto wide) {
+#pragma unroll
+      for (int k = 0; k < kL; ++k) {
+        token(load_two(in + 64 * k), load_two(up + 64 * k), std::true_type{});
+        if (!live) continue;
+        if (k >= kTaps - 1 || t > t0)
+          store_two(dst + (int64_t)k * channels, open[0], wide, second);
+        else if (first && p.d_init)  // (else the run before stores it)
+          store_two((T *)p.d_init + (ib * (kTaps - 1) + k) * channels + c, open[0], wide, second);
+      }
+    };
+    if (p.wide_out) tile(std::true_type{});
+    else tile(std::false_type{});
+    __syncwarp();  // the tile is read
+    fetch(t + kStages * kL, stage);
+    if (++stage == kStages) stage = 0;
   }
-  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+  if (t0 < p.sizes.tokens || first) {
+    for (; t < end + kTaps - 1; t += 4) {
+      float2 in[4], up[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) in[i] = row.load(t + i), up[i] = dy.load(t + i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int now = t + i, at = now - (kTaps - 1);  // whose dx is complete
+        if (now >= end + kTaps - 1) break;
+        // (beyond the sequence dy is zero)
+        token(in[i], now < len ? up[i] : two(0.f), now < end);
+        if (!live || (at < t0 && !first)) continue;
+        const int back = at - (len - (kTaps - 1));  // its row of the final state
+        if (p.d_final && back >= 0 && back < kTaps - 1) {
+          const T *d = (const T *)p.d_final + (ib * (kTaps - 1) + back) * channels + c;
+          open[0] = __fadd2_rn(open[0], row.at(d));
+        }
+        if (at >= 0)
+          store_two(dx + (int64_t)at * channels, open[0], p.wide_out, second);
+        else if (p.d_init)
+          store_two((T *)p.d_init + (ib * (kTaps - 1) + at + kTaps - 1) * channels + c, open[0],
+                    p.wide_out, second);
+      }
+    }
+  }
+  if (p.partial) {
+#pragma unroll
+    for (int j = 0; j < kSums; ++j) part[warp][j][lane] = sums[j];
+    __syncthreads();
+    float *dst = p.partial + (int64_t)sums_row * channels * kSums;
+    for (int i = threadIdx.x; i < kSums * 64; i += kThreads) {
+      const int j = i / 64, channel = c0 + i % 64;
+      if (channel >= channels) continue;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float2 v = part[k][j][i % 64 / 2];
+        sum += i & 1 ? v.y : v.x;
+      }
+      if (j < kTaps) dst[(int64_t)channel * kTaps + j] = sum;
+      else dst[(int64_t)channels * kTaps + channel] = sum;
+    }
+  }
+  end_bars(bars, l.err);
 }
 
-template <typename T, int NP>
-int fwd_by_taps(const ConvCall &p, cudaStream_t s) {
-  if (p.taps == 2) return launch_fwd<T, NP, 2>(p, s);
-  if (p.taps == 3) return launch_fwd<T, NP, 3>(p, s);
-  return launch_fwd<T, NP, 4>(p, s);
+template <typename T, Fetch kF, int kIn>
+int make_maps(TileMaps *maps, const ConvCall &p) {
+  const TokenView *views[2] = {&p.x, &p.d_out};
+  for (int n = 0; kF == Fetch::kTma && n < kIn; ++n)
+    if (!tile_map(&maps->m[n], *views[n], p.sizes,
+                  sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16, 64, kL))
+      return LA_ERR_CUDA;
+  return LA_OK;
+}
+template <typename T, Fetch kF, int kIn>
+constexpr int tile_bytes() {
+  return kStages * kIn * kWarps * tile_elems<kF>(kL, 64) * (int)sizeof(T) + (int)sizeof(Bars);
+}
+
+template <typename T, int kTaps, bool kSilu, Fetch kF>
+int launch(const ConvCall &p, const TileLaunch &l, bool grad, cudaStream_t s) {
+  const int columns = (p.sizes.channels + 63) / 64, run = run_of(p.sizes);
+  const int64_t blocks = blocks_of(p.sizes, run);
+  if (blocks > INT32_MAX / p.sizes.batch / columns) return LA_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)(blocks * p.sizes.batch * columns);
+  TileMaps maps;
+  int st = grad ? make_maps<T, kF, 2>(&maps, p) : make_maps<T, kF, 1>(&maps, p);
+  if (st != LA_OK) return st;
+  const int smem = grad ? tile_bytes<T, kF, 2>() : tile_bytes<T, kF, 1>();
+  auto kernel = grad ? conv_bwd_kernel<T, kTaps, kSilu, kF> : conv_fwd_kernel<T, kTaps, kSilu, kF>;
+  if ((st = allow_dynamic_smem((const void *)kernel, smem)) != LA_OK) return st;
+  kernel<<<grid, kThreads, smem, s>>>(p, l, maps, run, columns, (int)blocks);
+  return check_launch();
+}
+template <typename T, int kTaps, Fetch kF>
+int by_silu(const ConvCall &p, const TileLaunch &l, bool grad, cudaStream_t s) {
+  return p.silu ? launch<T, kTaps, true, kF>(p, l, grad, s) : launch<T, kTaps, false, kF>(p, l, grad, s);
+}
+template <typename T, Fetch kF>
+int by_taps(const ConvCall &p, const TileLaunch &l, bool grad, cudaStream_t s) {
+  if (p.taps == 2) return by_silu<T, 2, kF>(p, l, grad, s);
+  if (p.taps == 3) return by_silu<T, 3, kF>(p, l, grad, s);
+  return by_silu<T, 4, kF>(p, l, grad, s);
 }
 
 template <typename T>
-int run_fwd(ConvCall p, cudaStream_t s) {
-  const int bytes = pack_of(p, false, sizeof(T));
-  p.wide = bytes >= 2 * (int)sizeof(T);
-  return bytes >= 4 * (int)sizeof(T) ? fwd_by_taps<T, 2>(p, s) : fwd_by_taps<T, 1>(p, s);
-}
-
-template <typename T>
-int run_bwd(ConvCall p, cudaStream_t s) {
-  p.wide = pack_of(p, true, sizeof(T)) >= 2 * (int)sizeof(T);
-  if (p.taps == 2) return launch_bwd<T, 2>(p, s);
-  if (p.taps == 3) return launch_bwd<T, 3>(p, s);
-  return launch_bwd<T, 4>(p, s);
+int run_conv(ConvCall p, bool grad, cudaStream_t s) {
+  constexpr int size = sizeof(T);
+  const TokenView *views[2] = {&p.x, &p.d_out};
+  TileLaunch l{64, 0, device_error_word()};
+  const Fetch f = fetch_of(views, 2, p.sizes, size, kL, &l.copy);
+  auto at = [&](std::initializer_list<const void *> q) {
+    uintptr_t bits = (uintptr_t)p.sizes.channels * size;
+    for (const void *v : q) bits |= (uintptr_t)v;
+    return bits % (2 * size) == 0;
+  };
+  p.wide_in = row_bytes(p.x, size) >= 2 * size && row_bytes(p.d_out, size) >= 2 * size &&
+              at({p.init, p.d_final});
+  p.wide_out = at({p.out, p.final_state, p.dx, p.d_init});
+  if (f == Fetch::kTma) return by_taps<T, Fetch::kTma>(p, l, grad, s);
+  if constexpr (size == 2) {
+    if (f == Fetch::kShifted) return by_taps<T, Fetch::kShifted>(p, l, grad, s);
+  }
+  return by_taps<T, Fetch::kAsync>(p, l, grad, s);
 }
 
 }  // namespace
 
-int64_t conv_partial_rows(int64_t batch, int64_t tokens) {
-  constexpr int64_t kSpan = (int64_t)kWarps * kBwdRun;
-  return batch * max64(1, (tokens + kSpan - 1) / kSpan);
-}
+int64_t conv_partial_rows(const TokenSizes &z) { return z.batch * blocks_of(z, run_of(z)); }
 
 int launch_conv_fwd(const ConvCall &p, int dtype, cudaStream_t s) {
-  return dtype == LA_DTYPE_FLOAT32 ? run_fwd<float>(p, s) : run_fwd<__nv_bfloat16>(p, s);
+  return dtype == LA_DTYPE_FLOAT32 ? run_conv<float>(p, false, s)
+                                   : run_conv<__nv_bfloat16>(p, false, s);
 }
 
 int launch_conv_bwd(const ConvCall &p, int dtype, cudaStream_t s) {
-  return dtype == LA_DTYPE_FLOAT32 ? run_bwd<float>(p, s) : run_bwd<__nv_bfloat16>(p, s);
+  return dtype == LA_DTYPE_FLOAT32 ? run_conv<float>(p, true, s)
+                                   : run_conv<__nv_bfloat16>(p, true, s);
 }
 
 }  // namespace la

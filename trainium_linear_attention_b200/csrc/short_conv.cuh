@@ -1,7 +1,8 @@
 // Causal convolution of each channel with a few taps: what its launchers take.
 #pragma once
 
-#include "recurrence.cuh"
+#include "pairs.cuh"
+#include "token_tiles.cuh"
 
 namespace la {
 
@@ -12,10 +13,12 @@ struct ConvCall {
   const void *init = nullptr;    // null, or (batch, taps - 1, channels): the tokens before
   const void *lengths = nullptr;
   int lengths64 = 0;
-  int64_t batch = 0, tokens = 0;
-  int channels = 0, taps = 0, silu = 0;
+  TokenSizes sizes;
+  int taps = 0, silu = 0;
   int weight_dtype = 0;          // of weight and bias
-  bool wide = false;             // pairs of channels start at their own size (set by the launchers)
+  bool wide_in = false, wide_out = false;  // pairs of channels that are read alone, and those
+                                           // that are written, start at their own size (set by
+                                           // the launchers)
   // forward
   void *out = nullptr, *final_state = nullptr;
   // gradient
@@ -29,6 +32,6 @@ constexpr int kConvMinTaps = 2, kConvMaxTaps = 4;
 int launch_conv_fwd(const ConvCall &c, int dtype, cudaStream_t s);
 int launch_conv_bwd(const ConvCall &c, int dtype, cudaStream_t s);
 // Rows of `partial`.
-int64_t conv_partial_rows(int64_t batch, int64_t tokens);
+int64_t conv_partial_rows(const TokenSizes &z);
 
 }  // namespace la

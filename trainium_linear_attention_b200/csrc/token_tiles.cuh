@@ -264,7 +264,7 @@ inline bool tile_map(CUtensorMap *map, const TokenView &v, const TokenSizes &s, 
 // copy should it be kAsync.
 inline Fetch fetch_of(const TokenView *const *views, int n, const TokenSizes &s, int size, int l,
                       int *copy) {
-  bool tma = encode_fn() != nullptr;
+  bool tma = encode_fn() != nullptr && s.tokens >= l;
   *copy = 16;
   for (int i = 0; i < n; ++i) {
     if (!views[i]->p) continue;
