@@ -33,8 +33,10 @@ __device__ __forceinline__ void store_two(float *p, float2 v, bool pair, bool se
   }
 }
 
-// Functions by the inputs' type: bf16 inputs are 2^-9 apart, and the special-
-// function unit's 2^-22 is far below what they carry; fp32 ones take the library's.
+// Functions by the inputs' type.  The special-function unit's reciprocal is within
+// an ulp, its roots and exponentials within 2^-22: for bf16 inputs, which are 2^-9
+// apart, that is far below what they carry.  fp32 ones take the library's
+// exponential, which is as near for large arguments too.
 template <typename T> struct Fn;
 template <> struct Fn<__nv_bfloat16> {
   static __device__ __forceinline__ float exp(float x) {
@@ -55,8 +57,8 @@ template <> struct Fn<__nv_bfloat16> {
 };
 template <> struct Fn<float> {
   static __device__ __forceinline__ float exp(float x) { return expf(x); }
-  static __device__ __forceinline__ float rcp(float x) { return 1.f / x; }
-  static __device__ __forceinline__ float rsqrt(float x) { return 1.f / sqrtf(x); }
+  static __device__ __forceinline__ float rcp(float x) { return Fn<__nv_bfloat16>::rcp(x); }
+  static __device__ __forceinline__ float rsqrt(float x) { return rsqrtf(x); }
 };
 
 // max that keeps a NaN

@@ -207,8 +207,8 @@ struct RecurLaunch {
 
 // (TMA kernels write pairs of channels.)
 inline Fetch recur_fetch(const RecurCall &p, const TokenView *const *views, int n, int size, int l,
-                         int *copy) {
-  const Fetch f = fetch_of(views, n, p.sizes, size, l, copy);
+                         TileLaunch *launch) {
+  const Fetch f = fetch_of(views, n, p.sizes, size, l, launch);
   return f == Fetch::kTma && !p.pairs ? Fetch::kAsync : f;
 }
 

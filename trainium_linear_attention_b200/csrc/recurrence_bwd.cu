@@ -64,17 +64,14 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
       (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
-      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
   const int rows = parts * kL;            // tokens of a warp and step
   const int block_rows = kRecurWarps * rows;
   const int blocks = (len + block_rows - 1) / block_rows;
   const int steps = (blocks + cluster - 1) / cluster;
   auto block_of = [&](int i) { return blocks - 1 - (i * cluster + rank); };  // < 0: none
-  // Tiles that the sequence fills; the last one is loaded where it is used.
   auto fetch = [&](int i, int stage) {
-    const int t0 = block_of(i) * block_rows + warp * rows;
-    if (i < steps && t0 >= 0 && t0 + rows <= len) tiles.fetch(t0, stage);
-    tiles.commit();
+    tiles.fetch(block_of(i) * block_rows + warp * rows, i < steps ? len : 0, stage);
   };
 
   float2 lambda = two(0.f), carry = two(0.f), d_lambda = two(0.f);
@@ -118,20 +115,11 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
             *us = tiles.tile(stage, kIn - 1);
     const int block = block_of(i);
     const int row0 = block * block_rows + warp * rows, t0 = row0 + part * kL;
-    const bool whole = block >= 0 && row0 + rows <= len;
+    const bool whole = tiles.whole(row0, len);
     float2 h = start;
     start = saved(i + 1);
-    if (whole) {
-      tiles.wait(row0, stage, &ex.abort);
-    } else {
-      // tokens outside the sequence keep the state and the gradient
-      tiles.load_ragged(row0, len, stage, 0, 0.f);
-      tiles.load_ragged(row0, len, stage, 1, kDecay ? -INFINITY : INFINITY);
-      tiles.load_ragged(row0, len, stage, 2, 0.f);
-      if (kInput) tiles.load_ragged(row0, len, stage, 3, 0.f);
-      if (kF == Fetch::kTma) tc::fence_proxy_async_smem();  // ahead of the next copy into this tile
-      __syncwarp();
-    }
+    // tokens outside the sequence keep the state and the gradient
+    tiles.wait(row0, len, stage, kDecay ? -INFINITY : INFINITY, &ex.abort);
     float2 am1[kL], bu[kL], s[kL], sc[kL], uc[kL];
     float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f), r = two(0.f);
 #pragma unroll
@@ -301,9 +289,9 @@ int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
 
 template <typename T, bool kDecay, bool kInput>
 int launch_by_fetch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
-  RecurLaunch l{{shape.ch, 0, device_error_word()}, shape.cluster};
+  RecurLaunch l{{shape.ch, 0, false, device_error_word()}, shape.cluster};
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
-  const Fetch f = recur_fetch(p, views, 4, sizeof(T), kL, &l.tile.copy);
+  const Fetch f = recur_fetch(p, views, 4, sizeof(T), kL, &l.tile);
   if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
   if constexpr (sizeof(T) == 2) {
     if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);

@@ -63,17 +63,12 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
       (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
-      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
   const int rows = parts * kL;                      // tokens of a warp and step
   const int step = cluster * kRecurWarps * rows;    // of all
   const int steps = (len + step - 1) / step;
   const int first = (rank * kRecurWarps + warp) * rows;
-  // Tiles that the sequence fills; the last one is loaded where it is used.
-  auto fetch = [&](int i, int stage) {
-    const int t0 = i * step + first;
-    if (t0 + rows <= len) tiles.fetch(t0, stage);
-    tiles.commit();
-  };
+  auto fetch = [&](int i, int stage) { tiles.fetch(i * step + first, i < steps ? len : 0, stage); };
 
   float2 lambda = two(0.f), carry = two(0.f);
   if (live) {
@@ -106,16 +101,9 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     const int buf = i & 1;
     const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *us = tiles.tile(stage, kIn - 1);
     const int row0 = i * step + first, t0 = row0 + part * kL;
-    const bool whole = row0 + rows <= len;
-    if (whole) {
-      tiles.wait(row0, stage, &ex.abort);
-    } else {
-      // tokens beyond the sequence keep the state
-      tiles.load_ragged(row0, len, stage, 0, 0.f);
-      tiles.load_ragged(row0, len, stage, 1, kDecay ? -INFINITY : INFINITY);
-      if (kInput) tiles.load_ragged(row0, len, stage, 2, 0.f);
-      __syncwarp();
-    }
+    const bool whole = tiles.whole(row0, len);
+    // tokens beyond the sequence keep the state
+    tiles.wait(row0, len, stage, kDecay ? -INFINITY : INFINITY, &ex.abort);
     float2 am1[kL], b[kL];
     float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f);
 #pragma unroll
@@ -232,9 +220,9 @@ int launch_by_fetch(const RecurCall &p, cudaStream_t s) {
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
   const RecurShape shape = recur_shape(p.sizes, info.sm_count, kL, 64);
-  RecurLaunch l{{shape.ch, 0, device_error_word()}, shape.cluster};
+  RecurLaunch l{{shape.ch, 0, false, device_error_word()}, shape.cluster};
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
-  const Fetch f = recur_fetch(p, views, 3, sizeof(T), kL, &l.tile.copy);
+  const Fetch f = recur_fetch(p, views, 3, sizeof(T), kL, &l.tile);
   if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
   if constexpr (sizeof(T) == 2) {
     if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);

@@ -52,10 +52,7 @@ struct Row {
   int64_t st;
   int channels, len;
   bool wide, second;  // pairs start at their own size; there is a second channel
-  __device__ __forceinline__ float2 at(const T *p) const {
-    if (wide) return load_two(p);
-    return make_float2(to_f32(p[0]), second ? to_f32(p[1]) : 0.f);
-  }
+  __device__ __forceinline__ float2 at(const T *p) const { return pair_at(p, wide, second); }
   __device__ __forceinline__ float2 load(int t) const {
     if (t >= 0) return t < len ? at(x + t * st) : two(0.f);
     return init && t >= -(kTaps - 1) ? at(init + (int64_t)(t + kTaps - 1) * channels) : two(0.f);
@@ -126,11 +123,9 @@ conv_fwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   const TokenView *views[1] = {&p.x};
   WarpTiles<T, kL, 1, kStages, kF> tiles{
       (T *)smem + warp * kElems, kWarps * kElems, kElems, &bars.full[0][warp], kWarps, views, maps.m, ib,
-      c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
-  auto fetch = [&](int t, int stage) {
-    if (t + kL <= whole) tiles.fetch(t, stage);
-    tiles.commit();
-  };
+      c0, 64, min(64, channels - c0), l.copy, l.wide, p.sizes, 0};
+  // Whole tiles, and the one that the run or the sequence ends in.
+  auto fetch = [&](int t, int stage) { tiles.fetch(t, whole, stage); };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) fetch(t0 + j * kL, j);
 
@@ -163,7 +158,7 @@ conv_fwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   };
   int t = t0, stage = 0;
   for (; t + kL <= whole; t += kL) {
-    tiles.wait(t, stage, &bars.abort);
+    tiles.wait(t, whole, stage, 0.f, &bars.abort);
     const T *in = tiles.tile(stage, 0) + 2 * lane;
     if (p.wide_out && live) {
 #pragma unroll
@@ -180,17 +175,16 @@ conv_fwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
     fetch(t + kStages * kL, stage);
     if (++stage == kStages) stage = 0;
   }
-  for (; t < end; t += 4) {  // where the sequence or the tensor ends
-    float2 in[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) in[i] = row.load(t + i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 y = token(in[i]);
-      if (live && t + i < end)
-        store_two(out + (int64_t)i * channels, t + i < len ? y : two(0.f), p.wide_out, second);
+  for (; t < end; t += kL) {  // where the sequence or the tensor ends
+    if (t < len) tiles.wait(t, whole, stage, 0.f, &bars.abort);
+    const T *in = tiles.tile(stage, 0) + 2 * lane;
+    const int left = min(kL, end - t);
+#pragma unroll 4
+    for (int k = 0; k < left; ++k, out += channels) {
+      float2 y = two(0.f);
+      if (t + k < len) y = token(load_two(in + 64 * k));
+      if (live) store_two(out, y, p.wide_out, second);
     }
-    out += (int64_t)4 * channels;
   }
   end_bars(bars, l.err);
 }
@@ -221,11 +215,11 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   const TokenView *views[2] = {&p.x, &p.d_out};
   WarpTiles<T, kL, 2, kStages, kF> tiles{
       (T *)smem + warp * 2 * kElems, kWarps * 2 * kElems, kElems, &bars.full[0][warp], kWarps, views,
-      maps.m, ib, c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
-  auto fetch = [&](int t, int stage) {
-    if (t + kL <= whole) tiles.fetch(t, stage);
-    tiles.commit();
-  };
+      maps.m, ib, c0, 64, min(64, channels - c0), l.copy, l.wide, p.sizes, 0};
+  // Whole tiles, and those that the run, its neighbour's first tokens or the sequence
+  // end in.
+  const int reach = min(len, end + kTaps - 1);
+  auto fetch = [&](int t, int stage) { tiles.fetch(t, reach, stage); };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) fetch(t0 + j * kL, j);
 
@@ -233,8 +227,6 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   Row<T, kTaps> row{(const T *)p.x.p + ib * p.x.sb + c,
                     p.init && live ? (const T *)p.init + ib * (kTaps - 1) * channels + c : nullptr,
                     p.x.st, channels, live ? len : 0, p.wide_in, second};
-  Row<T, kTaps> dy{(const T *)p.d_out.p + ib * p.d_out.sb + c, nullptr, p.d_out.st, channels,
-                   live ? len : 0, p.wide_in, second};
   float2 sums[kSums] = {};
   Weights<kTaps> w;
   w.load(p, live ? c : 0, second);
@@ -264,7 +256,7 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   };
   int t = t0, stage = 0;
   for (; t + kL <= whole; t += kL) {
-    tiles.wait(t, stage, &bars.abort);
+    tiles.wait(t, reach, stage, 0.f, &bars.abort);
     const T *in = tiles.tile(stage, 0) + 2 * lane, *up = tiles.tile(stage, 1) + 2 * lane;
     T *dst = dx + (int64_t)(t - (kTaps - 1)) * channels;
     auto tile = [&](auto wide) {
@@ -285,21 +277,19 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
     if (++stage == kStages) stage = 0;
   }
   if (t0 < p.sizes.tokens || first) {
-    for (; t < end + kTaps - 1; t += 4) {
-      float2 in[4], up[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) in[i] = row.load(t + i), up[i] = dy.load(t + i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int now = t + i, at = now - (kTaps - 1);  // whose dx is complete
-        if (now >= end + kTaps - 1) break;
-        // (beyond the sequence dy is zero)
-        token(in[i], now < len ? up[i] : two(0.f), now < end);
+    for (; t < end + kTaps - 1; t += kL) {
+      const int left = min(kL, end + kTaps - 1 - t);
+      tiles.wait(t, reach, stage, 0.f, &bars.abort);  // (x and dy beyond it are zero)
+      const T *in = tiles.tile(stage, 0) + 2 * lane, *up = tiles.tile(stage, 1) + 2 * lane;
+#pragma unroll 1
+      for (int k = 0; k < left; ++k) {
+        const int now = t + k, at = now - (kTaps - 1);  // whose dx is complete
+        token(load_two(in + 64 * k), load_two(up + 64 * k), now < end);
         if (!live || (at < t0 && !first)) continue;
         const int back = at - (len - (kTaps - 1));  // its row of the final state
         if (p.d_final && back >= 0 && back < kTaps - 1) {
           const T *d = (const T *)p.d_final + (ib * (kTaps - 1) + back) * channels + c;
-          open[0] = __fadd2_rn(open[0], row.at(d));
+          open[0] = __fadd2_rn(open[0], pair_at(d, p.wide_in, second));
         }
         if (at >= 0)
           store_two(dx + (int64_t)at * channels, open[0], p.wide_out, second);
@@ -307,6 +297,9 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
           store_two((T *)p.d_init + (ib * (kTaps - 1) + at + kTaps - 1) * channels + c, open[0],
                     p.wide_out, second);
       }
+      __syncwarp();  // the tile is read
+      fetch(t + kStages * kL, stage);
+      if (++stage == kStages) stage = 0;
     }
   }
   if (p.partial) {
@@ -374,8 +367,8 @@ template <typename T>
 int run_conv(ConvCall p, bool grad, cudaStream_t s) {
   constexpr int size = sizeof(T);
   const TokenView *views[2] = {&p.x, &p.d_out};
-  TileLaunch l{64, 0, device_error_word()};
-  const Fetch f = fetch_of(views, 2, p.sizes, size, kL, &l.copy);
+  TileLaunch l{64, 0, false, device_error_word()};
+  const Fetch f = fetch_of(views, 2, p.sizes, size, kL, &l);
   auto at = [&](std::initializer_list<const void *> q) {
     uintptr_t bits = (uintptr_t)p.sizes.channels * size;
     for (const void *v : q) bits |= (uintptr_t)v;

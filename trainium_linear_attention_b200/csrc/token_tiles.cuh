@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "tc_common.cuh"
 #include "tma_host.cuh"
 
@@ -61,18 +62,34 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // Tokens [t0, t0 + 64 / ch * kL) of `row0` (the tensor at this sequence's first
-// token and this CTA's first channel), all of which the sequence has; channels beyond
-// `width` are set to zero and not read.
+// token and this CTA's first channel); tokens outside [0, len) and channels beyond
+// `width` are set to zero and not read.  kN bytes a copy.
 template <typename T, int kL, int kN>
-__device__ __forceinline__ void copy_tile(T *tile, const T *row0, int64_t st, int t0, int ch,
+__device__ __forceinline__ void copy_tile(T *tile, const T *row0, int64_t st, int t0, int len, int ch,
                                           int width) {
   constexpr int kPer = kN / (int)sizeof(T);  // elements of a copy
-#pragma unroll 4
-  for (int n = threadIdx.x & 31; n < 64 * kL / kPer; n += 32) {
-    const int at = n * kPer, k = at / 64, part = at % 64 / ch, q = at % ch;
-    const T *src = row0 + (int64_t)(t0 + part * kL + k) * st + q;
+  const int lane = threadIdx.x & 31;
+  if constexpr (kPer >= 2) {  // a lane's copies are whole rows of 64 apart
+    const int at = lane * kPer, q = at % ch;
+    int k = at / 64, t = t0 + at % 64 / ch * kL + k;
+    const T *src = row0 + (int64_t)t * st + q;
+    uint32_t dst = (uint32_t)__cvta_generic_to_shared(tile + at);
     const int bytes = max(0, min(kN, (width - q) * (int)sizeof(T)));
-    copy_async<kN>((uint32_t)__cvta_generic_to_shared(tile + at), bytes ? src : row0, bytes);
+    const int64_t step = st * (kPer / 2);
+#pragma unroll
+    for (int n = 0; n < kL * 2 / kPer; ++n) {
+      const bool in = bytes > 0 && (unsigned)t < (unsigned)len;
+      copy_async<kN>(dst, in ? src : row0, in ? bytes : 0);
+      src += step, dst += 32 * kN, t += kPer / 2;
+    }
+  } else {
+#pragma unroll 4
+    for (int n = lane; n < 64 * kL; n += 32) {
+      const int t = t0 + n % 64 / ch * kL + n / 64, q = n % ch;
+      const bool in = q < width && (unsigned)t < (unsigned)len;
+      copy_async<kN>((uint32_t)__cvta_generic_to_shared(tile + n),
+                     in ? row0 + (int64_t)t * st + q : row0, in ? kN : 0);
+    }
   }
 }
 
@@ -125,19 +142,34 @@ __device__ __forceinline__ void align_shifted(__nv_bfloat16 *tile, const __nv_bf
   }
 }
 
-// A tile that the sequence ends in, or that lies beside it: tokens outside [0, len)
-// become `outside` and are not read.
-template <typename T, int kL>
-__device__ __forceinline__ void ragged_tile(T *tile, const T *row0, int64_t st, int t0, int len,
-                                            int ch, int width, float outside) {
-  const T none = from_f32<T>(outside);
-#pragma unroll 8
-  for (int at = threadIdx.x & 31; at < 64 * kL; at += 32) {
-    const int t = t0 + at % 64 / ch * kL + at / 64, q = at % ch;
-    T v = none;
-    if (t >= 0 && t < len && q < width) v = row0[(int64_t)t * st + q];
-    tile[at] = v;
+// A pair of channels at p, the second of which may be beyond the row.
+template <typename T>
+__device__ __forceinline__ float2 pair_at(const T *p, bool wide, bool second) {
+  if (wide && second) return load_two(p);
+  return make_float2(to_f32(p[0]), second ? to_f32(p[1]) : 0.f);
+}
+// The same by elements.
+template <int kL>
+__device__ __noinline__ void load_elements(__nv_bfloat16 *tile, const __nv_bfloat16 *row0, int64_t st,
+                                           int t0, int len, int ch, int width) {
+  const int lane = threadIdx.x & 31, half = ch / 2, q = 2 * (lane & (half - 1));
+  const int first = t0 + lane / half * kL;
+  float2 v[kL];
+#pragma unroll
+  for (int k = 0; k < kL; ++k) {
+    v[k] = two(0.f);
+    if ((unsigned)(first + k) < (unsigned)len && q < width)
+      v[k] = pair_at(row0 + (int64_t)(first + k) * st + q, false, q + 1 < width);
   }
+#pragma unroll
+  for (int k = 0; k < kL; ++k) store_two(tile + 64 * k + 2 * lane, v[k], true, true);
+}
+// The tokens of a tile outside [0, len) become `value`.
+template <typename T, int kL>
+__device__ __forceinline__ void fill_outside(T *tile, int t0, int len, int ch, float value) {
+  const int lane = threadIdx.x & 31, first = t0 + lane / (ch / 2) * kL;
+  for (int k = 0; k < kL; ++k)
+    if ((unsigned)(first + k) >= (unsigned)len) store_two(tile + 64 * k + 2 * lane, two(value), true, true);
 }
 
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, uint64_t *bar, int x,
@@ -153,6 +185,7 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
 struct TileLaunch {
   int ch;       // channels of a CTA
   int copy;     // kAsync: bytes of a copy, 4 or 8
+  bool wide;    // pairs of channels start at their own size
   int *err;     // the library's device error word
 };
 
@@ -167,6 +200,7 @@ struct WarpTiles {
   const CUtensorMap *maps;
   int64_t ib;
   int c0, ch, width, copy;
+  bool wide;
   TokenSizes sizes;
   uint32_t phases;          // kTma: a bit per stage
 
@@ -176,9 +210,13 @@ struct WarpTiles {
   __device__ __forceinline__ const T *row0(int n) const {
     return (const T *)views[n]->p + ib * views[n]->sb + c0;
   }
-  // Starts to fetch the tiles from token t0 on, all of whose tokens the sequence has.
-  __device__ __forceinline__ void fetch(int t0, int stage) const {
-    if constexpr (kF == Fetch::kTma) {
+  __device__ __forceinline__ bool whole(int t0, int len) const {
+    return t0 >= 0 && t0 + 64 / ch * kL <= len;
+  }
+  // Starts to fetch the tiles from token t0 on; a sequence of `len` tokens may end in
+  // them, or not reach them.
+  __device__ __forceinline__ void fetch(int t0, int len, int stage) const {
+    if (kF == Fetch::kTma && whole(t0, len)) {
       if ((threadIdx.x & 31) == 0) {
         uint64_t *bar = full + stage * full_step;
         tc::mbar_arrive_expect_tx(bar, kIn * 64 * kL * sizeof(T));
@@ -186,33 +224,35 @@ struct WarpTiles {
         for (int n = 0; n < kIn; ++n)
           tma_load_4d(tile(stage, n), maps + n, bar, c0, t0 / kL, 0, (int)ib);
       }
-    } else {
+    } else if (kF == Fetch::kShifted && whole(t0, len)) {
 #pragma unroll
       for (int n = 0; n < kIn; ++n) {
         const int64_t st = views[n]->st;
-        if constexpr (kF == Fetch::kShifted) {
-          const uintptr_t begin = (uintptr_t)views[n]->p;
-          const uintptr_t end = begin + 2 * ((sizes.batch - 1) * views[n]->sb +
-                                             (sizes.tokens - 1) * st + sizes.channels);
+        const uintptr_t begin = (uintptr_t)views[n]->p;
+        const uintptr_t end =
+            begin + 2 * ((sizes.batch - 1) * views[n]->sb + (sizes.tokens - 1) * st + sizes.channels);
+        if constexpr (kF == Fetch::kShifted)
           copy_shifted<kL>(tile(stage, n), row0(n), st, t0, ch, begin, end);
-        } else if (copy == 8) {
-          copy_tile<T, kL, 8>(tile(stage, n), row0(n), st, t0, ch, width);
-        } else {
-          copy_tile<T, kL, 4>(tile(stage, n), row0(n), st, t0, ch, width);
-        }
+      }
+    } else if (kF != Fetch::kShifted && t0 < len && t0 + 64 / ch * kL > 0) {
+#pragma unroll
+      for (int n = 0; n < kIn; ++n) {
+        if (copy == 8) copy_tile<T, kL, 8>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
+        else copy_tile<T, kL, 4>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
       }
     }
+    if (kF != Fetch::kTma) copy_commit();
   }
-  // Closes a step's fetches (also where there were none).
-  __device__ __forceinline__ void commit() const {
-    if constexpr (kF != Fetch::kTma) copy_commit();
-  }
-  // Waits for what was fetched from t0 on.
-  __device__ __forceinline__ void wait(int t0, int stage, volatile int *abort) {
-    if constexpr (kF == Fetch::kTma) {
-      tc::mbar_wait(full + stage * full_step, phases >> stage & 1, abort);
-      phases ^= 1u << stage;
-    } else {
+  // Waits for what was fetched from t0 on.  Tokens that the sequence does not have are
+  // zero, and those of tensor 1 `outside`.
+  __device__ __forceinline__ void wait(int t0, int len, int stage, float outside,
+                                       volatile int *abort) {
+    if (whole(t0, len)) {
+      if constexpr (kF == Fetch::kTma) {
+        tc::mbar_wait(full + stage * full_step, phases >> stage & 1, abort);
+        phases ^= 1u << stage;
+        return;
+      }
       copy_wait<kStages - 1>();
       __syncwarp();
       if constexpr (kF == Fetch::kShifted) {
@@ -220,12 +260,20 @@ struct WarpTiles {
         for (int n = 0; n < kIn; ++n)
           align_shifted<kL>(tile(stage, n), row0(n), views[n]->st, t0, ch);
       }
+      return;
     }
-  }
-  // Instead of both, for tiles that the sequence does not fill.  A __syncwarp()
-  // follows.
-  __device__ __forceinline__ void load_ragged(int t0, int len, int stage, int n, float outside) const {
-    ragged_tile<T, kL>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width, outside);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    const bool none = t0 >= len || t0 + 64 / ch * kL <= 0;
+#pragma unroll
+    for (int n = 0; n < kIn; ++n) {
+      if constexpr (kF == Fetch::kShifted) load_elements<kL>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
+      if ((none && kF != Fetch::kShifted) || (n == 1 && outside != 0.f))
+        fill_outside<T, kL>(tile(stage, n), t0, len, ch, n == 1 ? outside : 0.f);
+    }
+    // (ahead of the next copy into these tiles)
+    if (kF == Fetch::kTma) tc::fence_proxy_async_smem();
+    __syncwarp();
   }
 };
 
@@ -260,21 +308,20 @@ inline bool tile_map(CUtensorMap *map, const TokenView &v, const TokenSizes &s, 
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// The fetch for all of `views` (null pointers: absent tensors), and the bytes of a
-// copy should it be kAsync.
+// The fetch for all of `views` (null pointers: absent tensors).
 inline Fetch fetch_of(const TokenView *const *views, int n, const TokenSizes &s, int size, int l,
-                      int *copy) {
+                      TileLaunch *launch) {
   bool tma = encode_fn() != nullptr && s.tokens >= l;
-  *copy = 16;
+  int least = 16;
   for (int i = 0; i < n; ++i) {
     if (!views[i]->p) continue;
     tma = tma && tma_view(*views[i], s, size, l);
     const int bytes = row_bytes(*views[i], size);
-    *copy = bytes < *copy ? bytes : *copy;
+    least = bytes < least ? bytes : least;
   }
-  const Fetch f = tma ? Fetch::kTma : *copy < 4 ? Fetch::kShifted : Fetch::kAsync;
-  *copy = *copy >= 8 ? 8 : 4;
-  return f;
+  launch->copy = least >= 8 ? 8 : 4;
+  launch->wide = least >= 2 * size;
+  return tma ? Fetch::kTma : least < 4 ? Fetch::kShifted : Fetch::kAsync;
 }
 
 }  // namespace la
