@@ -142,6 +142,14 @@ __device__ __forceinline__ void align_shifted(__nv_bfloat16 *tile, const __nv_bf
   }
 }
 
+// The same out of the way of a loop that copies whole tiles by other means.
+template <typename T, int kL>
+__device__ __noinline__ void copy_edge(T *tile, const T *row0, int64_t st, int t0, int len, int ch,
+                                       int width, int copy) {
+  if (copy == 8) copy_tile<T, kL, 8>(tile, row0, st, t0, len, ch, width);
+  else copy_tile<T, kL, 4>(tile, row0, st, t0, len, ch, width);
+}
+
 // A pair of channels at p, the second of which may be beyond the row.
 template <typename T>
 __device__ __forceinline__ float2 pair_at(const T *p, bool wide, bool second) {
@@ -166,7 +174,7 @@ __device__ __noinline__ void load_elements(__nv_bfloat16 *tile, const __nv_bfloa
 }
 // The tokens of a tile outside [0, len) become `value`.
 template <typename T, int kL>
-__device__ __forceinline__ void fill_outside(T *tile, int t0, int len, int ch, float value) {
+__device__ __noinline__ void fill_outside(T *tile, int t0, int len, int ch, float value) {
   const int lane = threadIdx.x & 31, first = t0 + lane / (ch / 2) * kL;
   for (int k = 0; k < kL; ++k)
     if ((unsigned)(first + k) >= (unsigned)len) store_two(tile + 64 * k + 2 * lane, two(value), true, true);
@@ -237,8 +245,12 @@ struct WarpTiles {
     } else if (kF != Fetch::kShifted && t0 < len && t0 + 64 / ch * kL > 0) {
 #pragma unroll
       for (int n = 0; n < kIn; ++n) {
-        if (copy == 8) copy_tile<T, kL, 8>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
-        else copy_tile<T, kL, 4>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
+        if constexpr (kF == Fetch::kTma)
+          copy_edge<T, kL>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width, copy);
+        else if (copy == 8)
+          copy_tile<T, kL, 8>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
+        else
+          copy_tile<T, kL, 4>(tile(stage, n), row0(n), views[n]->st, t0, len, ch, width);
       }
     }
     if (kF != Fetch::kTma) copy_commit();
