@@ -37,10 +37,8 @@ struct RecurCall {
 
 // Tokens from one saved state to the next: those of a forward thread's step.
 constexpr int kRecurCheck = 16;
-constexpr int kRecurThreads = 256;
 constexpr int kRecurMaxCluster = 8;
 
-constexpr int kRecurWarps = kRecurThreads / 32;
 
 // The floor of 1 - a^2 under a root or a division, where it meets a zero.
 constexpr float kBetaFloor = 1e-36f;
@@ -181,22 +179,28 @@ __device__ __forceinline__ void store_remote(float4 *p, uint64_t *bar, uint32_t 
       : "memory");
 }
 
-// Channels of a CTA and CTAs along the tokens for a size: a CTA for every SM from
-// narrower channel groups, and only then from clusters along the tokens, each of
-// whose CTAs has tokens of its own (l for each of its parts).  A cluster's
-// exchange at every step costs more than an idle SM: 16384 x 2048 in 65 us by 128
-// CTAs of 16 channels, in 86 by 256 in clusters of two; 2048 x 1024 in 12.0 us by 64
-// CTAs, 10.7 by 128 in clusters of two.
+// Channels of a CTA, CTAs along the tokens and warps of a CTA for a size.  A CTA for
+// every SM comes from narrower channel groups, and only then from clusters along
+// the tokens, each of whose CTAs has tokens of its own (l for each of its parts):
+// a cluster's exchange at every step costs more than an idle SM (16384 x 2048 in
+// 69 us by 128 CTAs of 16 channels, in 85 by 256 in clusters of two).  One CTA of 16
+// warps on most SMs beats two of 8 on some, where instructions bound it (`heavy`: 8 x
+// 32768 x 1024 by 128 CTAs of 64 channels and 16 warps in 384 us, by 256 of 32 and 8
+// in 429; the gradient of 4 x 4096 x 1024 in 71 and 73); where memory does, all SMs'
+// loads count (8 x 8192 x 1024 without a decay: 84 and 72).  `roomy`: 16 warps' tiles
+// fit (bf16).
 struct RecurShape {
-  int ch, cluster;
+  int ch, cluster, warps;
 };
-inline RecurShape recur_shape(const TokenSizes &z, int sm_count, int l, int widest) {
-  RecurShape s{widest, 1};
+inline RecurShape recur_shape(const TokenSizes &z, int sm_count, int l, int widest, bool heavy,
+                              bool roomy) {
+  RecurShape s{widest, 1, 8};
   auto ctas = [&] { return z.batch * ((z.channels + s.ch - 1) / s.ch) * s.cluster; };
-  while (s.ch > 16 && ctas() < sm_count) s.ch /= 2;
-  while (s.cluster < kRecurMaxCluster && ctas() * 2 <= sm_count &&
-         z.tokens > (int64_t)s.cluster * (64 / s.ch) * l * kRecurWarps)
-    s.cluster *= 2;
+  auto tokens = [&] { return (int64_t)s.cluster * (64 / s.ch) * l * 8; };  // of 8 warps' step
+  const int64_t enough = heavy && roomy ? sm_count * 4 / 5 : sm_count;
+  while (s.ch > 16 && ctas() < enough) s.ch /= 2;
+  while (s.cluster < kRecurMaxCluster && ctas() * 2 <= sm_count && z.tokens > tokens()) s.cluster *= 2;
+  if (heavy && roomy && s.cluster == 1 && ctas() <= sm_count && z.tokens > tokens()) s.warps = 16;
   return s;
 }
 
@@ -214,14 +218,14 @@ inline Fetch recur_fetch(const RecurCall &p, const TokenView *const *views, int 
 
 template <class Kernel>
 int launch_clusters(Kernel kernel, const RecurCall &p, const RecurLaunch &l, const TileMaps &maps,
-                    int smem, cudaStream_t s) {
+                    int threads, int smem, cudaStream_t s) {
   const int64_t grid = p.sizes.batch * ((p.sizes.channels + l.tile.ch - 1) / l.tile.ch) * l.cluster;
   if (grid > INT32_MAX) return LA_ERR_UNSUPPORTED;
   const int st = allow_dynamic_smem((const void *)kernel, smem);
   if (st != LA_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kRecurThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr;

@@ -30,27 +30,28 @@ namespace {
 constexpr int kL = 8;       // tokens of a thread and step
 constexpr int kStages = 2;   // tiles of a warp
 
+template <int kWarps>
 struct Exchange {
   // What the warp behind hands to each warp: without a cluster a H (in xy), else the
   // summary (A, A, R, R) of the CTA's tokens behind its own.
-  float4 behind[kRecurWarps][32];
+  float4 behind[kWarps][32];
   float4 csums[2][kRecurMaxCluster][32];  // summaries of the cluster's CTAs
-  float2 sums[kRecurWarps][32];
-  uint64_t full[kStages][kRecurWarps], handed[kRecurWarps], arrived[2];
+  float2 sums[kWarps][32];
+  uint64_t full[kStages][kWarps], handed[kWarps], arrived[2];
   int abort;
 };
 
-template <typename T, bool kDecay, bool kInput, Fetch kF>
-__global__ void __launch_bounds__(kRecurThreads, 2)
+template <typename T, bool kDecay, bool kInput, Fetch kF, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
 recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ TileMaps maps) {
-  constexpr int kIn = kInput ? 4 : 3, kLast = kRecurWarps - 1;
+  constexpr int kIn = kInput ? 4 : 3, kLast = kWarps - 1;
   static_assert(kRecurCheck == 2 * kL, "every other part starts at a saved state");
   extern __shared__ __align__(1024) uint8_t smem[];
   column_sum_may_start();
   const int cluster = l.cluster, ch = l.tile.ch, half = ch / 2, parts = 64 / ch;
   const int channels = p.sizes.channels;
   const int elems = tile_elems<kF>(kL, ch);
-  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * elems * sizeof(T));
+  Exchange<kWarps> &ex = *(Exchange<kWarps> *)(smem + kStages * kIn * kWarps * elems * sizeof(T));
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int groups = (channels + ch - 1) / ch;
   const int64_t ib = blockIdx.x / cluster / groups;
@@ -63,10 +64,10 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
 
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
-      (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
+      (T *)smem + warp * kIn * elems, kWarps * kIn * elems, elems, &ex.full[0][warp], kWarps,
       views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
   const int rows = parts * kL;            // tokens of a warp and step
-  const int block_rows = kRecurWarps * rows;
+  const int block_rows = kWarps * rows;
   const int blocks = (len + block_rows - 1) / block_rows;
   const int steps = (blocks + cluster - 1) / cluster;
   auto block_of = [&](int i) { return blocks - 1 - (i * cluster + rank); };  // < 0: none
@@ -83,7 +84,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     }
   }
   if (threadIdx.x == 0) {
-    for (int w = 0; w < kRecurWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       for (int j = 0; j < kStages; ++j) tc::mbar_init(&ex.full[j][w], 1);
       tc::mbar_init(&ex.handed[w], 1);
     }
@@ -242,7 +243,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   }
   if (p.d_init && rank == 0 && warp == 0 && part == 0 && live)
     store_two(p.d_init + ib * channels + c, carry, pairs, second);
-  const int slots = kRecurWarps * parts;
+  const int slots = kWarps * parts;
   for (int64_t t = len + rank * slots + warp * parts + part; t < p.sizes.tokens && live; t += cluster * slots) {
     const int64_t o = origin + t * channels;
     store_two((T *)p.dx + o, two(0.f), pairs, second);
@@ -260,7 +261,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     if (warp == 0 && part == 0 && live) {
       float2 v = two(0.f);
 #pragma unroll
-      for (int j = 0; j < kRecurWarps; ++j) v = __fadd2_rn(v, ex.sums[j][pair]);
+      for (int j = 0; j < kWarps; ++j) v = __fadd2_rn(v, ex.sums[j][pair]);
       store_two(p.partial + (ib * cluster + rank) * channels + c, v, channels % 2 == 0, second);
     }
   }
@@ -271,9 +272,13 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   }
 }
 
-RecurShape shape_of(const TokenSizes &z, int sm_count) { return recur_shape(z, sm_count, kL, 32); }
+// (The rows of `partial` may not go by the inputs' alignment: the shape is that of 16
+// warps' tiles whether they are used or not.)
+RecurShape shape_of(const TokenSizes &z, int sm_count) {
+  return recur_shape(z, sm_count, kL, 32, true, true);
+}
 
-template <typename T, bool kDecay, bool kInput, Fetch kF>
+template <typename T, bool kDecay, bool kInput, Fetch kF, int kWarps = 8>
 int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
   constexpr int kIn = kInput ? 4 : 3;
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
@@ -282,9 +287,9 @@ int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
     if (!tile_map(&maps.m[n], *views[n], p.sizes, sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16,
                   l.tile.ch, kL))
       return LA_ERR_CUDA;
-  const int smem = kStages * kIn * kRecurWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
-                   (int)sizeof(Exchange);
-  return launch_clusters(recur_bwd_kernel<T, kDecay, kInput, kF>, p, l, maps, smem, s);
+  const int smem = kStages * kIn * kWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
+                   (int)sizeof(Exchange<kWarps>);
+  return launch_clusters(recur_bwd_kernel<T, kDecay, kInput, kF, kWarps>, p, l, maps, 32 * kWarps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
@@ -292,10 +297,12 @@ int launch_by_fetch(const RecurCall &p, const RecurShape &shape, cudaStream_t s)
   RecurLaunch l{{shape.ch, 0, false, device_error_word()}, shape.cluster};
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
   const Fetch f = recur_fetch(p, views, 4, sizeof(T), kL, &l.tile);
-  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
   if constexpr (sizeof(T) == 2) {
+    if (f == Fetch::kTma && shape.warps == 16)
+      return launch<T, kDecay, kInput, Fetch::kTma, 16>(p, l, s);
     if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);
   }
+  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
   return launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
 }
 

@@ -32,24 +32,25 @@ namespace {
 constexpr int kL = 16;       // tokens of a thread and step
 constexpr int kStages = 2;   // tiles of a warp
 
+template <int kWarps>
 struct Exchange {
   // What the warp before hands to each warp: without a cluster the state (in
   // xy), else the summary (A, A, E, E) of the CTA's tokens before its own.
-  float4 before[kRecurWarps][32];
+  float4 before[kWarps][32];
   float4 csums[2][kRecurMaxCluster][32];  // summaries of the cluster's CTAs
-  uint64_t full[kStages][kRecurWarps], handed[kRecurWarps], arrived[2];
+  uint64_t full[kStages][kWarps], handed[kWarps], arrived[2];
   int abort;
 };
 
-template <typename T, bool kDecay, bool kInput, Fetch kF>
-__global__ void __launch_bounds__(kRecurThreads, 2)
+template <typename T, bool kDecay, bool kInput, Fetch kF, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
 recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ TileMaps maps) {
-  constexpr int kIn = kInput ? 3 : 2, kLast = kRecurWarps - 1;
+  constexpr int kIn = kInput ? 3 : 2, kLast = kWarps - 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int cluster = l.cluster, ch = l.tile.ch, half = ch / 2, parts = 64 / ch;
   const int channels = p.sizes.channels;
   const int elems = tile_elems<kF>(kL, ch);
-  Exchange &ex = *(Exchange *)(smem + kStages * kIn * kRecurWarps * elems * sizeof(T));
+  Exchange<kWarps> &ex = *(Exchange<kWarps> *)(smem + kStages * kIn * kWarps * elems * sizeof(T));
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int groups = (channels + ch - 1) / ch;
   const int64_t ib = blockIdx.x / cluster / groups;
@@ -62,12 +63,12 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
 
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
-      (T *)smem + warp * kIn * elems, kRecurWarps * kIn * elems, elems, &ex.full[0][warp], kRecurWarps,
+      (T *)smem + warp * kIn * elems, kWarps * kIn * elems, elems, &ex.full[0][warp], kWarps,
       views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
   const int rows = parts * kL;                      // tokens of a warp and step
-  const int step = cluster * kRecurWarps * rows;    // of all
+  const int step = cluster * kWarps * rows;    // of all
   const int steps = (len + step - 1) / step;
-  const int first = (rank * kRecurWarps + warp) * rows;
+  const int first = (rank * kWarps + warp) * rows;
   auto fetch = [&](int i, int stage) { tiles.fetch(i * step + first, i < steps ? len : 0, stage); };
 
   float2 lambda = two(0.f), carry = two(0.f);
@@ -79,7 +80,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     }
   }
   if (threadIdx.x == 0) {
-    for (int w = 0; w < kRecurWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       for (int j = 0; j < kStages; ++j) tc::mbar_init(&ex.full[j][w], 1);
       tc::mbar_init(&ex.handed[w], 1);
     }
@@ -190,7 +191,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   if (p.final_state && rank == 0 && warp == kLast && part == 0 && live)
     store_two(p.final_state + ib * channels + c, carry, pairs, second);
   // zeros behind the sequence
-  const int slots = kRecurWarps * parts;
+  const int slots = kWarps * parts;
   for (int64_t t = len + rank * slots + warp * parts + part; t < p.sizes.tokens && live; t += cluster * slots)
     store_two(out + t * channels, two(0.f), pairs, second);
   if (ex.abort) {
@@ -200,7 +201,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   }
 }
 
-template <typename T, bool kDecay, bool kInput, Fetch kF>
+template <typename T, bool kDecay, bool kInput, Fetch kF, int kWarps = 8>
 int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
   constexpr int kIn = kInput ? 3 : 2;
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
@@ -209,9 +210,9 @@ int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
     if (!tile_map(&maps.m[n], *views[n], p.sizes, sizeof(T) == 4 ? LA_DTYPE_FLOAT32 : LA_DTYPE_BFLOAT16,
                   l.tile.ch, kL))
       return LA_ERR_CUDA;
-  const int smem = kStages * kIn * kRecurWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
-                   (int)sizeof(Exchange);
-  return launch_clusters(recur_fwd_kernel<T, kDecay, kInput, kF>, p, l, maps, smem, s);
+  const int smem = kStages * kIn * kWarps * tile_elems<kF>(kL, l.tile.ch) * (int)sizeof(T) +
+                   (int)sizeof(Exchange<kWarps>);
+  return launch_clusters(recur_fwd_kernel<T, kDecay, kInput, kF, kWarps>, p, l, maps, 32 * kWarps, smem, s);
 }
 
 template <typename T, bool kDecay, bool kInput>
@@ -219,14 +220,18 @@ int launch_by_fetch(const RecurCall &p, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  const RecurShape shape = recur_shape(p.sizes, info.sm_count, kL, 64);
-  RecurLaunch l{{shape.ch, 0, false, device_error_word()}, shape.cluster};
+  RecurLaunch l{{0, 0, false, device_error_word()}, 1};
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
   const Fetch f = recur_fetch(p, views, 3, sizeof(T), kL, &l.tile);
-  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
+  const RecurShape shape =
+      recur_shape(p.sizes, info.sm_count, kL, 64, kDecay, f == Fetch::kTma && sizeof(T) == 2);
+  l.tile.ch = shape.ch, l.cluster = shape.cluster;
   if constexpr (sizeof(T) == 2) {
+    if (f == Fetch::kTma && shape.warps == 16)
+      return launch<T, kDecay, kInput, Fetch::kTma, 16>(p, l, s);
     if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);
   }
+  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
   return launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
 }
 
