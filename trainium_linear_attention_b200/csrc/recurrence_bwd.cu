@@ -109,9 +109,18 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     return make_float2(v[0], second ? v[1] : 0.f);
   };
   float2 start = saved(0);
+  // Without a cluster the chain starts at the warp with the last token: the first
+  // step's warps behind it have nothing to do, and they and it are not handed anything then.
+  const int last = cluster > 1 ? kLast : max(len - 1, 0) % block_rows / rows;
   int stage = 0;
   for (int i = 0; i < steps; ++i) {
     const int buf = i & 1;
+    if (i == 0 && warp > last) {
+      start = saved(1);
+      fetch(kStages, 0);
+      stage = 1;
+      continue;
+    }
     const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *ds = tiles.tile(stage, 2),
             *us = tiles.tile(stage, kIn - 1);
     const int block = block_of(i);
@@ -151,8 +160,8 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     const int next = warp == 0 ? kLast : warp - 1;
     float2 ap = two(1.f), rp = two(0.f);  // of the CTA's warps behind (with a cluster)
     if (cluster == 1) {
-      if (warp < kLast || i > 0) {
-        tc::mbar_wait(&ex.handed[warp], (uint32_t)(warp < kLast ? i : i - 1) & 1, &ex.abort);
+      if (warp < last || i > 0) {
+        tc::mbar_wait(&ex.handed[warp], (uint32_t)(warp < last ? i : i - 1) & 1, &ex.abort);
         const float4 v = ex.behind[warp][pair];
         carry = make_float2(v.x, v.y);
       }

@@ -102,6 +102,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     const int buf = i & 1;
     const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *us = tiles.tile(stage, kIn - 1);
     const int row0 = i * step + first, t0 = row0 + part * kL;
+    if (cluster == 1 && row0 >= len) break;  // (nobody waits for the last step's other warps)
     const bool whole = tiles.whole(row0, len);
     // tokens beyond the sequence keep the state
     tiles.wait(row0, len, stage, kDecay ? -INFINITY : INFINITY, &ex.abort);
@@ -188,7 +189,9 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
       }
     }
   }
-  if (p.final_state && rank == 0 && warp == kLast && part == 0 && live)
+  // by the warp with the last token; with a cluster all warps have folded all summaries
+  const int last = cluster > 1 ? kLast : max(len - 1, 0) % step / rows;
+  if (p.final_state && rank == 0 && warp == last && part == 0 && live)
     store_two(p.final_state + ib * channels + c, carry, pairs, second);
   // zeros behind the sequence
   const int slots = kWarps * parts;
