@@ -234,8 +234,11 @@ int launch_by_fetch(const RecurCall &p, cudaStream_t s) {
       return launch<T, kDecay, kInput, Fetch::kTma, 16>(p, l, s);
     if (f == Fetch::kShifted) return launch<T, kDecay, kInput, Fetch::kShifted>(p, l, s);
   }
-  if (f == Fetch::kTma) return launch<T, kDecay, kInput, Fetch::kTma>(p, l, s);
-  return launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
+  if (shape.warps == 2)
+    return f == Fetch::kTma ? launch<T, kDecay, kInput, Fetch::kTma, 2>(p, l, s)
+                            : launch<T, kDecay, kInput, Fetch::kAsync, 2>(p, l, s);
+  return f == Fetch::kTma ? launch<T, kDecay, kInput, Fetch::kTma>(p, l, s)
+                          : launch<T, kDecay, kInput, Fetch::kAsync>(p, l, s);
 }
 
 template <typename T>
