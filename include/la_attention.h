@@ -345,7 +345,7 @@ int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight,
  * state and no gates.
  * ------------------------------------------------------------------------- */
 /* Bytes of `saved` (what la_recurrence_fwd keeps for the gradient) and of
- * la_recurrence_bwd's workspace, which only d_log_decay needs. */
+ * la_recurrence_bwd's workspace, which only d_log_decay needs (16-byte aligned). */
 int la_recurrence_plan(int64_t batch, int64_t tokens, int64_t channels, size_t *saved_bytes,
                        size_t *workspace_bytes);
 
@@ -394,7 +394,7 @@ int la_short_conv_fwd(const void *x, const int64_t *x_strides, const void *weigh
                       int64_t batch, int64_t tokens, int64_t channels, int64_t taps, int silu,
                       int dtype, void *stream);
 
-/* Bytes of workspace la_short_conv_bwd needs for d_weight or d_bias. */
+/* Bytes of workspace (16-byte aligned) la_short_conv_bwd needs for d_weight or d_bias. */
 int la_short_conv_workspace_size(int64_t batch, int64_t tokens, int64_t channels, int64_t taps,
                                  size_t *bytes);
 
@@ -426,8 +426,8 @@ int la_short_conv_step(const void *x, int64_t x_stride, const void *weight, cons
  * differences.  x, gate and d_out are rows (shape[0], shape[1], channels) with
  * a dense last dimension and strides {0, 1} in elements; out and the gradients
  * are contiguous.  weight (null: ones) and bias (null: zeros), (channels), are
- * fp32 or bf16 by weight_dtype.  stats (null, or fp32 (rows, groups, 2)) is what
- * the gradient needs.  The reference has no norm.
+ * fp32 or bf16 by weight_dtype.  stats (null, or fp32 (rows, groups, 2),
+ * 8-byte aligned) is what the gradient needs.  The reference has no norm.
  * ------------------------------------------------------------------------- */
 int la_group_norm_fwd(const void *x, const int64_t *x_strides, const void *gate,
                       const int64_t *gate_strides, const void *weight, const void *bias,
@@ -435,7 +435,8 @@ int la_group_norm_fwd(const void *x, const int64_t *x_strides, const void *gate,
                       int64_t channels, int64_t groups, int silu, int dtype, float eps,
                       void *stream);
 
-/* Bytes of workspace la_group_norm_bwd needs for d_weight or d_bias on this device. */
+/* Bytes of workspace (16-byte aligned) la_group_norm_bwd needs for d_weight or
+ * d_bias on this device. */
 int la_group_norm_bwd_workspace_size(int64_t rows, int64_t channels, size_t *bytes);
 
 /* Gradients; d_gate with a gate; d_weight and d_bias (in weight_dtype, summed in

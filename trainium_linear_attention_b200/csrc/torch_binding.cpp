@@ -3,10 +3,10 @@
 //
 // These operators' kernels take a few microseconds at small sizes, and a
 // training step of a few tens; from Python (arguments through ctypes, the backward
-// pass on a thread that first has to get the interpreter) the host would take 125
-// us for a step that this file does in about half.  The entry points' addresses come
-// from the library that the package has loaded: there is one library, one set
-// of kernels and no other implementation.
+// pass on a thread that first has to get the interpreter) the host took 120
+// us for a step that takes 72 here, 47 of them the engine's own for an empty node.
+// The entry points' addresses come from the library that the package has loaded:
+// there is one library, one set of kernels and no other implementation.
 #include <torch/extension.h>
 
 #include <c10/cuda/CUDAGuard.h>
