@@ -340,7 +340,9 @@ int la_rms_norm_bwd(const void *s, const int64_t *s_strides, const void *weight,
  * device memory, taken into [0, tokens]: only so many tokens of a sequence are
  * read, its outputs and gradients behind them are zero, and its final state is
  * the one after them.  A value that is not finite reaches its channel's
- * outputs from its own token on.  The reference has no such recurrence;
+ * outputs from its own token on.  Here and below pointers lie at multiples of
+ * their elements' size, and nothing that is written overlaps another argument
+ * (a step's state apart).  The reference has no such recurrence;
  * its chunked kernel's (kernels/nki_attention_chunked.py:20-113) has a matrix for a
  * state and no gates.
  * ------------------------------------------------------------------------- */

@@ -210,6 +210,22 @@ def test_infinite_gates(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("b,t,c", [(4, 300, 1024), (8, 300, 1024), (1, 1100, 2048), (4, 289, 1016),
+                                   (1, 4100, 128), (700, 40, 72)])
+def test_shapes_of_launches(b, t, c):
+    """Channel groups of each width by CTAs of 16 warps, a cluster of 8, CTAs of 2 warps."""
+    for i, (decay, gate) in enumerate([(True, True), (True, False), (False, True)]):
+        s = make(b, t, c, torch.bfloat16, decay, gate, state=i != 1, lengths=i == 1, seed=i)
+        check_forward(s)
+        check_gradients(s, seed=i)
+        if i == 1:  # sequences that end in the first and last tokens of a step's tiles
+            ends = [0, 1, t, t - 1, 255, 256, 257, 129]
+            s["lengths"] = torch.tensor([min(ends[j % 8], t) for j in range(b)], device="cuda")
+            check_forward(s)
+            check_gradients(s, seed=i)
+
+
+@gpu
 def test_slow_decays():
     """1 - a below fp32's step next to 1: the memory is 2^30 tokens long."""
     n = 20000
@@ -510,6 +526,31 @@ def test_c_refusals():
     plan = lambda b, t, c: lib.la_recurrence_plan(b, t, c, N.ctypes.byref(a), N.ctypes.byref(w))
     assert plan(1, 1, 0) == bad and plan(0, 5, 8) == N.LA_OK and a.value == 0
     assert strides[0] == 8
+
+
+def test_c_refuses_pointers_between_elements():
+    """Numbers in place of pointers, which no call gets as far as reading."""
+    lib, bad = N.lib(), N.LA_ERR_INVALID_ARGUMENT
+    strides = (N.ctypes.c_int64 * 2)(8, 8)
+    st = N.ctypes.addressof(strides)
+
+    def calls(odd, dtype, at):
+        p = [odd if i == at else 16 for i in range(9)]
+        x, g, u, lam, init, out, final, saved, lengths = p
+        return (lib.la_recurrence_fwd(x, st, g, st, u, st, lam, init, lengths, 64, out, final,
+                                      saved, 1, 1, 8, dtype, None),
+                lib.la_recurrence_bwd(x, st, g, st, u, st, lam, saved, lengths, 64, out, st, init,
+                                      16, 16, 16, final, None, 1, 1, 8, dtype, None, 0, None))
+
+    for at in range(9):
+        odd, dtype = (20 if at == 8 else 18, 0)  # lengths of 8 bytes, all else of 4
+        assert calls(odd, dtype, at) == (bad, bad), at
+    for at in (0, 1, 2, 5):
+        assert calls(17, 1, at) == (bad, bad), at
+    step = lambda x=16, g=16, u=16, lam=16, state=16, out=16: lib.la_recurrence_step(
+        x, 8, g, 8, u, 8, lam, state, 8, out, 2, 8, 0, None)
+    assert step(x=18) == step(g=18) == step(u=18) == step(lam=18) == step(state=18) == step(
+        out=18) == bad
 
 
 @gpu

@@ -310,6 +310,23 @@ def test_refusals_on_the_cpu():
     assert strides[0] == 8 and shape[1] == 3
 
 
+def test_c_refuses_pointers_between_elements():
+    """Numbers in place of pointers, which no call gets as far as reading."""
+    lib, bad = N.lib(), N.LA_ERR_INVALID_ARGUMENT
+    strides, shape = (N.ctypes.c_int64 * 2)(8, 8), (N.ctypes.c_int64 * 2)(1, 3)
+    st, sh = N.ctypes.addressof(strides), N.ctypes.addressof(shape)
+
+    def fwd(x=16, gate=16, w=16, b=16, out=16, stats=16, dtype=0, wd=0):
+        return lib.la_group_norm_fwd(x, st, gate, st, w, b, wd, out, stats, sh, 8, 2, 0, dtype,
+                                     1e-5, None)
+
+    assert fwd(x=18) == fwd(gate=18) == fwd(w=18) == fwd(b=18) == fwd(out=18) == bad
+    assert fwd(stats=20) == fwd(x=17, dtype=1) == fwd(w=17, wd=1) == bad
+    bwd = lambda d=16, dx=16, dg=16, dw=16: lib.la_group_norm_bwd(
+        16, st, 16, st, 16, 16, 0, 16, d, st, dx, dg, dw, None, sh, 8, 2, 0, 0, None, 0, None)
+    assert bwd(d=18) == bwd(dx=18) == bwd(dg=18) == bwd(dw=18) == bad
+
+
 @gpu
 def test_refusals():
     s = make((2, 5, 8), 2, torch.bfloat16)

@@ -310,6 +310,20 @@ def test_refusals_on_the_cpu():
     assert strides[0] == 8
 
 
+def test_c_refuses_pointers_between_elements():
+    """Numbers in place of pointers, which no call gets as far as reading."""
+    lib, bad = N.lib(), N.LA_ERR_INVALID_ARGUMENT
+    strides = (N.ctypes.c_int64 * 2)(8, 8)
+    st = N.ctypes.addressof(strides)
+    fwd = lambda x=16, w=16, b=16, init=16, lens=None, dtype=0, wd=0: lib.la_short_conv_fwd(
+        x, st, w, b, wd, init, lens, 32, 16, None, 1, 1, 8, 4, 0, dtype, None)
+    assert fwd(x=18) == fwd(w=18) == fwd(b=18) == fwd(init=18) == fwd(lens=18) == bad
+    assert fwd(x=17, dtype=1) == fwd(w=17, wd=1) == bad
+    step = lambda x=16, w=16, state=16, out=16: lib.la_short_conv_step(
+        x, 8, w, None, 0, state, 24, out, 2, 8, 4, 0, 0, None)
+    assert step(x=18) == step(w=18) == step(state=18) == step(out=18) == bad
+
+
 @gpu
 def test_refusals():
     s = make(2, 5, 8, 4, torch.bfloat16)

@@ -12,6 +12,14 @@ namespace {
 
 bool valid_type(int t) { return t == LA_DTYPE_FLOAT32 || t == LA_DTYPE_BFLOAT16; }
 
+// Whether all of them start at an element's size.
+bool placed(int size, std::initializer_list<const void *> pointers) {
+  uintptr_t bits = 0;
+  for (const void *p : pointers) bits |= (uintptr_t)p;
+  return bits % size == 0;
+}
+int size_of(int dtype) { return dtype == LA_DTYPE_FLOAT32 ? 4 : 2; }
+
 // Sizes whose elements, and the bytes of a few tensors of them, fit 63 bits.
 bool fits(int64_t batch, int64_t tokens, int64_t channels) {
   constexpr int64_t kMost = INT64_MAX / 64;
@@ -50,7 +58,8 @@ int check_sizes(int64_t batch, int64_t tokens, int64_t channels, int dtype) {
 }
 
 int check_lengths(const void *lengths, int bits) {
-  return lengths && bits != 32 && bits != 64 ? LA_ERR_INVALID_ARGUMENT : LA_OK;
+  if (!lengths) return LA_OK;
+  return (bits == 32 || bits == 64) && placed(bits / 8, {lengths}) ? LA_OK : LA_ERR_INVALID_ARGUMENT;
 }
 
 int zero(void *p, int64_t bytes, cudaStream_t s) {
@@ -97,7 +106,9 @@ int la_recurrence_fwd(const void *x, const int64_t *x_strides, const void *gate,
   cudaStream_t s = (cudaStream_t)stream;
   if (!tokens) return copy_or_zero(final_state, init_state, batch * channels * 4, s);
   if (!x || !gate || !out || !valid_strides(x_strides) || !valid_strides(gate_strides) ||
-      (input_gate && !valid_strides(input_strides)))
+      (input_gate && !valid_strides(input_strides)) ||
+      !placed(size_of(dtype), {x, gate, input_gate, out}) ||
+      !placed(4, {log_decay, init_state, final_state, saved}))
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
@@ -131,7 +142,9 @@ int la_recurrence_bwd(const void *x, const int64_t *x_strides, const void *gate,
   }
   if (!x || !gate || !saved || !d_out || !dx || !d_gate || !valid_strides(x_strides) ||
       !valid_strides(gate_strides) || !valid_strides(d_out_strides) ||
-      (input_gate && (!valid_strides(input_strides) || !d_input_gate)))
+      (input_gate && (!valid_strides(input_strides) || !d_input_gate)) ||
+      !placed(size_of(dtype), {x, gate, input_gate, d_out, dx, d_gate, d_input_gate}) ||
+      !placed(4, {log_decay, saved, d_final_state, d_log_decay, d_init_state}))
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
@@ -164,7 +177,8 @@ int la_recurrence_step(const void *x, int64_t x_stride, const void *gate, int64_
   if (st != LA_OK) return st;
   if (!batch) return LA_OK;
   if (!x || !gate || !state || !out || x_stride < 0 || gate_stride < 0 || input_stride < 0 ||
-      (batch > 1 && state_stride < channels))
+      (batch > 1 && state_stride < channels) ||
+      !placed(size_of(dtype), {x, gate, input_gate, out}) || !placed(4, {log_decay, state}))
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
@@ -192,7 +206,9 @@ static int conv_call(ConvCall *c, const void *x, const int64_t *x_strides, const
   if (!valid_type(weight_dtype)) return LA_ERR_INVALID_ARGUMENT;
   if (taps < kConvMinTaps || taps > kConvMaxTaps) return LA_ERR_UNSUPPORTED;
   if (!batch) return LA_OK;
-  if ((tokens && (!x || !valid_strides(x_strides))) || !weight) return LA_ERR_INVALID_ARGUMENT;
+  if ((tokens && (!x || !valid_strides(x_strides))) || !weight ||
+      !placed(size_of(dtype), {x, init_state}) || !placed(size_of(weight_dtype), {weight, bias}))
+    return LA_ERR_INVALID_ARGUMENT;
   c->x = tokens_of(tokens ? x : nullptr, x_strides);
   c->weight = weight, c->bias = bias, c->weight_dtype = weight_dtype, c->init = init_state;
   c->lengths = lengths, c->lengths64 = lengths_bits == 64;
@@ -211,7 +227,7 @@ int la_short_conv_fwd(const void *x, const int64_t *x_strides, const void *weigh
   const int st = conv_call(&c, x, x_strides, weight, bias, weight_dtype, init_state, lengths,
                            lengths_bits, batch, tokens, channels, taps, silu, dtype);
   if (st != LA_OK || !batch || (!tokens && !final_state)) return st;
-  if (tokens && !out) return LA_ERR_INVALID_ARGUMENT;
+  if ((tokens && !out) || !placed(size_of(dtype), {out, final_state})) return LA_ERR_INVALID_ARGUMENT;
   c.out = out, c.final_state = final_state;
   return launch_conv_fwd(c, dtype, (cudaStream_t)stream);
 }
@@ -229,11 +245,14 @@ int la_short_conv_bwd(const void *x, const int64_t *x_strides, const void *weigh
   if (st != LA_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
   if (!batch) {
-    const int64_t size = weight_dtype == LA_DTYPE_FLOAT32 ? 4 : 2;
+    const int64_t size = size_of(weight_dtype);
     if ((st = zero(d_weight, channels * taps * size, s)) != LA_OK) return st;
     return zero(d_bias, channels * size, s);
   }
-  if (tokens && (!d_out || !valid_strides(d_out_strides) || !dx)) return LA_ERR_INVALID_ARGUMENT;
+  if ((tokens && (!d_out || !valid_strides(d_out_strides) || !dx)) ||
+      !placed(size_of(dtype), {d_out, d_final_state, dx, d_init_state}) ||
+      !placed(size_of(weight_dtype), {d_weight, d_bias}))
+    return LA_ERR_INVALID_ARGUMENT;
   const int64_t rows = conv_partial_rows({batch, tokens, (int)channels});
   const bool sums = d_weight || d_bias;
   if (sums && (!workspace || ((uintptr_t)workspace & 15) ||
@@ -258,7 +277,8 @@ int la_short_conv_step(const void *x, int64_t x_stride, const void *weight, cons
   if (taps < kConvMinTaps || taps > kConvMaxTaps) return LA_ERR_UNSUPPORTED;
   if (!batch) return LA_OK;
   if (!x || !weight || !state || !out || x_stride < 0 ||
-      (batch > 1 && state_stride < (taps - 1) * channels))
+      (batch > 1 && state_stride < (taps - 1) * channels) ||
+      !placed(size_of(dtype), {x, state, out}) || !placed(size_of(weight_dtype), {weight, bias}))
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
@@ -280,7 +300,8 @@ static int norm_call(GroupNormCall *c, const void *x, const int64_t *x_strides, 
   c->rows = shape[0] * shape[1];
   if (!c->rows) return LA_OK;
   if (c->rows > INT32_MAX / 2) return LA_ERR_UNSUPPORTED;
-  if (!x || !valid_strides(x_strides) || (gate && !valid_strides(gate_strides)))
+  if (!x || !valid_strides(x_strides) || (gate && !valid_strides(gate_strides)) ||
+      !placed(size_of(dtype), {x, gate}) || !placed(size_of(weight_dtype), {weight, bias}))
     return LA_ERR_INVALID_ARGUMENT;
   c->n1 = (uint32_t)shape[1];
   c->x.p = x, c->x.s0 = x_strides[0], c->x.s1 = x_strides[1];
@@ -300,7 +321,7 @@ int la_group_norm_fwd(const void *x, const int64_t *x_strides, const void *gate,
   int st = norm_call(&c, x, x_strides, gate, gate_strides, weight, bias, weight_dtype, shape,
                      channels, groups, silu, dtype);
   if (st != LA_OK || !c.rows) return st;
-  if (!out || ((uintptr_t)stats & 7)) return LA_ERR_INVALID_ARGUMENT;
+  if (!out || !placed(size_of(dtype), {out}) || !placed(8, {stats})) return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
   c.out = out, c.stats = stats, c.eps = eps;
@@ -331,11 +352,13 @@ int la_group_norm_bwd(const void *x, const int64_t *x_strides, const void *gate,
   if (st != LA_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
   if (!c.rows) {
-    const int64_t bytes = channels * (weight_dtype == LA_DTYPE_FLOAT32 ? 4 : 2);
+    const int64_t bytes = channels * size_of(weight_dtype);
     if ((st = zero(d_weight, bytes, s)) != LA_OK) return st;
     return zero(d_bias, bytes, s);
   }
-  if (!stats || ((uintptr_t)stats & 7) || !d_out || !valid_strides(d_out_strides) || !dx || (gate && !d_gate))
+  if (!stats || !d_out || !valid_strides(d_out_strides) || !dx || (gate && !d_gate) ||
+      !placed(8, {stats}) || !placed(size_of(dtype), {d_out, dx, d_gate}) ||
+      !placed(size_of(weight_dtype), {d_weight, d_bias}))
     return LA_ERR_INVALID_ARGUMENT;
   DeviceInfo info;
   if ((st = check_device(&info)) != LA_OK) return st;
