@@ -75,7 +75,7 @@ def _build_binding(force: bool) -> None:
                  sysconfig.get_path("include")):
         cmd += ["-isystem", str(path)]
     cmd += [str(BINDING_SRC), "-o", str(tmp), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
-            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+            "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")

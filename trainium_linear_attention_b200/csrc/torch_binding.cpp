@@ -4,11 +4,12 @@
 // These operators' kernels take a few microseconds at small sizes, and a
 // training step of a few tens; from Python (arguments through ctypes, the backward
 // pass on a thread that first has to get the interpreter) the host took 120
-// us for a step that takes 72 here, 47 of them the engine's own for an empty node.
+// us for a step that takes 71 here, 47 of them the engine's own for an empty node.
 // The entry points' addresses come from the library that the package has loaded:
 // there is one library, one set of kernels and no other implementation.
 #include <torch/extension.h>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -184,7 +185,8 @@ struct Rows {
 };
 
 Tensor empty(at::IntArrayRef shape, at::ScalarType type, const Tensor &like) {
-  return at::empty(shape, like.options().dtype(type).requires_grad(false));
+  // (the allocator itself, without the dispatcher's way to it)
+  return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
 }
 Tensor workspace(size_t bytes, const Tensor &like) {
   return empty({(int64_t)bytes}, at::kByte, like);
