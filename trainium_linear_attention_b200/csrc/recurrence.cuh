@@ -161,6 +161,7 @@ __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
+  __syncwarp();  // (one lane may have been issuing copies)
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Into the shared memory of the cluster's CTA `rank`, at this CTA's address `p`,
