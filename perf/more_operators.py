@@ -242,7 +242,7 @@ def _recur(s):
         got["state"] = h[:, -1].clone()
     if s["op"] == "recur":
         return got
-    g = s["d_out"].float()
+    g = s["d_out"].to(torch.float32, copy=True)  # (the final state's gradient is added to it)
     if inside is not None:
         g = torch.where(inside, g, 0.0)
     if s["d_state"] is not None:
