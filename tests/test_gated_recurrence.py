@@ -586,3 +586,30 @@ def test_refusals():
         step(x, g, state.clone().requires_grad_())
     with pytest.raises(ValueError, match="batch, channels"):
         step(s["x"], g, state)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,c", [(2, 100, 40), (1, 70, 33), (1, 300, 1030), (8, 1400, 1024)])
+def test_nearly_closed_input_gates(b, t, c, dtype):
+    """sigmoid of -40 to -75 is far from 0 (e-18 to e-33) and reaches the outputs, with a
+    decay and without, among open gates and by itself.  The bound holds: exp's argument in
+    units of ln 2 is below 128, so its rounding (half of 2^-17) and the constant's (2^-26
+    of it) are below 2^-18 of u, F's fourfold is 2^-17."""
+    for decay in (True, False):
+        s = make(b, t, c, dtype, decay, state=False, seed=23)
+        gen = torch.Generator().manual_seed(24)
+        low = (-40 - 35 * torch.rand(b, t, c, generator=gen)).to(dtype).cuda()
+        s["x"] = s["x"].abs().clamp(min=2.0 ** -6) * 2.0 ** 20
+        mixed = torch.where(torch.rand(b, t, c, generator=gen).cuda() < 0.9, s["input_gate"], low)
+        for gates in (low, mixed):
+            s["input_gate"] = gates
+            out, _ = check_forward(s)
+            assert (out != 0).all()
+        s["input_gate"] = low
+        state = torch.zeros(b, c, device="cuda")
+        one = T.gated_recurrence_step(s["x"][:, 0], s["gate"][:, 0], state, s["log_decay"], low[:, 0])
+        h, e, _, _ = forward_bounds({n: v if v is None or v.dim() < 3 else v[:, :1]
+                                     for n, v in s.items()})
+        assert (one != 0).all()
+        assert ((one.double() - h[:, 0]).abs() <= e[:, 0] + HALF[dtype] * 1.01 * h[:, 0].abs()).all()

@@ -13,6 +13,18 @@ __device__ __forceinline__ float2 load_two(const __nv_bfloat16 *p) {
 }
 __device__ __forceinline__ float2 load_two(const float *p) { return *(const float2 *)p; }
 
+// Whether any of some bf16 values are below a negative bound: as unsigned numbers floats
+// below zero are the larger the lower they are, above all others.
+struct Least {
+  uint32_t v = 0;
+  __device__ __forceinline__ void take(const __nv_bfloat16 *p, const __nv_bfloat16 *q) {
+    v = __vimax3_u16x2(v, *(const uint32_t *)p, *(const uint32_t *)q);
+  }
+  __device__ __forceinline__ bool below(float bound) const {
+    return max(v & 0xFFFF, v >> 16) > __float_as_uint(bound) >> 16;
+  }
+};
+
 // Channels c and c + 1 of a row of n (the second may be beyond it); `pair`: the
 // row's pairs are aligned.
 __device__ __forceinline__ void store_two(__nv_bfloat16 *p, float2 v, bool pair, bool second) {

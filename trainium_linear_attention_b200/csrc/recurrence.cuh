@@ -84,8 +84,15 @@ __device__ __forceinline__ float2 beta_squared(float2 am1, float2 &floored) {
 // A closed gate (s = 0; s = 1 without a decay) and a closed input gate (u = 0)
 // give beta u = 0 to the bit, whatever the other is: a masked token changes
 // nothing even where its x is the type's lowest value.
-template <typename T, bool kDecay, bool kInput, bool kGrad>
+//
+// kOneRoot: beta u as one root, beta^2 / sqrt(beta^2 p^2) with p = 1 + exp(-i), for a
+// loop that the special-function unit bounds (8 x 32768 x 1024 in bf16: 392 us, with two
+// functions 412; fp32 gains nothing).  p^2 overflows from an input gate of -44.36 down, and
+// u is then 0: the caller takes tokens with such gates without it.
+constexpr float kOneRootLeast = -44.f;
+template <typename T, bool kDecay, bool kInput, bool kGrad, bool kOneRoot>
 __device__ __forceinline__ Token token_of(float2 g, float2 i, float2 lambda) {
+  static_assert(!kOneRoot || (kDecay && kInput && !kGrad), "");
   Token y;
   float2 eg = exp_minus<T>(g);
   if constexpr (!kDecay) eg = min_nan(eg, kExpMost);  // 1 - s = e s, and not inf * 0
@@ -96,15 +103,14 @@ __device__ __forceinline__ Token token_of(float2 g, float2 i, float2 lambda) {
   if constexpr (kInput) {
     eu = exp_minus<T>(i);
     pu = __fadd2_rn(eu, two(1.f));
-    if constexpr (!kDecay || kGrad) u = rcp_two<T>(pu);
+    if constexpr (!kOneRoot) u = rcp_two<T>(pu);
     if constexpr (kGrad) y.uc = __fmul2_rn(min_nan(eu, kExpMost), u);
   }
   if constexpr (kDecay) {
     y.am1 = expm1_neg(__fmul2_rn(lambda, y.s));
     float2 w;
     const float2 v = beta_squared(y.am1, w);
-    if constexpr (kInput && !kGrad) {
-      // one root for both: beta / p = beta^2 / sqrt(beta^2 p^2), p = 1 + exp(-i)
+    if constexpr (kOneRoot) {
       y.bu = __fmul2_rn(v, rsqrt_two<T>(__fmul2_rn(w, __fmul2_rn(pu, pu))));
     } else {
       y.bu = __fmul2_rn(v, rsqrt_two<T>(w));

@@ -136,7 +136,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
 #pragma unroll
     for (int k = 0; k < kL; ++k) {
       const int at = 64 * k + 2 * lane;
-      const Token y = token_of<T, kDecay, kInput, true>(
+      const Token y = token_of<T, kDecay, kInput, true, false>(
           load_two(gs + at), kInput ? load_two(us + at) : two(0.f), lambda);
       am1[k] = y.am1, bu[k] = y.bu, s[k] = y.s, sc[k] = y.sc;
       if (kInput) uc[k] = y.uc;

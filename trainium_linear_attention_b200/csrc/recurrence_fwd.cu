@@ -46,6 +46,19 @@ struct Exchange {
   int abort;
 };
 
+// beta u x of a thread's tokens, of any input gates, in the place of its x and input gates
+// (two fp32 values for each pair).  Out of the way of the loop that reads them back.
+__device__ __noinline__ void any_input_gates(__nv_bfloat16 *xs, const __nv_bfloat16 *gs,
+                                             __nv_bfloat16 *us, float2 lambda) {
+#pragma unroll 1
+  for (int k = 0; k < kL; ++k, xs += 64, gs += 64, us += 64) {
+    const Token y = token_of<__nv_bfloat16, true, true, false, false>(load_two(gs), load_two(us), lambda);
+    const float2 b = __fmul2_rn(y.bu, load_two(xs));
+    *(float *)xs = b.x;
+    *(float *)us = b.y;
+  }
+}
+
 template <typename T, bool kDecay, bool kInput, Fetch kF, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps)
 recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__ TileMaps maps) {
@@ -104,7 +117,8 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   int stage = 0;
   for (int i = 0; i < steps; ++i) {
     const int buf = i & 1;
-    const T *xs = tiles.tile(stage, 0), *gs = tiles.tile(stage, 1), *us = tiles.tile(stage, kIn - 1);
+    T *const xs = tiles.tile(stage, 0), *const gs = tiles.tile(stage, 1),
+            *const us = tiles.tile(stage, kIn - 1);
     const int row0 = i * step + first, t0 = row0 + part * kL;
     if (cluster == 1 && row0 >= len) break;  // (nobody waits for the last step's other warps)
     const bool whole = tiles.whole(row0, len);
@@ -112,10 +126,14 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     tiles.wait(row0, len, stage, kDecay ? -INFINITY : INFINITY, &ex.abort);
     float2 am1[kL], b[kL];
     float2 a = two(kDecay ? 0.f : 1.f), e = two(0.f);
+    constexpr bool kOneRoot = kDecay && kInput && sizeof(T) == 2;
+    Least least;  // of the input gates
 #pragma unroll
     for (int k = 0; k < kL; ++k) {
       const int at = 64 * k + 2 * lane;
-      const Token y = token_of<T, kDecay, kInput, false>(
+      if constexpr (kOneRoot)
+        if (k % 2) least.take(us + at - 64, us + at);
+      const Token y = token_of<T, kDecay, kInput, false, kOneRoot>(
           load_two(gs + at), kInput ? load_two(us + at) : two(0.f), lambda);
       am1[k] = y.am1;
       b[k] = __fmul2_rn(y.bu, load_two(xs + at));
@@ -125,6 +143,19 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
     if (kDecay) {
       a = __fmul2_rn(a, lambda);
       a = make_float2(Fn<T>::exp(a.x), Fn<T>::exp(a.y));
+    }
+    if constexpr (kOneRoot) {
+      if (least.below(kOneRootLeast)) {  // nearly closed input gates
+        any_input_gates(xs + 2 * lane, gs + 2 * lane, us + 2 * lane, lambda);
+        e = two(0.f);
+#pragma unroll
+        for (int k = 0; k < kL; ++k) {
+          const int at = 64 * k + 2 * lane;
+          b[k] = make_float2(*(const float *)(xs + at), *(const float *)(us + at));
+          e = __fadd2_rn(__ffma2_rn(am1[k], e, e), b[k]);
+        }
+        if (kF == Fetch::kTma) tc::fence_proxy_async_smem();  // (ahead of the next copy into it)
+      }
     }
     __syncwarp();  // the rows are read
     fetch(i + kStages, stage);

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kThreads) recur_step_kernel(const RecurStep p)
 #pragma unroll
   for (int e = 0; e < kVec; e += 2) {
     const int f = e + 1 < kVec ? e + 1 : e;
-    const Token y = token_of<T, kDecay, kInput, false>(
+    const Token y = token_of<T, kDecay, kInput, false, false>(
         make_float2(g[e], g[f]), make_float2(u[e], u[f]), make_float2(lambda[e], lambda[f]));
     const float2 old = make_float2(h[e], h[f]);
     const float2 now = __ffma2_rn(y.bu, make_float2(x[e], x[f]), __ffma2_rn(y.am1, old, old));
