@@ -344,3 +344,25 @@ def test_refusals():
             T.group_norm(**{**s, **change})
     with pytest.raises(N.LaError):
         T.group_norm(torch.zeros(2, 9000, device="cuda"), 1)
+
+
+@gpu
+@pytest.mark.parametrize("shape,groups", [((3, 64), 2), ((5, 33), 1), ((7, 60), 6), ((9, 96), 4),
+                                          ((40, 1000), 2), ((3, 2047), 1), ((2, 4096), 1),
+                                          ((1200, 40), 5)])
+def test_a_common_part_costs_the_gradient_nothing(shape, groups):
+    """Values on a grid of 2^-10 below 8, and the same with 2^13 added, are both exact in fp32,
+    and so are their differences: outputs and gradients are the same bits."""
+    for gate, silu in ((True, True), (False, True), (False, False)):
+        s = make(shape, groups, torch.float32, gate, silu, seed=21)
+        s["x"] = torch.round(s["x"].clamp(-7, 7) * 1024) / 1024
+        names = [n for n in ("x", "weight", "bias", "gate") if s[n] is not None]
+        up = torch.randn(shape, generator=torch.Generator().manual_seed(2)).cuda()
+        got = []
+        for common in (0.0, 8192.0):
+            leaves = {n: (s[n] + common if n == "x" else s[n].detach()).requires_grad_()
+                      for n in names}
+            y = T.group_norm(**{**s, **leaves}, eps=EPS)
+            got.append([y.detach(), *torch.autograd.grad(y, list(leaves.values()), up)])
+        for n, a, b in zip(["y", *names], *got):
+            assert torch.equal(a, b), n

@@ -230,6 +230,15 @@ struct Lanes {
   int across, rows, columns;  // columns: CTAs along a row's groups
 };
 
+// Whether a group's mean is kept for the gradient as it is found, from the group's first
+// value on.  Rounded together with that value it would be off by 2^-24 of it: beside fp32
+// values that differ by little that is much of their differences, and the gradient's n
+// would not be the forward pass'.  bf16 values that differ do so by 2^-8 of themselves at
+// least: a single one among 8192 leaves a deviation of 2^-14.5 of them, and the mean is off by
+// 2^-9.5 of that, under half a rounding of the outputs.  There the sum is kept (16384 x 1024,
+// gradient: 41 us, with the first value read again 52).
+template <typename T> constexpr bool kFromPivot = sizeof(T) == 4;
+
 // CTAs walk the rows, the next row's loads on their way ahead of a row's sums.
 template <typename T, int TPR, int NV, Access kA>
 __global__ void __launch_bounds__(threads_for(TPR), TPR <= 256 && NV == 1 ? 4 : 1)
@@ -275,7 +284,8 @@ group_norm_fwd_kernel(const GroupNormCall p, const Lanes lanes) {
     const float sq = H::sum(x, t, p.size, [](float2 v, float2 s) { return __ffma2_rn(v, v, s); });
     const float rstd = 1.f / sqrtf(fmaf(group_sum<TPR>(sq, slot), inv, p.eps));
     if (p.stats && live && t == 0)
-      *(float2 *)(p.stats + 2 * ((int64_t)row * p.groups + group)) = make_float2(pivot + mean, rstd);
+      *(float2 *)(p.stats + 2 * ((int64_t)row * p.groups + group)) =
+          make_float2(kFromPivot<T> ? mean : pivot + mean, rstd);
     each<NV>([&](int i, int e) {
       x[i][e] = __ffma2_rn(__fmul2_rn(x[i][e], two(rstd)), w[i][e], b[i][e]);
     });
@@ -311,9 +321,12 @@ __global__ void __launch_bounds__(threads_for(TPR), TPR <= 256 && NV == 1 ? 2 : 
   // The next row is loaded ahead of this one's sums.
   H hx, hd, hg;
   float2 next_st;
+  float next_pivot = 0.f;
   auto fetch = [&](int first) {
     const int row = member && first + lane_row < rows ? first + lane_row : first;
-    hx.load((const T *)p.x.p + row_offset(p.x, p.n1, row, rows) + c0, t, p.size);
+    const T *src = (const T *)p.x.p + row_offset(p.x, p.n1, row, rows) + c0;
+    hx.load(src, t, p.size);
+    if (kFromPivot<T>) next_pivot = to_f32(*src);
     hd.load((const T *)p.d_out.p + row_offset(p.d_out, p.n1, row, rows) + c0, t, p.size);
     if (p.gate.p)
       hg.load((const T *)p.gate.p + row_offset(p.gate, p.n1, row, rows) + c0, t, p.size);
@@ -328,8 +341,10 @@ __global__ void __launch_bounds__(threads_for(TPR), TPR <= 256 && NV == 1 ? 2 : 
     hd.get(g);
     if (p.gate.p) hg.get(u);
     const float2 st = next_st;
+    const float pivot = next_pivot;
     if (first + stride < rows) fetch(first + stride);
     each<NV>([&](int i, int e) {
+      if constexpr (kFromPivot<T>) n[i][e] = __fadd2_rn(n[i][e], two(-pivot));
       n[i][e] = __fmul2_rn(__fadd2_rn(n[i][e], two(-st.x)), two(st.y));
     });
     // act'(v) = s + v s (1 - s) with s = sigmoid(v); the activation v s

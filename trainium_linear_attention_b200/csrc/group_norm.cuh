@@ -20,7 +20,8 @@ struct GroupNormCall {
   int groups = 1, size = 1;     // channels = groups * size
   int silu = 0;
   float eps = 0.f;
-  float *stats = nullptr;       // (rows, groups, 2): mean and 1 / sqrt(var + eps); forward: or null
+  float *stats = nullptr;       // (rows, groups, 2): mean (fp32: less the group's first value) and
+                                // 1 / sqrt(var + eps); forward: or null
   void *out = nullptr;          // contiguous, as dx and d_gate
   void *dx = nullptr, *d_gate = nullptr;
   float *partial = nullptr;     // null, or rows of (channels for the weight, channels for the bias)
