@@ -366,3 +366,25 @@ def test_a_common_part_costs_the_gradient_nothing(shape, groups):
             got.append([y.detach(), *torch.autograd.grad(y, list(leaves.values()), up)])
         for n, a, b in zip(["y", *names], *got):
             assert torch.equal(a, b), n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((3, 48), 2), ((3, 30), 1), ((3, 33), 1), ((2, 1032), 1)])
+def test_gradients_of_equal_large_values(shape, groups, dtype):
+    """Equal values have n = 0 and rstd = 1 / sqrt(eps) = 316: finite gradients, whatever the
+    value (its product with rstd is not), in groups that leave threads without values too."""
+    for affine, silu in ((True, True), (False, True), (False, False)):
+        s = make(shape, groups, dtype, False, silu, affine, seed=25)
+        s["x"] = torch.full_like(s["x"], 2.0 ** 122).requires_grad_()
+        y = T.group_norm(**s, eps=EPS)
+        up = torch.randn(shape, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+        g, = torch.autograd.grad(y, [s["x"]], up)
+        w64 = s["x"].detach().double().requires_grad_()
+        args = {n: v.double() if isinstance(v, torch.Tensor) else v for n, v in s.items()}
+        want, = torch.autograd.grad(T.ref_group_norm(**{**args, "x": w64}, eps=EPS), [w64],
+                                    up.double())
+        # up to 1032 terms in a row at most in the mean, a few roundings beside it
+        size = 316.3 * 1.6 * 1.1 * up.double().abs().max()
+        near = 1100 * 2.0 ** -24 * size + F * size
+        assert ((g.double() - want).abs() <= near + HALF[dtype] * 1.01 * want.abs()).all()

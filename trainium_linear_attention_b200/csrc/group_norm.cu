@@ -102,6 +102,17 @@ struct Held {
           x[i][e] = make_float2(__uint_as_float(w[i][e] << 16), __uint_as_float(w[i][e] & 0xFFFF0000u));
       }
   }
+  // f of each pair, (1, 1) for values inside the group and 0 for those beyond it.
+  template <class F>
+  static __device__ __forceinline__ void each_inside(int t, int size, F &&f) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = column(t, i, kA == kPacked ? 0 : 2 * e) < size ? 1.f : 0.f;
+        f(i, e, make_float2(x, kA != kSingle ? x : column(t, i, 2 * e + 1) < size ? 1.f : 0.f));
+      }
+  }
   // Sum of f(x) over the values inside the group (a pack or pair is whole, or beyond it).
   template <class F>
   static __device__ __forceinline__ float sum(const float2 (&x)[NV][4], int t, int size, F &&f) {
@@ -343,9 +354,10 @@ __global__ void __launch_bounds__(threads_for(TPR), TPR <= 256 && NV == 1 ? 2 : 
     const float2 st = next_st;
     const float pivot = next_pivot;
     if (first + stride < rows) fetch(first + stride);
-    each<NV>([&](int i, int e) {
+    // (0 beyond the group, where the sums below would meet an infinite -mean rstd)
+    H::each_inside(t, p.size, [&](int i, int e, float2 in) {
       if constexpr (kFromPivot<T>) n[i][e] = __fadd2_rn(n[i][e], two(-pivot));
-      n[i][e] = __fmul2_rn(__fadd2_rn(n[i][e], two(-st.x)), two(st.y));
+      n[i][e] = __fmul2_rn(__fadd2_rn(n[i][e], two(-st.x)), make_float2(in.x * st.y, in.y * st.y));
     });
     // act'(v) = s + v s (1 - s) with s = sigmoid(v); the activation v s
     auto slope = [](float2 vs, float2 s) {
