@@ -346,3 +346,40 @@ def test_refusals():
                            s["initial_state"].transpose(1, 2).contiguous().transpose(1, 2))
     with pytest.raises(ValueError, match="in place"):
         T.causal_conv_step(s["x"][:, 0], s["weight"], s["initial_state"].clone().requires_grad_())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("silu", [True, False])
+def test_infinite_values_end_with_their_sequence(dtype, silu):
+    """An infinite last token (or state, of an empty sequence): nothing of it behind the
+    sequence, where gradients are zero and from which the weights get nothing."""
+    inf = float("inf")
+    s = make(5, 70, 40, 4, dtype, silu=silu, seed=31)
+    ends = [0, 1, 15, 40, 64]
+    s["lengths"] = torch.tensor(ends, device="cuda")
+    s["initial_state"][0] = inf
+    for i, n in enumerate(ends[1:], 1):
+        s["x"][i, n - 1] = inf
+    names = ["x", "weight", "bias", "initial_state"]
+    for n in names:
+        s[n].requires_grad_()
+    out, state = T.causal_conv(**s, return_state=True)
+    up = torch.randn(out.shape, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    d_state = torch.ones_like(state)
+    dx, dw, db, dh = torch.autograd.grad((out, state), [s[n] for n in names], (up, d_state))
+    behind = torch.arange(70, device="cuda") >= s["lengths"][:, None]
+    assert (out[behind] == 0).all() and (dx[behind] == 0).all()
+    assert (dh[0] == 1).all()
+    if silu:
+        return  # (the slope at an infinite z is 0 * inf, as PyTorch's)
+    assert torch.isfinite(dx).all() and torch.isfinite(db).all() and torch.isfinite(dh).all()
+    # the last tap alone meets the infinite tokens
+    first = s["initial_state"].detach().double()
+    whole = torch.cat([first, s["x"].detach().double()], 1).unfold(1, 4, 1)
+    g = up.double()[..., None]
+    for j in range(3):
+        terms = torch.where(behind[..., None], 0.0, whole[..., j] * g[..., 0])
+        want, size = terms.sum((0, 1)), terms.abs().sum((0, 1))
+        near = (5 * 70 / 8 + 64) * 2.0 ** -24 * size + HALF[dtype] * 1.01 * want.abs()
+        assert ((dw[:, j].double() - want).abs() <= near).all()

@@ -241,11 +241,14 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
 #pragma unroll
   for (int j = 0; j < kTaps - 1; ++j) x[j + 1] = row.load(t0 - (kTaps - 1) + j);
   T *dx = (T *)p.dx + ib * p.sizes.tokens * channels + c;
-  // Takes a token's x and dy; open[0] is then the gradient of the window's oldest.
-  auto token = [&](float2 in, float2 g, auto own) {
+  // Takes a token's x and dy; open[0] is then the gradient of the window's oldest.  Behind
+  // the sequence there is no z, and its window's values are not multiplied by a zero.
+  auto token = [&](float2 in, float2 g, auto own, auto inside) {
 #pragma unroll
     for (int j = 0; j < kTaps - 1; ++j) x[j] = x[j + 1], open[j] = open[j + 1];
     x[kTaps - 1] = in;
+    open[kTaps - 1] = two(0.f);
+    if (!inside) return;
     if constexpr (kSilu) {
       float2 z = w.b;
 #pragma unroll
@@ -269,7 +272,7 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
     auto tile = [&](auto wide) {
 #pragma unroll
       for (int k = 0; k < kL; ++k) {
-        token(load_two(in + 64 * k), load_two(up + 64 * k), std::true_type{});
+        token(load_two(in + 64 * k), load_two(up + 64 * k), std::true_type{}, std::true_type{});
         if (!live) continue;
         if (k >= kTaps - 1 || t > t0)
           store_two(dst + (int64_t)k * channels, open[0], wide, second);
@@ -291,7 +294,7 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
 #pragma unroll 1
       for (int k = 0; k < left; ++k) {
         const int now = t + k, at = now - (kTaps - 1);  // whose dx is complete
-        token(load_two(in + 64 * k), load_two(up + 64 * k), now < end);
+        token(load_two(in + 64 * k), load_two(up + 64 * k), now < end, now < len);
         if (!live || (at < t0 && !first)) continue;
         const int back = at - (len - (kTaps - 1));  // its row of the final state
         if (p.d_final && back >= 0 && back < kTaps - 1) {
