@@ -168,3 +168,22 @@ def test_training_runs():
     for n, p in m.named_parameters():
         assert torch.isfinite(p).all() and p.grad.abs().sum() > 0, n
     assert any(not torch.equal(p, before[n]) for n, p in m.named_parameters())
+
+
+@gpu
+def test_autocast():
+    """fp32 parameters under autocast to bf16: prompts, and tokens from a new sequence's state,
+    within a bf16 block's bound; a training step's gradients are fp32 and finite."""
+    m = make(seed=4)
+    x = torch.randn(2, 6, 256, device="cuda")
+    want = plain(m, x.double(), None)[0]
+    with torch.autocast("cuda", torch.bfloat16), torch.no_grad():
+        out, _ = m(x)
+        state = m.empty_state(2)
+        steps = torch.stack([m.step(t, state)[0] for t in x.unbind(1)], 1)
+    assert rel(out, want) <= BOUND[torch.bfloat16] and rel(steps, want) <= BOUND[torch.bfloat16]
+    with torch.autocast("cuda", torch.bfloat16):
+        out, _ = m(x)
+    grads = torch.autograd.grad(out.float().square().mean(), list(m.parameters()))
+    assert all(g.dtype == torch.float32 and torch.isfinite(g).all() for g in grads)
+    assert m.empty_state(1)[0].dtype == torch.float32

@@ -35,7 +35,8 @@ class GatedRecurrence(nn.Module):
     (output, residual stream) for one token per sequence (x: (b, dim)), ``state``
     updated in place.  ``state``: the last taps - 1 inputs of the convolution
     (b, taps - 1, dim) and the recurrence's fp32 (b, dim); ``empty_state(b)`` is that
-    of a new sequence.
+    of a new sequence (called under the autocast, if any, that the block is called under:
+    the convolution's inputs have the projections' type).
     """
 
     def __init__(self, dim: int, heads: int = 8, eps: float = 1e-6, taps: int = 4):
@@ -66,7 +67,9 @@ class GatedRecurrence(nn.Module):
 
     def empty_state(self, batch: int):
         w = self.conv_weight
-        return (w.new_zeros(batch, self.taps - 1, w.shape[0]),
+        dtype = (torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda")
+                 else self.in_proj.weight.dtype)
+        return (w.new_zeros(batch, self.taps - 1, w.shape[0], dtype=dtype),
                 torch.zeros(batch, w.shape[0], device=w.device))
 
     def forward(self, hidden_states: torch.Tensor, residual: torch.Tensor | None = None,
