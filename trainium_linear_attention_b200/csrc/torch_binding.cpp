@@ -54,6 +54,14 @@ void *stream_of(const Tensor &t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 
+// The allocations and the library's call, without the interpreter's lock (as ctypes calls
+// the other operators' entry points).
+template <class F>
+auto unlocked(F &&f) {
+  py::gil_scoped_release released;
+  return f();
+}
+
 // ---- checks ----------------------------------------------------------------------
 [[noreturn]] void type_error(const std::string &what) { throw py::type_error(what); }
 [[noreturn]] void value_error(const std::string &what) { throw py::value_error(what); }
@@ -315,12 +323,14 @@ py::object gated_recurrence(py::handle px, py::handle pg, py::handle pl, py::han
   check_lengths(lengths, x);
   const Maybe mx = x, mg = gate;
   if (wants_gradient({&mx, &mg, &log_decay, &input_gate, &init})) {
-    const variable_list r =
-        RecurrenceFunction::apply(x, gate, log_decay, input_gate, init, lengths, want_state);
+    const variable_list r = unlocked([&] {
+      return RecurrenceFunction::apply(x, gate, log_decay, input_gate, init, lengths, want_state);
+    });
     return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
   }
-  const Recurrence r =
-      recurrence_forward(x, gate, log_decay, input_gate, init, lengths, want_state, false);
+  const Recurrence r = unlocked([&] {
+    return recurrence_forward(x, gate, log_decay, input_gate, init, lengths, want_state, false);
+  });
   return want_state ? py::object(py::make_tuple(r.out, r.final_state)) : py::cast(r.out);
 }
 
@@ -339,16 +349,18 @@ Tensor gated_recurrence_step(py::handle px, py::handle pg, py::handle ps, py::ha
   check_like(input_gate, "input_gate", x);
   check_exact(log_decay, "log_decay", {c}, at::kFloat, x);
   const int64_t stride = check_state(state, {b, c}, at::kFloat, x);
-  const c10::cuda::CUDAGuard guard(x.device());
-  const Rows vx(x), vg(gate), vi(input_gate);
-  const Maybe decay = dense(log_decay);
-  const Tensor out = empty({b, c}, x.scalar_type(), x);
-  check(lib.la_recurrence_step(vx.p(), vx.stride, vg.p(), vg.stride, vi.p(), vi.stride, floats(decay),
-                               (float *)state.data_ptr(), stride, out.data_ptr(), b, c, code,
-                               stream_of(x)),
-        "la_recurrence_step");
-  changed(state);
-  return out;
+  return unlocked([&] {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Rows vx(x), vg(gate), vi(input_gate);
+    const Maybe decay = dense(log_decay);
+    const Tensor out = empty({b, c}, x.scalar_type(), x);
+    check(lib.la_recurrence_step(vx.p(), vx.stride, vg.p(), vg.stride, vi.p(), vi.stride,
+                                 floats(decay), (float *)state.data_ptr(), stride, out.data_ptr(), b,
+                                 c, code, stream_of(x)),
+          "la_recurrence_step");
+    changed(state);
+    return out;
+  });
 }
 
 // ---- short causal convolution -----------------------------------------------------
@@ -433,10 +445,12 @@ py::object causal_conv(py::handle px, py::handle pw, py::handle pb, bool silu, p
   check_lengths(lengths, x);
   const Maybe mx = x, mw = weight;
   if (wants_gradient({&mx, &mw, &bias, &init})) {
-    const variable_list r = ConvFunction::apply(x, weight, bias, init, lengths, silu, want_state);
+    const variable_list r = unlocked(
+        [&] { return ConvFunction::apply(x, weight, bias, init, lengths, silu, want_state); });
     return want_state ? py::object(py::make_tuple(r[0], r[1])) : py::cast(r[0]);
   }
-  const auto r = conv_forward(x, weight, bias, init, lengths, silu, want_state);
+  const auto r =
+      unlocked([&] { return conv_forward(x, weight, bias, init, lengths, silu, want_state); });
   return want_state ? py::object(py::make_tuple(r.first, r.second)) : py::cast(r.first);
 }
 
@@ -448,15 +462,17 @@ Tensor causal_conv_step(py::handle px, py::handle pw, py::handle ps, py::handle 
   const int64_t b = x.size(0), c = x.size(1), taps = check_taps(weight, c);
   const int wcode = check_affine(weight, bias, {c, taps}, x);
   const int64_t stride = check_state(state, {b, taps - 1, c}, x.scalar_type(), x);
-  const c10::cuda::CUDAGuard guard(x.device());
-  const Rows vx(x);
-  const Maybe w = dense(weight), bb = dense(bias);
-  const Tensor out = empty({b, c}, x.scalar_type(), x);
-  check(lib.la_short_conv_step(vx.p(), vx.stride, ptr(w), ptr(bb), wcode, state.data_ptr(), stride,
-                               out.data_ptr(), b, c, taps, silu, code, stream_of(x)),
-        "la_short_conv_step");
-  changed(state);
-  return out;
+  return unlocked([&] {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Rows vx(x);
+    const Maybe w = dense(weight), bb = dense(bias);
+    const Tensor out = empty({b, c}, x.scalar_type(), x);
+    check(lib.la_short_conv_step(vx.p(), vx.stride, ptr(w), ptr(bb), wcode, state.data_ptr(), stride,
+                                 out.data_ptr(), b, c, taps, silu, code, stream_of(x)),
+          "la_short_conv_step");
+    changed(state);
+    return out;
+  });
 }
 
 // ---- group norm -------------------------------------------------------------------
@@ -566,8 +582,10 @@ Tensor group_norm(py::handle px, int64_t groups, py::handle pw, py::handle pb, p
   check_affine(weight, bias, {c}, x);
   const Maybe mx = x;
   if (wants_gradient({&mx, &weight, &bias, &gate}))
-    return NormFunction::apply(x, groups, weight, bias, gate, silu, eps);
-  return norm_forward(x, groups, weight, bias, gate, silu, eps, false).first;
+    return unlocked(
+        [&] { return NormFunction::apply(x, groups, weight, bias, gate, silu, eps); });
+  return unlocked(
+      [&] { return norm_forward(x, groups, weight, bias, gate, silu, eps, false).first; });
 }
 
 // The library's entry points, and the exception of a status that is not LA_OK.
