@@ -48,3 +48,20 @@ def test_the_interpreter_is_free_during_a_call():
         for name, call in calls(grad).items():
             with bound({name: ctypes.pythonapi.PyGILState_Check}):
                 call()
+
+
+@gpu
+def test_statuses_raise_their_error():
+    """A status other than ok is a LaError that has it, from calls and from backward passes
+    (which run on the engine's thread)."""
+    unsupported = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: N.LA_ERR_UNSUPPORTED)
+    for name, call in calls().items():
+        with bound({name: unsupported}), pytest.raises(N.LaError, match=name) as caught:
+            call()
+        assert caught.value.status == N.LA_ERR_UNSUPPORTED
+    for name, call in calls(grad=True).items():
+        if name.endswith("_fwd"):
+            y, name = call(), name.replace("_fwd", "_bwd")
+            with bound({name: unsupported}), pytest.raises(N.LaError, match=name) as caught:
+                y.sum().backward()
+            assert caught.value.status == N.LA_ERR_UNSUPPORTED

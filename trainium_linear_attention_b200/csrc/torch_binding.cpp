@@ -12,6 +12,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <optional>
@@ -48,6 +49,25 @@ struct Failure : std::runtime_error {  // a status that is not LA_OK
 };
 void check(int status, const char *where) {
   if (status != LA_OK) throw Failure(status, where);
+}
+PyObject *error_type = nullptr;  // what Python sees of it
+void set_error(const Failure &f) {
+  py::object e = py::reinterpret_borrow<py::object>(error_type)(f.status, f.where);
+  PyErr_SetObject(error_type, e.ptr());
+}
+// A backward pass runs in the engine, which takes Python's exceptions to its caller as they
+// are and others as a RuntimeError.
+template <class F>
+variable_list raising(F &&f) {
+  try {
+    return f();
+  } catch (const Failure &failure) {
+    python_error error;
+    py::gil_scoped_acquire lock;
+    set_error(failure);
+    error.persist();
+    throw error;
+  }
 }
 
 void *stream_of(const Tensor &t) {
@@ -270,6 +290,9 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
     return outs;
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return raising([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext *ctx, const variable_list &grads) {
     const auto s = ctx->get_saved_variables();
     auto given = [](const Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; };
     const Tensor &x = s[0], &gate = s[1];
@@ -397,6 +420,9 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
     return outs;
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return raising([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext *ctx, const variable_list &grads) {
     const auto s = ctx->get_saved_variables();
     auto given = [](const Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; };
     const Tensor &x = s[0], &weight = s[1];
@@ -534,6 +560,9 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     return r.first;
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+    return raising([&] { return gradients(ctx, grads); });
+  }
+  static variable_list gradients(AutogradContext *ctx, const variable_list &grads) {
     variable_list r(7);
     if (!grads[0].defined()) return r;
     const auto s = ctx->get_saved_variables();
@@ -593,8 +622,7 @@ void bind(const std::map<std::string, uintptr_t> &entries, py::object error) {
 #define LA_TAKE(name) lib.name = reinterpret_cast<decltype(&::name)>(entries.at(#name));
   LA_ENTRIES(LA_TAKE)
 #undef LA_TAKE
-  static PyObject *raise = nullptr;
-  raise = error.release().ptr();
+  error_type = error.release().ptr();
   static bool registered = false;
   if (registered) return;
   registered = true;
@@ -602,8 +630,7 @@ void bind(const std::map<std::string, uintptr_t> &entries, py::object error) {
     try {
       if (p) std::rethrow_exception(p);
     } catch (const Failure &f) {
-      py::object e = py::reinterpret_borrow<py::object>(raise)(f.status, f.where);
-      PyErr_SetObject(raise, e.ptr());
+      set_error(f);
     }
   });
 }
