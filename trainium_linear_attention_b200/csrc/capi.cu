@@ -87,24 +87,24 @@ int allow_dynamic_smem(const void *func, int bytes) {
     int bytes;
   };
   static std::mutex mu;
-  static Entry cache[128];
+  static Entry cache[1024];  // (the library has about 200 such kernels)
   static int used = 0;
   unsigned long long ctx = 0;
   const bool known = current_context_id(&ctx);
-  if (known) {
-    std::lock_guard<std::mutex> lock(mu);
-    for (int i = 0; i < used; ++i)
-      if (cache[i].ctx == ctx && cache[i].func == func && cache[i].bytes >= bytes) return LA_OK;
-  }
+  // Held while the attribute is set: another thread's launch of the same kernel with more
+  // may not find it lowered again.
+  std::lock_guard<std::mutex> lock(mu);
+  Entry *entry = nullptr;
+  for (int i = 0; known && i < used && !entry; ++i)
+    if (cache[i].ctx == ctx && cache[i].func == func) entry = &cache[i];
+  if (entry && entry->bytes >= bytes) return LA_OK;
   if (cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
       cudaSuccess) {
     cudaGetLastError();
     return LA_ERR_CUDA;
   }
-  if (known) {
-    std::lock_guard<std::mutex> lock(mu);
-    if (used < 128) cache[used++] = Entry{ctx, func, bytes};
-  }
+  if (entry) entry->bytes = bytes;
+  else if (known && used < 1024) cache[used++] = Entry{ctx, func, bytes};
   return LA_OK;
 }
 
