@@ -3,6 +3,8 @@ how it calls the library, with other functions in the place of its entry points.
 
 import contextlib
 import ctypes
+import subprocess
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -10,8 +12,63 @@ import torch
 import trainium_linear_attention_b200 as T
 from trainium_linear_attention_b200 import _native as N
 from trainium_linear_attention_b200 import _torch_binding as B
+from trainium_linear_attention_b200 import build as build_module
 
 gpu = pytest.mark.gpu
+
+
+def test_a_binding_of_another_torch_is_not_loaded(monkeypatch):
+    """The file's name has the interpreter and the torch whose layouts it was built with."""
+    assert B.path().exists()
+    monkeypatch.setattr(B, "_module", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    with pytest.raises(RuntimeError, match="0.0.1.* is missing.*build"):
+        T.group_norm(torch.zeros(2, 8), 2)
+
+
+def test_what_a_binding_is_built_for(monkeypatch, tmp_path):
+    """Another torch gets a file of its own; the same one, and an older file than the sources,
+    are taken and built again."""
+    ran = []
+
+    def compiler(cmd, **_):
+        ran.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(B, "LIB_DIR", tmp_path)
+    monkeypatch.setattr(subprocess, "run", compiler)
+    build_module._build_binding(False)
+    build_module._build_binding(False)
+    assert len(ran) == 1 and B.path().exists()
+    build_module._build_binding(True)
+    assert len(ran) == 2
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build_module._build_binding(False)
+    assert len(ran) == 3 and len(list(tmp_path.iterdir())) == 2
+
+
+def test_the_library_is_linked_without_the_binding(monkeypatch, tmp_path):
+    """A binding that fails to build is an error, but the C library is there by then."""
+    (tmp_path / "a.cu").write_text("")
+    monkeypatch.setattr(build_module, "CSRC", tmp_path)
+    monkeypatch.setattr(build_module, "BUILD", tmp_path)
+    monkeypatch.setattr(build_module, "LIB", tmp_path / "lib" / "library.so")
+    monkeypatch.setattr(build_module, "nvcc", lambda: "nvcc")
+    monkeypatch.setattr(build_module, "_compile", lambda src, obj, verbose: obj.write_text(""))
+
+    def link(cmd, **_):
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    def fails(force):
+        raise RuntimeError("no headers")
+
+    monkeypatch.setattr(subprocess, "run", link)
+    monkeypatch.setattr(build_module, "_build_binding", fails)
+    with pytest.raises(RuntimeError, match="no headers"):
+        build_module.build()
+    assert build_module.LIB.exists()
 
 
 def address(function):

@@ -9,12 +9,23 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import sysconfig
 import threading
 from pathlib import Path
 
+import torch
+
 from . import _native as N
 
-PATH = Path(__file__).resolve().parent / "lib" / "_la_torch.so"
+LIB_DIR = Path(__file__).resolve().parent / "lib"
+
+
+def path() -> Path:
+    """The extension for this interpreter and this torch, whose layouts are compiled into
+    it: one built for others has another name and is not loaded."""
+    return LIB_DIR / (f"_la_torch.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}"
+                      f".abi{int(torch._C._GLIBCXX_USE_CXX11_ABI)}.so")
+
 
 _ENTRIES = tuple(n for n in N.EXPORTED_SYMBOLS
                  if n.startswith(("la_recurrence_", "la_short_conv_", "la_group_norm_")))
@@ -29,12 +40,14 @@ def module():
     if _module is None:
         with _lock:
             if _module is None:
-                if not PATH.exists():
-                    raise RuntimeError(f"{PATH} is missing; build it with "
+                file = path()
+                if not file.exists():
+                    raise RuntimeError(f"{file} (the one for this Python and torch) is missing; "
+                                       "build it with "
                                        "`python -m trainium_linear_attention_b200.build`")
                 lib = N.lib()
-                loader = importlib.machinery.ExtensionFileLoader("_la_torch", str(PATH))
-                spec = importlib.util.spec_from_file_location("_la_torch", PATH, loader=loader)
+                loader = importlib.machinery.ExtensionFileLoader("_la_torch", str(file))
+                spec = importlib.util.spec_from_file_location("_la_torch", file, loader=loader)
                 loaded = importlib.util.module_from_spec(spec)
                 loader.exec_module(loaded)
                 loaded.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value

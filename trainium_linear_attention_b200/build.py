@@ -8,9 +8,10 @@ linked into ``trainium_linear_attention_b200/lib/libla_attention.so``.  The
 CUDA runtime is linked statically; the CUDA driver is reached at run time
 through ``cudaGetDriverEntryPoint`` (TMA descriptors), so the library has no
 link-time dependency on ``libcuda``.  ``csrc/torch_binding.cpp`` becomes
-``lib/_la_torch.so`` (g++, torch's headers; it has no kernels and takes the C
-entry points from the library at run time).  Objects are rebuilt only when a
-source or header is newer than they are.
+``lib/_la_torch.*.so``, named for the interpreter and the torch that it is built
+for (g++, torch's headers; it has no kernels and takes the C entry points from
+the library at run time).  Objects are rebuilt only when a source or header is
+newer than they are.
 """
 
 from __future__ import annotations
@@ -31,7 +32,6 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB = PKG / "lib" / "libla_attention.so"
 BINDING_SRC = CSRC / "torch_binding.cpp"
-BINDING = PKG / "lib" / "_la_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3",
@@ -62,13 +62,17 @@ def _compile(src: Path, obj: Path, verbose: bool) -> str:
 
 def _build_binding(force: bool) -> None:
     """Compile the torch binding (no CUDA code: the C++ compiler alone)."""
-    newest = max(BINDING_SRC.stat().st_mtime, (INCLUDE / "la_attention.h").stat().st_mtime)
-    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest:
-        return
     import torch
+
+    from . import _torch_binding
+    binding = _torch_binding.path()
+    newest = max(f.stat().st_mtime for f in (BINDING_SRC, INCLUDE / "la_attention.h",
+                                             Path(__file__)))  # (which has the command)
+    if not force and binding.exists() and binding.stat().st_mtime >= newest:
+        return
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + str(INCLUDE),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for path in (root / "include", root / "include/torch/csrc/api/include", cuda / "include",
@@ -79,12 +83,13 @@ def _build_binding(force: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, BINDING)
+    os.replace(tmp, binding)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every kernel source, link the shared library and compile the torch
-    binding; returns the library's path."""
+    binding; returns the library's path.  A binding that cannot be built is an error
+    behind the linking: the library is there for C all the same."""
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     hdr = _headers_mtime()
@@ -99,16 +104,16 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         for out in ex.map(lambda j: _compile(j[0], j[1], verbose), jobs):
             if out:
                 print(out, file=sys.stderr)
+        objs = [BUILD / (s.stem + ".o") for s in srcs]
+        newest = max(o.stat().st_mtime for o in objs)
+        if force or jobs or not LIB.exists() or LIB.stat().st_mtime < newest:
+            tmp = LIB.with_suffix(".so.tmp")
+            cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs)]
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            if res.returncode != 0:
+                raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+            os.replace(tmp, LIB)
         binding.result()
-    objs = [BUILD / (s.stem + ".o") for s in srcs]
-    newest = max(o.stat().st_mtime for o in objs)
-    if force or jobs or not LIB.exists() or LIB.stat().st_mtime < newest:
-        tmp = LIB.with_suffix(".so.tmp")
-        cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs)]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
-        os.replace(tmp, LIB)
     return LIB
 
 
