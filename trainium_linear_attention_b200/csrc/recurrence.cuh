@@ -46,7 +46,7 @@ constexpr float kExpMost = 8.5070592e37f;  // 2^126, whose reciprocal is still n
 
 // exp(z) - 1 for z <= 0, to a relative 2^-23: z = n ln 2 + f with |f| <= ln 2 / 2,
 // exp(z) - 1 = 2^n (exp(f) - 1) + (2^n - 1), exp(f) - 1 = f + f^2 q(f).  q is the
-// Chebyshev fit of degree 4 on that interval (1.2e-8 of exp(f) - 1).  On the
+// Chebyshev fit of degree 4 on that interval (2.4e-8 of exp(f) - 1).  On the
 // FMA pipe: the special-function unit is as busy as memory without it.
 __device__ __forceinline__ float2 expm1_neg(float2 z) {
   z.x = max_nan(z.x, -80.f);  // exp(-80) is far below half an ulp of 1
@@ -61,8 +61,8 @@ __device__ __forceinline__ float2 expm1_neg(float2 z) {
   q = __ffma2_rn(q, f, two(0.16666504740715027f));
   q = __ffma2_rn(q, f, two(0.5f));
   const float2 p = __ffma2_rn(__fmul2_rn(f, f), q, f);
-  const float2 s = make_float2(__int_as_float(__float_as_int(t.x) * (1 << 23) + 0x3F800000),
-                               __int_as_float(__float_as_int(t.y) * (1 << 23) + 0x3F800000));
+  const float2 s = make_float2(__uint_as_float(__float_as_uint(t.x) * (1u << 23) + 0x3F800000u),
+                               __uint_as_float(__float_as_uint(t.y) * (1u << 23) + 0x3F800000u));
   return __ffma2_rn(s, p, __fadd2_rn(s, two(-1.f)));
 }
 
