@@ -66,7 +66,7 @@ recur_bwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
       (T *)smem + warp * kIn * elems, kWarps * kIn * elems, elems, &ex.full[0][warp], kWarps,
-      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
   const int rows = parts * kL;            // tokens of a warp and step
   const int block_rows = kWarps * rows;
   const int blocks = (len + block_rows - 1) / block_rows;
@@ -304,7 +304,7 @@ int launch(const RecurCall &p, RecurLaunch l, cudaStream_t s) {
 
 template <typename T, bool kDecay, bool kInput>
 int launch_by_fetch(const RecurCall &p, const RecurShape &shape, cudaStream_t s) {
-  RecurLaunch l{{shape.ch, 0, false, device_error_word()}, shape.cluster};
+  RecurLaunch l{{shape.ch, 0, device_error_word()}, shape.cluster};
   const TokenView *views[4] = {&p.x, &p.gate, &p.d_out, &p.input_gate};
   const Fetch f = recur_fetch(p, views, 4, sizeof(T), kL, &l.tile);
   if constexpr (sizeof(T) == 2) {

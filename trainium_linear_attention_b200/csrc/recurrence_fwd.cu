@@ -81,7 +81,7 @@ recur_fwd_kernel(const RecurCall p, const RecurLaunch l, const __grid_constant__
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
   WarpTiles<T, kL, kIn, kStages, kF> tiles{
       (T *)smem + warp * kIn * elems, kWarps * kIn * elems, elems, &ex.full[0][warp], kWarps,
-      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, l.tile.wide, p.sizes, 0};
+      views, maps.m, ib, c0, ch, min(ch, channels - c0), l.tile.copy, p.sizes, 0};
   const int rows = parts * kL;                      // tokens of a warp and step
   const int step = cluster * kWarps * rows;    // of all
   const int steps = (len + step - 1) / step;
@@ -258,7 +258,7 @@ int launch_by_fetch(const RecurCall &p, cudaStream_t s) {
   DeviceInfo info;
   const int st = current_device_info(&info);
   if (st != LA_OK) return st;
-  RecurLaunch l{{0, 0, false, device_error_word()}, 1};
+  RecurLaunch l{{0, 0, device_error_word()}, 1};
   const TokenView *views[3] = {&p.x, &p.gate, &p.input_gate};
   const Fetch f = recur_fetch(p, views, 3, sizeof(T), kL, &l.tile);
   const RecurShape shape =

@@ -130,7 +130,7 @@ conv_fwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   const TokenView *views[1] = {&p.x};
   WarpTiles<T, kL, 1, kStages, kF> tiles{
       (T *)smem + warp * kElems, kWarps * kElems, kElems, &bars.full[0][warp], kWarps, views, maps.m, ib,
-      c0, 64, min(64, channels - c0), l.copy, l.wide, p.sizes, 0};
+      c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
   // Whole tiles, and the one that the run or the sequence ends in.
   auto fetch = [&](int t, int stage) { tiles.fetch(t, whole, stage); };
 #pragma unroll
@@ -222,7 +222,7 @@ conv_bwd_kernel(const ConvCall p, const TileLaunch l, const __grid_constant__ Ti
   const TokenView *views[2] = {&p.x, &p.d_out};
   WarpTiles<T, kL, 2, kStages, kF> tiles{
       (T *)smem + warp * 2 * kElems, kWarps * 2 * kElems, kElems, &bars.full[0][warp], kWarps, views,
-      maps.m, ib, c0, 64, min(64, channels - c0), l.copy, l.wide, p.sizes, 0};
+      maps.m, ib, c0, 64, min(64, channels - c0), l.copy, p.sizes, 0};
   // Whole tiles, and those that the run, its neighbour's first tokens or the sequence
   // end in.
   const int reach = min(len, end + kTaps - 1);
@@ -377,7 +377,7 @@ template <typename T>
 int run_conv(ConvCall p, bool grad, cudaStream_t s) {
   constexpr int size = sizeof(T);
   const TokenView *views[2] = {&p.x, &p.d_out};
-  TileLaunch l{64, 0, false, device_error_word()};
+  TileLaunch l{64, 0, device_error_word()};
   const Fetch f = fetch_of(views, 2, p.sizes, size, kL, &l);
   auto at = [&](std::initializer_list<const void *> q) {
     uintptr_t bits = (uintptr_t)p.sizes.channels * size;

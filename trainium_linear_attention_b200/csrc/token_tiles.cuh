@@ -150,7 +150,8 @@ __device__ __noinline__ void copy_edge(T *tile, const T *row0, int64_t st, int t
   else copy_tile<T, kL, 4>(tile, row0, st, t0, len, ch, width);
 }
 
-// A pair of channels at p, the second of which may be beyond the row.
+// A pair of channels at p, the second of which may be beyond the row; `wide`: pairs
+// start at their own size.
 template <typename T>
 __device__ __forceinline__ float2 pair_at(const T *p, bool wide, bool second) {
   if (wide && second) return load_two(p);
@@ -193,7 +194,6 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
 struct TileLaunch {
   int ch;       // channels of a CTA
   int copy;     // kAsync: bytes of a copy, 4 or 8
-  bool wide;    // pairs of channels start at their own size
   int *err;     // the library's device error word
 };
 
@@ -208,7 +208,6 @@ struct WarpTiles {
   const CUtensorMap *maps;
   int64_t ib;
   int c0, ch, width, copy;
-  bool wide;
   TokenSizes sizes;
   uint32_t phases;          // kTma: a bit per stage
 
@@ -332,7 +331,6 @@ inline Fetch fetch_of(const TokenView *const *views, int n, const TokenSizes &s,
     least = bytes < least ? bytes : least;
   }
   launch->copy = least >= 8 ? 8 : 4;
-  launch->wide = least >= 2 * size;
   return tma ? Fetch::kTma : least < 4 ? Fetch::kShifted : Fetch::kAsync;
 }
 
