@@ -16,8 +16,9 @@
 // joined over the CTA's row lanes in shared memory, written as one row per CTA,
 // and added by a second kernel in a fixed order.
 //
-// 16384 x 1024 in 16 groups with a gate's SiLU in 27 us (57% of the copy rate, 62% of
-// the issue slots), its gradient in 40 (64%).  Groups whose starts are not on 16 bytes
+// 16384 x 1024 in 16 groups with a gate's SiLU in 27 us (57% of the copy rate), its gradient
+// in 41 (62%); the wait for loads, one row ahead, comes first (62 and 51% of the issue
+// slots).  In fp32 38 us (80%) and 60 (85%).  Groups whose starts are not on 16 bytes
 // take pairs or single values, whose accesses bound them: 16384 x 1023 in 11 groups 66.
 #include <initializer_list>
 

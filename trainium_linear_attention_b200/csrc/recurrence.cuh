@@ -192,7 +192,7 @@ __device__ __forceinline__ void store_remote(float4 *p, uint64_t *bar, uint32_t 
 // a cluster's exchange at every step costs more than an idle SM (16384 x 2048 in
 // 69 us by 128 CTAs of 16 channels, in 85 by 256 in clusters of two).  One CTA of 16
 // warps on most SMs beats two of 8 on some, where instructions bound it (`heavy`: 8 x
-// 32768 x 1024 by 128 CTAs of 64 channels and 16 warps in 384 us, by 256 of 32 and 8
+// 32768 x 1024 by 128 CTAs of 64 channels and 16 warps in 385 us, by 256 of 32 and 8
 // in 429; the gradient of 4 x 4096 x 1024 in 71 and 73); where memory does, all SMs'
 // loads count (8 x 8192 x 1024 without a decay: 84 and 72).  `roomy`: 16 warps' tiles
 // fit (bf16).  Many short sequences take CTAs of 2 warps, more of which start

@@ -16,7 +16,8 @@
 // tokens (a quarter of a byte per element, against two for an h rounded to
 // bf16); those states keep the forward chain out of the walk: with one state per
 // CTA's tile, handed on from warp to warp against the gradient's direction, 4 x
-// 4096 x 1024 took 125 us instead of 71 (52% of the copy rate; 61% of the issue slots).
+// 4096 x 1024 took 125 us instead of 71 (52% of the copy rate; no unit above 61%, the wait
+// for tiles comes first: 128 CTAs on 148 SMs, 16 warps on each).
 // d(lambda) is summed over a CTA's tokens and written as one row per CTA; a second
 // kernel adds the rows in a fixed order.
 #include <type_traits>

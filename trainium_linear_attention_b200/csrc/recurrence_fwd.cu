@@ -2,7 +2,7 @@
 //
 // Bound by memory and, nearly as much, by its instructions: x and the gates are
 // read once and h is written once (8 bytes per element in bf16 with both gates),
-// against 35 instructions and 4 of the special-function unit, which does 16 a cycle
+// against 36 instructions and 4 of the special-function unit, which does 16 a cycle
 // and SM.  A channel's sequence is a chain, and channels x batch are too few
 // chains for the SMs, so a CTA takes 64, 32 or 16 channels and its lanes and warps
 // neighbouring groups of kL tokens.  A thread
@@ -20,13 +20,13 @@
 //
 // A CTA has 2, 8 or 16 warps (recur_shape says when).
 //
-// 8 x 32768 x 1024 in 385 us (5.6 TB/s, 85% of the copy rate), 16384 x 2048 in 60
-// (128 CTAs: 68%), 4 x 4096 x 1024 in 33 (62%; 62% of the issue slots, 60% of the
-// special-function unit's).  What it took, for the first of these: one barrier-bound
-// form with cp.async 873 us, fewer instructions (one root for beta and u, no selects)
+// 8 x 32768 x 1024 in 392 us (5.5 TB/s, 83% of the copy rate), 16384 x 2048 in 61
+// (128 CTAs: 67%), 4 x 4096 x 1024 in 34 (60%; 62% of the issue slots, 59% of the
+// special-function unit's), in fp32 55 (74%).  What it took, for the first of these: one
+// barrier-bound form with cp.async 873 us, fewer instructions (one root for beta and u, no selects)
 // 663, TMA 524, the hand-over from warp to warp 451, tiles that any channel width reads
 // without bank conflicts and stores without predicates 421, 16 warps with one chain of
-// hand-overs for an SM 385.
+// hand-overs for an SM 385 (392 with input gates below -44).
 #include "recurrence.cuh"
 #include "tc_kernels.cuh"
 

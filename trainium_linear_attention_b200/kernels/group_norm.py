@@ -41,7 +41,8 @@ def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, ep
     channels into neighbours of up to 8192; ``weight`` and ``bias``: (channels,),
     fp32 or in x.dtype, or None for ones and zeros.  ``activation``: None or
     "silu", applied to the gate where there is one, else to the normed value.
-    Statistics in fp32, the variance from squared differences.  Returns y
+    Statistics in fp32, the variance from squared differences, the activation's
+    sigmoid to 2^-20 (0 below 2^-126).  Returns y
     (contiguous, in x.dtype).  Differentiable once, backward (forward mode is
     refused); the gradients of weight and bias are summed in a fixed order."""
     check_tangents(x, weight, bias, gate)

@@ -49,7 +49,8 @@ def causal_conv(x, weight, bias=None, activation=None, initial_state=None, retur
     ``lengths``: as for ``gated_recurrence``.
 
     Returns (b, t, channels) in x.dtype, contiguous, or with ``return_state``
-    also the last taps - 1 tokens.  Sums in fp32.  Differentiable once, backward,
+    also the last taps - 1 tokens.  Sums in fp32, the activation's sigmoid to 2^-20
+    (0 below 2^-126).  Differentiable once, backward,
     in x, weight, bias and ``initial_state`` (forward mode is refused); the
     gradients of weight and bias are summed in a fixed order."""
     check_tangents(x, weight, bias, initial_state)
