@@ -4,6 +4,7 @@ how it calls the library, with other functions in the place of its entry points.
 import contextlib
 import ctypes
 import subprocess
+import threading
 from types import SimpleNamespace
 
 import pytest
@@ -122,3 +123,46 @@ def test_statuses_raise_their_error():
             with bound({name: unsupported}), pytest.raises(N.LaError, match=name) as caught:
                 y.sum().backward()
             assert caught.value.status == N.LA_ERR_UNSUPPORTED
+
+
+@gpu
+def test_threads_on_streams_of_their_own():
+    """Two threads' calls and backward passes at a time, of sizes that differ in the kernels'
+    shared memory, give what they give one after the other."""
+    def chain(c, seed):
+        gen = torch.Generator().manual_seed(seed)
+        x, gate = (torch.randn(3, 200, c, generator=gen).bfloat16().cuda().requires_grad_()
+                   for _ in range(2))
+        w = torch.randn(c, 4, generator=gen).cuda().requires_grad_()
+        lam = -torch.rand(c, generator=gen).cuda().requires_grad_()
+
+        def run():
+            h = T.gated_recurrence(T.causal_conv(x, w, activation="silu"), gate, lam)
+            y = T.group_norm(h, 1, gate=gate, activation="silu")
+            return [y.detach(), *torch.autograd.grad(y, [x, gate, w, lam], torch.ones_like(y))]
+        return run
+
+    runs = [chain(c, i) for i, c in enumerate((63, 21, 64, 128))]
+    want = [run() for run in runs]
+    torch.cuda.synchronize()
+    found, failed = [[] for _ in runs], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    found[i].append(runs[i]())
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001 (told to the test's thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(runs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for i, expected in enumerate(want):
+        for got in found[i]:
+            assert all(torch.equal(a, b) for a, b in zip(expected, got))
